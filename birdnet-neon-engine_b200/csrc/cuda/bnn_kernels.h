@@ -310,6 +310,61 @@ int bnnk_pad_f16(int B, int H, int W, int C, int ld, int h, const uint16_t *x, l
 int bnnk_mean_f16(int B, int P, int C, int ld, const uint16_t *x, long long xws, float *out, long long ows,
                   bnn_stream_t st);
 
+/* ---- operators over sequences of windows (k_norm.cu, k_dattn.cu, k_lowrank.cu); element types 0 fp32, 1 fp16,
+ * 2 bf16, strides in elements */
+/* u = norm(f) wpost + bpost; xo = x + alpha gamma act(g) u; h = norm(xo) wpre + bpre over rows of D (f, xo, h and the
+ * vectors may be NULL); rows with live[r] == 0: xo = x, h = 0. gate: 0 none, 1 sigmoid, 2 SiLU; layer: 0 RMS norm, 1
+ * layer norm. xtype is 0 or type. */
+typedef struct {
+  int rows, D, xtype, type, layer, gate;
+  float eps, alpha;
+  const void *x, *f, *g;
+  long long xs, fs, gs;
+  const float *wpost, *bpost, *gamma, *wpre, *bpre;
+  const uint8_t *live;
+  void *xo, *h;
+  long long xos, hs;
+} bnnk_norm_gate_args;
+int bnnk_norm_gate(const bnnk_norm_gate_args *a, bnn_stream_t st);
+
+/* linear attention with a decay per k/v head over n sequences: tokens cu[i] .. cu[i + 1] (cu NULL: token i), states
+ * s0 -> s1 [slot[i]] (slot NULL: i; negative: from zero, not stored) [Hk][dk][dv]; pow [Hk][kDattnPow] holds
+ * lambda^0 .. lambda^128. type 1 or 2; dk, dv multiples of 8 up to 128, 16-byte aligned rows. */
+#define kDattnPow 132
+typedef struct {
+  int type, n, H, Hk, dk, dv;
+  long long tokens;
+  const int32_t *cu, *slot;
+  const uint8_t *live;
+  const void *q, *k, *v;
+  long long qts, kts, vts;
+  const float *s0;
+  float *s1;
+  void *o;
+  long long ots;
+  const float *pow;
+  float scale;
+} bnnk_dattn_args;
+int bnnk_dattn(const bnnk_dattn_args *a, bnn_stream_t st);
+
+/* y = x w^T + bias + scale[s] (x a[s]^T) b[s]^T, s = slot[row]; otype 0 or type; hid: scratch [rows][rank]. K and rank
+ * multiples of 8, x, w and a rows 16-byte aligned */
+typedef struct {
+  int type, otype, rows, N, K, slots, rank;
+  const void *x;
+  long long ldx;
+  const void *w;
+  long long ldw;
+  const float *bias;
+  const int32_t *slot;
+  const void *a, *b;
+  const float *scale;
+  float *hid;
+  void *y;
+  long long ldy;
+} bnnk_lowrank_args;
+int bnnk_lowrank(const bnnk_lowrank_args *a, bnn_stream_t st);
+
 #ifdef __cplusplus
 }
 #endif

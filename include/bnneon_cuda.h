@@ -225,6 +225,74 @@ int bnn_cuda_stem_f16(int B, const float *d_img, long long iws, int H, int W, in
                       const float *d_w, const float *d_b, int N, int Kp, int act, void *d_out, long long ows, int ldo,
                       int opad, void *stream);
 
+/* ---- operators over sequences of windows (no counterpart in the reference): a block that looks across the windows of
+ * a recording or of a live station, run by hosts on the embeddings this library writes. Activations are fp16 or bf16
+ * (BNN_T_*), states and statistics fp32. Strides are in elements; buffers are the caller's device memory. An op object
+ * belongs to the device that was current when it was made. */
+enum { BNN_T_F32 = 0, BNN_T_F16 = 1, BNN_T_BF16 = 2 };
+enum { BNN_NORM_RMS = 0, BNN_NORM_LAYER = 1 };
+enum { BNN_GATE_NONE = 0, BNN_GATE_SIGMOID = 1, BNN_GATE_SILU = 2 };
+
+/* Linear attention with a decay for each key / value head. Per sequence, in fp32,
+ *   S_t = decay[j] S_(t-1) + k_t^T v_t,   o_t = scale q_t S_t       S [dk][dv], decay in [0, 1]
+ * for q heads in groups of heads / kv_heads that share k/v head j and its S. Tokens lie as q [tokens][heads][dk], k
+ * [tokens][kv_heads][dk], v [tokens][kv_heads][dv], o [tokens][heads][dv] at token strides qts, kts, vts, ots (so q, k
+ * and v may be parts of one projection's rows; multiples of 8, 16-byte aligned pointers). dk and dv are multiples of 8
+ * up to 128. decay: kv_heads host floats. seqs and tokens are the most of a call. */
+typedef struct bnn_dattn bnn_dattn;
+bnn_dattn *bnn_dattn_new(int type, int heads, int kv_heads, int dk, int dv, const float *decay, float scale, int seqs,
+                         long long tokens);
+/* n sequences of any lengths, 0 included: sequence i is the tokens d_cu[i] .. d_cu[i + 1] - 1 (n + 1 ascending offsets
+ * in 0 .. tokens). It starts from the state d_s0[slot] and leaves its state in d_s1[slot], [kv_heads][dk][dv] floats a
+ * slot, slot = d_slot[i] (d_slot NULL: i; a negative slot starts from zero and its state is dropped; no two sequences
+ * of a call share a slot). d_s0 NULL: all start from zero; d_s1 NULL: no state is kept; d_s1 may be d_s0. A token whose
+ * byte of d_live (NULL: all live) is 0 is a window that failed or is missing: its q, k and v are not used, its o is 0,
+ * and the state decays by its step. */
+int bnn_dattn_run(bnn_dattn *op, int n, long long tokens, const int32_t *d_cu, const int32_t *d_slot,
+                  const uint8_t *d_live, const void *d_q, long long qts, const void *d_k, long long kts, const void *d_v,
+                  long long vts, const float *d_s0, float *d_s1, void *d_o, long long ots, void *stream);
+/* the same for n sequences of one token each (token i is sequence i's) */
+int bnn_dattn_step(bnn_dattn *op, int n, const int32_t *d_slot, const uint8_t *d_live, const void *d_q, long long qts,
+                   const void *d_k, long long kts, const void *d_v, long long vts, const float *d_s0, float *d_s1,
+                   void *d_o, long long ots, void *stream);
+/* the op's device error word (0 = no bounded wait ran out); synchronous */
+int bnn_dattn_error(bnn_dattn *op);
+void bnn_dattn_free(bnn_dattn *op);
+
+/* A projection shared by all rows, with a low-rank adapter of many for each row:
+ *   y_r = W x_r + bias + scale[s] B[s] (A[s] x_r),   s = d_slot[r]
+ * d_w [N][K] at row stride ldw, d_bias [N] fp32 or NULL, d_a [slots][rank][K], d_b [slots][N][rank], d_scale [slots]
+ * fp32 or NULL (1): the caller's device memory, read by every run, so an adapter can be replaced in stream order. K and
+ * ldw are multiples of 8, rank one in 8 .. 64, d_w, d_a and d_b 16-byte aligned. x, W, A and B are of `type` (fp16 or
+ * bf16), y of `out_type` (the same or fp32). rows: the most rows of a call. */
+typedef struct bnn_lowrank bnn_lowrank;
+bnn_lowrank *bnn_lowrank_new(int type, int out_type, int N, int K, const void *d_w, long long ldw, const float *d_bias,
+                             int slots, int rank, const void *d_a, const void *d_b, const float *d_scale, int rows);
+/* d_x [rows][K] at row stride ldx (a multiple of 8, 16-byte aligned) -> d_y [rows][N] at row stride ldy; d_slot [rows]:
+ * the rows' adapters in any order (outside 0 .. slots - 1: none), NULL: none for all */
+int bnn_lowrank_run(bnn_lowrank *op, int rows, const void *d_x, long long ldx, const int32_t *d_slot, void *d_y,
+                    long long ldy, void *stream);
+/* the op's device error word (0 = no bounded wait ran out); synchronous */
+int bnn_lowrank_error(bnn_lowrank *op);
+void bnn_lowrank_free(bnn_lowrank *op);
+
+/* The norms before and after a block with its gate and residual scale, over rows of D:
+ *   u = norm(f) wpost + bpost,  x' = x + alpha gamma act(g) u,  h = norm(x') wpre + bpre
+ * norm: BNN_NORM_RMS v / sqrt(mean v^2 + eps), or BNN_NORM_LAYER, which takes the mean out first; act: BNN_GATE_*.
+ * x and x' are of x_type (fp32, or `type`), f, g and h of `type`; the vectors (the caller's fp32 device memory, [D])
+ * may be NULL: 1 for wpost, gamma and wpre, 0 for bpost and bpre. */
+typedef struct bnn_norm_gate bnn_norm_gate;
+bnn_norm_gate *bnn_norm_gate_new(int D, int x_type, int type, int norm, int gate, float eps, float alpha,
+                                 const float *d_wpost, const float *d_bpost, const float *d_gamma, const float *d_wpre,
+                                 const float *d_bpre);
+/* rows at strides xs, fs, gs, xos, hs. d_f NULL: x' = x (the norm before the first block; d_g is not read); d_xo or d_h
+ * NULL: not written; d_xo may be d_x and d_h may be d_f at equal strides. A row whose byte of d_live (NULL: all live) is
+ * 0: its f and g are not used, x' = x and h = 0. */
+int bnn_norm_gate_run(bnn_norm_gate *op, int rows, const void *d_x, long long xs, const void *d_f, long long fs,
+                      const void *d_g, long long gs, const uint8_t *d_live, void *d_xo, long long xos, void *d_h,
+                      long long hs, void *stream);
+void bnn_norm_gate_free(bnn_norm_gate *op);
+
 /* the current device's error word of the per-op entry points (0 = no bounded device wait ran out; then reset to 0;
  * -1 if it cannot be read); synchronous */
 int bnn_cuda_op_error(void);

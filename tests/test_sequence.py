@@ -1,0 +1,599 @@
+"""The operators over sequences of windows (bnn_dattn_*, bnn_lowrank_*, bnn_norm_gate_*) against their definitions in 64
+bits, and their refusals.
+
+Tolerances, element by element. An output of t bits of significand is rounded once: u |want|, u = 2^-8 (bf16), 2^-11
+(fp16), 2^-24 (fp32), and half the type's smallest step. A sum of n terms in fp32 is off by at most n 2^-24 times the sum
+M of the terms' magnitudes. An fp32 factor that the tensor cores take as two 16-bit parts is off by the square of their
+unit roundoff, 2^-16 for bf16: two such factors in a term (a chunk's products, the state before it) give 2^-15 M.
+"""
+import math
+
+import numpy as np
+import pytest
+
+from bnneon_b200 import BnnError, load_library, sequence
+
+torch = pytest.importorskip("torch")
+gpu = pytest.mark.gpu
+DT = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
+U = {"bf16": 2.0 ** -8, "f16": 2.0 ** -11, "f32": 2.0 ** -24}
+TINY = {"bf16": 2.0 ** -134, "f16": 2.0 ** -25, "f32": 2.0 ** -150}
+
+
+@pytest.fixture(scope="module")
+def cuda():
+    if not torch.cuda.is_available():
+        pytest.fail("a GPU test ran without a visible CUDA device")
+    torch.cuda.init()
+    load_library()
+    return torch.device("cuda")
+
+
+def rand(gen, *shape):
+    return torch.randn(*shape, device="cuda", generator=gen)
+
+
+def generator(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+def check(got, want, slack, dtype, what):
+    got, want = got.double(), want.double()
+    assert bool(torch.isfinite(got).all()), f"{what}: not finite"
+    off = (got - want).abs() - (U[dtype] * want.abs() + TINY[dtype] + slack)
+    assert float(off.max() if off.numel() else 0) <= 0, (
+        f"{what}: {int((off > 0).sum())} of {off.numel()} beyond, worst by {float(off.max()):.3g} "
+        f"(error {float((got - want).abs().max()):.3g})")
+
+
+# ------------------------------------------------------------------ linear attention with decay
+
+
+class Attention:
+    """inputs of one call; tokens of dead rows hold NaN"""
+
+    def __init__(self, dtype, H, Hk, dk, dv, lens, masked=0.0, states=None, seed=0, decay=None, row=0, k_scale=1.0):
+        gen = generator(seed)
+        self.dtype, self.H, self.Hk, self.dk, self.dv, self.lens = dtype, H, Hk, dk, dv, lens
+        T = sum(lens)
+        t = DT[dtype]
+        # q, k and v as parts of one projection's rows, with `row` more elements a row
+        width = H * dk + Hk * (dk + dv) + row
+        buf = rand(gen, T + 1, width)[:T]
+        buf[:, H * dk:H * dk + Hk * dk] *= k_scale
+        self.buf = buf.to(t)
+        self.q = self.buf[:, :H * dk].unflatten(1, (H, dk))
+        self.k = self.buf[:, H * dk:(H + Hk) * dk].unflatten(1, (Hk, dk))
+        self.v = self.buf[:, (H + Hk) * dk:(H + Hk) * dk + Hk * dv].unflatten(1, (Hk, dv))
+        self.ts = width
+        self.live = None
+        if masked:
+            self.live = torch.rand(T, device="cuda", generator=gen) >= masked
+            self.buf[~self.live] = math.nan
+        n = len(lens)
+        self.cu = torch.tensor([0] + lens).cumsum(0).int().cuda()
+        self.slot = torch.randperm(n + 3, device="cuda", generator=gen)[:n].int() if states is None else states.int()
+        self.s0 = rand(gen, n + 3, Hk, dk, dv)
+        self.decay = np.asarray(decay if decay is not None else 1 - 2.0 ** -np.linspace(0.5, 9, Hk), np.float32)
+        self.scale = dk ** -0.5
+        self.o = torch.full((T, H, dv), 7.0, device="cuda", dtype=t)
+
+    def op(self, **kw):
+        return sequence.DecayAttention(self.dtype, self.H, self.dk, self.dv, self.decay, kv_heads=self.Hk,
+                                       scale=self.scale, seqs=max(1, len(self.lens)), tokens=max(1, sum(self.lens)), **kw)
+
+    def run(self, op, s0=True, s1=None, slot=True, stream=None, step=False):
+        args = [self.q.data_ptr(), self.k.data_ptr(), self.v.data_ptr(), self.o.data_ptr(),
+                self.s0.data_ptr() if s0 else None, None if s1 is None else s1.data_ptr()]
+        kw = dict(slot=self.slot.data_ptr() if slot else None, live=None if self.live is None else self.live.data_ptr(),
+                  qts=self.ts, kts=self.ts, vts=self.ts, stream=stream)
+        if step:
+            op.step(len(self.lens), *args, **kw)
+        else:
+            op.run(len(self.lens), sum(self.lens), self.cu.data_ptr(), *args, **kw)
+
+    def want(self, s0=True, slot=True):
+        """(o, {sequence: state}) and the sums of their terms' magnitudes, token by token"""
+        out, states = [], []
+        lam = torch.from_numpy(self.decay.astype(np.float64)).cuda()[:, None, None]
+        G = self.H // self.Hk
+        t0 = 0
+        o, mo = (torch.zeros(self.o.shape, dtype=torch.float64, device="cuda") for _ in range(2))
+        for i, L in enumerate(self.lens):
+            at = int(self.slot[i]) if slot else i
+            S = self.s0[at].double() if s0 and at >= 0 else torch.zeros_like(self.s0[0], dtype=torch.float64)
+            M = S.abs()
+            for t in range(t0, t0 + L):
+                S, M = lam * S, lam * M
+                if self.live is None or bool(self.live[t]):
+                    kv = self.k[t].double()[:, :, None] * self.v[t].double()[:, None, :]
+                    S, M = S + kv, M + kv.abs()
+                    q = self.q[t].double().view(self.Hk, G, self.dk)
+                    o[t] = self.scale * torch.matmul(q, S).view(self.H, self.dv)
+                    # the chunk form's terms are (q . k) v: their magnitude is at most |q| |k| |v| summed, as M has it
+                    mo[t] = self.scale * torch.matmul(q.abs(), M).view(self.H, self.dv)
+            states.append((S, M))
+            t0 += L
+        out = (o, mo)
+        return out, states
+
+    def check(self, s1, s0=True, slot=True, what=""):
+        (o, mo), states = self.want(s0, slot)
+        n = max(self.lens + [0]) + self.dk + 4
+        rel = 2.0 ** -15 + n * 2.0 ** -24
+        check(self.o, o, rel * mo, self.dtype, what + "o")
+        if s1 is not None:
+            for i, (S, M) in enumerate(states):
+                at = int(self.slot[i]) if slot else i
+                if at >= 0:
+                    check(s1[at], S, rel * M, "f32", f"{what}state {i} of {self.lens[i]} tokens")
+
+
+ATTENTION = [
+    # dtype, heads, kv heads, dk, dv, lengths, share of masked tokens
+    ("bf16", 2, 2, 128, 128, [1], 0),
+    ("f16", 2, 2, 64, 64, [3, 0, 1, 17], 0),
+    ("bf16", 2, 2, 128, 128, [128, 129, 127, 0, 255, 1, 300], 0),
+    ("f16", 2, 2, 128, 128, [384, 63, 65], 0.2),
+    ("bf16", 3, 1, 64, 64, [200, 130, 64], 0.1),
+    ("f16", 6, 2, 96, 72, [150, 1, 290], 0.3),
+    ("bf16", 4, 4, 40, 24, [333, 90], 0),
+    ("f16", 1, 1, 8, 8, [513], 0),
+    ("bf16", 8, 1, 72, 128, [140, 260], 0.5),
+    ("f16", 2, 1, 128, 16, [700], 0),
+    ("bf16", 1, 1, 128, 64, [2500], 0.05),
+    ("bf16", 1, 1, 64, 128, [1900, 5], 0),
+    ("f16", 20, 1, 32, 32, [131], 0.1),
+]
+
+
+@gpu
+@pytest.mark.parametrize("case", range(len(ATTENTION)))
+def test_dattn_against_64_bits(cuda, case):
+    dtype, H, Hk, dk, dv, lens, masked = ATTENTION[case]
+    a = Attention(dtype, H, Hk, dk, dv, lens, masked, seed=case, row=8 * (case % 3))
+    s1 = torch.full_like(a.s0, 9.0)
+    op = a.op()
+    a.run(op, s1=s1)
+    a.check(s1)
+    untouched = [i for i in range(len(a.s0)) if i not in set(a.slot.tolist())]
+    assert bool((s1[untouched] == 9.0).all())
+    assert op.error == 0
+    # the same call again gives the same bits, in place too
+    o, s = a.o.clone(), s1.clone()
+    a.run(op, s1=s1)
+    assert torch.equal(a.o, o) and torch.equal(s1, s)
+    keep = a.s0.clone()
+    a.run(op, s1=a.s0)
+    assert torch.equal(a.o, o)
+    assert torch.equal(a.s0[a.slot.long()], s[a.slot.long()])
+    a.s0 = keep
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("heads", [(2, 2, 128, 128), (8, 2, 64, 64), (3, 1, 96, 72), (12, 1, 8, 104), (1, 1, 24, 128)])
+@pytest.mark.parametrize("n, masked", [(1, 0), (7, 0.4), (130, 0.1)])
+def test_dattn_step(cuda, dtype, heads, n, masked):
+    a = Attention(dtype, *heads, [1] * n, masked, seed=n)
+    s1 = torch.zeros_like(a.s0)
+    a.run(a.op(), s1=s1, step=True)
+    a.check(s1)
+
+
+@gpu
+def test_dattn_states_optional(cuda):
+    a = Attention("bf16", 2, 2, 64, 64, [140, 5, 0, 260], seed=3)
+    op = a.op()
+    s1 = torch.zeros_like(a.s0)
+    a.run(op, s0=False, s1=s1)
+    a.check(s1, s0=False, what="from zero: ")
+    a.run(op)
+    a.check(None, what="no state kept: ")
+    a.run(op, s1=s1, slot=False)
+    a.check(s1, slot=False, what="slots in order: ")
+    a.slot = torch.tensor([2, -1, 0, -1], device="cuda").int()
+    s1.fill_(5.0)
+    a.run(op, s1=s1)
+    a.check(s1, what="negative slots: ")
+    assert bool((s1[1] == 5.0).all()) and bool((s1[3:] == 5.0).all())
+
+
+@gpu
+@pytest.mark.parametrize("decay", [[0.0, 1.0], [0.5, 2.0 ** -30], [1.0, 1.0 - 2.0 ** -24]])
+def test_dattn_extreme_decays(cuda, decay):
+    a = Attention("bf16", 2, 2, 64, 64, [300, 1, 129], seed=5, decay=decay)
+    s1 = torch.zeros_like(a.s0)
+    a.run(a.op(), s1=s1)
+    a.check(s1)
+
+
+@gpu
+def test_dattn_all_masked(cuda):
+    a = Attention("f16", 2, 2, 64, 64, [200, 1, 128], 0.5, seed=6)
+    a.live.fill_(False)
+    a.buf.fill_(math.inf)
+    s1 = torch.zeros_like(a.s0)
+    a.run(a.op(), s1=s1)
+    assert bool((a.o == 0).all())
+    a.check(s1)
+
+
+@gpu
+def test_dattn_neighbours_do_not_leak(cuda):
+    """a sequence's results do not change when the tokens around it hold NaN"""
+    a = Attention("bf16", 2, 2, 128, 128, [70, 77, 300], seed=7)
+    s1 = torch.zeros_like(a.s0)
+    op = a.op()
+    a.run(op, s1=s1)
+    o = a.o.clone()
+    a.buf[:70] = math.nan
+    a.buf[147:] = math.inf
+    s2 = torch.zeros_like(a.s0)
+    a.run(op, s1=s2)
+    at = int(a.slot[1])
+    assert torch.equal(a.o[70:147], o[70:147]) and torch.equal(s2[at], s1[at])
+
+
+@gpu
+def test_dattn_prompt_then_steps(cuda):
+    """a prompt in one call, and the same tokens as a shorter prompt and single steps on its state"""
+    a = Attention("bf16", 4, 2, 64, 64, [140], seed=8)
+    whole = torch.zeros_like(a.s0)
+    a.run(a.op(), s1=whole)
+    want = a.o.clone()
+    state = a.s0.clone()
+    op = a.op()
+    cu = torch.tensor([0, 130]).int().cuda()
+    args = lambda t: (a.q[t].data_ptr(), a.k[t].data_ptr(), a.v[t].data_ptr(), a.o[t].data_ptr())  # noqa: E731
+    kw = dict(slot=a.slot.data_ptr(), qts=a.ts, kts=a.ts, vts=a.ts)
+    a.o.zero_()
+    op.run(1, 130, cu.data_ptr(), *args(0), state.data_ptr(), state.data_ptr(), **kw)
+    for t in range(130, 140):
+        op.step(1, *args(t), state.data_ptr(), state.data_ptr(), **kw)
+    a.check(state)
+    assert float((a.o.double() - want.double()).abs().max()) < 0.1
+
+
+@gpu
+def test_dattn_many_tokens_few_heads(cuda):
+    """long enough for the work to be split along the sequence; the definition in chunks of 64-bit products"""
+    a = Attention("bf16", 1, 1, 64, 64, [20011, 3000], 0.05, seed=9)
+    s1 = torch.zeros_like(a.s0)
+    a.run(a.op(), s1=s1)
+    a.check(s1)
+
+
+@gpu
+def test_dattn_offsets_past_32_bits(cuda):
+    """states and rows more than 2^32 bytes and 2^31 elements into their buffers"""
+    torch.cuda.empty_cache()
+    a = Attention("bf16", 16, 16, 128, 128, [130, 2], seed=10)
+    per = 16 * 128 * 128
+    pool = torch.empty((1 << 31) // per + 3, 16, 128, 128, device="cuda")
+    at = [len(pool) - 1, len(pool) - 2]
+    slot = torch.tensor(at).int().cuda()
+    for i, s in enumerate(at):
+        pool[s] = a.s0[i]
+    stride = 1 << 24
+    big = torch.empty(132 * stride + 4096, device="cuda", dtype=torch.bfloat16)
+    q = big.as_strided((132, 2048), (stride, 1))
+    q.copy_(a.q.reshape(132, 2048))
+    op = a.op()
+    op.run(2, 132, a.cu.data_ptr(), big.data_ptr(), a.k.data_ptr(), a.v.data_ptr(), a.o.data_ptr(), pool.data_ptr(),
+           pool.data_ptr(), slot=slot.data_ptr(), qts=stride, kts=a.ts, vts=a.ts)
+    a.slot = torch.tensor([0, 1]).int().cuda()
+    s1 = torch.stack([pool[s] for s in at])
+    a.check(s1)
+    del pool, big, q
+    torch.cuda.empty_cache()
+
+
+@gpu
+def test_operators_on_a_stream_of_their_own(cuda):
+    """inputs written on a side stream, the calls on that stream, with work before them that a wrong stream would miss"""
+    a = Attention("bf16", 2, 2, 64, 64, [150, 4], seed=11)
+    op = a.op()
+    s1 = torch.zeros_like(a.s0)
+    a.run(op, s1=s1)
+    want = a.o.clone()
+    side = torch.cuda.Stream()
+    keep = a.buf.clone()
+    a.buf.zero_()
+    a.o.zero_()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        big = torch.randn(4096, 4096, device="cuda")
+        for _ in range(10):
+            big = big @ big * 1e-4
+        a.buf.copy_(keep)
+        a.run(op, s1=s1, stream=side.cuda_stream)
+        got = a.o.clone()
+    side.synchronize()
+    assert torch.equal(got, want)
+
+
+# ------------------------------------------------------------------ shared projection, low-rank adapters
+
+
+def lowrank_case(dtype, out, rows, N, K, rank, slots, order, seed, bias=True, scale=True, xpad=0, ypad=0, wpad=0):
+    gen, t = generator(seed), DT[dtype]
+    x = rand(gen, rows, K + xpad).to(t)
+    w = (rand(gen, N, K + wpad) * K ** -0.5).to(t)
+    x[:, K:] = math.nan
+    w[:, K:] = math.nan
+    A, B = (rand(gen, slots, rank, K) * K ** -0.5).to(t), rand(gen, slots, N, rank).to(t)
+    b = rand(gen, N) if bias else None
+    s = torch.rand(slots, device="cuda", generator=gen) + 0.5 if scale else None
+    if order == "none":
+        slot = None
+    elif order == "runs":
+        slot = torch.sort(torch.randint(-1, slots, (rows,), device="cuda", generator=gen))[0].int()
+    else:
+        slot = torch.randint(-1, slots + 1, (rows,), device="cuda", generator=gen).int()  # slots: none, too
+    y = torch.full((rows, N + ypad), 7.0, device="cuda", dtype=DT[out])
+    op = sequence.LowRank(dtype, out, N, K, w.data_ptr(), None if b is None else b.data_ptr(), slots, rank, A.data_ptr(),
+                          B.data_ptr(), None if s is None else s.data_ptr(), rows=rows, ldw=K + wpad)
+    op.run(rows, x.data_ptr(), None if slot is None else slot.data_ptr(), y.data_ptr(), ldx=K + xpad, ldy=N + ypad)
+    first = y.clone()
+    op.run(rows, x.data_ptr(), None if slot is None else slot.data_ptr(), y.data_ptr(), ldx=K + xpad, ldy=N + ypad)
+    assert torch.equal(first, y), "the same call again"
+    assert op.error == 0
+    xd, wd = x[:, :K].double(), w[:, :K].double()
+    want, M = xd @ wd.t(), xd.abs() @ wd.abs().t()
+    if b is not None:
+        want, M = want + b.double(), M + b.double().abs()
+    if slot is not None:
+        for a in range(slots):
+            at = torch.nonzero(slot == a).flatten()
+            f = 1.0 if s is None else s[a].double()
+            want[at] += f * ((xd[at] @ A[a].double().t()) @ B[a].double().t())
+            M[at] += f * ((xd[at].abs() @ A[a].double().abs().t()) @ B[a].double().abs().t())
+    check(y[:, :N], want, (2.0 ** -15 + (K + rank + 4) * 2.0 ** -24) * M, out, "y")
+    assert bool((y[:, N:] == 7.0).all()), "outside the rows"
+
+
+LOWRANK = [
+    # dtype, out, rows, N, K, rank, slots, order of the slots
+    ("bf16", "bf16", 1, 1024, 1024, 16, 4, "any"),
+    ("f16", "f32", 1, 61, 64, 8, 1, "any"),
+    ("bf16", "f32", 5, 6522, 1024, 16, 5, "any"),
+    ("f16", "f16", 16, 512, 1536, 64, 20, "any"),
+    ("bf16", "bf16", 17, 129, 72, 24, 3, "any"),
+    ("f16", "f32", 64, 1000, 520, 32, 64, "any"),
+    ("bf16", "bf16", 128, 256, 256, 16, 2, "runs"),
+    ("bf16", "f32", 300, 333, 200, 40, 7, "any"),
+    ("f16", "f16", 1000, 1024, 1024, 16, 12, "runs"),
+    ("bf16", "bf16", 2049, 640, 8, 8, 3, "runs"),
+    ("f16", "f16", 129, 64, 128, 48, 130, "any"),
+    ("bf16", "bf16", 257, 6522, 64, 56, 2, "any"),
+    ("bf16", "f32", 31, 1, 40, 16, 2, "any"),
+    ("f16", "f16", 77, 200, 96, 16, 2, "none"),
+    ("bf16", "bf16", 2, 200, 96, 16, 2, "none"),
+]
+
+
+@gpu
+@pytest.mark.parametrize("case", range(len(LOWRANK)))
+def test_lowrank_against_64_bits(cuda, case):
+    lowrank_case(*LOWRANK[case], seed=case, bias=case % 3 != 1, scale=case % 4 != 2, xpad=8 * (case % 2),
+                 ypad=case % 5, wpad=8 * (case % 3))
+
+
+@gpu
+def test_lowrank_adapter_replaced_between_runs(cuda):
+    """the adapters are read by every run: one that is written in stream order counts from the next run on"""
+    gen = generator(1)
+    x, w = rand(gen, 40, 64).bfloat16(), rand(gen, 96, 64).bfloat16()
+    A, B = rand(gen, 2, 8, 64).bfloat16(), rand(gen, 2, 96, 8).bfloat16()
+    slot = torch.zeros(40, device="cuda").int()
+    y = torch.empty(40, 96, device="cuda")
+    op = sequence.LowRank("bf16", "f32", 96, 64, w.data_ptr(), None, 2, 8, A.data_ptr(), B.data_ptr(), rows=40)
+    op.run(40, x.data_ptr(), slot.data_ptr(), y.data_ptr())
+    before = y.clone()
+    B[0] = 0
+    op.run(40, x.data_ptr(), slot.data_ptr(), y.data_ptr())
+    assert not torch.equal(before, y)
+    xd, wd = x.double(), w.double()
+    check(y, xd @ wd.t(), 2.0 ** -17 * (xd.abs() @ wd.abs().t()), "f32", "without the adapter")
+
+
+# ------------------------------------------------------------------ norms around a block
+
+
+def norm_case(D, xtype, dtype, norm, gate, rows, seed, masked=False, f=True, vectors="all", pad=0, inplace=False,
+              offset=0, outputs="both"):
+    gen, t, xt = generator(seed), DT[dtype], DT[xtype]
+
+    def matrix(ty, scale=1.0, shift=0.0):
+        flat = torch.full((rows * (D + pad) + offset,), math.nan, device="cuda", dtype=ty)
+        m = flat[offset:].view(rows, D + pad)[:, :D]
+        m.copy_((rand(gen, rows, D) * scale + shift).to(ty))
+        return m
+
+    x, ff, g = matrix(xt), matrix(t, 3.0, 0.5), matrix(t, 2.0)
+    live = None
+    if masked:
+        live = torch.rand(rows, device="cuda", generator=gen) > 0.3
+        ff[~live] = math.nan
+        g[~live] = math.inf
+    vec = {k: None for k in ("wpost", "bpost", "gamma", "wpre", "bpre")}
+    if vectors == "all":
+        vec = {k: rand(gen, D) for k in vec}
+    eps, alpha = 1e-5, 0.7
+    op = sequence.NormGate(D, xtype, dtype, norm, gate, eps, alpha, **{k: None if v is None else v.data_ptr()
+                                                                         for k, v in vec.items()})
+    x0, f0 = x.clone(), ff.clone()
+    xo, h = (x, ff) if inplace else (matrix(xt), matrix(t))
+    op.run(rows, x.data_ptr(), ff.data_ptr() if f else None, g.data_ptr() if gate != "none" else None,
+           xo.data_ptr() if outputs != "h" else None, h.data_ptr() if outputs != "xo" else None,
+           live=None if live is None else live.data_ptr(), xs=D + pad, fs=D + pad, gs=D + pad, xos=D + pad, hs=D + pad)
+
+    def normed(v, m, w, b):
+        """norm(v) w + b and the sum of its terms' magnitudes, m those of v"""
+        mean = v.mean(-1, keepdim=True) if norm == "layer" else 0.0
+        mm = m.mean(-1, keepdim=True) if norm == "layer" else 0.0
+        r = 1 / torch.sqrt((v - mean).pow(2).mean(-1, keepdim=True) + eps)
+        w = 1.0 if w is None else w.double()
+        b = torch.zeros((), device="cuda").double() if b is None else b.double()
+        return (v - mean) * r * w + b, (m + mm) * r * abs(w) + b.abs()
+
+    y, my = x0.double(), x0.double().abs()
+    if f:
+        fd = f0.double()
+        gd = g.double()
+        if live is not None:
+            fd = torch.where(live[:, None], fd, 0.0)
+            gd = torch.where(live[:, None], gd, 0.0)
+        u, mu = normed(fd, fd.abs(), vec["wpost"], vec["bpost"])
+        act = {"none": torch.ones_like(gd), "sigmoid": torch.sigmoid(gd), "silu": gd * torch.sigmoid(gd)}[gate]
+        coef = alpha * (1.0 if vec["gamma"] is None else vec["gamma"].double()) * act
+        keep = torch.ones(rows, 1, device="cuda").double() if live is None else live[:, None].double()
+        y, my = y + keep * coef * u, my + keep * coef.abs() * mu
+    # the sums are trees: a thread's own terms, then the lanes and warps; 2^-19: the exponential and reciprocal
+    rel = 2.0 ** -19 + (D / 32 + 64) * 2.0 ** -24
+    if outputs != "h":
+        check(xo, y, rel * my, xtype, "x'")
+    if outputs != "xo":
+        hh, mh = normed(y, my, vec["wpre"], vec["bpre"])
+        if live is not None:
+            hh, mh = torch.where(live[:, None], hh, 0.0), torch.where(live[:, None], mh, 0.0)
+        # the statistics of h see x' off by rel my: relative to its norm, at most as much again
+        check(h, hh, 4 * rel * mh * (1 + my.pow(2).mean(-1, keepdim=True).sqrt()
+                                     / (y.pow(2).mean(-1, keepdim=True).sqrt() + 1e-30)), dtype, "h")
+
+
+@gpu
+@pytest.mark.parametrize("D", [1, 7, 8, 64, 250, 256, 1000, 1021, 1024, 1536, 2040, 2048, 2056, 5001, 8192, 8200, 20000])
+@pytest.mark.parametrize("types", [("f32", "bf16"), ("f16", "f16"), ("f32", "f32")])
+@pytest.mark.parametrize("norm, gate", [("rms", "silu"), ("layer", "sigmoid")])
+def test_norm_gate_widths(cuda, D, types, norm, gate):
+    if norm == "layer" and D == 1:
+        pytest.skip("a layer norm of one value is its bias")
+    norm_case(D, *types, norm, gate, rows=5, seed=D, masked=D % 3 == 0)
+
+
+@gpu
+@pytest.mark.parametrize("case", [
+    dict(D=1024, rows=3000), dict(D=1536, rows=2500, masked=True), dict(D=136, rows=9001), dict(D=1021, rows=1300),
+    dict(D=200, rows=1301, pad=3), dict(D=512, rows=33, offset=1), dict(D=512, rows=33, pad=8, offset=8),
+    dict(D=1024, rows=9, inplace=True), dict(D=999, rows=9, inplace=True), dict(D=9000, rows=9, inplace=True),
+    dict(D=1024, rows=9, vectors="none"), dict(D=700, rows=20, f=False), dict(D=9001, rows=3, f=False, masked=True),
+    dict(D=64, rows=1300, outputs="h"), dict(D=64, rows=1, outputs="xo"), dict(D=2000, rows=1, masked=True)])
+@pytest.mark.parametrize("norm, gate, types", [("rms", "none", ("bf16", "bf16")), ("layer", "silu", ("f32", "f16"))])
+def test_norm_gate_forms(cuda, case, norm, gate, types):
+    kw = dict(case)
+    norm_case(kw.pop("D"), *types, norm, gate, kw.pop("rows"), seed=3, **kw)
+
+
+@gpu
+def test_norm_gate_zero_rows_and_zero_values(cuda):
+    op = sequence.NormGate(64, "f32", "bf16", "rms", "none")
+    x = torch.zeros(4, 64, device="cuda")
+    f = torch.zeros(4, 64, device="cuda").bfloat16()
+    xo, h = torch.full_like(x, 3), torch.full_like(f, 3)
+    op.run(0, None, None, None, None, None)
+    op.run(4, x.data_ptr(), f.data_ptr(), None, xo.data_ptr(), h.data_ptr())
+    assert bool((xo == 0).all()) and bool((h == 0).all())
+
+
+# ------------------------------------------------------------------ refusals (no GPU needed)
+
+
+def usage(make, text):
+    with pytest.raises(BnnError) as e:
+        make()
+    assert e.value.kind == "USAGE" and text in str(e.value), str(e.value)
+
+
+P = 1 << 20  # a pointer that is never followed: the checks come first
+
+
+@pytest.mark.parametrize("kw, text", [
+    (dict(dtype="f32"), "type fp16 or bf16"), (dict(dtype="f64"), "one of"), (dict(heads=3, kv_heads=2), "multiple of kv_heads"),
+    (dict(dk=12), "multiples of 8"), (dict(dv=136), "up to 128"), (dict(dk=0), "multiples of 8"),
+    (dict(decay=[1.5, 0.5]), "decay[0] = 1.5"), (dict(decay=[0.5, math.nan]), "decay[1]"), (dict(decay=[0.5, -0.1]), "decay[1]"),
+    (dict(decay=[0.5]), "1 values for 2"), (dict(scale=math.inf), "a finite scale"), (dict(seqs=0), "at least one sequence"),
+    (dict(tokens=1 << 31), "2^31 - 1"), (dict(tokens=0), "1 .. 2^31 - 1")])
+def test_dattn_new_refuses(kw, text):
+    a = dict(dtype="bf16", heads=2, kv_heads=2, dk=64, dv=64, decay=[0.9, 0.5])
+    a.update(kw)
+    usage(lambda: sequence.DecayAttention(**a), text)
+
+
+@pytest.mark.parametrize("kw, text", [
+    (dict(dtype="f32"), "type fp16 or bf16"), (dict(out="f16"), "out fp32 or the same"), (dict(K=12), "multiples of 8"),
+    (dict(N=0), "N 0"), (dict(rank=12), "rank a multiple of 8"), (dict(rank=72), "8 .. 64"), (dict(slots=0), "slots 0"),
+    (dict(rows=0), "rows 0"), (dict(w=P + 2), "16-byte aligned"), (dict(a=None), "16-byte aligned"),
+    (dict(b=P + 8), "16-byte aligned"), (dict(ldw=56), "ldw >= K"), (dict(ldw=68), "multiples of 8")])
+def test_lowrank_new_refuses(kw, text):
+    a = dict(dtype="bf16", out="bf16", N=10, K=64, w=P, bias=None, slots=2, rank=8, a=P, b=P, rows=4)
+    a.update(kw)
+    usage(lambda: sequence.LowRank(**a), text)
+
+
+@pytest.mark.parametrize("kw, text", [
+    (dict(D=0), "D in 1"), (dict(xtype="f16"), "x_type fp32 or type"), (dict(norm="max"), "one of"),
+    (dict(gate="tanh"), "one of"), (dict(eps=-1.0), "eps >= 0"), (dict(eps=math.nan), "eps >= 0"),
+    (dict(alpha=math.inf), "finite")])
+def test_norm_gate_new_refuses(kw, text):
+    a = dict(D=64, xtype="f32", dtype="bf16")
+    a.update(kw)
+    usage(lambda: sequence.NormGate(**a), text)
+
+
+def test_norm_gate_run_refuses():
+    op = sequence.NormGate(64, "f32", "bf16", "rms", "silu")
+    ok = dict(rows=2, x=P, f=P, g=P, xo=P, h=P)
+    for kw, text in [(dict(rows=-1), "-1 rows"), (dict(x=None), "strides"), (dict(g=None), "g where f is given"),
+                     (dict(xo=None, h=None), "an output"), (dict(xs=63), "strides >= the width"),
+                     (dict(hs=10), "strides >= the width"), (dict(x=P + 2), "not aligned"), (dict(h=P + 1), "not aligned")]:
+        usage(lambda kw=kw: op.run(**dict(ok, **kw)), text)
+    op.run(0, None, None, None, None, None)
+    op.close()
+    with pytest.raises(BnnError):
+        op.run(**ok)
+
+
+@gpu
+def test_run_refuses(cuda):
+    op = sequence.DecayAttention("bf16", 4, 64, 32, [0.9, 0.5], kv_heads=2, seqs=2, tokens=10)
+    ok = dict(n=2, tokens=10, cu=P, q=P, k=P, v=P, o=P)
+    for kw, text in [(dict(n=3), "capacity 2"), (dict(n=-1), "capacity"), (dict(tokens=11), "capacity"), (dict(cu=None), "offsets"),
+                     (dict(q=None), "16-byte aligned"), (dict(k=P + 8), "16-byte aligned"), (dict(s0=P + 4), "16-byte aligned"),
+                     (dict(qts=255), "token strides"), (dict(kts=132), "token strides"), (dict(ots=127), "token strides")]:
+        usage(lambda kw=kw: op.run(**dict(ok, **kw)), text)
+    usage(lambda: op.step(3, P, P, P, P), "capacity 2")
+    op.run(0, 0, None, None, None, None, None)
+    op.step(0, None, None, None, None)
+    w = torch.zeros(10, 64, device="cuda").bfloat16()
+    low = sequence.LowRank("bf16", "f32", 10, 64, w.data_ptr(), None, 1, 8, w.data_ptr(), w.data_ptr(), rows=4)
+    ok = dict(rows=4, x=P, slot=P, y=P)
+    for kw, text in [(dict(rows=5), "capacity 4"), (dict(rows=-1), "capacity"), (dict(x=None), "16-byte aligned"),
+                     (dict(x=P + 8), "16-byte aligned"), (dict(ldx=60), ">= K"), (dict(ldy=9), ">= N"), (dict(y=P + 2), "y")]:
+        usage(lambda kw=kw: low.run(**dict(ok, **kw)), text)
+    low.run(0, None, None, None)
+
+
+@gpu
+def test_new_reports_out_of_memory(cuda):
+    h = load_library()
+    w = torch.zeros(10, 64, device="cuda").bfloat16()
+    try:
+        for k in (1, 2):
+            h.bnn_debug_fail_alloc(0, k)
+            with pytest.raises(BnnError) as e:
+                sequence.DecayAttention("bf16", 2, 64, 64, [0.9, 0.5])
+            assert e.value.kind == "OOM"
+            h.bnn_debug_fail_alloc(0, k)
+            with pytest.raises(BnnError) as e:
+                sequence.LowRank("bf16", "f32", 10, 64, w.data_ptr(), None, 1, 8, w.data_ptr(), w.data_ptr())
+            assert e.value.kind == "OOM"
+        h.bnn_debug_fail_alloc(1, 0)
+        with pytest.raises(BnnError) as e:
+            sequence.NormGate(64, "f32", "bf16")
+        assert e.value.kind == "OOM"
+    finally:
+        h.bnn_debug_fail_alloc(0, 0)
