@@ -344,7 +344,11 @@ typedef struct {
   long long ots;
   const float *pow;
   float scale;
+  float *scratch; /* bnnk_dattn_scratch_states(n, Hk, tokens) x dk dv floats */
+  int *err;       /* the device error word of the bounded waits */
 } bnnk_dattn_args;
+/* states of scratch a call of up to n sequences and `tokens` tokens may need */
+long long bnnk_dattn_scratch_states(int n, int Hk, long long tokens);
 int bnnk_dattn(const bnnk_dattn_args *a, bnn_stream_t st);
 
 /* y = x w^T + bias + scale[s] (x a[s]^T) b[s]^T, s = slot[row]; otype 0 or type; hid: scratch [rows][rank]. K and rank

@@ -3,11 +3,17 @@
 //   S_t = lambda S_{t-1} + live_t k_t^T v_t,   o_t = live_t scale q_t S_t
 //
 // S [dk][dv] fp32, q heads in groups of G that share one k/v head and its S.
+#include <cuda.h>
+#include <cudaTypedefs.h>
 #include <cuda_runtime.h>
+
+#include <mutex>
 
 #include "bnn_kernels.h"
 #include "seq.cuh"
-#include "tc.cuh"
+#include "smem_attr.cuh"
+#include "sync.cuh"
+#include "tc16.cuh"
 
 namespace bnn {
 namespace {
@@ -131,18 +137,646 @@ __global__ void __launch_bounds__(256) k_dattn_rec(const DattnArgs a) {
   }
 }
 
+
+// ------------------------------------------------------------------ the chunk form
+//
+// 128 tokens at a time, i, j in the chunk, S the state before it, n its tokens (lambda^x from a table):
+//   o_i = scale (lambda^(i+1) q_i S + sum_{j <= i} lambda^(i-j) (q_i . k_j) v_j)
+//   S'  = lambda^n S + sum_j lambda^(n-1-j) k_j^T v_j
+// as four products on the tensor cores (tcgen05 kind::f16, fp32 accumulators in TMEM): QK = Q K^T, O1 = Q S, DS = K'^T V
+// with K'_j = lambda^(n-1-j) k_j, and O2 = P V with P = QK times the decays below the diagonal. Q, K and V arrive by TMA
+// (128-byte swizzle, heads narrower than the padded width DP read as zero past their end). What is computed and goes back
+// into a product (P, S, K') goes as two 16-bit parts whose sum keeps 16 bits or more of significand, so that a 16-bit
+// output's error stays that of its one rounding and the fp32 state is off by about 6e-7 of its size, as an fp32 sum of
+// these terms is; one part alone would add an error as large as the output's rounding for each of P and S.
+//
+// One CTA per (segment of a sequence, k/v head) walks the segment's chunks, and for each the G q heads of the group
+// ("unit" u = (chunk, q head)). Roles: warp 0 TMA, warp 1 MMA issue, 4 warps turn QK into P (in place in TMEM, as the A
+// operand of the last product), 4 warps join O1 and O2 and store o, 8 warps hold S in registers, form K' and the S
+// operand. S in registers stays fp32: lambda^n S + DS, once a chunk.
+// A masked token, and a row past the segment's end, has its k and v rows taken as zero (K' zero, V zeroed in shared
+// memory, its P column zero by selection, so that NaN and infinities there stay out); its o row is zero or not stored.
+constexpr int kChunk = 128;
+constexpr int kDaThreads = 640;
+
+struct DaArgs {
+  DattnArgs d;
+  int seg_tokens;     // tokens of a segment (a multiple of kChunk), 0: a sequence is one segment
+  int segs;           // the most segments of the call, and CTAs of a head
+  float *seg_state;   // [segment][Hk][dk][dv]: a segment's own sum (kState), then the state before it
+  int *err;
+};
+
+// the sequence, part, tokens and last-part flag of segment s: sequence i has max(1, ceil(length / seg_tokens)) segments,
+// in order. One warp; false past the last segment.
+__device__ bool find_segment(const DaArgs &a, int s, int &seq, int &part, long long &t0, long long &t1, bool &last) {
+  const int lane = threadIdx.x % 32;
+  long long b0, b1;
+  if (!a.seg_tokens) {
+    if (s >= a.d.n) return false;
+    seq = s; part = 0; last = true;
+    seq_range(a.d, s, t0, t1);
+    return true;
+  }
+  int base = 0;
+  for (int i0 = 0; i0 < a.d.n; i0 += 32) {
+    const int i = i0 + lane;
+    int parts = 0;
+    if (i < a.d.n) {
+      seq_range(a.d, i, b0, b1);
+      parts = max(1, (int)((b1 - b0 + a.seg_tokens - 1) / a.seg_tokens));
+    }
+    int sum = parts;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += v;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, s < base + sum);
+    if (hit) {
+      const int l = __ffs(hit) - 1;
+      seq = i0 + l;
+      const int end = __shfl_sync(0xffffffffu, sum, l), np = __shfl_sync(0xffffffffu, parts, l);
+      part = s - (base + end - np);
+      last = part == np - 1;
+      seq_range(a.d, seq, b0, b1);
+      t0 = b0 + (long long)part * a.seg_tokens;
+      t1 = last ? b1 : t0 + a.seg_tokens;
+      return true;
+    }
+    base += __shfl_sync(0xffffffffu, sum, 31);
+  }
+  return false;
+}
+
+template <int DP>
+struct DaLayout {
+  static constexpr int stages = DP == 64 ? 2 : 1;   // Q, K, V tiles in flight
+  static constexpr int qk_bufs = DP == 64 ? 2 : 1;  // QK / P regions in TMEM
+  static constexpr uint32_t panel = kChunk * 128;   // 64 columns of a 128-row tile
+  static constexpr uint32_t tile = kChunk * DP * 2;
+  static constexpr uint32_t s_panel = DP * 128, s_tile = DP * DP * 2;
+  static constexpr uint32_t q = 0, k = q + stages * tile, v = k + stages * tile, kp = v + stages * tile,
+                            st = kp + 2 * tile, end = st + 2 * s_tile;
+  static constexpr uint32_t t_qk = 0, t_o1 = qk_bufs * 128, t_o2 = t_o1 + DP, t_ds = t_o2 + DP;  // TMEM columns
+  static constexpr size_t smem = end + 1024;
+};
+
+// the live tokens among a chunk's 128, bit j % 32 of word j / 32 (one warp; every lane gets all words)
+__device__ __forceinline__ void live_words(const DattnArgs &a, long long t, int n, uint32_t (&w)[4]) {
+  const int lane = threadIdx.x % 32;
+#pragma unroll
+  for (int b = 0; b < 4; b++) {
+    const int j = 32 * b + lane;
+    w[b] = __ballot_sync(0xffffffffu, j < n && (!a.live || a.live[t + j]));
+  }
+}
+
+template <int T, int DP, bool kState>
+__global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_constant__ CUtensorMap mq,
+                                                              const __grid_constant__ CUtensorMap mk,
+                                                              const __grid_constant__ CUtensorMap mv, const DaArgs a) {
+  using L = DaLayout<DP>;
+  constexpr int NS = L::stages, NB = L::qk_bufs, PN = DP / 64;
+  extern __shared__ uint8_t dsmem[];
+  __shared__ __align__(8) unsigned long long b_qfull[NS], b_kfull[NS], b_vfull[NS], b_qempty[NS], b_kempty[NS],
+      b_vempty[NS], b_qk[NB], b_p[NB], b_s, b_kp, b_ds, b_o, b_oempty;
+  __shared__ uint32_t tmem_s;
+  __shared__ volatile int abort_s;
+  __shared__ float s_pow[32 + kDattnPow];  // s_pow[32 + x] = lambda^x, 0 for x < 0
+  __shared__ long long s_range[2];
+  __shared__ int s_seg[3];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const DattnArgs &d = a.d;
+  const int hk = blockIdx.y, G = kState ? 1 : d.G;
+
+  if (warp == 0) {
+    int seq = 0, part = 0;
+    long long t0 = 0, t1 = 0;
+    bool last = false;
+    const bool any = find_segment(a, blockIdx.x, seq, part, t0, t1, last);
+    if (lane == 0) {
+      s_range[0] = t0;
+      s_range[1] = t1;
+      s_seg[0] = any ? seq : -1;
+      s_seg[1] = part;
+      s_seg[2] = last;
+      for (int s = 0; s < NS; s++) {
+        mbar_init(smem_u32(&b_qfull[s]), 1); mbar_init(smem_u32(&b_kfull[s]), 1); mbar_init(smem_u32(&b_vfull[s]), 1);
+        mbar_init(smem_u32(&b_qempty[s]), 1); mbar_init(smem_u32(&b_kempty[s]), 1); mbar_init(smem_u32(&b_vempty[s]), 1);
+      }
+      for (int b = 0; b < NB; b++) { mbar_init(smem_u32(&b_qk[b]), 1); mbar_init(smem_u32(&b_p[b]), 4); }
+      mbar_init(smem_u32(&b_s), 8); mbar_init(smem_u32(&b_kp), 8); mbar_init(smem_u32(&b_ds), 1);
+      mbar_init(smem_u32(&b_o), 1); mbar_init(smem_u32(&b_oempty), 4);
+      abort_s = 0;
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+  } else if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_s)), "r"(512));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  } else if (warp == 2) {
+    for (int x = lane; x < 32 + kDattnPow; x += 32) s_pow[x] = x < 32 ? 0.f : d.pow[hk * kDattnPow + x - 32];
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_s, base = (smem_u32(dsmem) + 1023u) & ~1023u;
+  const long long t0 = s_range[0], t1 = s_range[1];
+  const int seq = s_seg[0];
+  // a segment's own sum is needed where another follows it
+  const bool work = seq >= 0 && !(kState && s_seg[2]);
+  const int nc = work ? (int)((t1 - t0 + kChunk - 1) / kChunk) : 0, nu = nc * G;
+  const float *pw = s_pow + 32;
+
+#define DA_WAIT(bar, parity, code)                \
+  if (!mbar_wait(smem_u32(&(bar)), (parity))) {   \
+    atomicExch(a.err, code);                      \
+    abort_s = 1;                                  \
+    break;                                        \
+  }
+
+  if (warp == 0) {
+    if (lane == 0) {  // TMA
+      int nq = 0, c = 0;
+      for (; c < nc && !abort_s; c++) {
+        const long long t = t0 + (long long)c * kChunk;
+        const int s = c % NS, use = c / NS;
+        bool ok = true;
+        for (int g = 0; g < G && ok; g++) {
+          if (!kState) {
+            const int sq = nq % NS;
+            if (nq >= NS && !mbar_wait(smem_u32(&b_qempty[sq]), (nq / NS - 1) & 1)) { ok = false; break; }
+            mbar_expect_tx(smem_u32(&b_qfull[sq]), L::tile);
+            for (int p = 0; p < PN; p++)
+              tma_load_3d(base + L::q + sq * L::tile + p * L::panel, &mq, smem_u32(&b_qfull[sq]), 64 * p, hk * G + g, (int)t);
+            nq++;
+          }
+          if (g) continue;
+          if (use && !mbar_wait(smem_u32(&b_kempty[s]), (use - 1) & 1)) { ok = false; break; }
+          mbar_expect_tx(smem_u32(&b_kfull[s]), L::tile);
+          for (int p = 0; p < PN; p++)
+            tma_load_3d(base + L::k + s * L::tile + p * L::panel, &mk, smem_u32(&b_kfull[s]), 64 * p, hk, (int)t);
+          if (use && !mbar_wait(smem_u32(&b_vempty[s]), (use - 1) & 1)) { ok = false; break; }
+          mbar_expect_tx(smem_u32(&b_vfull[s]), L::tile);
+          for (int p = 0; p < PN; p++)
+            tma_load_3d(base + L::v + s * L::tile + p * L::panel, &mv, smem_u32(&b_vfull[s]), 64 * p, hk, (int)t);
+        }
+        if (!ok) {
+          atomicExch(a.err, BNNK_ERR_TMA_WAIT);
+          abort_s = 1;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {  // MMA
+      constexpr uint32_t bt = T - 1;
+      constexpr uint32_t i_qk = idesc_16(bt, 128, 0, 0), i_qs = idesc_16(bt, DP, 0, 1), i_ds = idesc_16(bt, DP, 1, 1),
+                         i_pv = idesc_16(bt, DP, 0, 1);
+      auto issue_qk = [&](int u) {
+        const int c = u / G, sq = u % NS, s = c % NS, b = u % NB;
+        if (!mbar_wait(smem_u32(&b_qfull[sq]), (u / NS) & 1) || !mbar_wait(smem_u32(&b_kfull[s]), (c / NS) & 1)) return false;
+        tc_fence_after();
+        const uint32_t qa = base + L::q + sq * L::tile, ka = base + L::k + s * L::tile;
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; kk++) {
+          const uint32_t off = (kk / 4) * L::panel + (kk % 4) * 32;
+          mma16_ss(tmem + L::t_qk + b * 128, smem_desc<128>(qa + off), smem_desc<128>(ka + off), i_qk, kk != 0);
+        }
+        mma_commit(smem_u32(&b_qk[b]));
+        return true;
+      };
+      if (!kState && nu > 0 && !issue_qk(0)) { atomicExch(a.err, BNNK_ERR_MMA_WAIT); abort_s = 1; }
+      for (int u = 0; u < nu && !abort_s; u++) {
+        const int c = u / G, g = u % G, sq = u % NS, s = c % NS, b = u % NB;
+        const uint32_t va = base + L::v + s * L::tile;
+        if (!kState) {
+          if (NB > 1 && u + 1 < nu && !issue_qk(u + 1)) { atomicExch(a.err, BNNK_ERR_MMA_WAIT); abort_s = 1; break; }
+          if (g == 0) DA_WAIT(b_s, c & 1, BNNK_ERR_MMA_WAIT)
+          if (u) DA_WAIT(b_oempty, (u - 1) & 1, BNNK_ERR_MMA_WAIT)
+          tc_fence_after();
+          const uint32_t qa = base + L::q + sq * L::tile;
+#pragma unroll
+          for (int part = 0; part < 2; part++)
+#pragma unroll
+            for (int kk = 0; kk < DP / 16; kk++)
+              mma16_ss(tmem + L::t_o1, smem_desc<128>(qa + (kk / 4) * L::panel + (kk % 4) * 32),
+                       smem_desc_mn(base + L::st + part * L::s_tile + kk * 2048, L::s_panel), i_qs, (part | kk) != 0);
+          mma_commit(smem_u32(&b_qempty[sq]));
+        }
+        if (g == 0) {
+          DA_WAIT(b_vfull[s], (c / NS) & 1, BNNK_ERR_MMA_WAIT)
+          DA_WAIT(b_kp, c & 1, BNNK_ERR_MMA_WAIT)
+          tc_fence_after();
+        }
+        if (g == G - 1) {
+#pragma unroll
+          for (int part = 0; part < 2; part++)
+#pragma unroll
+            for (int kk = 0; kk < 8; kk++)
+              mma16_ss(tmem + L::t_ds, smem_desc_mn(base + L::kp + part * L::tile + kk * 2048, L::panel),
+                       smem_desc_mn(va + kk * 2048, L::panel), i_ds, (part | kk) != 0);
+          mma_commit(smem_u32(&b_ds));
+          mma_commit(smem_u32(&b_kempty[s]));
+        }
+        if (!kState) {
+          DA_WAIT(b_p[b], (u / NB) & 1, BNNK_ERR_MMA_WAIT)
+          tc_fence_after();
+          // P: 32 columns j a block, its high parts in the block's first 16 TMEM columns, the low parts in the others
+#pragma unroll
+          for (int kk = 0; kk < 8; kk++)
+#pragma unroll
+            for (int part = 0; part < 2; part++)
+              mma16_ts(tmem + L::t_o2, tmem + L::t_qk + b * 128 + (kk / 2) * 32 + part * 16 + (kk % 2) * 8,
+                       smem_desc_mn(va + kk * 2048, L::panel), i_pv, (part | kk) != 0);
+          mma_commit(smem_u32(&b_o));
+        }
+        if (g == G - 1) mma_commit(smem_u32(&b_vempty[s]));
+        if (!kState && NB == 1 && u + 1 < nu && !issue_qk(u + 1)) { atomicExch(a.err, BNNK_ERR_MMA_WAIT); abort_s = 1; }
+      }
+    }
+  } else if (warp >= 4 && warp < 8) {
+    // P: this thread's row i against the columns j <= i
+    const int qd = warp % 4, i = 32 * qd + lane;
+    for (int u = 0; u < (kState ? 0 : nu); u++) {
+      const int c = u / G, b = u % NB;
+      const long long t = t0 + (long long)c * kChunk;
+      const int n = (int)min((long long)kChunk, t1 - t);
+      uint32_t lw[4];
+      live_words(d, t, n, lw);
+      bool ok = mbar_wait(smem_u32(&b_qk[b]), (u / NB) & 1);
+      ok = __all_sync(0xffffffffu, ok && !abort_s);
+      if (!ok) {
+        if (lane == 0) { atomicExch(a.err, BNNK_ERR_EPI_WAIT); abort_s = 1; }
+        break;
+      }
+      tc_fence_after();
+      const uint32_t tq = tmem + L::t_qk + b * 128 + ((uint32_t)(qd * 32) << 16);
+#pragma unroll
+      for (int blk = 0; blk < 4; blk++) {
+        uint32_t hi[16], lo[16];
+        if (blk > qd) {
+#pragma unroll
+          for (int j = 0; j < 16; j++) hi[j] = lo[j] = 0;
+        } else {
+          uint32_t x[32];
+          tmem_ld32(tq + blk * 32, x);
+          tmem_wait_ld(x);
+          const uint32_t w = lw[blk];
+          if (w != 0xffffffffu) {
+#pragma unroll
+            for (int j = 0; j < 32; j++) x[j] = (w >> j) & 1 ? x[j] : 0u;
+          }
+          if (blk == qd) {  // the diagonal block: lambda^(i - j), zero above
+#pragma unroll
+            for (int j = 0; j < 32; j += 2)
+              split2<T>(__uint_as_float(x[j]) * pw[lane - j], __uint_as_float(x[j + 1]) * pw[lane - j - 1], hi[j / 2],
+                        lo[j / 2]);
+          } else {  // lambda^(i - 32 blk - 31) lambda^(31 - j): no power that overflows, one factor the same for all rows
+            const float f = pw[i - 32 * blk - 31];
+#pragma unroll
+            for (int j = 0; j < 32; j += 2)
+              split2<T>(__uint_as_float(x[j]) * f * pw[31 - j], __uint_as_float(x[j + 1]) * f * pw[30 - j], hi[j / 2],
+                        lo[j / 2]);
+          }
+        }
+        tmem_st16(tq + blk * 32, hi);
+        tmem_st16(tq + blk * 32 + 16, lo);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&b_p[b]));
+    }
+  } else if (warp >= 8 && warp < 12) {
+    // o: this thread's row i
+    const int qd = warp % 4, i = 32 * qd + lane;
+    const bool wide = (d.dv % 16 | d.ots % 16) == 0 && ((uintptr_t)d.o & 31) == 0;
+    for (int u = 0; u < (kState ? 0 : nu); u++) {
+      const int c = u / G, g = u % G;
+      const long long t = t0 + (long long)c * kChunk;
+      const int n = (int)min((long long)kChunk, t1 - t);
+      const bool live = i < n && (!d.live || d.live[t + i]);
+      bool ok = mbar_wait(smem_u32(&b_o), u & 1);
+      ok = __all_sync(0xffffffffu, ok && !abort_s);
+      if (!ok) {
+        if (lane == 0) { atomicExch(a.err, BNNK_ERR_EPI_WAIT); abort_s = 1; }
+        break;
+      }
+      tc_fence_after();
+      const float c1 = d.scale * pw[i + 1], c2 = d.scale;
+      elem_t<T> *o = (elem_t<T> *)d.o + (t + i) * d.ots + (long long)(hk * G + g) * d.dv;
+      const uint32_t tq = tmem + ((uint32_t)(qd * 32) << 16);
+#pragma unroll
+      for (int col = 0; col < DP; col += 16) {
+        uint32_t x[16], y[16], z[8];
+        tmem_ld16(tq + L::t_o1 + col, x);
+        tmem_ld16(tq + L::t_o2 + col, y);
+        tmem_wait_ld(x, y);
+#pragma unroll
+        for (int j = 0; j < 16; j += 2) {
+          const float p = c1 * __uint_as_float(x[j]) + c2 * __uint_as_float(y[j]);
+          const float q = c1 * __uint_as_float(x[j + 1]) + c2 * __uint_as_float(y[j + 1]);
+          z[j / 2] = live ? pack2f<T>(p, q) : 0u;
+        }
+        if (i < n && col < d.dv) {
+          if (wide) {
+            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(o + col), "r"(z[0]), "r"(z[1]),
+                         "r"(z[2]), "r"(z[3]), "r"(z[4]), "r"(z[5]), "r"(z[6]), "r"(z[7])
+                         : "memory");
+          } else {
+            *reinterpret_cast<uint4 *>(o + col) = make_uint4(z[0], z[1], z[2], z[3]);
+            if (col + 8 < d.dv) *reinterpret_cast<uint4 *>(o + col + 8) = make_uint4(z[4], z[5], z[6], z[7]);
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&b_oempty));
+    }
+  } else if (warp >= 12 && seq >= 0) {
+    // the state: row r = dk index, DP / 2 columns from c0 in registers
+    constexpr int HC = DP / 2;
+    const int w8 = warp - 12, r = 32 * (warp % 4) + lane, c0 = (w8 / 4) * HC, tid = threadIdx.x - 384;
+    const bool mine = r < DP;
+    float S[HC];
+    const long long slot = d.slot ? d.slot[seq] : seq;
+    const float *from = nullptr;
+    if (!kState) {
+      if (a.seg_tokens) from = a.seg_state + ((long long)blockIdx.x * d.Hk + hk) * d.dk * d.dv;
+      else if (d.s0 && slot >= 0) from = d.s0 + (slot * d.Hk + hk) * (long long)d.dk * d.dv;
+    }
+#pragma unroll
+    for (int j = 0; j < HC; j += 4) {
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (from && r < d.dk && c0 + j < d.dv) v = *reinterpret_cast<const float4 *>(from + (long long)r * d.dv + c0 + j);
+      S[j] = v.x; S[j + 1] = v.y; S[j + 2] = v.z; S[j + 3] = v.w;
+    }
+    auto put_state = [&]() {  // S as the B operand of O1: row r, MN-major panels of 64 columns
+      if (mine) {
+#pragma unroll
+        for (int j = 0; j < HC; j += 8) {
+          uint32_t h[4], l[4];
+#pragma unroll
+          for (int e = 0; e < 4; e++) split2<T>(S[j + 2 * e], S[j + 2 * e + 1], h[e], l[e]);
+          const int col = c0 + j;
+          const uint32_t at = base + L::st + (col / 64) * L::s_panel + r * 128 + ((((col % 64) / 8) ^ (r & 7)) << 4);
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3])
+                       : "memory");
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + L::s_tile), "r"(l[0]), "r"(l[1]), "r"(l[2]),
+                       "r"(l[3])
+                       : "memory");
+        }
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&b_s));
+    };
+    if (!kState && nc > 0) put_state();
+    bool ok = true;
+    for (int c = 0; c < nc; c++) {
+      const int s = c % NS;
+      const long long t = t0 + (long long)c * kChunk;
+      const int n = (int)min((long long)kChunk, t1 - t);
+      // K' and the dead rows of V: 16-byte slots, a row's 8 by 8 lanes; both tiles keep the swizzle's order
+      bool dead[4];
+      float wt[4];
+#pragma unroll
+      for (int m = 0; m < 4; m++) {
+        const int row = tid / 8 + 32 * m;
+        dead[m] = row >= n || (d.live && !d.live[t + row]);
+        wt[m] = row < n ? pw[n - 1 - row] : 0.f;
+      }
+      ok = mbar_wait(smem_u32(&b_kfull[s]), (c / NS) & 1);
+      ok = __all_sync(0xffffffffu, ok && !abort_s);
+      if (!ok) break;
+#pragma unroll
+      for (int p = 0; p < PN; p++)
+#pragma unroll
+        for (int m = 0; m < 4; m++) {
+          const uint32_t off = p * L::panel + (tid + 256 * m) * 16;
+          uint32_t x[4], h[4], l[4];
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
+                       : "r"(base + L::k + s * L::tile + off)
+                       : "memory");
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const float2 f = unpack2<T>(dead[m] ? 0u : x[e]);
+            split2<T>(f.x * wt[m], f.y * wt[m], h[e], l[e]);
+          }
+          const uint32_t at = base + L::kp + off;
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3])
+                       : "memory");
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + L::tile), "r"(l[0]), "r"(l[1]), "r"(l[2]),
+                       "r"(l[3])
+                       : "memory");
+        }
+      if (n < kChunk || d.live) {
+        ok = mbar_wait(smem_u32(&b_vfull[s]), (c / NS) & 1);
+        ok = __all_sync(0xffffffffu, ok && !abort_s);
+        if (!ok) break;
+#pragma unroll
+        for (int p = 0; p < PN; p++)
+#pragma unroll
+          for (int m = 0; m < 4; m++)
+            if (dead[m])
+              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(base + L::v + s * L::tile + p * L::panel +
+                                                                            (tid + 256 * m) * 16),
+                           "r"(0)
+                           : "memory");
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&b_kp));
+      ok = mbar_wait(smem_u32(&b_ds), c & 1);
+      ok = __all_sync(0xffffffffu, ok && !abort_s);
+      if (!ok) break;
+      tc_fence_after();
+      const float dec = pw[n];
+      const uint32_t td = tmem + L::t_ds + c0 + ((uint32_t)((warp % 4) * 32) << 16);
+#pragma unroll
+      for (int j = 0; j < HC; j += 32) {
+        uint32_t x[32];
+        tmem_ld32(td + j, x);
+        tmem_wait_ld(x);
+#pragma unroll
+        for (int e = 0; e < 32; e++) S[j + e] = fmaf(dec, S[j + e], __uint_as_float(x[e]));
+      }
+      tc_fence_before();
+      if (!kState && c + 1 < nc) put_state();
+    }
+    if (!ok) {
+      if (lane == 0) { atomicExch(a.err, BNNK_ERR_EPI_WAIT); abort_s = 1; }
+    } else {
+      float *to = nullptr;
+      if (kState) {
+        if (work) to = a.seg_state + ((long long)blockIdx.x * d.Hk + hk) * d.dk * d.dv;
+      } else if (s_seg[2] && d.s1 && slot >= 0) {
+        to = d.s1 + (slot * d.Hk + hk) * (long long)d.dk * d.dv;
+      }
+      if (to && r < d.dk) {
+#pragma unroll
+        for (int j = 0; j < HC; j += 4)
+          if (c0 + j < d.dv)
+            *reinterpret_cast<float4 *>(to + (long long)r * d.dv + c0 + j) = make_float4(S[j], S[j + 1], S[j + 2], S[j + 3]);
+      }
+    }
+  }
+#undef DA_WAIT
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+}
+
+// the states before each segment: S = s0, then S = lambda^seg_tokens S + (the segment's own sum), in place in seg_state.
+// One thread per state element.
+__global__ void __launch_bounds__(256) k_dattn_scan(const DaArgs a) {
+  const DattnArgs &d = a.d;
+  __shared__ int s_first, s_parts;
+  __shared__ float s_dec;
+  const int i = blockIdx.z, hk = blockIdx.y;
+  if (threadIdx.x < 32) {
+    int before = 0, mine = 0;
+    for (int j = threadIdx.x; j <= i; j += 32) {
+      long long b0, b1;
+      seq_range(d, j, b0, b1);
+      const int parts = max(1, (int)((b1 - b0 + a.seg_tokens - 1) / a.seg_tokens));
+      if (j < i) before += parts;
+      else mine = parts;
+    }
+    for (int o = 16; o; o >>= 1) {
+      before += __shfl_xor_sync(0xffffffffu, before, o);
+      mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    }
+    if (threadIdx.x == 0) {
+      s_first = before;
+      s_parts = min(mine, a.segs - before);  // offsets that do not ascend could ask for more
+      s_dec = (float)pow((double)d.pow[hk * kDattnPow + 1], (double)a.seg_tokens);
+    }
+  }
+  __syncthreads();
+  const int e = blockIdx.x * 256 + threadIdx.x, size = d.dk * d.dv;
+  if (e >= size) return;
+  const long long slot = d.slot ? d.slot[i] : i;
+  float S = d.s0 && slot >= 0 ? d.s0[(slot * d.Hk + hk) * (long long)size + e] : 0.f;
+  float *p = a.seg_state + ((long long)s_first * d.Hk + hk) * size + e;
+  const long long step = (long long)d.Hk * size;
+  const int parts = s_parts;
+  const float dec = s_dec;
+  for (int k0 = 0; k0 < parts; k0 += 8) {  // 8 loads in flight
+    float own[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++) own[k] = k0 + k < parts - 1 ? p[(k0 + k) * step] : 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; k++)
+      if (k0 + k < parts) {
+        p[(k0 + k) * step] = S;
+        S = fmaf(dec, S, own[k]);
+      }
+  }
+}
+
+template <int T, int DP>
+int run_chunk(const DaArgs &a, cudaStream_t st) {
+  const DattnArgs &d = a.d;
+  CUtensorMap mq, mk, mv;
+  int e = encode_heads(&mq, d.q, T == 2, d.dk, d.H, d.tokens, d.qts, kChunk);
+  if (!e) e = encode_heads(&mk, d.k, T == 2, d.dk, d.Hk, d.tokens, d.kts, kChunk);
+  if (!e) e = encode_heads(&mv, d.v, T == 2, d.dv, d.Hk, d.tokens, d.vts, kChunk);
+  if (e) return e;
+  static SmemAttr attr_s, attr;
+  const dim3 grid(a.segs, d.Hk);
+  constexpr size_t smem = DaLayout<DP>::smem;
+  if (a.seg_tokens) {
+    e = attr_s.ensure(k_dattn_chunk<T, DP, true>, smem);
+    if (e) return e;
+    k_dattn_chunk<T, DP, true><<<grid, kDaThreads, smem, st>>>(mq, mk, mv, a);
+    k_dattn_scan<<<dim3((d.dk * d.dv + 255) / 256, d.Hk, d.n), 256, 0, st>>>(a);
+  }
+  e = attr.ensure(k_dattn_chunk<T, DP, false>, smem);
+  if (e) return e;
+  k_dattn_chunk<T, DP, false><<<grid, kDaThreads, smem, st>>>(mq, mk, mv, a);
+  return cudaGetLastError();
+}
+
 }  // namespace
 }  // namespace bnn
 
 using namespace bnn;
 
+static PFN_cuTensorMapEncodeTiled_v12000 seq_encode_fn(void) {
+  static std::once_flag once;
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  std::call_once(once, [] {
+    void *p = nullptr;
+    cudaDriverEntryPointQueryResult qr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &qr) == cudaSuccess &&
+        qr == cudaDriverEntryPointSuccess)
+      fn = (PFN_cuTensorMapEncodeTiled_v12000)p;
+  });
+  return fn;
+}
+
+int bnn::encode_heads(CUtensorMap *m, const void *base, int bf16, int width, int heads, long long rows, long long rs,
+                      int box_rows) {
+  PFN_cuTensorMapEncodeTiled_v12000 enc = seq_encode_fn();
+  if (!enc) return cudaErrorNotSupported;
+  const cuuint64_t dims[3] = {(cuuint64_t)width, (cuuint64_t)heads, (cuuint64_t)rows};
+  const cuuint64_t strides[2] = {(cuuint64_t)width * 2, (cuuint64_t)rs * 2};
+  const cuuint32_t box[3] = {64, 1, (cuuint32_t)box_rows}, es[3] = {1, 1, 1};
+  return enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void *>(base),
+             dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE)
+             ? cudaErrorInvalidValue
+             : 0;
+}
+
+int bnn::encode_rows16(CUtensorMap *m, const void *base, int bf16, int width, long long rows, long long rs, int box_w,
+                       int box_rows, int sw) {
+  PFN_cuTensorMapEncodeTiled_v12000 enc = seq_encode_fn();
+  if (!enc) return cudaErrorNotSupported;
+  const cuuint64_t dims[2] = {(cuuint64_t)width, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)rs * 2};
+  const cuuint32_t box[2] = {(cuuint32_t)box_w, (cuuint32_t)box_rows}, es[2] = {1, 1};
+  return enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void *>(base),
+             dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             sw == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : sw == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE)
+             ? cudaErrorInvalidValue
+             : 0;
+}
+
+// Tokens of a segment, 0 for whole sequences. Whole sequences where they are enough CTAs for the SMs: one pass. Fewer:
+// parts of about equal length, one per SM, whose states come from a first pass over K and V.
+static int segment_tokens(int n, int Hk, long long tokens) {
+  const long long sms = num_sms(), ctas = (long long)n * Hk;
+  if (ctas * 2 > sms) return 0;
+  const long long parts = sms / Hk < 1 ? 1 : sms / Hk;  // of all sequences together
+  const long long len = ((tokens + parts - 1) / parts + kChunk - 1) / kChunk * kChunk;
+  return tokens <= (long long)n * len ? 0 : (int)len;
+}
+
+extern "C" long long bnnk_dattn_scratch_states(int n, int Hk, long long tokens) {
+  if ((long long)n * Hk * 2 > num_sms()) n = num_sms() / (2 * Hk);  // the most sequences that are split
+  return n < 1 ? 0 : (long long)(n + num_sms() / Hk + 1) * Hk;
+}
+
 extern "C" int bnnk_dattn(const bnnk_dattn_args *p, bnn_stream_t st) {
   if (p->n <= 0) return 0;
-  DattnArgs a = {p->n, p->H, p->Hk, p->H / p->Hk, p->dk, p->dv, p->tokens, p->cu, p->slot, p->live, p->q, p->k, p->v,
-                 p->qts, p->kts, p->vts, p->s0, p->s1, p->o, p->ots, p->pow, p->scale};
-  const int warps = (p->dk + 15) / 16;
-  const dim3 grid(p->n, p->Hk, (p->dv + 31) / 32);
-  if (p->type == 1) k_dattn_rec<1><<<grid, 32 * warps, 0, (cudaStream_t)st>>>(a);
-  else k_dattn_rec<2><<<grid, 32 * warps, 0, (cudaStream_t)st>>>(a);
-  return cudaGetLastError();
+  const DattnArgs d = {p->n, p->H, p->Hk, p->H / p->Hk, p->dk, p->dv, p->tokens, p->cu, p->slot, p->live, p->q, p->k, p->v,
+                       p->qts, p->kts, p->vts, p->s0, p->s1, p->o, p->ots, p->pow, p->scale};
+  const cudaStream_t s = (cudaStream_t)st;
+  // short sequences: the recurrent form
+  if (!p->cu || p->tokens <= 8ll * p->n) {
+    const int warps = (p->dk + 15) / 16;
+    const dim3 grid(p->n, p->Hk, (p->dv + 31) / 32);
+    if (p->type == 1) k_dattn_rec<1><<<grid, 32 * warps, 0, s>>>(d);
+    else k_dattn_rec<2><<<grid, 32 * warps, 0, s>>>(d);
+    return cudaGetLastError();
+  }
+  DaArgs a = {d, segment_tokens(p->n, p->Hk, p->tokens), p->n, p->scratch, p->err};
+  if (a.seg_tokens) a.segs += (int)(p->tokens / a.seg_tokens);
+  const bool wide = p->dk > 64 || p->dv > 64;
+  if (p->type == 1) return wide ? run_chunk<1, 128>(a, s) : run_chunk<1, 64>(a, s);
+  return wide ? run_chunk<2, 128>(a, s) : run_chunk<2, 64>(a, s);
 }

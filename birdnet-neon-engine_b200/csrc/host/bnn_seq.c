@@ -15,10 +15,10 @@ static int launch_rc(const char *what, int e) {
   return -1;
 }
 
-/* zeroed device memory of an op; -1 with the error set */
+/* device memory of an op, the first word zero (an error word); -1 with the error set */
 static int dev_alloc(const char *what, void **p, size_t bytes) {
   cudaError_t e = bnn_fail_dev_alloc() ? cudaErrorMemoryAllocation : cudaMalloc(p, bytes);
-  if (!e) e = cudaMemset(*p, 0, bytes);
+  if (!e) e = cudaMemset(*p, 0, sizeof(int));
   if (!e) return 0;
   ERR(e == cudaErrorMemoryAllocation ? BNN_ERR_OOM : BNN_ERR_CPU, "%s: %zu bytes of device memory: CUDA error %d (%s)",
       what, bytes, (int)e, cudaGetErrorString(e));
@@ -45,7 +45,8 @@ struct bnn_dattn {
   int type, H, Hk, dk, dv, seqs;
   long long tokens;
   float scale;
-  float *pow;  /* [Hk][kDattnPow] */
+  float *pow;      /* [Hk][kDattnPow] */
+  float *scratch;  /* the states of the parts of long sequences */
   int *err;
 };
 
@@ -73,6 +74,8 @@ bnn_dattn *bnn_dattn_new(int type, int heads, int kv_heads, int dk, int dv, cons
   const size_t bytes = sizeof(float) * kDattnPow * kv_heads;
   int bad = !t || dev_alloc("bnn_dattn_new", (void **)&o->pow, bytes) ||
             dev_alloc("bnn_dattn_new", (void **)&o->err, sizeof(int));
+  const long long states = bad ? 0 : bnnk_dattn_scratch_states(seqs, kv_heads, tokens);
+  if (states > 0) bad = dev_alloc("bnn_dattn_new", (void **)&o->scratch, sizeof(float) * states * dk * dv);
   if (!bad) {
     for (int h = 0; h < kv_heads; h++)
       for (int i = 0; i < kDattnPow; i++) t[h * kDattnPow + i] = (float)pow((double)decay[h], i);
@@ -105,7 +108,7 @@ static int dattn_launch(const char *what, bnn_dattn *o, int n, long long tokens,
     return -1;
   }
   const bnnk_dattn_args a = {o->type, n, o->H, o->Hk, o->dk, o->dv, tokens, d_cu, d_slot, d_live, d_q, d_k, d_v,
-                             qts, kts, vts, d_s0, d_s1, d_o, ots, o->pow, o->scale};
+                             qts, kts, vts, d_s0, d_s1, d_o, ots, o->pow, o->scale, o->scratch, o->err};
   return launch_rc(what, bnnk_dattn(&a, (bnn_stream_t)stream));
 }
 
@@ -129,6 +132,7 @@ int bnn_dattn_error(bnn_dattn *o) { return o ? read_word(o->err) : -1; }
 void bnn_dattn_free(bnn_dattn *o) {
   if (!o) return;
   cudaFree(o->pow);
+  cudaFree(o->scratch);
   cudaFree(o->err);
   free(o);
 }
