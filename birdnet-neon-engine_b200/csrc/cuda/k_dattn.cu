@@ -410,7 +410,9 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
       }
       tc_fence_after();
       const uint32_t tq = tmem + L::t_qk + b * 128 + ((uint32_t)(qd * 32) << 16);
-#pragma unroll
+      // 32 columns at a time, in a loop: the roles' code has to stay in the instruction cache together (unrolled four
+      // times, with the other roles' loops, a unit took twice as long, its warps waiting for instructions)
+#pragma unroll 1
       for (int blk = 0; blk < 4; blk++) {
         uint32_t hi[16], lo[16];
         if (blk > qd) {
@@ -419,24 +421,16 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
         } else {
           uint32_t x[32];
           tmem_ld32(tq + blk * 32, x);
+          const uint32_t w = blk == 0 ? lw[0] : blk == 1 ? lw[1] : blk == 2 ? lw[2] : lw[3];
+          const float *f = pw + i - 32 * blk;  // f[-j] = lambda^(i - j), 0 above the diagonal
           tmem_wait_ld(x);
-          const uint32_t w = lw[blk];
           if (w != 0xffffffffu) {
 #pragma unroll
             for (int j = 0; j < 32; j++) x[j] = (w >> j) & 1 ? x[j] : 0u;
           }
-          if (blk == qd) {  // the diagonal block: lambda^(i - j), zero above
 #pragma unroll
-            for (int j = 0; j < 32; j += 2)
-              split2<T>(__uint_as_float(x[j]) * pw[lane - j], __uint_as_float(x[j + 1]) * pw[lane - j - 1], hi[j / 2],
-                        lo[j / 2]);
-          } else {  // lambda^(i - 32 blk - 31) lambda^(31 - j): no power that overflows, one factor the same for all rows
-            const float f = pw[i - 32 * blk - 31];
-#pragma unroll
-            for (int j = 0; j < 32; j += 2)
-              split2<T>(__uint_as_float(x[j]) * f * pw[31 - j], __uint_as_float(x[j + 1]) * f * pw[30 - j], hi[j / 2],
-                        lo[j / 2]);
-          }
+          for (int j = 0; j < 32; j += 2)
+            split2<T>(__uint_as_float(x[j]) * f[-j], __uint_as_float(x[j + 1]) * f[-j - 1], hi[j / 2], lo[j / 2]);
         }
         tmem_st16(tq + blk * 32, hi);
         tmem_st16(tq + blk * 32 + 16, lo);
@@ -465,7 +459,7 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
       const float c1 = d.scale * pw[i + 1], c2 = d.scale;
       elem_t<T> *o = (elem_t<T> *)d.o + (t + i) * d.ots + (long long)(hk * G + g) * d.dv;
       const uint32_t tq = tmem + ((uint32_t)(qd * 32) << 16);
-#pragma unroll
+#pragma unroll 1
       for (int col = 0; col < DP; col += 16) {
         uint32_t x[16], y[16], z[8];
         tmem_ld16(tq + L::t_o1 + col, x);
@@ -537,21 +531,20 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
       const long long t = t0 + (long long)c * kChunk;
       const int n = (int)min((long long)kChunk, t1 - t);
       // K' and the dead rows of V: 16-byte slots, a row's 8 by 8 lanes; both tiles keep the swizzle's order
-      bool dead[4];
-      float wt[4];
-#pragma unroll
-      for (int m = 0; m < 4; m++) {
-        const int row = tid / 8 + 32 * m;
-        dead[m] = row >= n || (d.live && !d.live[t + row]);
-        wt[m] = row < n ? pw[n - 1 - row] : 0.f;
-      }
+      uint32_t lw[4];
+      live_words(d, t, n, lw);
+      auto dead = [&](int m) {
+        return !(((m == 0 ? lw[0] : m == 1 ? lw[1] : m == 2 ? lw[2] : lw[3]) >> (tid / 8)) & 1);
+      };
       ok = mbar_wait(smem_u32(&b_kfull[s]), (c / NS) & 1);
       ok = __all_sync(0xffffffffu, ok && !abort_s);
       if (!ok) break;
+#pragma unroll 1
+      for (int m = 0; m < 4; m++) {
+        const float wt = pw[n - 1 - min(tid / 8 + 32 * m, n - 1)];
+        const bool off_row = dead(m);
 #pragma unroll
-      for (int p = 0; p < PN; p++)
-#pragma unroll
-        for (int m = 0; m < 4; m++) {
+        for (int p = 0; p < PN; p++) {
           const uint32_t off = p * L::panel + (tid + 256 * m) * 16;
           uint32_t x[4], h[4], l[4];
           asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
@@ -560,8 +553,8 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
                        : "memory");
 #pragma unroll
           for (int e = 0; e < 4; e++) {
-            const float2 f = unpack2<T>(dead[m] ? 0u : x[e]);
-            split2<T>(f.x * wt[m], f.y * wt[m], h[e], l[e]);
+            const float2 f = unpack2<T>(off_row ? 0u : x[e]);
+            split2<T>(f.x * wt, f.y * wt, h[e], l[e]);
           }
           const uint32_t at = base + L::kp + off;
           asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3])
@@ -570,15 +563,15 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
                        "r"(l[3])
                        : "memory");
         }
+      }
       if (n < kChunk || d.live) {
         ok = mbar_wait(smem_u32(&b_vfull[s]), (c / NS) & 1);
         ok = __all_sync(0xffffffffu, ok && !abort_s);
         if (!ok) break;
-#pragma unroll
-        for (int p = 0; p < PN; p++)
-#pragma unroll
-          for (int m = 0; m < 4; m++)
-            if (dead[m])
+#pragma unroll 1
+        for (int m = 0; m < 4; m++)
+          if (dead(m))
+            for (int p = 0; p < PN; p++)
               asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(base + L::v + s * L::tile + p * L::panel +
                                                                             (tid + 256 * m) * 16),
                            "r"(0)
