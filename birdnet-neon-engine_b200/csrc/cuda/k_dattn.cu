@@ -145,19 +145,27 @@ __global__ void __launch_bounds__(256) k_dattn_rec(const DattnArgs a) {
 //   S'  = lambda^n S + sum_j lambda^(n-1-j) k_j^T v_j
 // as four products on the tensor cores (tcgen05 kind::f16, fp32 accumulators in TMEM): QK = Q K^T, O1 = Q S, DS = K'^T V
 // with K'_j = lambda^(n-1-j) k_j, and O2 = P V with P = QK times the decays below the diagonal. Q, K and V arrive by TMA
-// (128-byte swizzle, heads narrower than the padded width DP read as zero past their end). What is computed and goes back
-// into a product (P, S, K') goes as two 16-bit parts whose sum keeps 16 bits or more of significand, so that a 16-bit
-// output's error stays that of its one rounding and the fp32 state is off by about 6e-7 of its size, as an fp32 sum of
-// these terms is; one part alone would add an error as large as the output's rounding for each of P and S.
+// (128-byte swizzle, heads narrower than the padded width DP read as zero past their end).
+//
+// What is computed and goes back into a product (P, S, K') goes as 16-bit parts whose sum keeps enough of the fp32 value:
+//  - bf16: P and S as two parts (2^-16 of a value, so that o keeps the error of its one rounding; one part each would add
+//    1.4 times that rounding), K' as three (all 24 bits: the state is fp32 and sums K' over every chunk; with two parts
+//    it was 2.4e-6 off, against 4.5e-7 for fp32 products).
+//  - fp16: two parts are 22 bits, but only within the type's range, so each is scaled by a power of two that a maximum
+//    gives: P by its row's, S and K' by their tile's, and K' has the decays counted from the chunk's last live token. The
+//    scales go into the fp32 steps after the products. Values 2^28 below the maximum are the first to lose bits.
 //
 // One CTA per (segment of a sequence, k/v head) walks the segment's chunks, and for each the G q heads of the group
-// ("unit" u = (chunk, q head)). Roles: warp 0 TMA, warp 1 MMA issue, 4 warps turn QK into P (in place in TMEM, as the A
-// operand of the last product), 4 warps join O1 and O2 and store o, 8 warps hold S in registers, form K' and the S
-// operand. S in registers stays fp32: lambda^n S + DS, once a chunk.
+// ("unit" u = (chunk, q head)). Roles: warp 0 TMA, warp 1 MMA issue, 8 warps turn QK into P (in place in TMEM, as the A
+// operand of the last product), 4 warps join O1 and O2 and store o, 16 warps hold S in registers, form K' and the S
+// operand. S in registers stays fp32: lambda^n S + DS, once a chunk. The roles' loops are rolled: unrolled, their code
+// did not stay in the instruction cache together and a unit took twice as long. The issuing warp stays converged
+// (elect.sync): from one lane's branch each tcgen05.mma took 70 cycles to issue, more than a 128 x 64 x 16 product.
 // A masked token, and a row past the segment's end, has its k and v rows taken as zero (K' zero, V zeroed in shared
 // memory, its P column zero by selection, so that NaN and infinities there stay out); its o row is zero or not stored.
 constexpr int kChunk = 128;
-constexpr int kDaThreads = 640;
+constexpr int kDaThreads = 1024;
+constexpr int kDaP = 4, kDaO = 12, kDaS = 16;  // first warps of the P, output and state roles
 
 struct DaArgs {
   DattnArgs d;
@@ -208,17 +216,26 @@ __device__ bool find_segment(const DaArgs &a, int s, int &seq, int &part, long l
   return false;
 }
 
-template <int DP>
+// Shared memory and TMEM. DP 128: one stage of Q, K, V, and the first part of K' in K's place (it waits for QK to have
+// read K); DP 64: three stages, two QK / P regions, K' apart.
+template <int T, int DP>
 struct DaLayout {
-  static constexpr int stages = DP == 64 ? 2 : 1;   // Q, K, V tiles in flight
+  static constexpr int parts = T == 2 ? 3 : 2;      // of K'
+  static constexpr bool in_place = DP == 128;
+  static constexpr int stages = DP == 64 ? 3 : 1;   // Q, K, V tiles in flight
   static constexpr int qk_bufs = DP == 64 ? 2 : 1;  // QK / P regions in TMEM
   static constexpr uint32_t panel = kChunk * 128;   // 64 columns of a 128-row tile
   static constexpr uint32_t tile = kChunk * DP * 2;
   static constexpr uint32_t s_panel = DP * 128, s_tile = DP * DP * 2;
   static constexpr uint32_t q = 0, k = q + stages * tile, v = k + stages * tile, kp = v + stages * tile,
-                            st = kp + 2 * tile, end = st + 2 * s_tile;
+                            st = kp + (parts - in_place) * tile, end = st + 2 * s_tile;
   static constexpr uint32_t t_qk = 0, t_o1 = qk_bufs * 128, t_o2 = t_o1 + DP, t_ds = t_o2 + DP;  // TMEM columns
   static constexpr size_t smem = end + 1024;
+  static constexpr int scales = T == 1 ? (qk_bufs == 2 ? 4 : 2) : 1;  // P row scales: units until o has read them
+  // part x of K' for stage s
+  static __device__ __forceinline__ uint32_t kpart(uint32_t base, int s, int x) {
+    return in_place ? (x ? base + kp + (x - 1) * tile : base + k + s * tile) : base + kp + x * tile;
+  }
 };
 
 // the live tokens among a chunk's 128, bit j % 32 of word j / 32 (one warp; every lane gets all words)
@@ -230,22 +247,44 @@ __device__ __forceinline__ void live_words(const DattnArgs &a, long long t, int 
     w[b] = __ballot_sync(0xffffffffu, j < n && (!a.live || a.live[t + j]));
   }
 }
+__device__ __forceinline__ uint32_t word_of(const uint32_t (&w)[4], int b) {
+  return b == 0 ? w[0] : b == 1 ? w[1] : b == 2 ? w[2] : w[3];
+}
+
+// the power of two that brings a magnitude m to [2^14, 2^15), and its inverse; 1 where m is zero or not finite
+__device__ __forceinline__ float scale_to_f16(float m, float &inv) {
+  const int e = (int)(__float_as_uint(m) >> 23);
+  if (e == 0 || e == 255) { inv = 1.f; return 1.f; }
+  const int x = min(max(14 + 127 - e, -126), 126);
+  inv = __uint_as_float((uint32_t)(127 - x) << 23);
+  return __uint_as_float((uint32_t)(127 + x) << 23);
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+__device__ __forceinline__ void sts128(uint32_t at, const uint32_t (&x)[4]) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+}
 
 template <int T, int DP, bool kState>
 __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_constant__ CUtensorMap mq,
                                                               const __grid_constant__ CUtensorMap mk,
                                                               const __grid_constant__ CUtensorMap mv, const DaArgs a) {
-  using L = DaLayout<DP>;
+  using L = DaLayout<T, DP>;
   constexpr int NS = L::stages, NB = L::qk_bufs, PN = DP / 64;
   extern __shared__ uint8_t dsmem[];
   __shared__ __align__(8) unsigned long long b_qfull[NS], b_kfull[NS], b_vfull[NS], b_qempty[NS], b_kempty[NS],
-      b_vempty[NS], b_qk[NB], b_p[NB], b_s, b_kp, b_ds, b_o, b_oempty;
+      b_vempty[NS], b_qk[NB], b_p[NB], b_s, b_vfix, b_kp, b_ds, b_o, b_oempty, b_max, b_row[4];
   __shared__ uint32_t tmem_s;
   __shared__ volatile int abort_s;
   __shared__ float s_pow[32 + kDattnPow];  // s_pow[32 + x] = lambda^x, 0 for x < 0
   __shared__ long long s_range[2];
   __shared__ int s_seg[3];
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  __shared__ float s_max[2][16], s_inv[2];  // fp16: the state warps' maxima, the inverse scale of S by chunk
+  __shared__ float s_pinv[L::scales][T == 1 ? kChunk : 1];  // fp16: the inverse row scales of P
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   const DattnArgs &d = a.d;
   const int hk = blockIdx.y, G = kState ? 1 : d.G;
 
@@ -264,12 +303,15 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
         mbar_init(smem_u32(&b_qfull[s]), 1); mbar_init(smem_u32(&b_kfull[s]), 1); mbar_init(smem_u32(&b_vfull[s]), 1);
         mbar_init(smem_u32(&b_qempty[s]), 1); mbar_init(smem_u32(&b_kempty[s]), 1); mbar_init(smem_u32(&b_vempty[s]), 1);
       }
-      for (int b = 0; b < NB; b++) { mbar_init(smem_u32(&b_qk[b]), 1); mbar_init(smem_u32(&b_p[b]), 4); }
-      mbar_init(smem_u32(&b_s), 8); mbar_init(smem_u32(&b_kp), 8); mbar_init(smem_u32(&b_ds), 1);
-      mbar_init(smem_u32(&b_o), 1); mbar_init(smem_u32(&b_oempty), 4);
+      for (int b = 0; b < NB; b++) { mbar_init(smem_u32(&b_qk[b]), 1); mbar_init(smem_u32(&b_p[b]), 8); }
+      mbar_init(smem_u32(&b_s), 16); mbar_init(smem_u32(&b_vfix), 16); mbar_init(smem_u32(&b_kp), 16);
+      mbar_init(smem_u32(&b_ds), 1); mbar_init(smem_u32(&b_o), 1); mbar_init(smem_u32(&b_oempty), 4);
+      mbar_init(smem_u32(&b_max), 16);
+      for (int w = 0; w < 4; w++) mbar_init(smem_u32(&b_row[w]), 2);
       abort_s = 0;
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    __syncwarp();
   } else if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_s)), "r"(512));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
@@ -286,74 +328,83 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
   const bool work = seq >= 0 && !(kState && s_seg[2]);
   const int nc = work ? (int)((t1 - t0 + kChunk - 1) / kChunk) : 0, nu = nc * G;
   const float *pw = s_pow + 32;
+  // a whole warp waits; false (and the error word set) when the time limit or another role's ran out
+  auto wait = [&](unsigned long long &bar, int parity, int code) {
+    bool ok = mbar_wait(smem_u32(&bar), parity);
+    ok = __all_sync(0xffffffffu, ok && !abort_s);
+    if (!ok && lane == 0) {
+      if (!abort_s) atomicExch(a.err, code);
+      abort_s = 1;
+    }
+    return ok;
+  };
 
-#define DA_WAIT(bar, parity, code)                \
-  if (!mbar_wait(smem_u32(&(bar)), (parity))) {   \
-    atomicExch(a.err, code);                      \
-    abort_s = 1;                                  \
-    break;                                        \
-  }
-
-  if (warp == 0) {
-    if (lane == 0) {  // TMA
-      int nq = 0, c = 0;
-      for (; c < nc && !abort_s; c++) {
-        const long long t = t0 + (long long)c * kChunk;
-        const int s = c % NS, use = c / NS;
-        bool ok = true;
-        for (int g = 0; g < G && ok; g++) {
-          if (!kState) {
-            const int sq = nq % NS;
-            if (nq >= NS && !mbar_wait(smem_u32(&b_qempty[sq]), (nq / NS - 1) & 1)) { ok = false; break; }
+  if (warp == 0) {  // TMA
+    int nq = 0;
+    bool ok = true;
+    for (int c = 0; c < nc && ok; c++) {
+      const int t = (int)(t0 + (long long)c * kChunk);
+      const int s = c % NS, use = c / NS;
+      for (int g = 0; g < G && ok; g++) {
+        if (!kState) {
+          const int sq = nq % NS;
+          if (nq >= NS && !(ok = wait(b_qempty[sq], (nq / NS - 1) & 1, BNNK_ERR_TMA_WAIT))) break;
+          if (elect_one()) {
             mbar_expect_tx(smem_u32(&b_qfull[sq]), L::tile);
+#pragma unroll
             for (int p = 0; p < PN; p++)
-              tma_load_3d(base + L::q + sq * L::tile + p * L::panel, &mq, smem_u32(&b_qfull[sq]), 64 * p, hk * G + g, (int)t);
-            nq++;
+              tma_load_3d(base + L::q + sq * L::tile + p * L::panel, &mq, smem_u32(&b_qfull[sq]), 64 * p, hk * G + g, t);
           }
-          if (g) continue;
-          if (use && !mbar_wait(smem_u32(&b_kempty[s]), (use - 1) & 1)) { ok = false; break; }
-          mbar_expect_tx(smem_u32(&b_kfull[s]), L::tile);
-          for (int p = 0; p < PN; p++)
-            tma_load_3d(base + L::k + s * L::tile + p * L::panel, &mk, smem_u32(&b_kfull[s]), 64 * p, hk, (int)t);
-          if (use && !mbar_wait(smem_u32(&b_vempty[s]), (use - 1) & 1)) { ok = false; break; }
-          mbar_expect_tx(smem_u32(&b_vfull[s]), L::tile);
-          for (int p = 0; p < PN; p++)
-            tma_load_3d(base + L::v + s * L::tile + p * L::panel, &mv, smem_u32(&b_vfull[s]), 64 * p, hk, (int)t);
+          nq++;
         }
-        if (!ok) {
-          atomicExch(a.err, BNNK_ERR_TMA_WAIT);
-          abort_s = 1;
+        if (g) continue;
+        if (use && !(ok = wait(b_kempty[s], (use - 1) & 1, BNNK_ERR_TMA_WAIT))) break;
+        if (elect_one()) {
+          mbar_expect_tx(smem_u32(&b_kfull[s]), L::tile);
+#pragma unroll
+          for (int p = 0; p < PN; p++)
+            tma_load_3d(base + L::k + s * L::tile + p * L::panel, &mk, smem_u32(&b_kfull[s]), 64 * p, hk, t);
+        }
+        if (use && !(ok = wait(b_vempty[s], (use - 1) & 1, BNNK_ERR_TMA_WAIT))) break;
+        if (elect_one()) {
+          mbar_expect_tx(smem_u32(&b_vfull[s]), L::tile);
+#pragma unroll
+          for (int p = 0; p < PN; p++)
+            tma_load_3d(base + L::v + s * L::tile + p * L::panel, &mv, smem_u32(&b_vfull[s]), 64 * p, hk, t);
         }
       }
     }
-  } else if (warp == 1) {
-    if (lane == 0) {  // MMA
-      constexpr uint32_t bt = T - 1;
-      constexpr uint32_t i_qk = idesc_16(bt, 128, 0, 0), i_qs = idesc_16(bt, DP, 0, 1), i_ds = idesc_16(bt, DP, 1, 1),
-                         i_pv = idesc_16(bt, DP, 0, 1);
-      auto issue_qk = [&](int u) {
-        const int c = u / G, sq = u % NS, s = c % NS, b = u % NB;
-        if (!mbar_wait(smem_u32(&b_qfull[sq]), (u / NS) & 1) || !mbar_wait(smem_u32(&b_kfull[s]), (c / NS) & 1)) return false;
-        tc_fence_after();
-        const uint32_t qa = base + L::q + sq * L::tile, ka = base + L::k + s * L::tile;
+  } else if (warp == 1) {  // MMA
+    constexpr uint32_t bt = T - 1;
+    constexpr uint32_t i_qk = idesc_16(bt, 128, 0, 0), i_qs = idesc_16(bt, DP, 0, 1), i_ds = idesc_16(bt, DP, 1, 1),
+                       i_pv = idesc_16(bt, DP, 0, 1);
+    auto issue_qk = [&](int u) {
+      const int c = u / G, sq = u % NS, s = c % NS, b = u % NB;
+      if (!wait(b_qfull[sq], (u / NS) & 1, BNNK_ERR_MMA_WAIT)) return false;
+      if (u % G == 0 && !wait(b_kfull[s], (c / NS) & 1, BNNK_ERR_MMA_WAIT)) return false;
+      tc_fence_after();
+      const uint32_t qa = base + L::q + sq * L::tile, ka = base + L::k + s * L::tile;
+      if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < DP / 16; kk++) {
           const uint32_t off = (kk / 4) * L::panel + (kk % 4) * 32;
           mma16_ss(tmem + L::t_qk + b * 128, smem_desc<128>(qa + off), smem_desc<128>(ka + off), i_qk, kk != 0);
         }
         mma_commit(smem_u32(&b_qk[b]));
-        return true;
-      };
-      if (!kState && nu > 0 && !issue_qk(0)) { atomicExch(a.err, BNNK_ERR_MMA_WAIT); abort_s = 1; }
-      for (int u = 0; u < nu && !abort_s; u++) {
-        const int c = u / G, g = u % G, sq = u % NS, s = c % NS, b = u % NB;
-        const uint32_t va = base + L::v + s * L::tile;
-        if (!kState) {
-          if (NB > 1 && u + 1 < nu && !issue_qk(u + 1)) { atomicExch(a.err, BNNK_ERR_MMA_WAIT); abort_s = 1; break; }
-          if (g == 0) DA_WAIT(b_s, c & 1, BNNK_ERR_MMA_WAIT)
-          if (u) DA_WAIT(b_oempty, (u - 1) & 1, BNNK_ERR_MMA_WAIT)
-          tc_fence_after();
-          const uint32_t qa = base + L::q + sq * L::tile;
+      }
+      return true;
+    };
+    bool ok = kState || nu == 0 || issue_qk(0);
+    for (int u = 0; u < nu && ok; u++) {
+      const int c = u / G, g = u % G, sq = u % NS, s = c % NS, b = u % NB;
+      const uint32_t va = base + L::v + s * L::tile;
+      if (!kState) {
+        if (NB > 1 && u + 1 < nu && !(ok = issue_qk(u + 1))) break;
+        if (g == 0 && !(ok = wait(b_s, c & 1, BNNK_ERR_MMA_WAIT))) break;
+        if (u && !(ok = wait(b_oempty, (u - 1) & 1, BNNK_ERR_MMA_WAIT))) break;
+        tc_fence_after();
+        const uint32_t qa = base + L::q + sq * L::tile;
+        if (elect_one()) {
 #pragma unroll
           for (int part = 0; part < 2; part++)
 #pragma unroll
@@ -362,85 +413,107 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
                        smem_desc_mn(base + L::st + part * L::s_tile + kk * 2048, L::s_panel), i_qs, (part | kk) != 0);
           mma_commit(smem_u32(&b_qempty[sq]));
         }
-        if (g == 0) {
-          DA_WAIT(b_vfull[s], (c / NS) & 1, BNNK_ERR_MMA_WAIT)
-          DA_WAIT(b_kp, c & 1, BNNK_ERR_MMA_WAIT)
-          tc_fence_after();
-        }
-        if (g == G - 1) {
+      }
+      if (g == 0) {
+        if (!(ok = wait(b_vfull[s], (c / NS) & 1, BNNK_ERR_MMA_WAIT))) break;
+        if (!(ok = wait(b_vfix, c & 1, BNNK_ERR_MMA_WAIT))) break;
+      }
+      if (g == G - 1) {
+        if (!(ok = wait(b_kp, c & 1, BNNK_ERR_MMA_WAIT))) break;
+        tc_fence_after();
+        if (elect_one()) {
 #pragma unroll
-          for (int part = 0; part < 2; part++)
+          for (int part = 0; part < L::parts; part++)
 #pragma unroll
             for (int kk = 0; kk < 8; kk++)
-              mma16_ss(tmem + L::t_ds, smem_desc_mn(base + L::kp + part * L::tile + kk * 2048, L::panel),
+              mma16_ss(tmem + L::t_ds, smem_desc_mn(L::kpart(base, s, part) + kk * 2048, L::panel),
                        smem_desc_mn(va + kk * 2048, L::panel), i_ds, (part | kk) != 0);
           mma_commit(smem_u32(&b_ds));
           mma_commit(smem_u32(&b_kempty[s]));
         }
-        if (!kState) {
-          DA_WAIT(b_p[b], (u / NB) & 1, BNNK_ERR_MMA_WAIT)
-          tc_fence_after();
-          // P: 32 columns j a block, its high parts in the block's first 16 TMEM columns, the low parts in the others
+      }
+      if (!kState) {
+        if (!(ok = wait(b_p[b], (u / NB) & 1, BNNK_ERR_MMA_WAIT))) break;
+        tc_fence_after();
+        if (elect_one()) {  // P: 16 columns j a block, its first parts in 8 TMEM columns, the second parts in the next 8
 #pragma unroll
           for (int kk = 0; kk < 8; kk++)
 #pragma unroll
             for (int part = 0; part < 2; part++)
-              mma16_ts(tmem + L::t_o2, tmem + L::t_qk + b * 128 + (kk / 2) * 32 + part * 16 + (kk % 2) * 8,
-                       smem_desc_mn(va + kk * 2048, L::panel), i_pv, (part | kk) != 0);
+              mma16_ts(tmem + L::t_o2, tmem + L::t_qk + b * 128 + kk * 16 + part * 8, smem_desc_mn(va + kk * 2048, L::panel),
+                       i_pv, (part | kk) != 0);
           mma_commit(smem_u32(&b_o));
         }
-        if (g == G - 1) mma_commit(smem_u32(&b_vempty[s]));
-        if (!kState && NB == 1 && u + 1 < nu && !issue_qk(u + 1)) { atomicExch(a.err, BNNK_ERR_MMA_WAIT); abort_s = 1; }
       }
+      if (g == G - 1 && elect_one()) mma_commit(smem_u32(&b_vempty[s]));
+      if (!kState && NB == 1 && u + 1 < nu) ok = issue_qk(u + 1);
     }
-  } else if (warp >= 4 && warp < 8) {
-    // P: this thread's row i against the columns j <= i
-    const int qd = warp % 4, i = 32 * qd + lane;
+  } else if (warp >= kDaP && warp < kDaO) {
+    // P: row i against the columns j <= i, blocks of 16 columns alternating between two warps
+    const int qd = warp % 4, h = (warp - kDaP) / 4, i = 32 * qd + lane;
     for (int u = 0; u < (kState ? 0 : nu); u++) {
       const int c = u / G, b = u % NB;
       const long long t = t0 + (long long)c * kChunk;
       const int n = (int)min((long long)kChunk, t1 - t);
       uint32_t lw[4];
       live_words(d, t, n, lw);
-      bool ok = mbar_wait(smem_u32(&b_qk[b]), (u / NB) & 1);
-      ok = __all_sync(0xffffffffu, ok && !abort_s);
-      if (!ok) {
-        if (lane == 0) { atomicExch(a.err, BNNK_ERR_EPI_WAIT); abort_s = 1; }
-        break;
-      }
+      if (!wait(b_qk[b], (u / NB) & 1, BNNK_ERR_EPI_WAIT)) break;
       tc_fence_after();
       const uint32_t tq = tmem + L::t_qk + b * 128 + ((uint32_t)(qd * 32) << 16);
-      // 32 columns at a time, in a loop: the roles' code has to stay in the instruction cache together (unrolled four
-      // times, with the other roles' loops, a unit took twice as long, its warps waiting for instructions)
+      float sc = 1.f;
+      if constexpr (T == 1) {  // the row's largest product (the dead columns' and those above the diagonal left out)
+        float m = 0.f;
 #pragma unroll 1
-      for (int blk = 0; blk < 4; blk++) {
-        uint32_t hi[16], lo[16];
-        if (blk > qd) {
-#pragma unroll
-          for (int j = 0; j < 16; j++) hi[j] = lo[j] = 0;
-        } else {
-          uint32_t x[32];
-          tmem_ld32(tq + blk * 32, x);
-          const uint32_t w = blk == 0 ? lw[0] : blk == 1 ? lw[1] : blk == 2 ? lw[2] : lw[3];
-          const float *f = pw + i - 32 * blk;  // f[-j] = lambda^(i - j), 0 above the diagonal
+        for (int blk = 0; blk < 2 * qd + 2; blk++) {
+          uint32_t x[16];
+          tmem_ld16(tq + blk * 16, x);
+          const uint32_t w = word_of(lw, blk / 2) >> (blk % 2 * 16);
+          const int left = i - 16 * blk;
           tmem_wait_ld(x);
-          if (w != 0xffffffffu) {
 #pragma unroll
-            for (int j = 0; j < 32; j++) x[j] = (w >> j) & 1 ? x[j] : 0u;
+          for (int j = 0; j < 16; j++) m = fmaxf(m, (w >> j) & 1 && j <= left ? fabsf(__uint_as_float(x[j])) : 0.f);
+        }
+        float inv;
+        sc = scale_to_f16(m, inv);
+        if (h == 0) s_pinv[u % L::scales][i] = inv;
+        // every column is read before another warp of this row writes P over it
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&b_row[qd]));
+        if (!wait(b_row[qd], u & 1, BNNK_ERR_EPI_WAIT)) break;
+      }
+#pragma unroll 1
+      for (int blk = h; blk < 8; blk += 2) {
+        uint32_t x[16];
+        if (blk >= 2 * qd + 2) {
+#pragma unroll
+          for (int j = 0; j < 16; j++) x[j] = 0;
+        } else {
+          tmem_ld16(tq + blk * 16, x);
+          const uint32_t w = word_of(lw, blk / 2) >> (blk % 2 * 16);
+          const float *f = pw + i - 16 * blk;  // f[-j] = lambda^(i - j), 0 above the diagonal
+          tmem_wait_ld(x);
+          if ((w & 0xffffu) != 0xffffu) {
+#pragma unroll
+            for (int j = 0; j < 16; j++) x[j] = (w >> j) & 1 ? x[j] : 0u;
+          }
+          uint32_t p[16];
+#pragma unroll
+          for (int j = 0; j < 16; j += 2) {
+            float f0 = f[-j], f1 = f[-j - 1];
+            if constexpr (T == 1) { f0 *= sc; f1 *= sc; }
+            split2<T>(__uint_as_float(x[j]) * f0, __uint_as_float(x[j + 1]) * f1, p[j / 2], p[8 + j / 2]);
           }
 #pragma unroll
-          for (int j = 0; j < 32; j += 2)
-            split2<T>(__uint_as_float(x[j]) * f[-j], __uint_as_float(x[j + 1]) * f[-j - 1], hi[j / 2], lo[j / 2]);
+          for (int j = 0; j < 16; j++) x[j] = p[j];
         }
-        tmem_st16(tq + blk * 32, hi);
-        tmem_st16(tq + blk * 32 + 16, lo);
+        tmem_st16(tq + blk * 16, x);
       }
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&b_p[b]));
     }
-  } else if (warp >= 8 && warp < 12) {
+  } else if (warp >= kDaO && warp < kDaS) {
     // o: this thread's row i
     const int qd = warp % 4, i = 32 * qd + lane;
     const bool wide = (d.dv % 16 | d.ots % 16) == 0 && ((uintptr_t)d.o & 31) == 0;
@@ -449,14 +522,13 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
       const long long t = t0 + (long long)c * kChunk;
       const int n = (int)min((long long)kChunk, t1 - t);
       const bool live = i < n && (!d.live || d.live[t + i]);
-      bool ok = mbar_wait(smem_u32(&b_o), u & 1);
-      ok = __all_sync(0xffffffffu, ok && !abort_s);
-      if (!ok) {
-        if (lane == 0) { atomicExch(a.err, BNNK_ERR_EPI_WAIT); abort_s = 1; }
-        break;
-      }
+      if (!wait(b_o, u & 1, BNNK_ERR_EPI_WAIT)) break;
       tc_fence_after();
-      const float c1 = d.scale * pw[i + 1], c2 = d.scale;
+      float c1 = d.scale * pw[i + 1], c2 = d.scale;
+      if constexpr (T == 1) {
+        c1 *= s_inv[c & 1];
+        c2 *= s_pinv[u % L::scales][i];
+      }
       elem_t<T> *o = (elem_t<T> *)d.o + (t + i) * d.ots + (long long)(hk * G + g) * d.dv;
       const uint32_t tq = tmem + ((uint32_t)(qd * 32) << 16);
 #pragma unroll 1
@@ -486,11 +558,10 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&b_oempty));
     }
-  } else if (warp >= 12 && seq >= 0) {
-    // the state: row r = dk index, DP / 2 columns from c0 in registers
-    constexpr int HC = DP / 2;
-    const int w8 = warp - 12, r = 32 * (warp % 4) + lane, c0 = (w8 / 4) * HC, tid = threadIdx.x - 384;
-    const bool mine = r < DP;
+  } else if (warp >= kDaS && seq >= 0) {
+    // the state: row r = dk index, DP / 4 columns from c0 in registers
+    constexpr int HC = DP / 4;
+    const int r = 32 * (warp % 4) + lane, c0 = (warp - kDaS) / 4 * HC, tid = threadIdx.x - 32 * kDaS;
     float S[HC];
     const long long slot = d.slot ? d.slot[seq] : seq;
     const float *from = nullptr;
@@ -504,102 +575,140 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
       if (from && r < d.dk && c0 + j < d.dv) v = *reinterpret_cast<const float4 *>(from + (long long)r * d.dv + c0 + j);
       S[j] = v.x; S[j + 1] = v.y; S[j + 2] = v.z; S[j + 3] = v.w;
     }
-    auto put_state = [&]() {  // S as the B operand of O1: row r, MN-major panels of 64 columns
-      if (mine) {
+    // the maximum over the role's threads; a buffer is written again two calls later, when every warp has arrived at
+    // the call between and so has read it
+    int calls = 0;
+    bool ok = true;
+    auto role_max = [&](float v) {
+      v = warp_max(v);
+      if (lane == 0) {
+        s_max[calls & 1][warp - kDaS] = v;
+        mbar_arrive(smem_u32(&b_max));
+      }
+      if (ok) ok = wait(b_max, calls & 1, BNNK_ERR_EPI_WAIT);
+      return warp_max(s_max[calls++ & 1][lane % 16]);
+    };
+    auto put_state = [&](int c) {  // S before chunk c as the B operand of O1: row r, MN-major panels of 64 columns
+      float sc = 1.f;
+      if constexpr (T == 1) {
+        float m = 0.f, inv;
+#pragma unroll
+        for (int j = 0; j < HC; j++) m = fmaxf(m, fabsf(S[j]));
+        sc = scale_to_f16(role_max(r < DP ? m : 0.f), inv);
+        if (tid == 0) s_inv[c & 1] = inv;
+      }
+      if (r < DP) {
 #pragma unroll
         for (int j = 0; j < HC; j += 8) {
           uint32_t h[4], l[4];
 #pragma unroll
-          for (int e = 0; e < 4; e++) split2<T>(S[j + 2 * e], S[j + 2 * e + 1], h[e], l[e]);
+          for (int e = 0; e < 4; e++) split2<T>(S[j + 2 * e] * sc, S[j + 2 * e + 1] * sc, h[e], l[e]);
           const int col = c0 + j;
           const uint32_t at = base + L::st + (col / 64) * L::s_panel + r * 128 + ((((col % 64) / 8) ^ (r & 7)) << 4);
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3])
-                       : "memory");
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + L::s_tile), "r"(l[0]), "r"(l[1]), "r"(l[2]),
-                       "r"(l[3])
-                       : "memory");
+          sts128(at, h);
+          sts128(at + L::s_tile, l);
         }
       }
       fence_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&b_s));
     };
-    if (!kState && nc > 0) put_state();
-    bool ok = true;
-    for (int c = 0; c < nc; c++) {
+    if (!kState && nc > 0) put_state(0);
+    for (int c = 0; c < nc && ok; c++) {
       const int s = c % NS;
       const long long t = t0 + (long long)c * kChunk;
       const int n = (int)min((long long)kChunk, t1 - t);
-      // K' and the dead rows of V: 16-byte slots, a row's 8 by 8 lanes; both tiles keep the swizzle's order
+      // 16-byte slots of the tiles, a row's 8 by 8 lanes: row tid / 8, then 64 rows on. A slot stays where it is, so the
+      // tiles written here have the swizzle of the one they come from
       uint32_t lw[4];
       live_words(d, t, n, lw);
-      auto dead = [&](int m) {
-        return !(((m == 0 ? lw[0] : m == 1 ? lw[1] : m == 2 ? lw[2] : lw[3]) >> (tid / 8)) & 1);
-      };
-      ok = mbar_wait(smem_u32(&b_kfull[s]), (c / NS) & 1);
-      ok = __all_sync(0xffffffffu, ok && !abort_s);
-      if (!ok) break;
+      auto dead = [&](int m) { return !((word_of(lw, 2 * m + tid / 256) >> (tid / 8 % 32)) & 1); };
+      if (n < kChunk || d.live) {
+        if (!(ok = wait(b_vfull[s], (c / NS) & 1, BNNK_ERR_EPI_WAIT))) break;
+        const uint32_t zero[4] = {0, 0, 0, 0};
 #pragma unroll 1
-      for (int m = 0; m < 4; m++) {
-        const float wt = pw[n - 1 - min(tid / 8 + 32 * m, n - 1)];
+        for (int m = 0; m < 2; m++)
+          if (dead(m))
+            for (int p = 0; p < PN; p++) sts128(base + L::v + s * L::tile + p * L::panel + (tid + 512 * m) * 16, zero);
+        fence_async_smem();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&b_vfix));
+      if (!(ok = wait(b_kfull[s], (c / NS) & 1, BNNK_ERR_EPI_WAIT))) break;
+      int from_j = n - 1;  // the token whose decay counts as 1
+      float ksc = 1.f, dsc = 1.f;
+      auto load = [&](int m, int p, uint32_t (&x)[4]) {
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
+                     : "r"(base + L::k + s * L::tile + p * L::panel + (tid + 512 * m) * 16)
+                     : "memory");
+      };
+      if constexpr (T == 1) {
+        float mx = 0.f;
+#pragma unroll 1
+        for (int m = 0; m < 2; m++)
+          if (!dead(m))
+            for (int p = 0; p < PN; p++) {
+              uint32_t x[4];
+              load(m, p, x);
+#pragma unroll
+              for (int e = 0; e < 4; e++) {
+                const float2 f = unpack2<T>(x[e]);
+                mx = fmaxf(mx, fmaxf(fabsf(f.x), fabsf(f.y)));
+              }
+            }
+        from_j = lw[3] ? 127 - __clz(lw[3]) : lw[2] ? 95 - __clz(lw[2]) : lw[1] ? 63 - __clz(lw[1]) : lw[0] ? 31 - __clz(lw[0]) : 0;
+        ksc = scale_to_f16(role_max(mx), dsc);
+        if (!ok) break;
+        dsc *= pw[n - 1 - from_j];
+      }
+      if (L::in_place && !kState) {  // K has been read by the products of all its q heads
+        for (int g = 0; g < G && ok; g++) ok = wait(b_qk[0], (c * G + g) & 1, BNNK_ERR_EPI_WAIT);
+        if (!ok) break;
+      }
+#pragma unroll 1
+      for (int m = 0; m < 2; m++) {
+        const int row = tid / 8 + 64 * m;
         const bool off_row = dead(m);
+        const float wt = off_row ? 0.f : pw[from_j - row] * ksc;
 #pragma unroll
         for (int p = 0; p < PN; p++) {
-          const uint32_t off = p * L::panel + (tid + 256 * m) * 16;
-          uint32_t x[4], h[4], l[4];
-          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                       : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
-                       : "r"(base + L::k + s * L::tile + off)
-                       : "memory");
+          const uint32_t off = p * L::panel + (tid + 512 * m) * 16;
+          uint32_t x[4], h[4], l[4], l2[4];
+          load(m, p, x);
 #pragma unroll
           for (int e = 0; e < 4; e++) {
             const float2 f = unpack2<T>(off_row ? 0u : x[e]);
-            split2<T>(f.x * wt, f.y * wt, h[e], l[e]);
+            if constexpr (L::parts == 3) split3<T>(f.x * wt, f.y * wt, h[e], l[e], l2[e]);
+            else split2<T>(f.x * wt, f.y * wt, h[e], l[e]);
           }
-          const uint32_t at = base + L::kp + off;
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3])
-                       : "memory");
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + L::tile), "r"(l[0]), "r"(l[1]), "r"(l[2]),
-                       "r"(l[3])
-                       : "memory");
+          sts128(L::kpart(base, s, 0) + off, h);
+          sts128(L::kpart(base, s, 1) + off, l);
+          if constexpr (L::parts == 3) sts128(L::kpart(base, s, 2) + off, l2);
         }
-      }
-      if (n < kChunk || d.live) {
-        ok = mbar_wait(smem_u32(&b_vfull[s]), (c / NS) & 1);
-        ok = __all_sync(0xffffffffu, ok && !abort_s);
-        if (!ok) break;
-#pragma unroll 1
-        for (int m = 0; m < 4; m++)
-          if (dead(m))
-            for (int p = 0; p < PN; p++)
-              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(base + L::v + s * L::tile + p * L::panel +
-                                                                            (tid + 256 * m) * 16),
-                           "r"(0)
-                           : "memory");
       }
       fence_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&b_kp));
-      ok = mbar_wait(smem_u32(&b_ds), c & 1);
-      ok = __all_sync(0xffffffffu, ok && !abort_s);
-      if (!ok) break;
+      if (!(ok = wait(b_ds, c & 1, BNNK_ERR_EPI_WAIT))) break;
       tc_fence_after();
       const float dec = pw[n];
       const uint32_t td = tmem + L::t_ds + c0 + ((uint32_t)((warp % 4) * 32) << 16);
 #pragma unroll
-      for (int j = 0; j < HC; j += 32) {
-        uint32_t x[32];
-        tmem_ld32(td + j, x);
+      for (int j = 0; j < HC; j += 16) {
+        uint32_t x[16];
+        tmem_ld16(td + j, x);
         tmem_wait_ld(x);
 #pragma unroll
-        for (int e = 0; e < 32; e++) S[j + e] = fmaf(dec, S[j + e], __uint_as_float(x[e]));
+        for (int e = 0; e < 16; e++) {
+          const float v = __uint_as_float(x[e]);
+          S[j + e] = fmaf(dec, S[j + e], T == 1 ? v * dsc : v);
+        }
       }
       tc_fence_before();
-      if (!kState && c + 1 < nc) put_state();
+      if (!kState && c + 1 < nc) put_state(c + 1);
     }
-    if (!ok) {
-      if (lane == 0) { atomicExch(a.err, BNNK_ERR_EPI_WAIT); abort_s = 1; }
-    } else {
+    if (ok) {
       float *to = nullptr;
       if (kState) {
         if (work) to = a.seg_state + ((long long)blockIdx.x * d.Hk + hk) * d.dk * d.dv;
@@ -614,7 +723,6 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
       }
     }
   }
-#undef DA_WAIT
   tc_fence_before();
   __syncthreads();
   if (warp == 1)
@@ -679,7 +787,7 @@ int run_chunk(const DaArgs &a, cudaStream_t st) {
   if (e) return e;
   static SmemAttr attr_s, attr;
   const dim3 grid(a.segs, d.Hk);
-  constexpr size_t smem = DaLayout<DP>::smem;
+  constexpr size_t smem = DaLayout<T, DP>::smem;
   if (a.seg_tokens) {
     e = attr_s.ensure(k_dattn_chunk<T, DP, true>, smem);
     if (e) return e;

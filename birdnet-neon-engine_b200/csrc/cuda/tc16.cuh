@@ -101,6 +101,23 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t &hi, uint32_t 
   lo = pack2f<T>(a - h.x, b - h.y);
 }
 
+// three parts: all of an fp32 value's 24 bits (bf16)
+template <int T>
+__device__ __forceinline__ void split3(float a, float b, uint32_t &hi, uint32_t &lo, uint32_t &lo2) {
+  hi = pack2f<T>(a, b);
+  const float2 h = unpack2<T>(hi);
+  const float ra = a - h.x, rb = b - h.y;
+  lo = pack2f<T>(ra, rb);
+  const float2 l = unpack2<T>(lo);
+  lo2 = pack2f<T>(ra - l.x, rb - l.y);
+}
+// one lane of a converged warp, the same for every call
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
 // host: a 3-D map of a 16-bit tensor [rows][heads][width] (row stride rs elements, heads back to back), boxes of 64
 // elements x 1 head x box_rows rows, 128-byte swizzle, zero fill out of bounds: a width that ends inside a box reads
 // zero past it, never the next head; 0 or a cudaError_t
