@@ -238,6 +238,20 @@ struct DaLayout {
   }
 };
 
+// a place in a ring of N and the parity of its use
+template <int N>
+struct Ring {
+  int at = 0, parity = 0;
+  bool used = false;  // every place has been used once
+  __device__ __forceinline__ void next() {
+    if (N == 1 || ++at == N) {
+      at = 0;
+      parity ^= 1;
+      used = true;
+    }
+  }
+};
+
 // the live tokens among a chunk's 128, bit j % 32 of word j / 32 (one warp; every lane gets all words)
 __device__ __forceinline__ void live_words(const DattnArgs &a, long long t, int n, uint32_t (&w)[4]) {
   const int lane = threadIdx.x % 32;
@@ -330,7 +344,8 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
   const float *pw = s_pow + 32;
   // a whole warp waits; false (and the error word set) when the time limit or another role's ran out
   auto wait = [&](unsigned long long &bar, int parity, int code) {
-    bool ok = mbar_wait(smem_u32(&bar), parity);
+    if (__all_sync(0xffffffffu, mbar_try(smem_u32(&bar), parity))) return true;
+    bool ok = mbar_wait_asleep(smem_u32(&bar), parity);
     ok = __all_sync(0xffffffffu, ok && !abort_s);
     if (!ok && lane == 0) {
       if (!abort_s) atomicExch(a.err, code);
@@ -340,32 +355,30 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
   };
 
   if (warp == 0) {  // TMA
-    int nq = 0;
+    Ring<NS> rq, rc;  // tiles of Q (one a unit), of K and V (one a chunk)
     bool ok = true;
     for (int c = 0; c < nc && ok; c++) {
-      const int t = (int)(t0 + (long long)c * kChunk);
-      const int s = c % NS, use = c / NS;
+      const int t = (int)(t0 + (long long)c * kChunk), s = rc.at;
       for (int g = 0; g < G && ok; g++) {
         if (!kState) {
-          const int sq = nq % NS;
-          if (nq >= NS && !(ok = wait(b_qempty[sq], (nq / NS - 1) & 1, BNNK_ERR_TMA_WAIT))) break;
+          if (rq.used && !(ok = wait(b_qempty[rq.at], rq.parity ^ 1, BNNK_ERR_TMA_WAIT))) break;
           if (elect_one()) {
-            mbar_expect_tx(smem_u32(&b_qfull[sq]), L::tile);
+            mbar_expect_tx(smem_u32(&b_qfull[rq.at]), L::tile);
 #pragma unroll
             for (int p = 0; p < PN; p++)
-              tma_load_3d(base + L::q + sq * L::tile + p * L::panel, &mq, smem_u32(&b_qfull[sq]), 64 * p, hk * G + g, t);
+              tma_load_3d(base + L::q + rq.at * L::tile + p * L::panel, &mq, smem_u32(&b_qfull[rq.at]), 64 * p, hk * G + g, t);
           }
-          nq++;
+          rq.next();
         }
         if (g) continue;
-        if (use && !(ok = wait(b_kempty[s], (use - 1) & 1, BNNK_ERR_TMA_WAIT))) break;
+        if (rc.used && !(ok = wait(b_kempty[s], rc.parity ^ 1, BNNK_ERR_TMA_WAIT))) break;
         if (elect_one()) {
           mbar_expect_tx(smem_u32(&b_kfull[s]), L::tile);
 #pragma unroll
           for (int p = 0; p < PN; p++)
             tma_load_3d(base + L::k + s * L::tile + p * L::panel, &mk, smem_u32(&b_kfull[s]), 64 * p, hk, t);
         }
-        if (use && !(ok = wait(b_vempty[s], (use - 1) & 1, BNNK_ERR_TMA_WAIT))) break;
+        if (rc.used && !(ok = wait(b_vempty[s], rc.parity ^ 1, BNNK_ERR_TMA_WAIT))) break;
         if (elect_one()) {
           mbar_expect_tx(smem_u32(&b_vfull[s]), L::tile);
 #pragma unroll
@@ -373,37 +386,45 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
             tma_load_3d(base + L::v + s * L::tile + p * L::panel, &mv, smem_u32(&b_vfull[s]), 64 * p, hk, t);
         }
       }
+      rc.next();
     }
   } else if (warp == 1) {  // MMA
     constexpr uint32_t bt = T - 1;
     constexpr uint32_t i_qk = idesc_16(bt, 128, 0, 0), i_qs = idesc_16(bt, DP, 0, 1), i_ds = idesc_16(bt, DP, 1, 1),
                        i_pv = idesc_16(bt, DP, 0, 1);
-    auto issue_qk = [&](int u) {
-      const int c = u / G, sq = u % NS, s = c % NS, b = u % NB;
-      if (!wait(b_qfull[sq], (u / NS) & 1, BNNK_ERR_MMA_WAIT)) return false;
-      if (u % G == 0 && !wait(b_kfull[s], (c / NS) & 1, BNNK_ERR_MMA_WAIT)) return false;
+    Ring<NS> kq, kc, rq, rc;  // the next QK's tiles (kq, kc), this unit's (rq, rc)
+    Ring<NB> kb, rb;          // and their QK / P regions
+    int kg = 0;
+    auto issue_qk = [&]() {
+      if (!wait(b_qfull[kq.at], kq.parity, BNNK_ERR_MMA_WAIT)) return false;
+      if (kg == 0 && !wait(b_kfull[kc.at], kc.parity, BNNK_ERR_MMA_WAIT)) return false;
       tc_fence_after();
-      const uint32_t qa = base + L::q + sq * L::tile, ka = base + L::k + s * L::tile;
+      const uint32_t qa = base + L::q + kq.at * L::tile, ka = base + L::k + kc.at * L::tile;
       if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < DP / 16; kk++) {
           const uint32_t off = (kk / 4) * L::panel + (kk % 4) * 32;
-          mma16_ss(tmem + L::t_qk + b * 128, smem_desc<128>(qa + off), smem_desc<128>(ka + off), i_qk, kk != 0);
+          mma16_ss(tmem + L::t_qk + kb.at * 128, smem_desc<128>(qa + off), smem_desc<128>(ka + off), i_qk, kk != 0);
         }
-        mma_commit(smem_u32(&b_qk[b]));
+        mma_commit(smem_u32(&b_qk[kb.at]));
       }
+      kq.next();
+      kb.next();
+      if (++kg == G) { kg = 0; kc.next(); }
       return true;
     };
-    bool ok = kState || nu == 0 || issue_qk(0);
+    bool ok = kState || nu == 0 || issue_qk();
+    int g = 0;
+    Ring<1> ru, rk;  // single barriers: a phase a unit, a phase a chunk
     for (int u = 0; u < nu && ok; u++) {
-      const int c = u / G, g = u % G, sq = u % NS, s = c % NS, b = u % NB;
+      const int s = rc.at;
       const uint32_t va = base + L::v + s * L::tile;
       if (!kState) {
-        if (NB > 1 && u + 1 < nu && !(ok = issue_qk(u + 1))) break;
-        if (g == 0 && !(ok = wait(b_s, c & 1, BNNK_ERR_MMA_WAIT))) break;
-        if (u && !(ok = wait(b_oempty, (u - 1) & 1, BNNK_ERR_MMA_WAIT))) break;
+        if (NB > 1 && u + 1 < nu && !(ok = issue_qk())) break;
+        if (g == 0 && !(ok = wait(b_s, rk.parity, BNNK_ERR_MMA_WAIT))) break;
+        if (u && !(ok = wait(b_oempty, ru.parity ^ 1, BNNK_ERR_MMA_WAIT))) break;
         tc_fence_after();
-        const uint32_t qa = base + L::q + sq * L::tile;
+        const uint32_t qa = base + L::q + rq.at * L::tile;
         if (elect_one()) {
 #pragma unroll
           for (int part = 0; part < 2; part++)
@@ -411,15 +432,18 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
             for (int kk = 0; kk < DP / 16; kk++)
               mma16_ss(tmem + L::t_o1, smem_desc<128>(qa + (kk / 4) * L::panel + (kk % 4) * 32),
                        smem_desc_mn(base + L::st + part * L::s_tile + kk * 2048, L::s_panel), i_qs, (part | kk) != 0);
-          mma_commit(smem_u32(&b_qempty[sq]));
+          mma_commit(smem_u32(&b_qempty[rq.at]));
         }
+        rq.next();
       }
       if (g == 0) {
-        if (!(ok = wait(b_vfull[s], (c / NS) & 1, BNNK_ERR_MMA_WAIT))) break;
-        if (!(ok = wait(b_vfix, c & 1, BNNK_ERR_MMA_WAIT))) break;
+        if (!(ok = wait(b_vfull[s], rc.parity, BNNK_ERR_MMA_WAIT))) break;
+        if (!(ok = wait(b_vfix, rk.parity, BNNK_ERR_MMA_WAIT))) break;
       }
-      if (g == G - 1) {
-        if (!(ok = wait(b_kp, c & 1, BNNK_ERR_MMA_WAIT))) break;
+      const bool last = ++g == G;
+      if (last) {
+        g = 0;
+        if (!(ok = wait(b_kp, rk.parity, BNNK_ERR_MMA_WAIT))) break;
         tc_fence_after();
         if (elect_one()) {
 #pragma unroll
@@ -431,22 +455,26 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
           mma_commit(smem_u32(&b_ds));
           mma_commit(smem_u32(&b_kempty[s]));
         }
+        rk.next();
+        rc.next();
       }
       if (!kState) {
-        if (!(ok = wait(b_p[b], (u / NB) & 1, BNNK_ERR_MMA_WAIT))) break;
+        if (!(ok = wait(b_p[rb.at], rb.parity, BNNK_ERR_MMA_WAIT))) break;
         tc_fence_after();
         if (elect_one()) {  // P: 16 columns j a block, its first parts in 8 TMEM columns, the second parts in the next 8
 #pragma unroll
           for (int kk = 0; kk < 8; kk++)
 #pragma unroll
             for (int part = 0; part < 2; part++)
-              mma16_ts(tmem + L::t_o2, tmem + L::t_qk + b * 128 + kk * 16 + part * 8, smem_desc_mn(va + kk * 2048, L::panel),
-                       i_pv, (part | kk) != 0);
+              mma16_ts(tmem + L::t_o2, tmem + L::t_qk + rb.at * 128 + kk * 16 + part * 8,
+                       smem_desc_mn(va + kk * 2048, L::panel), i_pv, (part | kk) != 0);
           mma_commit(smem_u32(&b_o));
         }
+        rb.next();
+        ru.next();
       }
-      if (g == G - 1 && elect_one()) mma_commit(smem_u32(&b_vempty[s]));
-      if (!kState && NB == 1 && u + 1 < nu) ok = issue_qk(u + 1);
+      if (last && elect_one()) mma_commit(smem_u32(&b_vempty[s]));
+      if (!kState && NB == 1 && u + 1 < nu) ok = issue_qk();
     }
   } else if (warp >= kDaP && warp < kDaO) {
     // P: row i against the columns j <= i, blocks of 16 columns alternating between two warps

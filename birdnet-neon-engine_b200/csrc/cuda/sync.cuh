@@ -45,6 +45,23 @@ __device__ __forceinline__ bool mbar_wait_ns(uint32_t bar, uint32_t parity, unsi
     if (gtimer() - t0 > limit_ns) return false;
   }
 }
+// the same for kernels with many warps waiting at once: a try may sleep in hardware until the phase completes (up to
+// 100 us), so that waiting warps take few issue slots and few timer reads
+__device__ __forceinline__ bool mbar_wait_asleep(uint32_t bar, uint32_t parity) {
+  const unsigned long long t0 = gtimer();
+  for (;;) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(bar), "r"(parity), "r"(100000u)
+        : "memory");
+    if (done) return true;
+    if (gtimer() - t0 > kWaitNs) return false;
+  }
+}
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) { return mbar_wait_ns(bar, parity, kWaitNs); }
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y) {
   asm volatile(
