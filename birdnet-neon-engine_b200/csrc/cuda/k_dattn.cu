@@ -156,16 +156,16 @@ __global__ void __launch_bounds__(256) k_dattn_rec(const DattnArgs a) {
 //    scales go into the fp32 steps after the products. Values 2^28 below the maximum are the first to lose bits.
 //
 // One CTA per (segment of a sequence, k/v head) walks the segment's chunks, and for each the G q heads of the group
-// ("unit" u = (chunk, q head)). Roles: warp 0 TMA, warp 1 MMA issue, 8 warps turn QK into P (in place in TMEM, as the A
-// operand of the last product), 4 warps join O1 and O2 and store o, 16 warps hold S in registers, form K' and the S
-// operand. S in registers stays fp32: lambda^n S + DS, once a chunk. The roles' loops are rolled: unrolled, their code
+// ("unit" u = (chunk, q head)). Roles: warp 0 MMA issue, warp 1 TMA, 8 warps turn QK into P (in place in TMEM, as the A
+// operand of the last product), 16 warps hold S in registers, form K' and the S operand, and join O1 and O2 into o. S in
+// registers stays fp32: lambda^n S + DS, once a chunk. The roles' loops are rolled: unrolled, their code
 // did not stay in the instruction cache together and a unit took twice as long. The issuing warp stays converged
 // (elect.sync): from one lane's branch each tcgen05.mma took 70 cycles to issue, more than a 128 x 64 x 16 product.
 // A masked token, and a row past the segment's end, has its k and v rows taken as zero (K' zero, V zeroed in shared
 // memory, its P column zero by selection, so that NaN and infinities there stay out); its o row is zero or not stored.
 constexpr int kChunk = 128;
-constexpr int kDaThreads = 1024;
-constexpr int kDaP = 4, kDaO = 12, kDaS = 16;  // first warps of the P, output and state roles
+constexpr int kDaThreads = 896;
+constexpr int kDaP = 4, kDaS = 12;  // first warps of the P and state roles
 
 struct DaArgs {
   DattnArgs d;
@@ -217,24 +217,26 @@ __device__ bool find_segment(const DaArgs &a, int s, int &seq, int &part, long l
 }
 
 // Shared memory and TMEM. DP 128: one stage of Q, K, V, and the first part of K' in K's place (it waits for QK to have
-// read K); DP 64: three stages, two QK / P regions, K' apart.
+// read K); DP 64: two stages, two QK / P regions, two sets of K', formed a chunk ahead.
 template <int T, int DP>
 struct DaLayout {
   static constexpr int parts = T == 2 ? 3 : 2;      // of K'
   static constexpr bool in_place = DP == 128;
-  static constexpr int stages = DP == 64 ? 3 : 1;   // Q, K, V tiles in flight
+  static constexpr int stages = DP == 64 ? 2 : 1;   // Q, K, V tiles in flight, sets of K'
   static constexpr int qk_bufs = DP == 64 ? 2 : 1;  // QK / P regions in TMEM
   static constexpr uint32_t panel = kChunk * 128;   // 64 columns of a 128-row tile
   static constexpr uint32_t tile = kChunk * DP * 2;
   static constexpr uint32_t s_panel = DP * 128, s_tile = DP * DP * 2;
   static constexpr uint32_t q = 0, k = q + stages * tile, v = k + stages * tile, kp = v + stages * tile,
-                            st = kp + (parts - in_place) * tile, end = st + 2 * s_tile;
+                            st = kp + (in_place ? parts - 1 : stages * parts) * tile,
+                            o = in_place ? kp : st + 2 * s_tile,  // o on its way out: in place of K''s second part, or apart
+                            end = st + 2 * s_tile + (in_place ? 0 : tile);
   static constexpr uint32_t t_qk = 0, t_o1 = qk_bufs * 128, t_o2 = t_o1 + DP, t_ds = t_o2 + DP;  // TMEM columns
   static constexpr size_t smem = end + 1024;
   static constexpr int scales = T == 1 ? (qk_bufs == 2 ? 4 : 2) : 1;  // P row scales: units until o has read them
   // part x of K' for stage s
   static __device__ __forceinline__ uint32_t kpart(uint32_t base, int s, int x) {
-    return in_place ? (x ? base + kp + (x - 1) * tile : base + k + s * tile) : base + kp + x * tile;
+    return in_place ? (x ? base + kp + (x - 1) * tile : base + k + s * tile) : base + kp + (s * parts + x) * tile;
   }
 };
 
@@ -290,13 +292,13 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
   constexpr int NS = L::stages, NB = L::qk_bufs, PN = DP / 64;
   extern __shared__ uint8_t dsmem[];
   __shared__ __align__(8) unsigned long long b_qfull[NS], b_kfull[NS], b_vfull[NS], b_qempty[NS], b_kempty[NS],
-      b_vempty[NS], b_qk[NB], b_p[NB], b_s, b_vfix, b_kp, b_ds, b_o, b_oempty, b_max, b_row[4];
+      b_vempty[NS], b_qk[NB], b_p[NB], b_s, b_vfix[NS], b_kp[NS], b_ds, b_o, b_oempty, b_max, b_row[4];
   __shared__ uint32_t tmem_s;
   __shared__ volatile int abort_s;
   __shared__ float s_pow[32 + kDattnPow];  // s_pow[32 + x] = lambda^x, 0 for x < 0
   __shared__ long long s_range[2];
   __shared__ int s_seg[3];
-  __shared__ float s_max[2][16], s_inv[2];  // fp16: the state warps' maxima, the inverse scale of S by chunk
+  __shared__ float s_max[2][16], s_inv[2], s_dsc[2];  // fp16: the state warps' maxima, scales of S and of its sums by chunk
   __shared__ float s_pinv[L::scales][T == 1 ? kChunk : 1];  // fp16: the inverse row scales of P
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   const DattnArgs &d = a.d;
@@ -316,10 +318,11 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
       for (int s = 0; s < NS; s++) {
         mbar_init(smem_u32(&b_qfull[s]), 1); mbar_init(smem_u32(&b_kfull[s]), 1); mbar_init(smem_u32(&b_vfull[s]), 1);
         mbar_init(smem_u32(&b_qempty[s]), 1); mbar_init(smem_u32(&b_kempty[s]), 1); mbar_init(smem_u32(&b_vempty[s]), 1);
+        mbar_init(smem_u32(&b_vfix[s]), 16); mbar_init(smem_u32(&b_kp[s]), 16);
       }
       for (int b = 0; b < NB; b++) { mbar_init(smem_u32(&b_qk[b]), 1); mbar_init(smem_u32(&b_p[b]), 8); }
-      mbar_init(smem_u32(&b_s), 16); mbar_init(smem_u32(&b_vfix), 16); mbar_init(smem_u32(&b_kp), 16);
-      mbar_init(smem_u32(&b_ds), 1); mbar_init(smem_u32(&b_o), 1); mbar_init(smem_u32(&b_oempty), 4);
+      mbar_init(smem_u32(&b_s), 16); mbar_init(smem_u32(&b_ds), 1); mbar_init(smem_u32(&b_o), 1);
+      mbar_init(smem_u32(&b_oempty), 16);
       mbar_init(smem_u32(&b_max), 16);
       for (int w = 0; w < 4; w++) mbar_init(smem_u32(&b_row[w]), 2);
       abort_s = 0;
@@ -335,7 +338,7 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_s, base = (smem_u32(dsmem) + 1023u) & ~1023u;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_s, 0), base = (smem_u32(dsmem) + 1023u) & ~1023u;
   const long long t0 = s_range[0], t1 = s_range[1];
   const int seq = s_seg[0];
   // a segment's own sum is needed where another follows it
@@ -354,7 +357,7 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
     return ok;
   };
 
-  if (warp == 0) {  // TMA
+  if (warp == 1) {  // TMA
     Ring<NS> rq, rc;  // tiles of Q (one a unit), of K and V (one a chunk)
     bool ok = true;
     for (int c = 0; c < nc && ok; c++) {
@@ -388,10 +391,14 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
       }
       rc.next();
     }
-  } else if (warp == 1) {  // MMA
+  } else if (warp == 0) {  // MMA (the warp of the first TMEM quarter, whose scheduler has the fewest P blocks)
     constexpr uint32_t bt = T - 1;
     constexpr uint32_t i_qk = idesc_16(bt, 128, 0, 0), i_qs = idesc_16(bt, DP, 0, 1), i_ds = idesc_16(bt, DP, 1, 1),
                        i_pv = idesc_16(bt, DP, 0, 1);
+    // a descriptor's address is its low bits, in 16 bytes: K-major steps of 16 lie 32 bytes apart in a panel of 64,
+    // MN-major steps 16 rows of 128 bytes
+    auto kstep = [](int kk) { return (uint64_t)(((kk / 4) * L::panel + (kk % 4) * 32) >> 4); };
+    constexpr uint64_t mnstep = 2048 >> 4;
     Ring<NS> kq, kc, rq, rc;  // the next QK's tiles (kq, kc), this unit's (rq, rc)
     Ring<NB> kb, rb;          // and their QK / P regions
     int kg = 0;
@@ -399,13 +406,11 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
       if (!wait(b_qfull[kq.at], kq.parity, BNNK_ERR_MMA_WAIT)) return false;
       if (kg == 0 && !wait(b_kfull[kc.at], kc.parity, BNNK_ERR_MMA_WAIT)) return false;
       tc_fence_after();
-      const uint32_t qa = base + L::q + kq.at * L::tile, ka = base + L::k + kc.at * L::tile;
+      const uint64_t dq = smem_desc<128>(base + L::q + kq.at * L::tile), dk = smem_desc<128>(base + L::k + kc.at * L::tile);
       if (elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < DP / 16; kk++) {
-          const uint32_t off = (kk / 4) * L::panel + (kk % 4) * 32;
-          mma16_ss(tmem + L::t_qk + kb.at * 128, smem_desc<128>(qa + off), smem_desc<128>(ka + off), i_qk, kk != 0);
-        }
+        for (int kk = 0; kk < DP / 16; kk++)
+          mma16_ss(tmem + L::t_qk + kb.at * 128, dq + kstep(kk), dk + kstep(kk), i_qk, kk != 0);
         mma_commit(smem_u32(&b_qk[kb.at]));
       }
       kq.next();
@@ -418,40 +423,40 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
     Ring<1> ru, rk;  // single barriers: a phase a unit, a phase a chunk
     for (int u = 0; u < nu && ok; u++) {
       const int s = rc.at;
-      const uint32_t va = base + L::v + s * L::tile;
+      const uint64_t dv = smem_desc_mn(base + L::v + s * L::tile, L::panel);
       if (!kState) {
         if (NB > 1 && u + 1 < nu && !(ok = issue_qk())) break;
         if (g == 0 && !(ok = wait(b_s, rk.parity, BNNK_ERR_MMA_WAIT))) break;
         if (u && !(ok = wait(b_oempty, ru.parity ^ 1, BNNK_ERR_MMA_WAIT))) break;
         tc_fence_after();
-        const uint32_t qa = base + L::q + rq.at * L::tile;
+        const uint64_t dq = smem_desc<128>(base + L::q + rq.at * L::tile), ds = smem_desc_mn(base + L::st, L::s_panel);
         if (elect_one()) {
 #pragma unroll
           for (int part = 0; part < 2; part++)
 #pragma unroll
             for (int kk = 0; kk < DP / 16; kk++)
-              mma16_ss(tmem + L::t_o1, smem_desc<128>(qa + (kk / 4) * L::panel + (kk % 4) * 32),
-                       smem_desc_mn(base + L::st + part * L::s_tile + kk * 2048, L::s_panel), i_qs, (part | kk) != 0);
+              mma16_ss(tmem + L::t_o1, dq + kstep(kk), ds + (part * L::s_tile >> 4) + kk * mnstep, i_qs, (part | kk) != 0);
           mma_commit(smem_u32(&b_qempty[rq.at]));
         }
         rq.next();
       }
       if (g == 0) {
         if (!(ok = wait(b_vfull[s], rc.parity, BNNK_ERR_MMA_WAIT))) break;
-        if (!(ok = wait(b_vfix, rk.parity, BNNK_ERR_MMA_WAIT))) break;
+        if (!(ok = wait(b_vfix[s], rc.parity, BNNK_ERR_MMA_WAIT))) break;
       }
       const bool last = ++g == G;
       if (last) {
         g = 0;
-        if (!(ok = wait(b_kp, rk.parity, BNNK_ERR_MMA_WAIT))) break;
+        if (!(ok = wait(b_kp[s], rc.parity, BNNK_ERR_MMA_WAIT))) break;
         tc_fence_after();
+        const uint64_t dk0 = smem_desc_mn(L::kpart(base, s, 0), L::panel), dk1 = smem_desc_mn(L::kpart(base, s, 1), L::panel);
         if (elect_one()) {
 #pragma unroll
           for (int part = 0; part < L::parts; part++)
 #pragma unroll
             for (int kk = 0; kk < 8; kk++)
-              mma16_ss(tmem + L::t_ds, smem_desc_mn(L::kpart(base, s, part) + kk * 2048, L::panel),
-                       smem_desc_mn(va + kk * 2048, L::panel), i_ds, (part | kk) != 0);
+              mma16_ss(tmem + L::t_ds, (part ? dk1 + ((part - 1) * L::tile >> 4) : dk0) + kk * mnstep, dv + kk * mnstep, i_ds,
+                       (part | kk) != 0);
           mma_commit(smem_u32(&b_ds));
           mma_commit(smem_u32(&b_kempty[s]));
         }
@@ -466,8 +471,8 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
           for (int kk = 0; kk < 8; kk++)
 #pragma unroll
             for (int part = 0; part < 2; part++)
-              mma16_ts(tmem + L::t_o2, tmem + L::t_qk + rb.at * 128 + kk * 16 + part * 8,
-                       smem_desc_mn(va + kk * 2048, L::panel), i_pv, (part | kk) != 0);
+              mma16_ts(tmem + L::t_o2, tmem + L::t_qk + rb.at * 128 + kk * 16 + part * 8, dv + kk * mnstep, i_pv,
+                       (part | kk) != 0);
           mma_commit(smem_u32(&b_o));
         }
         rb.next();
@@ -476,19 +481,19 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
       if (last && elect_one()) mma_commit(smem_u32(&b_vempty[s]));
       if (!kState && NB == 1 && u + 1 < nu) ok = issue_qk();
     }
-  } else if (warp >= kDaP && warp < kDaO) {
+  } else if (warp >= kDaP && warp < kDaS) {
     // P: row i against the columns j <= i, blocks of 16 columns alternating between two warps
     const int qd = warp % 4, h = (warp - kDaP) / 4, i = 32 * qd + lane;
     for (int u = 0; u < (kState ? 0 : nu); u++) {
       const int c = u / G, b = u % NB;
       const long long t = t0 + (long long)c * kChunk;
       const int n = (int)min((long long)kChunk, t1 - t);
-      uint32_t lw[4];
-      live_words(d, t, n, lw);
+      uint32_t lw[4] = {~0u, ~0u, ~0u, ~0u};
+      if (n < kChunk || d.live) live_words(d, t, n, lw);
       if (!wait(b_qk[b], (u / NB) & 1, BNNK_ERR_EPI_WAIT)) break;
       tc_fence_after();
       const uint32_t tq = tmem + L::t_qk + b * 128 + ((uint32_t)(qd * 32) << 16);
-      float sc = 1.f;
+      float sc = d.scale;
       if constexpr (T == 1) {  // the row's largest product (the dead columns' and those above the diagonal left out)
         float m = 0.f;
 #pragma unroll 1
@@ -509,88 +514,41 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
         if (lane == 0) mbar_arrive(smem_u32(&b_row[qd]));
         if (!wait(b_row[qd], u & 1, BNNK_ERR_EPI_WAIT)) break;
       }
+      const int blocks = 2 * qd + 2;  // those that reach the diagonal
+      uint32_t x[16];
+      if (h < blocks) tmem_ld16(tq + h * 16, x);
 #pragma unroll 1
-      for (int blk = h; blk < 8; blk += 2) {
-        uint32_t x[16];
-        if (blk >= 2 * qd + 2) {
+      for (int blk = h; blk < blocks; blk += 2) {
+        uint32_t p[16];
+        const uint32_t w = word_of(lw, blk / 2) >> (blk % 2 * 16);
+        const float *f = pw + i - 16 * blk;  // f[-j] = lambda^(i - j), 0 above the diagonal
+        tmem_wait_ld(x);
+        if ((w & 0xffffu) != 0xffffu) {
 #pragma unroll
-          for (int j = 0; j < 16; j++) x[j] = 0;
-        } else {
-          tmem_ld16(tq + blk * 16, x);
-          const uint32_t w = word_of(lw, blk / 2) >> (blk % 2 * 16);
-          const float *f = pw + i - 16 * blk;  // f[-j] = lambda^(i - j), 0 above the diagonal
-          tmem_wait_ld(x);
-          if ((w & 0xffffu) != 0xffffu) {
-#pragma unroll
-            for (int j = 0; j < 16; j++) x[j] = (w >> j) & 1 ? x[j] : 0u;
-          }
-          uint32_t p[16];
-#pragma unroll
-          for (int j = 0; j < 16; j += 2) {
-            float f0 = f[-j], f1 = f[-j - 1];
-            if constexpr (T == 1) { f0 *= sc; f1 *= sc; }
-            split2<T>(__uint_as_float(x[j]) * f0, __uint_as_float(x[j + 1]) * f1, p[j / 2], p[8 + j / 2]);
-          }
-#pragma unroll
-          for (int j = 0; j < 16; j++) x[j] = p[j];
+          for (int j = 0; j < 16; j++) x[j] = (w >> j) & 1 ? x[j] : 0u;
         }
-        tmem_st16(tq + blk * 16, x);
+#pragma unroll
+        for (int j = 0; j < 16; j += 2)
+          split2<T>(__uint_as_float(x[j]) * (f[-j] * sc), __uint_as_float(x[j + 1]) * (f[-j - 1] * sc), p[j / 2],
+                    p[8 + j / 2]);
+        if (blk + 2 < blocks) tmem_ld16(tq + (blk + 2) * 16, x);  // the next block, while this one is stored
+        tmem_st16(tq + blk * 16, p);
       }
+#pragma unroll
+      for (int j = 0; j < 16; j++) x[j] = 0;
+#pragma unroll 1
+      for (int blk = blocks + h; blk < 8; blk += 2) tmem_st16(tq + blk * 16, x);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&b_p[b]));
-    }
-  } else if (warp >= kDaO && warp < kDaS) {
-    // o: this thread's row i
-    const int qd = warp % 4, i = 32 * qd + lane;
-    const bool wide = (d.dv % 16 | d.ots % 16) == 0 && ((uintptr_t)d.o & 31) == 0;
-    for (int u = 0; u < (kState ? 0 : nu); u++) {
-      const int c = u / G, g = u % G;
-      const long long t = t0 + (long long)c * kChunk;
-      const int n = (int)min((long long)kChunk, t1 - t);
-      const bool live = i < n && (!d.live || d.live[t + i]);
-      if (!wait(b_o, u & 1, BNNK_ERR_EPI_WAIT)) break;
-      tc_fence_after();
-      float c1 = d.scale * pw[i + 1], c2 = d.scale;
-      if constexpr (T == 1) {
-        c1 *= s_inv[c & 1];
-        c2 *= s_pinv[u % L::scales][i];
-      }
-      elem_t<T> *o = (elem_t<T> *)d.o + (t + i) * d.ots + (long long)(hk * G + g) * d.dv;
-      const uint32_t tq = tmem + ((uint32_t)(qd * 32) << 16);
-#pragma unroll 1
-      for (int col = 0; col < DP; col += 16) {
-        uint32_t x[16], y[16], z[8];
-        tmem_ld16(tq + L::t_o1 + col, x);
-        tmem_ld16(tq + L::t_o2 + col, y);
-        tmem_wait_ld(x, y);
-#pragma unroll
-        for (int j = 0; j < 16; j += 2) {
-          const float p = c1 * __uint_as_float(x[j]) + c2 * __uint_as_float(y[j]);
-          const float q = c1 * __uint_as_float(x[j + 1]) + c2 * __uint_as_float(y[j + 1]);
-          z[j / 2] = live ? pack2f<T>(p, q) : 0u;
-        }
-        if (i < n && col < d.dv) {
-          if (wide) {
-            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(o + col), "r"(z[0]), "r"(z[1]),
-                         "r"(z[2]), "r"(z[3]), "r"(z[4]), "r"(z[5]), "r"(z[6]), "r"(z[7])
-                         : "memory");
-          } else {
-            *reinterpret_cast<uint4 *>(o + col) = make_uint4(z[0], z[1], z[2], z[3]);
-            if (col + 8 < d.dv) *reinterpret_cast<uint4 *>(o + col + 8) = make_uint4(z[4], z[5], z[6], z[7]);
-          }
-        }
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&b_oempty));
     }
   } else if (warp >= kDaS && seq >= 0) {
     // the state: row r = dk index, DP / 4 columns from c0 in registers
     constexpr int HC = DP / 4;
     const int r = 32 * (warp % 4) + lane, c0 = (warp - kDaS) / 4 * HC, tid = threadIdx.x - 32 * kDaS;
     float S[HC];
+    const float o1_scale = d.scale;  // bf16: P has the scale already
     const long long slot = d.slot ? d.slot[seq] : seq;
     const float *from = nullptr;
     if (!kState) {
@@ -641,30 +599,37 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&b_s));
     };
-    if (!kState && nc > 0) put_state(0);
-    for (int c = 0; c < nc && ok; c++) {
-      const int s = c % NS;
+    // the dead rows of V and K' of chunk c; false where a wait ran out. dsc: what the state's sum is multiplied by
+    float dsc = 1.f;
+    uint32_t lw[4] = {~0u, ~0u, ~0u, ~0u};
+    auto dead = [&](int m) { return !((word_of(lw, 2 * m + tid / 256) >> (tid / 8 % 32)) & 1); };
+    auto fix_v = [&](int c, const Ring<NS> &rc) {
+      const int s = rc.at;
       const long long t = t0 + (long long)c * kChunk;
       const int n = (int)min((long long)kChunk, t1 - t);
       // 16-byte slots of the tiles, a row's 8 by 8 lanes: row tid / 8, then 64 rows on. A slot stays where it is, so the
       // tiles written here have the swizzle of the one they come from
-      uint32_t lw[4];
-      live_words(d, t, n, lw);
-      auto dead = [&](int m) { return !((word_of(lw, 2 * m + tid / 256) >> (tid / 8 % 32)) & 1); };
-      if (n < kChunk || d.live) {
-        if (!(ok = wait(b_vfull[s], (c / NS) & 1, BNNK_ERR_EPI_WAIT))) break;
+      const bool whole = n == kChunk && !d.live;
+      if (!whole) {
+        live_words(d, t, n, lw);
+        if (!(ok = wait(b_vfull[s], rc.parity, BNNK_ERR_EPI_WAIT))) return false;
         const uint32_t zero[4] = {0, 0, 0, 0};
 #pragma unroll 1
         for (int m = 0; m < 2; m++)
           if (dead(m))
             for (int p = 0; p < PN; p++) sts128(base + L::v + s * L::tile + p * L::panel + (tid + 512 * m) * 16, zero);
         fence_async_smem();
+        __syncwarp();
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&b_vfix));
-      if (!(ok = wait(b_kfull[s], (c / NS) & 1, BNNK_ERR_EPI_WAIT))) break;
+      if (lane == 0) mbar_arrive(smem_u32(&b_vfix[s]));
+      return true;
+    };
+    auto make_kp = [&](int c, const Ring<NS> &rc) {
+      const int s = rc.at;
+      const int n = (int)min((long long)kChunk, t1 - (t0 + (long long)c * kChunk));
+      if (!(ok = wait(b_kfull[s], rc.parity, BNNK_ERR_EPI_WAIT))) return false;
       int from_j = n - 1;  // the token whose decay counts as 1
-      float ksc = 1.f, dsc = 1.f;
+      float ksc = 1.f;
       auto load = [&](int m, int p, uint32_t (&x)[4]) {
         asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                      : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
@@ -685,15 +650,14 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
                 mx = fmaxf(mx, fmaxf(fabsf(f.x), fabsf(f.y)));
               }
             }
-        from_j = lw[3] ? 127 - __clz(lw[3]) : lw[2] ? 95 - __clz(lw[2]) : lw[1] ? 63 - __clz(lw[1]) : lw[0] ? 31 - __clz(lw[0]) : 0;
-        ksc = scale_to_f16(role_max(mx), dsc);
-        if (!ok) break;
-        dsc *= pw[n - 1 - from_j];
+        if (n < kChunk || d.live)
+          from_j = lw[3] ? 127 - __clz(lw[3]) : lw[2] ? 95 - __clz(lw[2]) : lw[1] ? 63 - __clz(lw[1]) : lw[0] ? 31 - __clz(lw[0]) : 0;
+        float inv;
+        ksc = scale_to_f16(role_max(mx), inv);
+        if (!ok) return false;
+        if (tid == 0) s_dsc[c & 1] = inv * pw[n - 1 - from_j];
       }
-      if (L::in_place && !kState) {  // K has been read by the products of all its q heads
-        for (int g = 0; g < G && ok; g++) ok = wait(b_qk[0], (c * G + g) & 1, BNNK_ERR_EPI_WAIT);
-        if (!ok) break;
-      }
+      if (L::in_place && !kState && !(ok = wait(b_qk[0], (c * G + G - 1) & 1, BNNK_ERR_EPI_WAIT))) return false;
 #pragma unroll 1
       for (int m = 0; m < 2; m++) {
         const int row = tid / 8 + 64 * m;
@@ -717,10 +681,98 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
       }
       fence_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&b_kp));
+      if (lane == 0) mbar_arrive(smem_u32(&b_kp[s]));
+      return true;
+    };
+    // o of unit u: this warp's 32 rows and quarter of the columns, through its own part of shared memory, so that a store
+    // covers whole 32-byte sectors of few rows (16 bytes of 32 rows a store cost 3300 cycles a chunk of 128 x 128)
+    auto put_o = [&](int c, int g, int u) {
+      const long long t = t0 + (long long)c * kChunk;
+      constexpr int LR = HC / 8, RI = 32 / LR;  // lanes a row, rows a store
+      const int n = (int)min((long long)kChunk, t1 - t) - 32 * (warp % 4);  // this warp's rows inside the segment
+      uint32_t alive = ~0u;
+      if (d.live) alive = __ballot_sync(0xffffffffu, lane < n && d.live[t + r]);
+      if (!(ok = wait(b_o, u & 1, BNNK_ERR_EPI_WAIT))) return false;
+      tc_fence_after();
+      float c1 = o1_scale * pw[r + 1], c2 = 1.f;
+      if constexpr (T == 1) {
+        c1 *= s_inv[c & 1];
+        c2 = d.scale * s_pinv[u % L::scales][r];
+      }
+      const uint32_t tq = tmem + c0 + ((uint32_t)((warp % 4) * 32) << 16);
+      // in K''s place: the slots that this warp writes of K', so that no other warp's come in between
+      auto slot_at = [&](int row, int k) {
+        const uint32_t in = L::in_place ? (row / 16) * L::panel + (row / 8 % 2) * 8192 + (warp - kDaS) * 512 + row % 8 * 64
+                                        : (warp - kDaS) * 32 * HC * 2 + row * HC * 2;
+        return base + L::o + in + ((k ^ (row * LR / 8 % LR)) << 4);  // turned by the rows that share 128 bytes of banks
+      };
+#pragma unroll
+      for (int j = 0; j < HC; j += 8) {
+        uint32_t x[8], y[8], z[4];
+        tmem_ld8(tq + L::t_o1 + j, x);
+        tmem_ld8(tq + L::t_o2 + j, y);
+        tmem_wait_ld(x, y);
+        if (j + 8 == HC) {  // the last read: the next unit's products may be written
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&b_oempty));
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const float y0 = __uint_as_float(y[2 * e]), y1 = __uint_as_float(y[2 * e + 1]);
+          z[e] = pack2f<T>(fmaf(c1, __uint_as_float(x[2 * e]), T == 1 ? c2 * y0 : y0),
+                           fmaf(c1, __uint_as_float(x[2 * e + 1]), T == 1 ? c2 * y1 : y1));
+        }
+        sts128(slot_at(lane, j / 8), z);
+      }
+      __syncwarp();
+      const int part = lane % LR;
+      elem_t<T> *o = (elem_t<T> *)d.o + (t + 32 * (warp % 4) + lane / LR) * d.ots + (long long)(hk * G + g) * d.dv + c0 + part * 8;
+#pragma unroll
+      for (int k = 0; k < 32; k += RI) {
+        const int row = k + lane / LR;
+        uint4 z;
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(z.x), "=r"(z.y), "=r"(z.z), "=r"(z.w)
+                     : "r"(slot_at(row, part))
+                     : "memory");
+        if (!((alive >> row) & 1)) z = make_uint4(0, 0, 0, 0);
+        if (row < n && c0 + part * 8 < d.dv) *reinterpret_cast<uint4 *>(o + (long long)k * d.ots) = z;
+      }
+      __syncwarp();  // before the next unit's values go there
+      return true;
+    };
+    // Order for a chunk: o of all but its last unit, K', then the state, o of the last unit. K' waits for the chunk's
+    // last QK where it goes in K's place; elsewhere it is formed a chunk ahead, while the products of this one run.
+    if (!kState && nc > 0) put_state(0);
+    Ring<NS> rc;
+    if (!L::in_place && nc > 0 && ok && fix_v(0, rc) && make_kp(0, rc)) rc.next();
+    for (int c = 0, u = 0; c < nc && ok; c++, u++) {
+      const int n = (int)min((long long)kChunk, t1 - (t0 + (long long)c * kChunk));
+      if (L::in_place) {
+        if (!fix_v(c, rc)) break;
+        if (!kState) {
+          bool more = true;
+          for (int g = 0; g < G - 1 && more; g++, u++) more = put_o(c, g, u);
+          if (!more) break;
+        }
+        if (!make_kp(c, rc)) break;
+        rc.next();
+      } else {
+        if (c + 1 < nc) {
+          if (!fix_v(c + 1, rc) || !make_kp(c + 1, rc)) break;
+          rc.next();
+        }
+        if (!kState) {
+          bool more = true;
+          for (int g = 0; g < G - 1 && more; g++, u++) more = put_o(c, g, u);
+          if (!more) break;
+        }
+      }
       if (!(ok = wait(b_ds, c & 1, BNNK_ERR_EPI_WAIT))) break;
       tc_fence_after();
       const float dec = pw[n];
+      if constexpr (T == 1) dsc = s_dsc[c & 1];
       const uint32_t td = tmem + L::t_ds + c0 + ((uint32_t)((warp % 4) * 32) << 16);
 #pragma unroll
       for (int j = 0; j < HC; j += 16) {
@@ -735,6 +787,7 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
       }
       tc_fence_before();
       if (!kState && c + 1 < nc) put_state(c + 1);
+      if (!kState && ok && !put_o(c, G - 1, u)) break;
     }
     if (ok) {
       float *to = nullptr;

@@ -82,6 +82,9 @@ __device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[16], uint32_t (&q)[16
                : BNN_P4(r, 0), BNN_P4(r, 4), BNN_P4(r, 8), BNN_P4(r, 12), BNN_P4(q, 0), BNN_P4(q, 4), BNN_P4(q, 8),
                  BNN_P4(q, 12)::"memory");
 }
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[8], uint32_t (&q)[8]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : BNN_P4(r, 0), BNN_P4(r, 4), BNN_P4(q, 0), BNN_P4(q, 4)::"memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
