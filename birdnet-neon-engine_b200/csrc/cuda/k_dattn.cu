@@ -157,8 +157,8 @@ __global__ void __launch_bounds__(256) k_dattn_rec(const DattnArgs a) {
 //
 // One CTA per (segment of a sequence, k/v head) walks the segment's chunks, and for each the G q heads of the group
 // ("unit" u = (chunk, q head)). Roles: warp 0 MMA issue, warp 1 TMA, 8 warps turn QK into P (in place in TMEM, as the A
-// operand of the last product), 16 warps hold S in registers, form K' and the S operand, and join O1 and O2 into o. S in
-// registers stays fp32: lambda^n S + DS, once a chunk. The roles' loops are rolled: unrolled, their code
+// operand of the last product), 16 warps hold S in registers, form K' and the S operand; one of the two joins O1 and O2
+// into o. S in registers stays fp32: lambda^n S + DS, once a chunk. The roles' loops are rolled: unrolled, their code
 // did not stay in the instruction cache together and a unit took twice as long. The issuing warp stays converged
 // (elect.sync): from one lane's branch each tcgen05.mma took 70 cycles to issue, more than a 128 x 64 x 16 product.
 // A masked token, and a row past the segment's end, has its k and v rows taken as zero (K' zero, V zeroed in shared
@@ -217,26 +217,26 @@ __device__ bool find_segment(const DaArgs &a, int s, int &seq, int &part, long l
 }
 
 // Shared memory and TMEM. DP 128: one stage of Q, K, V, and the first part of K' in K's place (it waits for QK to have
-// read K); DP 64: two stages, two QK / P regions, two sets of K', formed a chunk ahead.
+// read K); DP 64: two stages (three of K), two QK / P regions, two sets of K', formed a chunk ahead.
 template <int T, int DP>
 struct DaLayout {
   static constexpr int parts = T == 2 ? 3 : 2;      // of K'
   static constexpr bool in_place = DP == 128;
-  static constexpr int stages = DP == 64 ? 2 : 1;   // Q, K, V tiles in flight, sets of K'
+  static constexpr int o_warps = in_place ? 8 : 16;  // that store o: P's, which wait for the next K there, or the state's
+  static constexpr int stages = DP == 64 ? 2 : 1;    // Q and V tiles in flight, sets of K'
+  static constexpr int k_stages = DP == 64 ? 3 : 1;  // K tiles: the last to be free again (after DS) and the first needed
   static constexpr int qk_bufs = DP == 64 ? 2 : 1;  // QK / P regions in TMEM
   static constexpr uint32_t panel = kChunk * 128;   // 64 columns of a 128-row tile
   static constexpr uint32_t tile = kChunk * DP * 2;
   static constexpr uint32_t s_panel = DP * 128, s_tile = DP * DP * 2;
-  static constexpr uint32_t q = 0, k = q + stages * tile, v = k + stages * tile, kp = v + stages * tile,
-                            st = kp + (in_place ? parts - 1 : stages * parts) * tile,
-                            o = in_place ? kp : st + 2 * s_tile,  // o on its way out: in place of K''s second part, or apart
-                            end = st + 2 * s_tile + (in_place ? 0 : tile);
+  static constexpr uint32_t q = 0, k = q + stages * tile, v = k + k_stages * tile, kp = v + stages * tile,
+                            st = kp + (in_place ? parts - 1 : stages * parts) * tile, end = st + 2 * s_tile;
   static constexpr uint32_t t_qk = 0, t_o1 = qk_bufs * 128, t_o2 = t_o1 + DP, t_ds = t_o2 + DP;  // TMEM columns
   static constexpr size_t smem = end + 1024;
   static constexpr int scales = T == 1 ? (qk_bufs == 2 ? 4 : 2) : 1;  // P row scales: units until o has read them
-  // part x of K' for stage s
+  // part x of K' of set s
   static __device__ __forceinline__ uint32_t kpart(uint32_t base, int s, int x) {
-    return in_place ? (x ? base + kp + (x - 1) * tile : base + k + s * tile) : base + kp + (s * parts + x) * tile;
+    return in_place ? (x ? base + kp + (x - 1) * tile : base + k) : base + kp + (s * parts + x) * tile;
   }
 };
 
@@ -289,10 +289,10 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
                                                               const __grid_constant__ CUtensorMap mk,
                                                               const __grid_constant__ CUtensorMap mv, const DaArgs a) {
   using L = DaLayout<T, DP>;
-  constexpr int NS = L::stages, NB = L::qk_bufs, PN = DP / 64;
+  constexpr int NS = L::stages, NK = L::k_stages, NB = L::qk_bufs, PN = DP / 64;
   extern __shared__ uint8_t dsmem[];
-  __shared__ __align__(8) unsigned long long b_qfull[NS], b_kfull[NS], b_vfull[NS], b_qempty[NS], b_kempty[NS],
-      b_vempty[NS], b_qk[NB], b_p[NB], b_s, b_vfix[NS], b_kp[NS], b_ds, b_o, b_oempty, b_max, b_row[4];
+  __shared__ __align__(8) unsigned long long b_qfull[NS], b_kfull[NK], b_vfull[NS], b_qempty[NS], b_kempty[NK],
+      b_vempty[NS], b_qk[NB], b_p[NB], b_s, b_vfix[NS], b_kp[NS], b_kq, b_ds, b_o, b_oempty, b_max, b_row[4];
   __shared__ uint32_t tmem_s;
   __shared__ volatile int abort_s;
   __shared__ float s_pow[32 + kDattnPow];  // s_pow[32 + x] = lambda^x, 0 for x < 0
@@ -316,13 +316,14 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
       s_seg[1] = part;
       s_seg[2] = last;
       for (int s = 0; s < NS; s++) {
-        mbar_init(smem_u32(&b_qfull[s]), 1); mbar_init(smem_u32(&b_kfull[s]), 1); mbar_init(smem_u32(&b_vfull[s]), 1);
-        mbar_init(smem_u32(&b_qempty[s]), 1); mbar_init(smem_u32(&b_kempty[s]), 1); mbar_init(smem_u32(&b_vempty[s]), 1);
+        mbar_init(smem_u32(&b_qfull[s]), 1); mbar_init(smem_u32(&b_vfull[s]), 1);
+        mbar_init(smem_u32(&b_qempty[s]), 1); mbar_init(smem_u32(&b_vempty[s]), 1);
         mbar_init(smem_u32(&b_vfix[s]), 16); mbar_init(smem_u32(&b_kp[s]), 16);
       }
+      for (int s = 0; s < NK; s++) { mbar_init(smem_u32(&b_kfull[s]), 1); mbar_init(smem_u32(&b_kempty[s]), 1); }
       for (int b = 0; b < NB; b++) { mbar_init(smem_u32(&b_qk[b]), 1); mbar_init(smem_u32(&b_p[b]), 8); }
       mbar_init(smem_u32(&b_s), 16); mbar_init(smem_u32(&b_ds), 1); mbar_init(smem_u32(&b_o), 1);
-      mbar_init(smem_u32(&b_oempty), 16);
+      mbar_init(smem_u32(&b_oempty), L::o_warps); mbar_init(smem_u32(&b_kq), 1);
       mbar_init(smem_u32(&b_max), 16);
       for (int w = 0; w < 4; w++) mbar_init(smem_u32(&b_row[w]), 2);
       abort_s = 0;
@@ -357,38 +358,94 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
     return ok;
   };
 
+  // o of unit u: this warp's 32 rows and CN columns from c0, 16 at a time. Two neighbouring lanes exchange halves of
+  // their rows, so that a store covers whole sectors of 32 bytes: with 16 bytes of 32 rows a store it took 3300 cycles
+  // a chunk of 128 x 128
+  auto put_o = [&](int c, int g, int u, int c0) {
+    constexpr int CN = DP * 4 / L::o_warps;
+    const int r = 32 * (warp % 4) + lane;
+    const long long t = t0 + (long long)c * kChunk;
+    const int n = (int)min((long long)kChunk, t1 - t) - 32 * (warp % 4);  // this warp's rows inside the segment
+    uint32_t alive = ~0u;
+    if (d.live) alive = __ballot_sync(0xffffffffu, lane < n && d.live[t + r]);
+    if (!wait(b_o, u & 1, BNNK_ERR_EPI_WAIT)) return false;
+    tc_fence_after();
+    float c1 = d.scale * pw[r + 1], c2 = 1.f;  // bf16: P has the scale already
+    if constexpr (T == 1) {
+      c1 *= s_inv[c & 1];
+      c2 = d.scale * s_pinv[u % L::scales][r];
+    }
+    const uint32_t tq = tmem + c0 + ((uint32_t)((warp % 4) * 32) << 16);
+    const int half = lane & 1, row0 = lane - half;
+    elem_t<T> *o = (elem_t<T> *)d.o + (t + 32 * (warp % 4) + row0) * d.ots + (long long)(hk * G + g) * d.dv + c0 + half * 8;
+#pragma unroll
+    for (int j = 0; j < CN; j += 16) {
+      uint32_t z[2][4];
+#pragma unroll
+      for (int k = 0; k < 2; k++) {
+        uint32_t x[8], y[8];
+        tmem_ld8(tq + L::t_o1 + j + 8 * k, x);
+        tmem_ld8(tq + L::t_o2 + j + 8 * k, y);
+        tmem_wait_ld(x, y);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const float y0 = __uint_as_float(y[2 * e]), y1 = __uint_as_float(y[2 * e + 1]);
+          z[k][e] = pack2f<T>(fmaf(c1, __uint_as_float(x[2 * e]), T == 1 ? c2 * y0 : y0),
+                              fmaf(c1, __uint_as_float(x[2 * e + 1]), T == 1 ? c2 * y1 : y1));
+        }
+      }
+      if (j + 16 == CN) {  // the last read: the next unit's products may be written
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&b_oempty));
+      }
+#pragma unroll
+      for (int e = 0; e < 4; e++) {  // half k of this lane's row <-> this lane's half of row row0 + k
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, half ? z[0][e] : z[1][e], 1);
+        if (half) z[0][e] = got;
+        else z[1][e] = got;
+      }
+#pragma unroll
+      for (int k = 0; k < 2; k++)
+        if (row0 + k < n && c0 + j + half * 8 < d.dv)
+          *reinterpret_cast<uint4 *>(o + k * d.ots + j) =
+              (alive >> (row0 + k)) & 1 ? make_uint4(z[k][0], z[k][1], z[k][2], z[k][3]) : make_uint4(0, 0, 0, 0);
+    }
+    return true;
+  };
   if (warp == 1) {  // TMA
-    Ring<NS> rq, rc;  // tiles of Q (one a unit), of K and V (one a chunk)
+    Ring<NS> rq, rc;  // tiles of Q (one a unit), of V (one a chunk)
+    Ring<NK> rk;      // of K
     bool ok = true;
     for (int c = 0; c < nc && ok; c++) {
       const int t = (int)(t0 + (long long)c * kChunk), s = rc.at;
-      for (int g = 0; g < G && ok; g++) {
-        if (!kState) {
-          if (rq.used && !(ok = wait(b_qempty[rq.at], rq.parity ^ 1, BNNK_ERR_TMA_WAIT))) break;
-          if (elect_one()) {
-            mbar_expect_tx(smem_u32(&b_qfull[rq.at]), L::tile);
-#pragma unroll
-            for (int p = 0; p < PN; p++)
-              tma_load_3d(base + L::q + rq.at * L::tile + p * L::panel, &mq, smem_u32(&b_qfull[rq.at]), 64 * p, hk * G + g, t);
-          }
-          rq.next();
-        }
-        if (g) continue;
-        if (rc.used && !(ok = wait(b_kempty[s], rc.parity ^ 1, BNNK_ERR_TMA_WAIT))) break;
+      auto load_q = [&](int g) {
+        if (rq.used && !(ok = wait(b_qempty[rq.at], rq.parity ^ 1, BNNK_ERR_TMA_WAIT))) return;
         if (elect_one()) {
-          mbar_expect_tx(smem_u32(&b_kfull[s]), L::tile);
+          mbar_expect_tx(smem_u32(&b_qfull[rq.at]), L::tile);
 #pragma unroll
           for (int p = 0; p < PN; p++)
-            tma_load_3d(base + L::k + s * L::tile + p * L::panel, &mk, smem_u32(&b_kfull[s]), 64 * p, hk, t);
+            tma_load_3d(base + L::q + rq.at * L::tile + p * L::panel, &mq, smem_u32(&b_qfull[rq.at]), 64 * p, hk * G + g, t);
         }
-        if (rc.used && !(ok = wait(b_vempty[s], rc.parity ^ 1, BNNK_ERR_TMA_WAIT))) break;
-        if (elect_one()) {
-          mbar_expect_tx(smem_u32(&b_vfull[s]), L::tile);
+        rq.next();
+      };
+      if (!kState) load_q(0);  // in the order in which the tiles are free again
+      if (!ok || (rk.used && !(ok = wait(b_kempty[rk.at], rk.parity ^ 1, BNNK_ERR_TMA_WAIT)))) break;
+      if (elect_one()) {
+        mbar_expect_tx(smem_u32(&b_kfull[rk.at]), L::tile);
 #pragma unroll
-          for (int p = 0; p < PN; p++)
-            tma_load_3d(base + L::v + s * L::tile + p * L::panel, &mv, smem_u32(&b_vfull[s]), 64 * p, hk, t);
-        }
+        for (int p = 0; p < PN; p++)
+          tma_load_3d(base + L::k + rk.at * L::tile + p * L::panel, &mk, smem_u32(&b_kfull[rk.at]), 64 * p, hk, t);
       }
+      rk.next();
+      if (!ok || (rc.used && !(ok = wait(b_vempty[s], rc.parity ^ 1, BNNK_ERR_TMA_WAIT)))) break;
+      if (elect_one()) {
+        mbar_expect_tx(smem_u32(&b_vfull[s]), L::tile);
+#pragma unroll
+        for (int p = 0; p < PN; p++)
+          tma_load_3d(base + L::v + s * L::tile + p * L::panel, &mv, smem_u32(&b_vfull[s]), 64 * p, hk, t);
+      }
+      for (int g = 1; g < G && ok; g++) load_q(g);
       rc.next();
     }
   } else if (warp == 0) {  // MMA (the warp of the first TMEM quarter, whose scheduler has the fewest P blocks)
@@ -399,7 +456,8 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
     // MN-major steps 16 rows of 128 bytes
     auto kstep = [](int kk) { return (uint64_t)(((kk / 4) * L::panel + (kk % 4) * 32) >> 4); };
     constexpr uint64_t mnstep = 2048 >> 4;
-    Ring<NS> kq, kc, rq, rc;  // the next QK's tiles (kq, kc), this unit's (rq, rc)
+    Ring<NS> kq, rq, rc;  // the next QK's Q tile, this unit's, this chunk's V tile and set of K'
+    Ring<NK> kc, rn;      // the next QK's K tile, this chunk's
     Ring<NB> kb, rb;          // and their QK / P regions
     int kg = 0;
     auto issue_qk = [&]() {
@@ -412,6 +470,7 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
         for (int kk = 0; kk < DP / 16; kk++)
           mma16_ss(tmem + L::t_qk + kb.at * 128, dq + kstep(kk), dk + kstep(kk), i_qk, kk != 0);
         mma_commit(smem_u32(&b_qk[kb.at]));
+        if (L::in_place && kg == G - 1) mma_commit(smem_u32(&b_kq));
       }
       kq.next();
       kb.next();
@@ -424,10 +483,9 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
     for (int u = 0; u < nu && ok; u++) {
       const int s = rc.at;
       const uint64_t dv = smem_desc_mn(base + L::v + s * L::tile, L::panel);
-      if (!kState) {
-        if (NB > 1 && u + 1 < nu && !(ok = issue_qk())) break;
-        if (g == 0 && !(ok = wait(b_s, rk.parity, BNNK_ERR_MMA_WAIT))) break;
-        if (u && !(ok = wait(b_oempty, ru.parity ^ 1, BNNK_ERR_MMA_WAIT))) break;
+      auto issue_qs = [&]() {
+        if (g == 0 && !wait(b_s, rk.parity, BNNK_ERR_MMA_WAIT)) return false;
+        if (u && !wait(b_oempty, ru.parity ^ 1, BNNK_ERR_MMA_WAIT)) return false;
         tc_fence_after();
         const uint64_t dq = smem_desc<128>(base + L::q + rq.at * L::tile), ds = smem_desc_mn(base + L::st, L::s_panel);
         if (elect_one()) {
@@ -439,15 +497,10 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
           mma_commit(smem_u32(&b_qempty[rq.at]));
         }
         rq.next();
-      }
-      if (g == 0) {
-        if (!(ok = wait(b_vfull[s], rc.parity, BNNK_ERR_MMA_WAIT))) break;
-        if (!(ok = wait(b_vfix[s], rc.parity, BNNK_ERR_MMA_WAIT))) break;
-      }
-      const bool last = ++g == G;
-      if (last) {
-        g = 0;
-        if (!(ok = wait(b_kp[s], rc.parity, BNNK_ERR_MMA_WAIT))) break;
+        return true;
+      };
+      auto issue_ds = [&]() {
+        if (!wait(b_kp[s], rc.parity, BNNK_ERR_MMA_WAIT)) return false;
         tc_fence_after();
         const uint64_t dk0 = smem_desc_mn(L::kpart(base, s, 0), L::panel), dk1 = smem_desc_mn(L::kpart(base, s, 1), L::panel);
         if (elect_one()) {
@@ -458,10 +511,25 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
               mma16_ss(tmem + L::t_ds, (part ? dk1 + ((part - 1) * L::tile >> 4) : dk0) + kk * mnstep, dv + kk * mnstep, i_ds,
                        (part | kk) != 0);
           mma_commit(smem_u32(&b_ds));
-          mma_commit(smem_u32(&b_kempty[s]));
+          mma_commit(smem_u32(&b_kempty[rn.at]));
         }
+        rn.next();
+        return true;
+      };
+      const bool last = g == G - 1;
+      if (!kState && NB > 1 && u + 1 < nu && !(ok = issue_qk())) break;
+      if (!kState && !(ok = issue_qs())) break;
+      if (g == 0) {
+        if (!(ok = wait(b_vfull[s], rc.parity, BNNK_ERR_MMA_WAIT))) break;
+        if (!(ok = wait(b_vfix[s], rc.parity, BNNK_ERR_MMA_WAIT))) break;
+      }
+      if (last && !(ok = issue_ds())) break;
+      if (last) {
+        g = 0;
         rk.next();
         rc.next();
+      } else {
+        g++;
       }
       if (!kState) {
         if (!(ok = wait(b_p[rb.at], rb.parity, BNNK_ERR_MMA_WAIT))) break;
@@ -542,13 +610,13 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&b_p[b]));
+      if (L::in_place && !put_o(c, u % G, u, h * (DP / 2))) break;
     }
   } else if (warp >= kDaS && seq >= 0) {
     // the state: row r = dk index, DP / 4 columns from c0 in registers
     constexpr int HC = DP / 4;
     const int r = 32 * (warp % 4) + lane, c0 = (warp - kDaS) / 4 * HC, tid = threadIdx.x - 32 * kDaS;
     float S[HC];
-    const float o1_scale = d.scale;  // bf16: P has the scale already
     const long long slot = d.slot ? d.slot[seq] : seq;
     const float *from = nullptr;
     if (!kState) {
@@ -624,16 +692,16 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
       if (lane == 0) mbar_arrive(smem_u32(&b_vfix[s]));
       return true;
     };
-    auto make_kp = [&](int c, const Ring<NS> &rc) {
+    auto make_kp = [&](int c, const Ring<NS> &rc, const Ring<NK> &rk) {
       const int s = rc.at;
       const int n = (int)min((long long)kChunk, t1 - (t0 + (long long)c * kChunk));
-      if (!(ok = wait(b_kfull[s], rc.parity, BNNK_ERR_EPI_WAIT))) return false;
+      if (!(ok = wait(b_kfull[rk.at], rk.parity, BNNK_ERR_EPI_WAIT))) return false;
       int from_j = n - 1;  // the token whose decay counts as 1
       float ksc = 1.f;
       auto load = [&](int m, int p, uint32_t (&x)[4]) {
         asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                      : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
-                     : "r"(base + L::k + s * L::tile + p * L::panel + (tid + 512 * m) * 16)
+                     : "r"(base + L::k + rk.at * L::tile + p * L::panel + (tid + 512 * m) * 16)
                      : "memory");
       };
       if constexpr (T == 1) {
@@ -657,7 +725,7 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
         if (!ok) return false;
         if (tid == 0) s_dsc[c & 1] = inv * pw[n - 1 - from_j];
       }
-      if (L::in_place && !kState && !(ok = wait(b_qk[0], (c * G + G - 1) & 1, BNNK_ERR_EPI_WAIT))) return false;
+      if (L::in_place && !kState && !(ok = wait(b_kq, c & 1, BNNK_ERR_EPI_WAIT))) return false;
 #pragma unroll 1
       for (int m = 0; m < 2; m++) {
         const int row = tid / 8 + 64 * m;
@@ -684,91 +752,23 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
       if (lane == 0) mbar_arrive(smem_u32(&b_kp[s]));
       return true;
     };
-    // o of unit u: this warp's 32 rows and quarter of the columns, through its own part of shared memory, so that a store
-    // covers whole 32-byte sectors of few rows (16 bytes of 32 rows a store cost 3300 cycles a chunk of 128 x 128)
-    auto put_o = [&](int c, int g, int u) {
-      const long long t = t0 + (long long)c * kChunk;
-      constexpr int LR = HC / 8, RI = 32 / LR;  // lanes a row, rows a store
-      const int n = (int)min((long long)kChunk, t1 - t) - 32 * (warp % 4);  // this warp's rows inside the segment
-      uint32_t alive = ~0u;
-      if (d.live) alive = __ballot_sync(0xffffffffu, lane < n && d.live[t + r]);
-      if (!(ok = wait(b_o, u & 1, BNNK_ERR_EPI_WAIT))) return false;
-      tc_fence_after();
-      float c1 = o1_scale * pw[r + 1], c2 = 1.f;
-      if constexpr (T == 1) {
-        c1 *= s_inv[c & 1];
-        c2 = d.scale * s_pinv[u % L::scales][r];
-      }
-      const uint32_t tq = tmem + c0 + ((uint32_t)((warp % 4) * 32) << 16);
-      // in K''s place: the slots that this warp writes of K', so that no other warp's come in between
-      auto slot_at = [&](int row, int k) {
-        const uint32_t in = L::in_place ? (row / 16) * L::panel + (row / 8 % 2) * 8192 + (warp - kDaS) * 512 + row % 8 * 64
-                                        : (warp - kDaS) * 32 * HC * 2 + row * HC * 2;
-        return base + L::o + in + ((k ^ (row * LR / 8 % LR)) << 4);  // turned by the rows that share 128 bytes of banks
-      };
-#pragma unroll
-      for (int j = 0; j < HC; j += 8) {
-        uint32_t x[8], y[8], z[4];
-        tmem_ld8(tq + L::t_o1 + j, x);
-        tmem_ld8(tq + L::t_o2 + j, y);
-        tmem_wait_ld(x, y);
-        if (j + 8 == HC) {  // the last read: the next unit's products may be written
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(&b_oempty));
-        }
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const float y0 = __uint_as_float(y[2 * e]), y1 = __uint_as_float(y[2 * e + 1]);
-          z[e] = pack2f<T>(fmaf(c1, __uint_as_float(x[2 * e]), T == 1 ? c2 * y0 : y0),
-                           fmaf(c1, __uint_as_float(x[2 * e + 1]), T == 1 ? c2 * y1 : y1));
-        }
-        sts128(slot_at(lane, j / 8), z);
-      }
-      __syncwarp();
-      const int part = lane % LR;
-      elem_t<T> *o = (elem_t<T> *)d.o + (t + 32 * (warp % 4) + lane / LR) * d.ots + (long long)(hk * G + g) * d.dv + c0 + part * 8;
-#pragma unroll
-      for (int k = 0; k < 32; k += RI) {
-        const int row = k + lane / LR;
-        uint4 z;
-        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                     : "=r"(z.x), "=r"(z.y), "=r"(z.z), "=r"(z.w)
-                     : "r"(slot_at(row, part))
-                     : "memory");
-        if (!((alive >> row) & 1)) z = make_uint4(0, 0, 0, 0);
-        if (row < n && c0 + part * 8 < d.dv) *reinterpret_cast<uint4 *>(o + (long long)k * d.ots) = z;
-      }
-      __syncwarp();  // before the next unit's values go there
-      return true;
-    };
-    // Order for a chunk: o of all but its last unit, K', then the state, o of the last unit. K' waits for the chunk's
-    // last QK where it goes in K's place; elsewhere it is formed a chunk ahead, while the products of this one run.
+    // K' in K's place waits for the chunk's last QK; else it is formed a chunk ahead, while the products of this one run
     if (!kState && nc > 0) put_state(0);
     Ring<NS> rc;
-    if (!L::in_place && nc > 0 && ok && fix_v(0, rc) && make_kp(0, rc)) rc.next();
-    for (int c = 0, u = 0; c < nc && ok; c++, u++) {
+    Ring<NK> rk;
+    auto next_kp = [&](int c) {
+      if (!fix_v(c, rc) || !make_kp(c, rc, rk)) return false;
+      rc.next();
+      rk.next();
+      return true;
+    };
+    if (!L::in_place && nc > 0 && ok) next_kp(0);
+    for (int c = 0, u = 0; c < nc && ok; c++) {
       const int n = (int)min((long long)kChunk, t1 - (t0 + (long long)c * kChunk));
-      if (L::in_place) {
-        if (!fix_v(c, rc)) break;
-        if (!kState) {
-          bool more = true;
-          for (int g = 0; g < G - 1 && more; g++, u++) more = put_o(c, g, u);
-          if (!more) break;
-        }
-        if (!make_kp(c, rc)) break;
-        rc.next();
-      } else {
-        if (c + 1 < nc) {
-          if (!fix_v(c + 1, rc) || !make_kp(c + 1, rc)) break;
-          rc.next();
-        }
-        if (!kState) {
-          bool more = true;
-          for (int g = 0; g < G - 1 && more; g++, u++) more = put_o(c, g, u);
-          if (!more) break;
-        }
-      }
+      if (L::in_place ? !next_kp(c) : c + 1 < nc && !next_kp(c + 1)) break;
+      if (!L::in_place && !kState)
+        for (int g = 0; g < G - 1 && ok; g++) ok = put_o(c, g, u++, c0);
+      if (!ok) break;
       if (!(ok = wait(b_ds, c & 1, BNNK_ERR_EPI_WAIT))) break;
       tc_fence_after();
       const float dec = pw[n];
@@ -786,8 +786,9 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
         }
       }
       tc_fence_before();
-      if (!kState && c + 1 < nc) put_state(c + 1);
-      if (!kState && ok && !put_o(c, G - 1, u)) break;
+      if (kState) continue;
+      if (c + 1 < nc) put_state(c + 1);  // the S operand's last reader, the chunk's last O1, comes before DS
+      if (!L::in_place && ok) ok = put_o(c, G - 1, u++, c0);
     }
     if (ok) {
       float *to = nullptr;
