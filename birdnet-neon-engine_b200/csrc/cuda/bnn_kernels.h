@@ -328,9 +328,10 @@ typedef struct {
 int bnnk_norm_gate(const bnnk_norm_gate_args *a, bnn_stream_t st);
 
 /* linear attention with a decay per k/v head over n sequences: tokens cu[i] .. cu[i + 1] (cu NULL: token i), states
- * s0 -> s1 [slot[i]] (slot NULL: i; negative: from zero, not stored) [Hk][dk][dv]; pow [Hk][kDattnPow] holds
- * lambda^0 .. lambda^128. type 1 or 2; dk, dv multiples of 8 up to 128, 16-byte aligned rows. */
-#define kDattnPow 132
+ * s0 -> s1 [slot[i]] (slot NULL: i; negative: from zero, not stored) [Hk][dk][dv]; pow [Hk][kDattnPow] is the
+ * heads' table. type 1 or 2; dk, dv multiples of 8 up to 128, 16-byte aligned rows. */
+#define kDattnPow 192  /* a head's table: lambda^0 .. lambda^128, and from kDattnPow2 on lambda^(128 2^k), k 0 .. 24, */
+#define kDattnPow2 132 /* as pairs of floats whose sum has twice the significand */
 typedef struct {
   int type, n, H, Hk, dk, dv;
   long long tokens;

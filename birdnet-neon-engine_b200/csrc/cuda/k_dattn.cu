@@ -216,27 +216,28 @@ __device__ bool find_segment(const DaArgs &a, int s, int &seq, int &part, long l
   return false;
 }
 
-// Shared memory and TMEM. DP 128: one stage of Q, K, V, and the first part of K' in K's place (it waits for QK to have
+// Shared memory and TMEM. A pass for the state alone has no Q and no S operand. Else, DP 128: one stage of Q, K, V, and the first part of K' in K's place (it waits for QK to have
 // read K); DP 64: two stages (three of K), two QK / P regions, two sets of K', formed a chunk ahead.
-template <int T, int DP>
+template <int T, int DP, bool kState>
 struct DaLayout {
   static constexpr int parts = T == 2 ? 3 : 2;      // of K'
-  static constexpr bool in_place = DP == 128;
+  static constexpr bool in_place = DP == 128 && !kState;
   static constexpr int o_warps = in_place ? 8 : 16;  // that store o: P's, which wait for the next K there, or the state's
-  static constexpr int stages = DP == 64 ? 2 : 1;    // Q and V tiles in flight, sets of K'
-  static constexpr int k_stages = DP == 64 ? 3 : 1;  // K tiles: the last to be free again (after DS) and the first needed
+  static constexpr int stages = in_place ? 1 : 2;    // Q and V tiles in flight
+  static constexpr int kp_sets = DP == 64 ? 2 : 1;   // sets of K': with two it is formed a chunk ahead
+  static constexpr int k_stages = DP == 64 ? 3 : stages;  // K tiles: the last to be free again (after DS) and the first needed
   static constexpr int qk_bufs = DP == 64 ? 2 : 1;  // QK / P regions in TMEM
   static constexpr uint32_t panel = kChunk * 128;   // 64 columns of a 128-row tile
   static constexpr uint32_t tile = kChunk * DP * 2;
   static constexpr uint32_t s_panel = DP * 128, s_tile = DP * DP * 2;
-  static constexpr uint32_t q = 0, k = q + stages * tile, v = k + k_stages * tile, kp = v + stages * tile,
-                            st = kp + (in_place ? parts - 1 : stages * parts) * tile, end = st + 2 * s_tile;
+  static constexpr uint32_t q = 0, k = q + (kState ? 0 : stages * tile), v = k + k_stages * tile, kp = v + stages * tile,
+                            st = kp + (in_place ? parts - 1 : kp_sets * parts) * tile, end = st + (kState ? 0 : 2 * s_tile);
   static constexpr uint32_t t_qk = 0, t_o1 = qk_bufs * 128, t_o2 = t_o1 + DP, t_ds = t_o2 + DP;  // TMEM columns
-  static constexpr size_t smem = end + 1024;
+  static constexpr size_t smem = end + 1024 + (kState && DP == 64 ? panel : 0);  // the last part's second panel is read, not used
   static constexpr int scales = T == 1 ? (qk_bufs == 2 ? 4 : 2) : 1;  // P row scales: units until o has read them
   // part x of K' of set s
   static __device__ __forceinline__ uint32_t kpart(uint32_t base, int s, int x) {
-    return in_place ? (x ? base + kp + (x - 1) * tile : base + k) : base + kp + (s * parts + x) * tile;
+    return in_place ? (x ? base + kp + (x - 1) * tile : base + k) : base + kp + (s % kp_sets * parts + x) * tile;
   }
 };
 
@@ -288,14 +289,14 @@ template <int T, int DP, bool kState>
 __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_constant__ CUtensorMap mq,
                                                               const __grid_constant__ CUtensorMap mk,
                                                               const __grid_constant__ CUtensorMap mv, const DaArgs a) {
-  using L = DaLayout<T, DP>;
+  using L = DaLayout<T, DP, kState>;
   constexpr int NS = L::stages, NK = L::k_stages, NB = L::qk_bufs, PN = DP / 64;
   extern __shared__ uint8_t dsmem[];
   __shared__ __align__(8) unsigned long long b_qfull[NS], b_kfull[NK], b_vfull[NS], b_qempty[NS], b_kempty[NK],
       b_vempty[NS], b_qk[NB], b_p[NB], b_s, b_vfix[NS], b_kp[NS], b_kq, b_ds, b_o, b_oempty, b_max, b_row[4];
   __shared__ uint32_t tmem_s;
   __shared__ volatile int abort_s;
-  __shared__ float s_pow[32 + kDattnPow];  // s_pow[32 + x] = lambda^x, 0 for x < 0
+  __shared__ float s_pow[32 + 129];  // s_pow[32 + x] = lambda^x, 0 for x < 0
   __shared__ long long s_range[2];
   __shared__ int s_seg[3];
   __shared__ float s_max[2][16], s_inv[2], s_dsc[2];  // fp16: the state warps' maxima, scales of S and of its sums by chunk
@@ -334,7 +335,7 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_s)), "r"(512));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   } else if (warp == 2) {
-    for (int x = lane; x < 32 + kDattnPow; x += 32) s_pow[x] = x < 32 ? 0.f : d.pow[hk * kDattnPow + x - 32];
+    for (int x = lane; x < 32 + 129; x += 32) s_pow[x] = x < 32 ? 0.f : d.pow[hk * kDattnPow + x - 32];
   }
   tc_fence_before();
   __syncthreads();
@@ -725,7 +726,7 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
         if (!ok) return false;
         if (tid == 0) s_dsc[c & 1] = inv * pw[n - 1 - from_j];
       }
-      if (L::in_place && !kState && !(ok = wait(b_kq, c & 1, BNNK_ERR_EPI_WAIT))) return false;
+      if (L::in_place && !(ok = wait(b_kq, c & 1, BNNK_ERR_EPI_WAIT))) return false;
 #pragma unroll 1
       for (int m = 0; m < 2; m++) {
         const int row = tid / 8 + 64 * m;
@@ -752,7 +753,8 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
       if (lane == 0) mbar_arrive(smem_u32(&b_kp[s]));
       return true;
     };
-    // K' in K's place waits for the chunk's last QK; else it is formed a chunk ahead, while the products of this one run
+    // one set of K' is formed when DS has read the last (in K's place also when the chunk's last QK has read K); of two
+    // sets, one is formed a chunk ahead, while the products of this chunk run
     if (!kState && nc > 0) put_state(0);
     Ring<NS> rc;
     Ring<NK> rk;
@@ -762,10 +764,10 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
       rk.next();
       return true;
     };
-    if (!L::in_place && nc > 0 && ok) next_kp(0);
+    if (L::kp_sets == 2 && nc > 0 && ok) next_kp(0);
     for (int c = 0, u = 0; c < nc && ok; c++) {
       const int n = (int)min((long long)kChunk, t1 - (t0 + (long long)c * kChunk));
-      if (L::in_place ? !next_kp(c) : c + 1 < nc && !next_kp(c + 1)) break;
+      if (L::kp_sets == 1 ? !next_kp(c) : c + 1 < nc && !next_kp(c + 1)) break;
       if (!L::in_place && !kState)
         for (int g = 0; g < G - 1 && ok; g++) ok = put_o(c, g, u++, c0);
       if (!ok) break;
@@ -834,7 +836,12 @@ __global__ void __launch_bounds__(256) k_dattn_scan(const DaArgs a) {
     if (threadIdx.x == 0) {
       s_first = before;
       s_parts = min(mine, a.segs - before);  // offsets that do not ascend could ask for more
-      s_dec = (float)pow((double)d.pow[hk * kDattnPow + 1], (double)a.seg_tokens);
+      // lambda^seg_tokens from the table's lambda^(128 2^k), as two floats each
+      double dec = 1.0;
+      const float *pk = d.pow + hk * kDattnPow + kDattnPow2;
+      for (int k = 0, m = a.seg_tokens / kChunk; m; k++, m >>= 1)
+        if (m & 1) dec *= (double)pk[2 * k] + (double)pk[2 * k + 1];
+      s_dec = (float)dec;
     }
   }
   __syncthreads();
@@ -869,13 +876,14 @@ int run_chunk(const DaArgs &a, cudaStream_t st) {
   if (e) return e;
   static SmemAttr attr_s, attr;
   const dim3 grid(a.segs, d.Hk);
-  constexpr size_t smem = DaLayout<T, DP>::smem;
   if (a.seg_tokens) {
+    constexpr size_t smem = DaLayout<T, DP, true>::smem;
     e = attr_s.ensure(k_dattn_chunk<T, DP, true>, smem);
     if (e) return e;
     k_dattn_chunk<T, DP, true><<<grid, kDaThreads, smem, st>>>(mq, mk, mv, a);
     k_dattn_scan<<<dim3((d.dk * d.dv + 255) / 256, d.Hk, d.n), 256, 0, st>>>(a);
   }
+  constexpr size_t smem = DaLayout<T, DP, false>::smem;
   e = attr.ensure(k_dattn_chunk<T, DP, false>, smem);
   if (e) return e;
   k_dattn_chunk<T, DP, false><<<grid, kDaThreads, smem, st>>>(mq, mk, mv, a);

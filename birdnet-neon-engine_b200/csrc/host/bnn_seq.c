@@ -77,8 +77,15 @@ bnn_dattn *bnn_dattn_new(int type, int heads, int kv_heads, int dk, int dv, cons
   const long long states = bad ? 0 : bnnk_dattn_scratch_states(seqs, kv_heads, tokens);
   if (states > 0) bad = dev_alloc("bnn_dattn_new", (void **)&o->scratch, sizeof(float) * states * dk * dv);
   if (!bad) {
-    for (int h = 0; h < kv_heads; h++)
-      for (int i = 0; i < kDattnPow; i++) t[h * kDattnPow + i] = (float)pow((double)decay[h], i);
+    for (int h = 0; h < kv_heads; h++) {
+        float *th = t + h * kDattnPow;
+        for (int i = 0; i <= 128; i++) th[i] = (float)pow((double)decay[h], i);
+        double p = pow((double)decay[h], 128.0);
+        for (int k = 0; k < 25; k++, p *= p) {
+          th[kDattnPow2 + 2 * k] = (float)p;
+          th[kDattnPow2 + 2 * k + 1] = (float)(p - (double)(float)p);
+        }
+    }
     const cudaError_t e = cudaMemcpy(o->pow, t, bytes, cudaMemcpyHostToDevice);
     if (e) { ERR(BNN_ERR_CPU, "bnn_dattn_new: CUDA error %d (%s)", (int)e, cudaGetErrorString(e)); bad = 1; }
   }
