@@ -367,6 +367,7 @@ typedef struct {
   float *hid;
   void *y;
   long long ldy;
+  int *err; /* the device error word of the bounded waits */
 } bnnk_lowrank_args;
 int bnnk_lowrank(const bnnk_lowrank_args *a, bnn_stream_t st);
 

@@ -1,99 +1,610 @@
 // A projection shared by all rows beside low-rank adapters, one of many for each row (bnn_lowrank):
 //
-//   y_r = W x_r + bias + s_a B_a (A_a x_r),   a = slot[r] (none where it is outside [0, slots))
+//   y_r = W x_r + bias + h_r B_a^T,   h_r = s_a A_a x_r,   a = slot[r] (none where it is outside [0, slots))
 //
-// W [N][K], A [slots][rank][K], B [slots][N][rank]; sums in fp32.
+// W [N][K], A [slots][rank][K], B [slots][N][rank]; sums in fp32. Two launches: h (k_lowrank_down), then y in one of two
+// forms by the number of rows; the second launch starts while the first runs (programmatic dependent launch) and waits
+// for h only where it is used, after its sums over K.
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include "bnn_kernels.h"
 #include "seq.cuh"
-#include "tc.cuh"
+#include "smem_attr.cuh"
+#include "sync.cuh"
+#include "tc16.cuh"
 
 namespace bnn {
 namespace {
 
-// s_a A_a x_r: a warp a (row, rank index), hid [rows][rank]
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// the launch before it has ended, its writes are visible
+__device__ __forceinline__ void wait_launch_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// D (16 x 8) += A (16 x 16) B (16 x 8), fp32 sums
 template <int T>
+__device__ __forceinline__ void mma_sync(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  if constexpr (T == 1)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, "
+        "%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint4 ldg16(const void *p, bool in) {
+  return in ? __ldg(reinterpret_cast<const uint4 *>(p)) : make_uint4(0, 0, 0, 0);
+}
+
+// ------------------------------------------------------------------ h = s_a A_a x
+//
+// One CTA per (16 rows, one of the adapters among them): the rows against the adapter's rank rows with warp-level matrix
+// instructions (a product of 16 rows is too small for a 128-row tile, and bound by reading A and x), K in steps of 32
+// dealt to 8 warps, their sums joined in shared memory in warp order. A lane's 16 bytes are 8 consecutive k of a row: the
+// two instructions of a step take them in the same order from both operands, so their k are a permutation of the
+// layout's, the same for both. Rows of other adapters are computed and dropped.
+constexpr int kDownRows = 16;
+
+template <int T, int RT>  // RT: 8-wide tiles of the rank
 __global__ void __launch_bounds__(256) k_lowrank_down(int rows, int K, const elem_t<T> *x, long long ldx,
                                                       const int32_t *slot, int slots, int rank, const elem_t<T> *A,
                                                       const float *scale, float *hid) {
-  const long long u = (long long)blockIdx.x * 8 + threadIdx.x / 32;
-  const int lane = threadIdx.x % 32;
-  if (u >= (long long)rows * rank) return;
-  const long long r = u / rank;
-  const int j = (int)(u % rank), s = slot[r];
-  float sum = 0.f;
-  if (s >= 0 && s < slots) {
-    const elem_t<T> *w = A + ((long long)s * rank + j) * K;
-    for (int k = lane * 8; k < K; k += 256) {
-      float xv[8], wv[8];
-      load_elems<T, 8>(x + r * ldx + k, xv);
-      load_elems<T, 8>(w + k, wv);
-#pragma unroll
-      for (int e = 0; e < 8; e++) sum = fmaf(xv[e], wv[e], sum);
+  __shared__ float red[8][kDownRows][RT * 8 + 1];
+  __shared__ int s_slot[kDownRows];
+  launch_dependents();
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, q = lane % 4;
+  const long long r0 = (long long)blockIdx.x * kDownRows;
+  if (warp == 0) {
+    int s = -1;
+    if (lane < kDownRows && r0 + lane < rows) {
+      s = slot[r0 + lane];
+      if (s >= slots) s = -1;
     }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    sum *= scale ? scale[s] : 1.f;
+    if (lane < kDownRows) s_slot[lane] = s;
   }
-  if (lane == 0) hid[u] = sum;
+  __syncthreads();
+  const int mine = lane < kDownRows ? s_slot[lane] : -1;
+  // the first row of each adapter here
+  const unsigned same = __match_any_sync(0xffffffffu, mine);
+  unsigned first = __ballot_sync(0xffffffffu, mine >= 0 && __ffs(same) - 1 == lane);
+  for (int e = 0; first; first &= first - 1, e++) {
+    if (e % (int)gridDim.y != (int)blockIdx.y) continue;
+    const int s = s_slot[__ffs(first) - 1];
+    const elem_t<T> *a = A + (long long)s * rank * K;
+    const elem_t<T> *x0 = x + (r0 + g) * ldx, *x1 = x0 + 8 * ldx;
+    const bool in0 = r0 + g < rows, in1 = r0 + g + 8 < rows;
+    float acc[RT][4] = {};
+#pragma unroll 4
+    for (int k0 = 32 * warp; k0 < K; k0 += 256) {
+      const int k = k0 + 8 * q;
+      const uint4 xa = ldg16(x0 + k, in0 && k < K), xb = ldg16(x1 + k, in1 && k < K);
+#pragma unroll
+      for (int j = 0; j < RT; j++) {
+        const uint4 b = ldg16(a + (long long)(8 * j + g) * K + k, 8 * j + g < rank && k < K);
+        mma_sync<T>(acc[j], xa.x, xb.x, xa.y, xb.y, b.x, b.y);
+        mma_sync<T>(acc[j], xa.z, xb.z, xa.w, xb.w, b.z, b.w);
+      }
+    }
+    __syncthreads();  // the sums of the adapter before have been read
+#pragma unroll
+    for (int j = 0; j < RT; j++) {
+      red[warp][g][8 * j + 2 * q] = acc[j][0];
+      red[warp][g][8 * j + 2 * q + 1] = acc[j][1];
+      red[warp][g + 8][8 * j + 2 * q] = acc[j][2];
+      red[warp][g + 8][8 * j + 2 * q + 1] = acc[j][3];
+    }
+    __syncthreads();
+    const float f = scale ? scale[s] : 1.f;
+    for (int i = threadIdx.x; i < kDownRows * rank; i += 256) {
+      const int r = i / rank, c = i % rank;
+      if (s_slot[r] != s) continue;
+      float v = 0.f;
+#pragma unroll
+      for (int w = 0; w < 8; w++) v += red[w][r][c];
+      hid[(r0 + r) * rank + c] = f * v;
+    }
+  }
 }
 
-// y: a 64 x 64 tile a CTA, 4 x 4 outputs a thread, K in steps of 16 through shared memory
+// ------------------------------------------------------------------ few rows
+//
+// Bound by reading W (and the adapters' B) once. One CTA per 16 MT rows of W: warp-level matrix instructions with W as
+// the 16-row operand and 8 NT rows of x as the other, K dealt to 8 warps as above, all of a warp's loads independent; the
+// warps' sums are joined in shared memory, then a warp takes 32 neighbouring outputs of one row, and each lane adds its
+// output's rank products with B from the row's adapter (neighbouring outputs' rows of B are neighbours in memory).
+template <int T, int OT, int MT, int NT>
+__global__ void __launch_bounds__(256) k_lowrank_few(const bnnk_lowrank_args p) {
+  extern __shared__ float red[];  // [8][16 MT][8 NT + 1]
+  constexpr int P = 8 * NT + 1;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, q = lane % 4;
+  const int n0 = blockIdx.x * 16 * MT, K = p.K, rank = p.rank;
+  const elem_t<T> *W = (const elem_t<T> *)p.w, *x = (const elem_t<T> *)p.x, *B = (const elem_t<T> *)p.b;
+  // the rows of B that the outputs here need, on their way to L2 while W is read
+  if (p.slot)
+    for (int i = threadIdx.x; i < p.rows * 16 * MT; i += 256) {
+      const int n = n0 + i % (16 * MT), s = p.slot[i / (16 * MT)];
+      if (n < p.N && s >= 0 && s < p.slots) {
+        const elem_t<T> *b = B + ((long long)s * p.N + n) * rank;
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(b));
+        if (rank > 32) asm volatile("prefetch.global.L2 [%0];" ::"l"(b + rank - 1));
+      }
+    }
+  float acc[MT][NT][4] = {};
+#pragma unroll 2
+  for (int k0 = 32 * warp; k0 < K; k0 += 256) {
+    const int k = k0 + 8 * q;
+    uint4 wa[MT], wb[MT];
+#pragma unroll
+    for (int m = 0; m < MT; m++) {
+      const int n = n0 + 16 * m + g;
+      wa[m] = ldg16(W + (long long)n * p.ldw + k, n < p.N && k < K);
+      wb[m] = ldg16(W + (long long)(n + 8) * p.ldw + k, n + 8 < p.N && k < K);
+    }
+#pragma unroll
+    for (int j = 0; j < NT; j++) {
+      const uint4 b = ldg16(x + (8 * j + g) * p.ldx + k, 8 * j + g < p.rows && k < K);
+#pragma unroll
+      for (int m = 0; m < MT; m++) {
+        mma_sync<T>(acc[m][j], wa[m].x, wb[m].x, wa[m].y, wb[m].y, b.x, b.y);
+        mma_sync<T>(acc[m][j], wa[m].z, wb[m].z, wa[m].w, wb[m].w, b.z, b.w);
+      }
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < MT; m++)
+#pragma unroll
+    for (int j = 0; j < NT; j++) {
+      float *r = red + (warp * 16 * MT + 16 * m + g) * P + 8 * j + 2 * q;
+      r[0] = acc[m][j][0];
+      r[1] = acc[m][j][1];
+      r[8 * P] = acc[m][j][2];
+      r[8 * P + 1] = acc[m][j][3];
+    }
+  __syncthreads();
+  if (p.slot) wait_launch_before();
+  for (int i = threadIdx.x; i < p.rows * 16 * MT; i += 256) {
+    const int r = i / (16 * MT), c = i % (16 * MT), n = n0 + c;
+    if (n >= p.N) continue;
+    float v = p.bias ? p.bias[n] : 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; w++) v += red[(w * 16 * MT + c) * P + r];
+    const int s = p.slot ? p.slot[r] : -1;
+    if (s >= 0 && s < p.slots) {
+      const elem_t<T> *b = B + ((long long)s * p.N + n) * rank;
+      const float *h = p.hid + (long long)r * rank;
+      float u = 0.f;
+      for (int e = 0; e < rank; e += 8) {
+        float bv[8];
+        load_elems<T, 8>(b + e, bv);
+        const float4 h0 = *reinterpret_cast<const float4 *>(h + e), h1 = *reinterpret_cast<const float4 *>(h + e + 4);
+        u = fmaf(h0.x, bv[0], u); u = fmaf(h0.y, bv[1], u); u = fmaf(h0.z, bv[2], u); u = fmaf(h0.w, bv[3], u);
+        u = fmaf(h1.x, bv[4], u); u = fmaf(h1.y, bv[5], u); u = fmaf(h1.z, bv[6], u); u = fmaf(h1.w, bv[7], u);
+      }
+      v += u;
+    }
+    ((elem_t<OT> *)p.y)[r * p.ldy + n] = Elem<OT>::put(v);
+  }
+}
+
+// ------------------------------------------------------------------ many rows
+//
+// A tcgen05 GEMM of 128-row tiles, y's accumulators in TMEM, with the adapters as more steps of the sum: for each
+// adapter among the tile's rows (the list that 4 warps make from the rows' slots while W's steps run) the A operand is h
+// in the rows of that adapter and zero in the others, the B operand B_a. h is fp32 and goes as 16-bit parts: three for
+// bf16 (all 24 bits), two for fp16 (22 bits); a row with an |h| past fp16's range is left out of the operand and its
+// products are added in fp32 when y is stored. Slots of 64 / RB adapters share a stage (RB: the rank rounded up to 16, 32
+// or 64, a row of that many bytes swizzled as such).
+//
+// One persistent CTA per SM, column tiles fastest. Warp 0 streams 64-wide steps of x and W into a ring by TMA; warp 1
+// issues the MMAs into one of two accumulators; warps 2 .. 5 make the list and h's operand tiles and load the B_a tiles;
+// warps 6 .. 13 store y: accumulator rows through shared memory, so that a store covers 32 neighbouring words of a row at
+// any row alignment.
+constexpr int kLrThreads = 448;
+constexpr int kLrStages = 8;
+constexpr int kLrPad = 17;  // words a row of the stores' shared memory: blocks of 16 words
+
+struct LrArgs {
+  bnnk_lowrank_args p;
+  int nkb, bn, n_tiles, tiles, stages, acc_cols, tmem_cols;
+  int *err;
+};
+
+template <int T, int OT, int RB>
+__global__ void __launch_bounds__(kLrThreads, 1) k_lowrank_many(const __grid_constant__ CUtensorMap mx,
+                                                               const __grid_constant__ CUtensorMap mw,
+                                                               const __grid_constant__ CUtensorMap mb, const LrArgs a) {
+  constexpr int PARTS = T == 2 ? 3 : 2, GS = 64 / RB;  // adapters a stage
+  extern __shared__ uint8_t dsmem[];
+  __shared__ __align__(8) unsigned long long b_full[kLrStages], b_empty[kLrStages], b_acc[2], b_accempty[2], b_list[2],
+      b_listempty[2], b_turn[2], b_back[2];
+  __shared__ uint32_t tmem_s;
+  __shared__ volatile int abort_s;
+  __shared__ int s_n[2], s_list[2][128];
+  __shared__ volatile uint8_t s_big[2][128];
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
+  const bnnk_lowrank_args &p = a.p;
+  const int S = a.stages, bn = a.bn;
+  const uint32_t a_bytes = 128 * 128, stage = (128 + bn) * 128;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; s++) { mbar_init(smem_u32(&b_full[s]), 5); mbar_init(smem_u32(&b_empty[s]), 1); }
+    for (int g = 0; g < 2; g++) {
+      mbar_init(smem_u32(&b_acc[g]), 1);
+      mbar_init(smem_u32(&b_accempty[g]), 8);
+      mbar_init(smem_u32(&b_list[g]), 4);
+      mbar_init(smem_u32(&b_listempty[g]), 14);
+      mbar_init(smem_u32(&b_turn[g]), 1);
+      mbar_init(smem_u32(&b_back[g]), 4);
+    }
+    abort_s = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_s)),
+                 "r"(a.tmem_cols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_s, 0), base = (smem_u32(dsmem) + 1023u) & ~1023u;
+  auto wait = [&](unsigned long long &bar, int parity, int code) {
+    if (__all_sync(0xffffffffu, mbar_try(smem_u32(&bar), parity))) return true;
+    bool ok = mbar_wait_asleep(smem_u32(&bar), parity);
+    ok = __all_sync(0xffffffffu, ok && !abort_s);
+    if (!ok && lane == 0) {
+      if (!abort_s) atomicExch(a.err, code);
+      abort_s = 1;
+    }
+    return ok;
+  };
+  const bool adapters = p.slot != nullptr;
+  // a place in the ring of stages
+  struct Place {
+    int s = 0, parity = 0, used = 0;
+    __device__ __forceinline__ void next(int S) {
+      if (++s == S) { s = 0; parity ^= 1; used = 1; }
+    }
+  } at;
+  int lt = 0;       // tiles done
+  bool ok = true;
+  // the stages that the tile's adapters take (after list lt % 2 is made)
+  auto extra = [&](int &n) {
+    n = 0;
+    if (!adapters) return true;
+    if (!wait(b_list[lt & 1], (lt >> 1) & 1, BNNK_ERR_TMA_WAIT)) return false;
+    n = (s_n[lt & 1] + GS - 1) / GS * PARTS;
+    return true;
+  };
+  auto list_read = [&]() {
+    __syncwarp();
+    if (adapters && lane == 0) mbar_arrive(smem_u32(&b_listempty[lt & 1]));
+  };
+
+  if (warp == 0) {
+    for (int t = blockIdx.x; t < a.tiles && ok; t += gridDim.x, lt++) {
+      const int r0 = t / a.n_tiles * 128, n0 = t % a.n_tiles * bn;
+      for (int kb = 0; kb < a.nkb; kb++, at.next(S)) {
+        if (at.used && !(ok = wait(b_empty[at.s], at.parity ^ 1, BNNK_ERR_TMA_WAIT))) break;
+        const uint32_t st = base + at.s * stage, bar = smem_u32(&b_full[at.s]);
+        if (elect_one()) {
+          mbar_expect_tx(bar, stage);
+          asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], 4;" ::"r"(bar) : "memory");
+          tma_load_2d(st, &mx, bar, kb * 64, r0);
+          tma_load_2d(st + a_bytes, &mw, bar, kb * 64, n0);
+        }
+      }
+      // the ring's next places are the adapters': handed over and back, so that each side waits for a place whose use
+      // before has begun (a parity tells one use from the next, not from the one after)
+      if (!ok || !adapters) continue;
+      if (elect_one()) mbar_arrive(smem_u32(&b_turn[lt & 1]));
+      int n = 0;
+      if (!(ok = extra(n))) break;
+      list_read();
+      for (int k = 0; k < n; k++) at.next(S);
+      if (!(ok = wait(b_back[lt & 1], (lt >> 1) & 1, BNNK_ERR_TMA_WAIT))) break;
+    }
+  } else if (warp == 1) {
+    const uint32_t idesc = idesc_16(T - 1, bn, 0, 0);
+    for (int t = blockIdx.x; t < a.tiles && ok; t += gridDim.x, lt++) {
+      const int g = lt & 1;
+      if (lt >= 2 && !(ok = wait(b_accempty[g], (lt / 2 - 1) & 1, BNNK_ERR_MMA_WAIT))) break;
+      const uint32_t acc = tmem + g * a.acc_cols;
+      for (int kb = 0; kb < a.nkb; kb++, at.next(S)) {
+        if (!(ok = wait(b_full[at.s], at.parity, BNNK_ERR_MMA_WAIT))) break;
+        tc_fence_after();
+        const uint64_t da = smem_desc<128>(base + at.s * stage), db = smem_desc<128>(base + at.s * stage + a_bytes);
+        if (elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < 4; kk++) mma16_ss(acc, da + kk * 2, db + kk * 2, idesc, (kb | kk) != 0);
+          mma_commit(smem_u32(&b_empty[at.s]));
+        }
+      }
+      int n = 0;
+      if (!ok || !(ok = extra(n))) break;
+      const int used = n ? s_n[g] : 0;
+      list_read();
+      for (int k = 0; k < n; k++, at.next(S)) {
+        if (!(ok = wait(b_full[at.s], at.parity, BNNK_ERR_MMA_WAIT))) break;
+        tc_fence_after();
+        const int here = min(GS, used - k / PARTS * GS);
+        const uint64_t da = smem_desc<2 * RB>(base + at.s * stage), db = smem_desc<2 * RB>(base + at.s * stage + a_bytes);
+        if (elect_one()) {
+          for (int e = 0; e < here; e++)
+#pragma unroll
+            for (int kk = 0; kk < RB / 16; kk++)
+              mma16_ss(acc, da + e * (128 * RB * 2 >> 4) + kk * 2, db + e * (bn * RB * 2 >> 4) + kk * 2, idesc, 1);
+          mma_commit(smem_u32(&b_empty[at.s]));
+        }
+      }
+      if (ok && elect_one()) mma_commit(smem_u32(&b_acc[g]));
+    }
+  } else if (warp < 6) {
+    if (adapters) {
+      const int row = threadIdx.x - 64;
+      wait_launch_before();
+      for (int t = blockIdx.x; t < a.tiles && ok; t += gridDim.x, lt++) {
+        const int r0 = t / a.n_tiles * 128, n0 = t % a.n_tiles * bn, g = lt & 1;
+        if (lt >= 2 && !(ok = wait(b_listempty[g], (lt / 2 - 1) & 1, BNNK_ERR_TMA_WAIT))) break;
+        // the tile's adapters, in the order of their first rows: every warp makes the whole list from all 128 slots and
+        // writes its own part of it
+        int all[4], mine = -1, count = 0, before = 0;
+        unsigned firsts[4];
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+          const int r = r0 + 32 * w + lane;
+          int s = r < p.rows ? p.slot[r] : -1;
+          if (s >= p.slots) s = -1;
+          all[w] = s;
+          if (w == warp - 2) mine = s;
+        }
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+          const unsigned same = __match_any_sync(0xffffffffu, all[w]);  // every lane takes part, those without an adapter too
+          bool first = all[w] >= 0 && __ffs(same) - 1 == lane;
+#pragma unroll
+          for (int v = 0; v < w; v++)
+            for (int l = 0; l < 32; l++) first &= __shfl_sync(0xffffffffu, all[v], l) != all[w];
+          firsts[w] = __ballot_sync(0xffffffffu, first);
+          if (w < warp - 2) before += __popc(firsts[w]);
+          count += __popc(firsts[w]);
+        }
+        const unsigned own = firsts[0] * (warp == 2) | firsts[1] * (warp == 3) | firsts[2] * (warp == 4) | firsts[3] * (warp == 5);
+        if ((own >> lane) & 1) s_list[g][before + __popc(own & ((1u << lane) - 1))] = mine;
+        if (warp == 2 && lane == 0) s_n[g] = count;
+        // this row's h: rows past fp16's range are added when y is stored
+        const float *h = p.hid + (long long)(r0 + row) * p.rank;
+        bool big = false;
+        if (T == 1 && mine >= 0)
+          for (int e = 0; e < p.rank; e++) big |= fabsf(h[e]) > 65504.f && fabsf(h[e]) < __int_as_float(0x7f800000);
+        s_big[g][row] = big;
+        __threadfence_block();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&b_list[g]));
+        if (!(ok = wait(b_list[g], (lt >> 1) & 1, BNNK_ERR_TMA_WAIT))) break;
+        if (!(ok = wait(b_turn[g], (lt >> 1) & 1, BNNK_ERR_TMA_WAIT))) break;
+        // the ring's places of W's steps
+        for (int kb = 0; kb < a.nkb; kb++) at.next(S);
+        for (int e0 = 0; e0 < count && ok; e0 += GS) {
+          for (int part = 0; part < PARTS; part++, at.next(S)) {
+            if (at.used && !(ok = wait(b_empty[at.s], at.parity ^ 1, BNNK_ERR_TMA_WAIT))) break;
+            const uint32_t st = base + at.s * stage, bar = smem_u32(&b_full[at.s]);
+            const int here = min(GS, count - e0);
+#pragma unroll 1
+            for (int e = 0; e < here; e++) {
+              const bool on = mine >= 0 && s_list[g][e0 + e] == mine && !big;
+#pragma unroll 1
+              for (int c = 0; c < RB; c += 8) {
+                uint32_t z[4] = {0, 0, 0, 0};
+                if (on && c < p.rank) {
+                  const float4 u = *reinterpret_cast<const float4 *>(h + c), v = *reinterpret_cast<const float4 *>(h + c + 4);
+                  const float f[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+#pragma unroll
+                  for (int i = 0; i < 4; i++) {
+                    uint32_t x0, x1, x2 = 0;
+                    if constexpr (PARTS == 3) split3<T>(f[2 * i], f[2 * i + 1], x0, x1, x2);
+                    else split2<T>(f[2 * i], f[2 * i + 1], x0, x1);
+                    z[i] = part == 0 ? x0 : part == 1 ? x1 : x2;
+                  }
+                }
+                uint32_t off = e * 128 * RB * 2 + row * RB * 2 + c * 2;
+                off ^= (off >> 3) & (RB == 64 ? 0x70 : RB == 32 ? 0x30 : 0x10);  // the swizzle of 2 RB bytes a row
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(st + off), "r"(z[0]), "r"(z[1]), "r"(z[2]),
+                             "r"(z[3])
+                             : "memory");
+              }
+            }
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar);
+            if (warp == 2 && elect_one()) {
+              mbar_expect_tx(bar, here * bn * RB * 2);
+              for (int e = 0; e < here; e++)
+                tma_load_3d(st + a_bytes + e * bn * RB * 2, &mb, bar, 0, n0, s_list[g][e0 + e]);
+            }
+          }
+        }
+        if (!ok) break;
+        list_read();
+        if (lane == 0) mbar_arrive(smem_u32(&b_back[g]));
+      }
+    }
+  } else {
+    // y: rows of this warp's TMEM quarter, blocks of 16 words a row alternating between two warps of a quarter
+    constexpr int PW = OT == 0 ? 1 : 2, CW = 16 * PW;  // values a word, columns a block
+    const int qd = warp % 4, h = (warp - 6) / 4;
+    const uint32_t buf = base + S * stage + (warp - 6) * 32 * kLrPad * 4;
+    const bool even = PW == 1 || (((uintptr_t)p.y | (uintptr_t)(p.ldy * 2)) & 3) == 0;  // word-aligned rows
+    for (int t = blockIdx.x; t < a.tiles; t += gridDim.x, lt++) {
+      const int r0 = t / a.n_tiles * 128 + 32 * qd, n0 = t % a.n_tiles * bn, g = lt & 1;
+      if (!wait(b_acc[g], (lt >> 1) & 1, BNNK_ERR_EPI_WAIT)) break;
+      tc_fence_after();
+      const bool big = T == 1 && adapters && s_big[g][32 * qd + lane];
+      const uint32_t tq = tmem + g * a.acc_cols + ((uint32_t)(32 * qd) << 16);
+      const int width = min(bn, p.N - n0), rows = min(32, p.rows - r0);
+#pragma unroll 1
+      for (int c0 = h * CW; c0 < width; c0 += 2 * CW) {
+#pragma unroll
+        for (int w0 = 0; w0 < PW; w0++) {
+          const int c = c0 + 16 * w0;
+          if (c >= bn) break;
+          uint32_t x[16];
+          tmem_ld16(tq + c, x);
+          tmem_wait_ld(x);
+          float v[16];
+#pragma unroll
+          for (int j = 0; j < 16; j++)
+            v[j] = __uint_as_float(x[j]) + (p.bias && c + j < width ? __ldg(p.bias + n0 + c + j) : 0.f);
+          if (big) {  // h past fp16's range: its products here
+            const int s = p.slot[r0 + lane];
+            const float *hh = p.hid + (long long)(r0 + lane) * p.rank;
+#pragma unroll 1
+            for (int j = 0; j < 16 && c + j < width; j++) {
+              const elem_t<T> *b = (const elem_t<T> *)p.b + ((long long)s * p.N + n0 + c + j) * p.rank;
+              float u = 0.f;
+              for (int e = 0; e < p.rank; e++) u = fmaf(hh[e], Elem<T>::get(b[e]), u);
+#pragma unroll
+              for (int i = 0; i < 16; i++) v[i] += i == j ? u : 0.f;
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 16; j += PW) {
+            const uint32_t z = PW == 1 ? __float_as_uint(v[j]) : pack2f<T>(v[j], v[j + PW - 1]);
+            asm volatile("st.shared.b32 [%0], %1;" ::"r"(buf + (lane * kLrPad + (16 * w0 + j) / PW) * 4), "r"(z) : "memory");
+          }
+        }
+        __syncwarp();
+        const int c = c0 + lane % 16 * PW;
+        elem_t<OT> *y = (elem_t<OT> *)p.y + (long long)(r0 + lane / 16) * p.ldy + n0 + c;
+#pragma unroll 4
+        for (int r = lane / 16; r < rows; r += 2, y += 2 * p.ldy) {
+          uint32_t z;
+          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(z) : "r"(buf + (r * kLrPad + lane % 16) * 4) : "memory");
+          if constexpr (PW == 1) {
+            if (c < width) *y = __uint_as_float(z);
+          } else if (even && c + 1 < width) {
+            *reinterpret_cast<uint32_t *>(y) = z;
+          } else {
+            if (c < width) reinterpret_cast<uint16_t *>(y)[0] = (uint16_t)z;
+            if (c + 1 < width) reinterpret_cast<uint16_t *>(y)[1] = (uint16_t)(z >> 16);
+          }
+        }
+        __syncwarp();
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(smem_u32(&b_accempty[g]));
+        if (adapters) mbar_arrive(smem_u32(&b_listempty[g]));
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(a.tmem_cols));
+}
+
+// a launch that may start before the one before it has ended
+template <typename... Args>
+cudaError_t launch_early(void (*kernel)(Args...), dim3 grid, int threads, size_t smem, cudaStream_t st, Args... args) {
+  cudaLaunchConfig_t c = {};
+  c.gridDim = grid;
+  c.blockDim = dim3(threads);
+  c.dynamicSmemBytes = smem;
+  c.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  c.attrs = at;
+  c.numAttrs = 1;
+  return cudaLaunchKernelEx(&c, kernel, args...);
+}
+
+template <int T, int OT, int MT, int NT>
+cudaError_t few_nt(const bnnk_lowrank_args &p, cudaStream_t st) {
+  static SmemAttr attr;
+  const size_t smem = sizeof(float) * 8 * 16 * MT * (8 * NT + 1);
+  const cudaError_t e = attr.ensure(k_lowrank_few<T, OT, MT, NT>, smem);
+  if (e) return e;
+  const dim3 grid((p.N + 16 * MT - 1) / (16 * MT));
+  if (p.slot) return launch_early(k_lowrank_few<T, OT, MT, NT>, grid, 256, smem, st, p);
+  k_lowrank_few<T, OT, MT, NT><<<grid, 256, smem, st>>>(p);
+  return cudaGetLastError();
+}
+
 template <int T, int OT>
-__global__ void __launch_bounds__(256) k_lowrank_up(int rows, int N, int K, const elem_t<T> *x, long long ldx,
-                                                    const elem_t<T> *W, long long ldw, const float *bias,
-                                                    const int32_t *slot, int slots, int rank, const elem_t<T> *B,
-                                                    const float *hid, elem_t<OT> *y, long long ldy) {
-  __shared__ float xs[16][65], ws[16][65];
-  const long long r0 = (long long)blockIdx.y * 64;
-  const int n0 = blockIdx.x * 64, tr = threadIdx.x / 16, tn = threadIdx.x % 16;
-  float acc[4][4] = {};
-  for (int k0 = 0; k0 < K; k0 += 16) {
-    for (int e = threadIdx.x; e < 1024; e += 256) {
-      const int m = e / 16, k = e % 16;
-      xs[k][m] = r0 + m < rows && k0 + k < K ? Elem<T>::get(x[(r0 + m) * ldx + k0 + k]) : 0.f;
-      ws[k][m] = n0 + m < N && k0 + k < K ? Elem<T>::get(W[(n0 + m) * ldw + k0 + k]) : 0.f;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 16; k++)
-#pragma unroll
-      for (int i = 0; i < 4; i++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) acc[i][j] = fmaf(xs[k][tr + 16 * i], ws[k][tn + 16 * j], acc[i][j]);
-    __syncthreads();
-  }
-  for (int i = 0; i < 4; i++) {
-    const long long r = r0 + tr + 16 * i;
-    if (r >= rows) continue;
-    const int s = slot ? slot[r] : -1;
-    for (int j = 0; j < 4; j++) {
-      const int n = n0 + tn + 16 * j;
-      if (n >= N) continue;
-      float v = acc[i][j] + (bias ? bias[n] : 0.f);
-      if (s >= 0 && s < slots)
-        for (int e = 0; e < rank; e++)
-          v = fmaf(hid[r * rank + e], Elem<T>::get(B[((long long)s * N + n) * rank + e]), v);
-      y[r * ldy + n] = Elem<OT>::put(v);
-    }
-  }
+cudaError_t run_few(const bnnk_lowrank_args &p, cudaStream_t st) {
+  // 32 rows of W a CTA halve the reads of x; 16 where they would leave SMs idle
+  const bool two = (p.N + 31) / 32 >= num_sms();
+  const int nt = (p.rows + 7) / 8;
+  if (two)
+    return nt <= 1 ? few_nt<T, OT, 2, 1>(p, st) : nt <= 2 ? few_nt<T, OT, 2, 2>(p, st)
+         : nt <= 4 ? few_nt<T, OT, 2, 4>(p, st) : few_nt<T, OT, 2, 8>(p, st);
+  return nt <= 1 ? few_nt<T, OT, 1, 1>(p, st) : nt <= 2 ? few_nt<T, OT, 1, 2>(p, st)
+       : nt <= 4 ? few_nt<T, OT, 1, 4>(p, st) : few_nt<T, OT, 1, 8>(p, st);
+}
+
+template <int T, int OT, int RB>
+int run_many(const bnnk_lowrank_args &p, int *err, cudaStream_t st) {
+  LrArgs a = {};
+  a.p = p;
+  a.err = err;
+  a.nkb = (p.K + 63) / 64;
+  // column tiles of at most 256, of equal widths, narrower while there are fewer tiles than SMs
+  const int n16 = (p.N + 15) & ~15, mt = (p.rows + 127) / 128;
+  int nt = (n16 + 255) / 256;
+  while ((long long)mt * nt < num_sms() && ((n16 + nt) / (nt + 1) + 15) / 16 * 16 >= 32) nt++;
+  a.bn = ((n16 + nt - 1) / nt + 15) & ~15;
+  a.n_tiles = (p.N + a.bn - 1) / a.bn;
+  if ((long long)mt * a.n_tiles > 0x7fffffffLL) return cudaErrorInvalidValue;
+  a.tiles = mt * a.n_tiles;
+  a.acc_cols = a.bn <= 32 ? 32 : a.bn <= 64 ? 64 : a.bn <= 128 ? 128 : 256;
+  a.tmem_cols = 2 * a.acc_cols;
+  const size_t stage = (size_t)(128 + a.bn) * 128, out = 8 * 32 * kLrPad * 4;
+  const int s = (int)((227 * 1024 - 4096 - out) / stage);
+  a.stages = s > kLrStages ? kLrStages : s;
+  const size_t smem = a.stages * stage + out + 1024;
+  CUtensorMap mx, mw, mb;
+  int e = encode_rows16(&mx, p.x, T == 2, p.K, p.rows, p.ldx, 64, 128, 128);
+  if (!e) e = encode_rows16(&mw, p.w, T == 2, p.K, p.N, p.ldw, 64, a.bn, 128);
+  if (!e) e = encode_slots16(&mb, p.b, T == 2, p.rank, p.N, p.slots, RB, a.bn);
+  static SmemAttr attr;
+  if (!e) e = attr.ensure(k_lowrank_many<T, OT, RB>, smem);
+  if (e) return e;
+  const int grid = a.tiles < num_sms() ? a.tiles : num_sms();
+  if (p.slot) return launch_early(k_lowrank_many<T, OT, RB>, dim3(grid), kLrThreads, smem, st, mx, mw, mb, a);
+  k_lowrank_many<T, OT, RB><<<grid, kLrThreads, smem, st>>>(mx, mw, mb, a);
+  return cudaGetLastError();
+}
+
+template <int T, int RT>
+void run_down(const bnnk_lowrank_args &p, cudaStream_t st) {
+  // an adapter a CTA where there are few rows; of many rows' tiles most hold one adapter
+  const dim3 grid((p.rows + kDownRows - 1) / kDownRows, p.rows <= 512 ? kDownRows : 4);
+  k_lowrank_down<T, RT><<<grid, 256, 0, st>>>(p.rows, p.K, (const elem_t<T> *)p.x, p.ldx, p.slot, p.slots, p.rank,
+                                              (const elem_t<T> *)p.a, p.scale, p.hid);
 }
 
 template <int T>
-cudaError_t run_lowrank(const bnnk_lowrank_args &p, cudaStream_t st) {
-  using E = elem_t<T>;
-  if (p.slot)
-    k_lowrank_down<T><<<(int)(((long long)p.rows * p.rank + 7) / 8), 256, 0, st>>>(
-        p.rows, p.K, (const E *)p.x, p.ldx, p.slot, p.slots, p.rank, (const E *)p.a, p.scale, p.hid);
-  const dim3 grid((p.N + 63) / 64, (p.rows + 63) / 64);
+int run_lowrank(const bnnk_lowrank_args &p, int *err, cudaStream_t st) {
+  if (p.slot) {
+    if (p.rank <= 16) run_down<T, 2>(p, st);
+    else if (p.rank <= 32) run_down<T, 4>(p, st);
+    else run_down<T, 8>(p, st);
+    const cudaError_t e = cudaGetLastError();
+    if (e) return e;
+  }
+  if (p.rows <= 64) return p.otype == 0 ? run_few<T, 0>(p, st) : run_few<T, T>(p, st);
   if (p.otype == 0)
-    k_lowrank_up<T, 0><<<grid, 256, 0, st>>>(p.rows, p.N, p.K, (const E *)p.x, p.ldx, (const E *)p.w, p.ldw, p.bias,
-                                             p.slot, p.slots, p.rank, (const E *)p.b, p.hid, (float *)p.y, p.ldy);
-  else
-    k_lowrank_up<T, T><<<grid, 256, 0, st>>>(p.rows, p.N, p.K, (const E *)p.x, p.ldx, (const E *)p.w, p.ldw, p.bias,
-                                             p.slot, p.slots, p.rank, (const E *)p.b, p.hid, (E *)p.y, p.ldy);
-  return cudaGetLastError();
+    return p.rank <= 16 ? run_many<T, 0, 16>(p, err, st) : p.rank <= 32 ? run_many<T, 0, 32>(p, err, st)
+                                                                         : run_many<T, 0, 64>(p, err, st);
+  return p.rank <= 16 ? run_many<T, T, 16>(p, err, st) : p.rank <= 32 ? run_many<T, T, 32>(p, err, st)
+                                                                       : run_many<T, T, 64>(p, err, st);
 }
 
 }  // namespace
@@ -103,5 +614,5 @@ using namespace bnn;
 
 extern "C" int bnnk_lowrank(const bnnk_lowrank_args *p, bnn_stream_t st) {
   if (p->rows <= 0) return 0;
-  return p->type == 1 ? run_lowrank<1>(*p, (cudaStream_t)st) : run_lowrank<2>(*p, (cudaStream_t)st);
+  return p->type == 1 ? run_lowrank<1>(*p, p->err, (cudaStream_t)st) : run_lowrank<2>(*p, p->err, (cudaStream_t)st);
 }

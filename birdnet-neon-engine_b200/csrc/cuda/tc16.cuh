@@ -129,5 +129,7 @@ int encode_heads(CUtensorMap *m, const void *base, int bf16, int width, int head
 // host: a 2-D map of a 16-bit matrix [rows][width] (row stride rs elements), boxes of box_w x box_rows, swizzle sw bytes
 int encode_rows16(CUtensorMap *m, const void *base, int bf16, int width, long long rows, long long rs, int box_w,
                   int box_rows, int sw);
+// host: a 3-D map of [slots][rows][width] back to back, boxes of box_w x box_rows x 1 slot, swizzle 2 box_w bytes
+int encode_slots16(CUtensorMap *m, const void *base, int bf16, int width, int rows, int slots, int box_w, int box_rows);
 
 }  // namespace bnn

@@ -149,7 +149,6 @@ void bnn_dattn_free(bnn_dattn *o) {
 struct bnn_lowrank {
   bnnk_lowrank_args a;
   int rows;
-  int *err;
 };
 
 bnn_lowrank *bnn_lowrank_new(int type, int out_type, int N, int K, const void *d_w, long long ldw, const float *d_bias,
@@ -168,7 +167,7 @@ bnn_lowrank *bnn_lowrank_new(int type, int out_type, int N, int K, const void *d
   o->a.type = type; o->a.otype = out_type; o->a.N = N; o->a.K = K; o->a.slots = slots; o->a.rank = rank;
   o->a.w = d_w; o->a.ldw = ldw; o->a.bias = d_bias; o->a.a = d_a; o->a.b = d_b; o->a.scale = d_scale;
   if (dev_alloc("bnn_lowrank_new", (void **)&o->a.hid, sizeof(float) * (size_t)rows * rank) ||
-      dev_alloc("bnn_lowrank_new", (void **)&o->err, sizeof(int))) {
+      dev_alloc("bnn_lowrank_new", (void **)&o->a.err, sizeof(int))) {
     bnn_lowrank_free(o);
     return NULL;
   }
@@ -194,12 +193,12 @@ int bnn_lowrank_run(bnn_lowrank *o, int rows, const void *d_x, long long ldx, co
   return launch_rc("bnn_lowrank_run", bnnk_lowrank(&a, (bnn_stream_t)stream));
 }
 
-int bnn_lowrank_error(bnn_lowrank *o) { return o ? read_word(o->err) : -1; }
+int bnn_lowrank_error(bnn_lowrank *o) { return o ? read_word(o->a.err) : -1; }
 
 void bnn_lowrank_free(bnn_lowrank *o) {
   if (!o) return;
   cudaFree(o->a.hid);
-  cudaFree(o->err);
+  cudaFree(o->a.err);
   free(o);
 }
 
