@@ -69,8 +69,20 @@ __global__ void __launch_bounds__(256) k_dattn_rec(const DattnArgs a) {
   const float lam = a.pow[hk * kDattnPow + 1];
   int buf = 0;
   for (long long t = t0; t < t1; t++) {
-    const bool live = !a.live || a.live[t];
+    const elem_t<T> *k = (const elem_t<T> *)a.k + t * a.kts + (long long)hk * dk;
+    const elem_t<T> *v = (const elem_t<T> *)a.v + t * a.vts + (long long)hk * dv + c0;
+    const elem_t<T> *q = (const elem_t<T> *)a.q + t * a.qts + (long long)hk * a.G * dk;
     elem_t<T> *o = (elem_t<T> *)a.o + t * a.ots + (long long)hk * a.G * dv;
+    // all of the token's loads before the first use, a dead token's too: one wait for memory, with that for S
+    const bool live = !a.live || a.live[t];
+    const uint2 vw = col ? *reinterpret_cast<const uint2 *>(v) : make_uint2(0, 0);
+    elem_t<T> kw[4], qw[4];
+#pragma unroll
+    for (int p = 0; p < 4; p++) {
+      const int r = min(row[p], dk - 1);
+      kw[p] = k[r];
+      qw[p] = q[r];
+    }
     if (!live) {
 #pragma unroll
       for (int p = 0; p < 4; p++) { S[p].x *= lam; S[p].y *= lam; S[p].z *= lam; S[p].w *= lam; }
@@ -78,18 +90,11 @@ __global__ void __launch_bounds__(256) k_dattn_rec(const DattnArgs a) {
         if (cs + lane < dv) o[(long long)g * dv + cs + lane] = Elem<T>::put(0.f);
       continue;
     }
-    const elem_t<T> *k = (const elem_t<T> *)a.k + t * a.kts + (long long)hk * dk;
-    const elem_t<T> *v = (const elem_t<T> *)a.v + t * a.vts + (long long)hk * dv + c0;
-    const elem_t<T> *q = (const elem_t<T> *)a.q + t * a.qts + (long long)hk * a.G * dk;
-    float4 vv = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (col) {
-      const uint2 w = *reinterpret_cast<const uint2 *>(v);
-      const float2 x = unpack2<T>(w.x), y = unpack2<T>(w.y);
-      vv = make_float4(x.x, x.y, y.x, y.y);
-    }
+    const float2 v0 = unpack2<T>(vw.x), v1 = unpack2<T>(vw.y);
+    const float4 vv = make_float4(v0.x, v0.y, v1.x, v1.y);
 #pragma unroll
     for (int p = 0; p < 4; p++) {
-      const float kk = row[p] < dk ? Elem<T>::get(k[row[p]]) : 0.f;
+      const float kk = row[p] < dk ? Elem<T>::get(kw[p]) : 0.f;
       S[p].x = fmaf(kk, vv.x, lam * S[p].x);
       S[p].y = fmaf(kk, vv.y, lam * S[p].y);
       S[p].z = fmaf(kk, vv.z, lam * S[p].z);
@@ -102,7 +107,7 @@ __global__ void __launch_bounds__(256) k_dattn_rec(const DattnArgs a) {
 #pragma unroll
         for (int p = 0; p < 4; p++) {
           if (row[p] >= dk) continue;
-          const float qq = Elem<T>::get(q[(long long)(g0 + g) * dk + row[p]]);
+          const float qq = Elem<T>::get(g0 + g == 0 ? qw[p] : q[(long long)(g0 + g) * dk + row[p]]);
           s.x = fmaf(qq, S[p].x, s.x);
           s.y = fmaf(qq, S[p].y, s.y);
           s.z = fmaf(qq, S[p].z, s.z);

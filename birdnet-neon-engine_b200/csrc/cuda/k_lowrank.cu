@@ -115,8 +115,9 @@ __global__ void __launch_bounds__(256) k_lowrank_down(int rows, int K, const ele
 //
 // Bound by reading W (and the adapters' B) once. One CTA per 16 MT rows of W: warp-level matrix instructions with W as
 // the 16-row operand and 8 NT rows of x as the other, K dealt to 8 warps as above, all of a warp's loads independent; the
-// warps' sums are joined in shared memory, then a warp takes 32 neighbouring outputs of one row, and each lane adds its
-// output's rank products with B from the row's adapter (neighbouring outputs' rows of B are neighbours in memory).
+// warps' sums are joined in shared memory, then each lane takes some rows' outputs of one column and adds their rank
+// products with B from the rows' adapters (neighbouring lanes' rows of B are neighbours in memory; the loads of all of a
+// lane's outputs are in flight together, the first of them before the wait for h).
 template <int T, int OT, int MT, int NT>
 __global__ void __launch_bounds__(256) k_lowrank_few(const bnnk_lowrank_args p) {
   extern __shared__ float red[];  // [8][16 MT][8 NT + 1]
@@ -165,29 +166,46 @@ __global__ void __launch_bounds__(256) k_lowrank_few(const bnnk_lowrank_args p) 
       r[8 * P] = acc[m][j][2];
       r[8 * P + 1] = acc[m][j][3];
     }
-  __syncthreads();
-  if (p.slot) wait_launch_before();
-  for (int i = threadIdx.x; i < p.rows * 16 * MT; i += 256) {
-    const int r = i / (16 * MT), c = i % (16 * MT), n = n0 + c;
-    if (n >= p.N) continue;
-    float v = p.bias ? p.bias[n] : 0.f;
+  constexpr int CN = 16 * MT, OUTS = (8 * NT * CN + 255) / 256, RSTEP = 256 / CN;  // a lane's rows: r0, r0 + RSTEP, ..
+  const int c = threadIdx.x % CN, r0 = threadIdx.x / CN, n = n0 + c;
+  float u[OUTS];
+  int s[OUTS];
 #pragma unroll
-    for (int w = 0; w < 8; w++) v += red[(w * 16 * MT + c) * P + r];
-    const int s = p.slot ? p.slot[r] : -1;
-    if (s >= 0 && s < p.slots) {
-      const elem_t<T> *b = B + ((long long)s * p.N + n) * rank;
-      const float *h = p.hid + (long long)r * rank;
-      float u = 0.f;
-      for (int e = 0; e < rank; e += 8) {
-        float bv[8];
-        load_elems<T, 8>(b + e, bv);
-        const float4 h0 = *reinterpret_cast<const float4 *>(h + e), h1 = *reinterpret_cast<const float4 *>(h + e + 4);
-        u = fmaf(h0.x, bv[0], u); u = fmaf(h0.y, bv[1], u); u = fmaf(h0.z, bv[2], u); u = fmaf(h0.w, bv[3], u);
-        u = fmaf(h1.x, bv[4], u); u = fmaf(h1.y, bv[5], u); u = fmaf(h1.z, bv[6], u); u = fmaf(h1.w, bv[7], u);
+  for (int o = 0; o < OUTS; o++) {
+    const int r = r0 + o * RSTEP;
+    u[o] = 0.f;
+    s[o] = p.slot && r < p.rows && n < p.N ? p.slot[r] : -1;
+    if (s[o] >= p.slots) s[o] = -1;
+  }
+  if (p.slot) {
+    for (int e = 0; e < rank; e += 8) {
+      uint4 b[OUTS];
+#pragma unroll
+      for (int o = 0; o < OUTS; o++) b[o] = ldg16(B + ((long long)s[o] * p.N + n) * rank + e, s[o] >= 0);
+      if (e == 0) wait_launch_before();
+#pragma unroll
+      for (int o = 0; o < OUTS; o++) {
+        if (s[o] < 0) continue;
+        const float *h = p.hid + (long long)(r0 + o * RSTEP) * rank + e;
+        const float4 h0 = *reinterpret_cast<const float4 *>(h), h1 = *reinterpret_cast<const float4 *>(h + 4);
+        const float2 b0 = unpack2<T>(b[o].x), b1 = unpack2<T>(b[o].y), b2 = unpack2<T>(b[o].z), b3 = unpack2<T>(b[o].w);
+        u[o] = fmaf(h0.x, b0.x, u[o]); u[o] = fmaf(h0.y, b0.y, u[o]);
+        u[o] = fmaf(h0.z, b1.x, u[o]); u[o] = fmaf(h0.w, b1.y, u[o]);
+        u[o] = fmaf(h1.x, b2.x, u[o]); u[o] = fmaf(h1.y, b2.y, u[o]);
+        u[o] = fmaf(h1.z, b3.x, u[o]); u[o] = fmaf(h1.w, b3.y, u[o]);
       }
-      v += u;
     }
-    ((elem_t<OT> *)p.y)[r * p.ldy + n] = Elem<OT>::put(v);
+  }
+  __syncthreads();
+  const float bias = p.bias && n < p.N ? p.bias[n] : 0.f;
+#pragma unroll
+  for (int o = 0; o < OUTS; o++) {
+    const int r = r0 + o * RSTEP;
+    if (r >= p.rows || n >= p.N) continue;
+    float v = bias;
+#pragma unroll
+    for (int w = 0; w < 8; w++) v += red[(w * CN + c) * P + r];
+    ((elem_t<OT> *)p.y)[r * p.ldy + n] = Elem<OT>::put(v + u[o]);
   }
 }
 

@@ -7,7 +7,10 @@
 // nothing cancels), h is formed from x' before x' is rounded for its store. A row whose live byte is 0 keeps x and
 // gets h = 0 whatever its f and g hold (they are not read).
 //
-// Bound by memory: f, g, x in, x', h out.
+// Bound by memory: f, g, x in, x', h out. 28800 rows of 1536 (x fp32, the rest bf16, 619 MB): 119 us, 5.2 TB/s. A row
+// over the warps of a block keeps a thread's share small (56 registers); a warp a row took 242 us (250 registers, few
+// rows in flight), the same without the next row's loads ahead of this row's sums 141 us, without the vectors in registers
+// 149 us. Four blocks of 6 warps an SM: with five 143 us, with eight 120 us.
 #include <cuda_runtime.h>
 
 #include "bnn_kernels.h"
@@ -37,140 +40,175 @@ __device__ __forceinline__ float gate_of(int gate, float g) {
   return gate == 1 ? s : g * s;
 }
 
-// the sum of v over the W warps of a row (W a power of two; W > 1: through shared memory, every warp of the block at
-// the same call), in an order that does not depend on timing
-template <int W>
-__device__ __forceinline__ float row_sum(float v, float *red) {
+// the sum of v over the block's warps, in an order that does not depend on timing. calls: the block's calls so far; two
+// rows of 8 in turn, so that every warp has read a call's values (before it arrives at the next) when they are replaced
+__device__ __forceinline__ float block_sum(float v, float (*red)[8], int &calls) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if constexpr (W > 1) {
-    const int warp = threadIdx.x / 32;
-    __syncthreads();  // the sums of the call before have been read
-    if (threadIdx.x % 32 == 0) red[warp] = v;
+  const int warps = blockDim.x / 32;
+  if (warps > 1) {
+    const int buf = calls++ & 1;
+    if (threadIdx.x % 32 == 0) red[buf][threadIdx.x / 32] = v;
     __syncthreads();
     v = 0.f;
-    const int w0 = warp / W * W;
-#pragma unroll
-    for (int w = 0; w < W; w++) v += red[w0 + w];
+    for (int w = 0; w < warps; w++) v += red[buf][w];
   }
   return v;
 }
 
-template <int V>
-__device__ __forceinline__ void load_vec(const float *p, float (&v)[V]) { load_elems<0, V>(p, v); }
+// V consecutive elements as they lie in memory
+template <int T, int V>
+struct Raw {
+  static constexpr int words = V == 1 ? 1 : V * (T == 0 ? 4 : 2) / 4;
+  uint32_t w[words];
+  __device__ __forceinline__ void load(const elem_t<T> *p) {
+    if constexpr (V == 1) {
+      w[0] = T == 0 ? *reinterpret_cast<const uint32_t *>(p) : *reinterpret_cast<const uint16_t *>(p);
+    } else {
+#pragma unroll
+      for (int i = 0; i < words; i += 4) {
+        const uint4 v = reinterpret_cast<const uint4 *>(p)[i / 4];
+        w[i] = v.x; w[i + 1] = v.y; w[i + 2] = v.z; w[i + 3] = v.w;
+      }
+    }
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < words; i++) w[i] = 0;
+  }
+  __device__ __forceinline__ float at(int j) const {
+    if constexpr (T == 0) return __uint_as_float(w[j]);
+    else {
+      const float2 f = unpack2<T>(w[j / 2]);
+      return j & 1 ? f.y : f.x;
+    }
+  }
+};
 
-// W warps a row, each thread NV groups of V consecutive elements: D <= 32 W NV V
-template <int XT, int FT, int V, int NV, int W>
-__global__ void __launch_bounds__(kNormThreads) k_norm_gate(const NormArgs a) {
-  __shared__ float red[kNormThreads / 32];
-  constexpr int R = kNormThreads / (32 * W);
-  const int lane = threadIdx.x % (32 * W), sub = threadIdx.x / (32 * W), D = a.D;
+// A block a row, each thread NV groups of V consecutive columns (D <= blockDim NV V), the same for all its rows: the
+// vectors' values for them are read once and stay in registers (alpha gamma wpost as one). B: with bpost and bpre.
+template <int XT, int FT, int V, int NV, bool B>
+__global__ void __launch_bounds__(256) k_norm_gate(const NormArgs a) {
+  __shared__ float red[2][8];
+  int calls = 0;
+  const int D = a.D;
   const float inv = 1.f / (float)D;
-  for (long long r0 = (long long)blockIdx.x * R; r0 < a.rows; r0 += (long long)gridDim.x * R) {
-    const long long r = r0 + sub;
-    const bool in = r < a.rows, live = in && (!a.live || a.live[r]);
+  float cu[NV][V], bu[NV][B ? V : 1], ch[NV][V], bh[NV][B ? V : 1];
+#pragma unroll
+  for (int k = 0; k < NV; k++)
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+      const int c = (k * blockDim.x + threadIdx.x) * V + j;
+      const bool in = c < D;
+      const float gm = a.alpha * (a.gamma && in ? a.gamma[c] : 1.f);
+      cu[k][j] = gm * (a.wpost && in ? a.wpost[c] : 1.f);
+      ch[k][j] = a.wpre && in ? a.wpre[c] : 1.f;
+      if constexpr (B) {
+        bu[k][j] = a.bpost && in ? gm * a.bpost[c] : 0.f;
+        bh[k][j] = a.bpre && in ? a.bpre[c] : 0.f;
+      }
+    }
+  Raw<XT, V> rx[NV], nx[NV];
+  Raw<FT, V> rf[NV], rg[NV], nf[NV], ng[NV];
+  // a row's values; a dead row's f and g are not read
+  auto load = [&](long long r, bool live, Raw<XT, V> (&vx)[NV], Raw<FT, V> (&vf)[NV], Raw<FT, V> (&vg)[NV]) {
     const elem_t<XT> *x = (const elem_t<XT> *)a.x + r * a.xs;
-    float y[NV][V];
-    if (a.f) {
-      const elem_t<FT> *f = (const elem_t<FT> *)a.f + r * a.fs, *g = (const elem_t<FT> *)a.g + r * a.gs;
-      float u[NV][V], gg[NV][V];
+    const elem_t<FT> *f = (const elem_t<FT> *)a.f + r * a.fs, *g = (const elem_t<FT> *)a.g + r * a.gs;
 #pragma unroll
-      for (int k = 0; k < NV; k++) {
-        const int c = (k * 32 * W + lane) * V;
-#pragma unroll
-        for (int j = 0; j < V; j++) u[k][j] = 0.f, gg[k][j] = 0.f, y[k][j] = 0.f;
-        if (c < D && in) {
-          load_elems<XT, V>(x + c, y[k]);
-          if (live) {
-            load_elems<FT, V>(f + c, u[k]);
-            if (a.gate) load_elems<FT, V>(g + c, gg[k]);
-          }
+    for (int k = 0; k < NV; k++) {
+      const int c = (k * blockDim.x + threadIdx.x) * V;
+      vx[k].zero();
+      vf[k].zero();
+      vg[k].zero();
+      if (c < D) {
+        vx[k].load(x + c);
+        if (a.f && live) {
+          vf[k].load(f + c);
+          if (a.gate) vg[k].load(g + c);
         }
       }
+    }
+  };
+  bool live = blockIdx.x < a.rows && (!a.live || a.live[blockIdx.x]), next_live = false;
+  if (blockIdx.x < a.rows) load(blockIdx.x, live, rx, rf, rg);
+  for (long long r = blockIdx.x; r < a.rows; r += gridDim.x) {
+    const bool upd = a.f && live;
+    // the block's next row, on its way while this one's sums wait for its warps
+    const long long rn = r + gridDim.x;
+    if (rn < a.rows) {
+      next_live = !a.live || a.live[rn];
+      load(rn, next_live, nx, nf, ng);
+    }
+    float y[NV][V];
+#pragma unroll
+    for (int k = 0; k < NV; k++)
+#pragma unroll
+      for (int j = 0; j < V; j++) y[k][j] = rx[k].at(j);
+    // v is zero past the row's end, and stays out of the squares there
+    auto in_row = [&](int k) { return (k * (int)blockDim.x + (int)threadIdx.x) * V < D; };
+    if (upd) {
       float mean = 0.f, ss = 0.f;
       if (a.layer) {
 #pragma unroll
         for (int k = 0; k < NV; k++)
 #pragma unroll
-          for (int j = 0; j < V; j++) mean += u[k][j];
-        mean = row_sum<W>(mean, red) * inv;
+          for (int j = 0; j < V; j++) mean += rf[k].at(j);
+        mean = block_sum(mean, red, calls) * inv;
       }
 #pragma unroll
-      for (int k = 0; k < NV; k++) {
-        if ((k * 32 * W + lane) * V >= D) continue;
+      for (int k = 0; k < NV; k++)
+        if (in_row(k))
 #pragma unroll
-        for (int j = 0; j < V; j++) ss += (u[k][j] - mean) * (u[k][j] - mean);
-      }
-      const float rs = rsqrtf(row_sum<W>(ss, red) * inv + a.eps);
-#pragma unroll
-      for (int k = 0; k < NV; k++) {
-        const int c = (k * 32 * W + lane) * V;
-        if (c < D && live) {
-          float w[V];
-          if (a.wpost) load_vec<V>(a.wpost + c, w);
-#pragma unroll
-          for (int j = 0; j < V; j++) u[k][j] = (u[k][j] - mean) * rs * (a.wpost ? w[j] : 1.f);
-          if (a.bpost) {
-            load_vec<V>(a.bpost + c, w);
-#pragma unroll
-            for (int j = 0; j < V; j++) u[k][j] += w[j];
-          }
-          if (a.gamma) load_vec<V>(a.gamma + c, w);
-#pragma unroll
-          for (int j = 0; j < V; j++)
-            y[k][j] += a.alpha * (a.gamma ? w[j] : 1.f) * (gate_of(a.gate, gg[k][j]) * u[k][j]);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int k = 0; k < NV; k++) {
-        const int c = (k * 32 * W + lane) * V;
-#pragma unroll
-        for (int j = 0; j < V; j++) y[k][j] = 0.f;
-        if (c < D && in) load_elems<XT, V>(x + c, y[k]);
-      }
-    }
-    if (a.xo && in) {
-      elem_t<XT> *xo = (elem_t<XT> *)a.xo + r * a.xos;
-#pragma unroll
-      for (int k = 0; k < NV; k++) {
-        const int c = (k * 32 * W + lane) * V;
-        if (c < D) store_elems<XT, V>(xo + c, y[k]);
-      }
-    }
-    if (!a.h) continue;
-    float mean = 0.f, ss = 0.f;
-    if (a.layer) {
+          for (int j = 0; j < V; j++) ss += (rf[k].at(j) - mean) * (rf[k].at(j) - mean);
+      const float rs = rsqrtf(block_sum(ss, red, calls) * inv + a.eps);
 #pragma unroll
       for (int k = 0; k < NV; k++)
 #pragma unroll
-        for (int j = 0; j < V; j++) mean += y[k][j];
-      mean = row_sum<W>(mean, red) * inv;
+        for (int j = 0; j < V; j++) {
+          float u = (rf[k].at(j) - mean) * rs * cu[k][j];
+          if constexpr (B) u += bu[k][j];
+          y[k][j] += gate_of(a.gate, rg[k].at(j)) * u;
+        }
     }
+    if (a.xo) {
+      elem_t<XT> *xo = (elem_t<XT> *)a.xo + r * a.xos;
 #pragma unroll
-    for (int k = 0; k < NV; k++) {
-      if ((k * 32 * W + lane) * V >= D) continue;
-#pragma unroll
-      for (int j = 0; j < V; j++) ss += (y[k][j] - mean) * (y[k][j] - mean);
+      for (int k = 0; k < NV; k++)
+        if (in_row(k)) store_elems<XT, V>(xo + (k * blockDim.x + threadIdx.x) * V, y[k]);
     }
-    const float rs = rsqrtf(row_sum<W>(ss, red) * inv + a.eps);
-    if (!in) continue;
-    elem_t<FT> *h = (elem_t<FT> *)a.h + r * a.hs;
+    if (a.h) {
+      float mean = 0.f, ss = 0.f;
+      if (a.layer) {
 #pragma unroll
-    for (int k = 0; k < NV; k++) {
-      const int c = (k * 32 * W + lane) * V;
-      if (c >= D) continue;
-      float w[V], b[V], o[V];
-      if (a.wpre) load_vec<V>(a.wpre + c, w);
-      if (a.bpre) load_vec<V>(a.bpre + c, b);
+        for (int k = 0; k < NV; k++)
+          if (in_row(k))
 #pragma unroll
-      for (int j = 0; j < V; j++) {
-        o[j] = (y[k][j] - mean) * rs * (a.wpre ? w[j] : 1.f);
-        if (a.bpre) o[j] += b[j];
-        if (!live) o[j] = 0.f;
+            for (int j = 0; j < V; j++) mean += y[k][j];
+        mean = block_sum(mean, red, calls) * inv;
       }
-      store_elems<FT, V>(h + c, o);
+#pragma unroll
+      for (int k = 0; k < NV; k++)
+        if (in_row(k))
+#pragma unroll
+          for (int j = 0; j < V; j++) ss += (y[k][j] - mean) * (y[k][j] - mean);
+      const float rs = rsqrtf(block_sum(ss, red, calls) * inv + a.eps);
+      elem_t<FT> *h = (elem_t<FT> *)a.h + r * a.hs;
+#pragma unroll
+      for (int k = 0; k < NV; k++) {
+        if (!in_row(k)) continue;
+        float o[V];
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+          o[j] = (y[k][j] - mean) * rs * ch[k][j];
+          if constexpr (B) o[j] += bh[k][j];
+          if (!live) o[j] = 0.f;
+        }
+        store_elems<FT, V>(h + (k * blockDim.x + threadIdx.x) * V, o);
+      }
     }
+#pragma unroll
+    for (int k = 0; k < NV; k++) { rx[k] = nx[k]; rf[k] = nf[k]; rg[k] = ng[k]; }
+    live = next_live;
   }
 }
 
@@ -178,7 +216,8 @@ __global__ void __launch_bounds__(kNormThreads) k_norm_gate(const NormArgs a) {
 // sum (the rows stay in L1 / L2), stored in the last pass, which reads an element's inputs before it writes there.
 template <int XT, int FT>
 __global__ void __launch_bounds__(kNormThreads) k_norm_gate_wide(const NormArgs a) {
-  __shared__ float red[kNormThreads / 32];
+  __shared__ float red[2][8];
+  int calls = 0;
   const int D = a.D;
   const float inv = 1.f / (float)D;
   for (long long r = blockIdx.x; r < a.rows; r += gridDim.x) {
@@ -190,14 +229,14 @@ __global__ void __launch_bounds__(kNormThreads) k_norm_gate_wide(const NormArgs 
       float s = 0.f;
       if (a.layer) {
         for (int c = threadIdx.x; c < D; c += kNormThreads) s += Elem<FT>::get(f[c]);
-        fm = row_sum<kNormThreads / 32>(s, red) * inv;
+        fm = block_sum(s, red, calls) * inv;
       }
       s = 0.f;
       for (int c = threadIdx.x; c < D; c += kNormThreads) {
         const float v = Elem<FT>::get(f[c]) - fm;
         s += v * v;
       }
-      frs = rsqrtf(row_sum<kNormThreads / 32>(s, red) * inv + a.eps);
+      frs = rsqrtf(block_sum(s, red, calls) * inv + a.eps);
     }
     auto y_at = [&](int c) {
       float y = Elem<XT>::get(x[c]);
@@ -213,14 +252,14 @@ __global__ void __launch_bounds__(kNormThreads) k_norm_gate_wide(const NormArgs 
       float s = 0.f;
       if (a.layer) {
         for (int c = threadIdx.x; c < D; c += kNormThreads) s += y_at(c);
-        mean = row_sum<kNormThreads / 32>(s, red) * inv;
+        mean = block_sum(s, red, calls) * inv;
       }
       s = 0.f;
       for (int c = threadIdx.x; c < D; c += kNormThreads) {
         const float v = y_at(c) - mean;
         s += v * v;
       }
-      rs = rsqrtf(row_sum<kNormThreads / 32>(s, red) * inv + a.eps);
+      rs = rsqrtf(block_sum(s, red, calls) * inv + a.eps);
     }
     for (int c = threadIdx.x; c < D; c += kNormThreads) {
       const float y = y_at(c);
@@ -234,34 +273,24 @@ __global__ void __launch_bounds__(kNormThreads) k_norm_gate_wide(const NormArgs 
   }
 }
 
-template <int XT, int FT, int V, int NV, int W>
-cudaError_t launch_w(const NormArgs &a, cudaStream_t st) {
-  constexpr int R = kNormThreads / (32 * W);
-  const long long blocks = (a.rows + (long long)R - 1) / R, most = 8LL * num_sms();
-  k_norm_gate<XT, FT, V, NV, W><<<(int)(blocks < most ? blocks : most), kNormThreads, 0, st>>>(a);
+template <int XT, int FT, int V, int NV>
+cudaError_t launch_rows(const NormArgs &a, cudaStream_t st) {
+  const int warps = (a.D + 32 * V * NV - 1) / (32 * V * NV);
+  const long long most = (long long)num_sms() * (24 / warps);
+  const int blocks = (int)(a.rows < most ? a.rows : most);
+  if (a.bpost || a.bpre) k_norm_gate<XT, FT, V, NV, true><<<blocks, 32 * warps, 0, st>>>(a);
+  else k_norm_gate<XT, FT, V, NV, false><<<blocks, 32 * warps, 0, st>>>(a);
   return cudaGetLastError();
 }
 
 template <int XT, int FT>
 cudaError_t launch_norm(const NormArgs &a, bool vec, cudaStream_t st) {
-  const int units = vec ? a.D / 8 : a.D;
-  // few rows: a row over as many warps as give each thread one group; many: as few warps as hold the row
-  const bool few = a.rows < 8 * num_sms();
   if (vec) {
-    if (few || units > 256) {
-      if (units <= 32) return launch_w<XT, FT, 8, 1, 1>(a, st);
-      if (units <= 128) return launch_w<XT, FT, 8, 1, 4>(a, st);
-      if (units <= 256) return launch_w<XT, FT, 8, 1, 8>(a, st);
-      if (units <= 1024) return launch_w<XT, FT, 8, 4, 8>(a, st);
-    } else {
-      if (units <= 32) return launch_w<XT, FT, 8, 1, 1>(a, st);
-      if (units <= 128) return launch_w<XT, FT, 8, 4, 1>(a, st);
-      return launch_w<XT, FT, 8, 8, 1>(a, st);
-    }
+    if (a.D <= 2048) return launch_rows<XT, FT, 8, 1>(a, st);
+    if (a.D <= 8192) return launch_rows<XT, FT, 8, 4>(a, st);
   } else {
-    if (units <= 256) return launch_w<XT, FT, 1, 8, 1>(a, st);
-    if (units <= 1024) return few ? launch_w<XT, FT, 1, 4, 8>(a, st) : launch_w<XT, FT, 1, 32, 1>(a, st);
-    if (units <= 2048) return launch_w<XT, FT, 1, 8, 8>(a, st);
+    if (a.D <= 1024) return launch_rows<XT, FT, 1, 4>(a, st);
+    if (a.D <= 2048) return launch_rows<XT, FT, 1, 8>(a, st);
   }
   const long long most = 8LL * num_sms();
   k_norm_gate_wide<XT, FT><<<(int)(a.rows < most ? a.rows : most), kNormThreads, 0, st>>>(a);
