@@ -2,8 +2,8 @@
 //
 //   y_r = W x_r + bias + h_r B_a^T,   h_r = s_a A_a x_r,   a = slot[r] (none where it is outside [0, slots))
 //
-// W [N][K], A [slots][rank][K], B [slots][N][rank]; sums in fp32. Two launches: h (k_lowrank_down), then y in one of two
-// forms by the number of rows; the second launch starts while the first runs (programmatic dependent launch) and waits
+// W [N][K], A [slots][rank][K], B [slots][N][rank]; sums in fp32. Two launches: h (k_lowrank_down), then y in one of three
+// forms by the number of rows (one launch for one or two rows); the second launch starts while the first runs (programmatic dependent launch) and waits
 // for h only where it is used, after its sums over K.
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -111,32 +111,27 @@ __global__ void __launch_bounds__(256) k_lowrank_down(int rows, int K, const ele
   }
 }
 
-// ------------------------------------------------------------------ few rows
+// ------------------------------------------------------------------ up to 16 rows
 //
-// Bound by reading W (and the adapters' B) once. One CTA per 16 MT rows of W: warp-level matrix instructions with W as
-// the 16-row operand and 8 NT rows of x as the other, K dealt to 8 warps as above, all of a warp's loads independent; the
-// warps' sums are joined in shared memory, then each lane takes some rows' outputs of one column and adds their rank
-// products with B from the rows' adapters (neighbouring lanes' rows of B are neighbours in memory; the loads of all of a
-// lane's outputs are in flight together, the first of them before the wait for h).
-template <int T, int OT, int MT, int NT>
+// Bound by reading W (and the adapters' B) once, and by latency. One CTA per 16 MT rows of W: warp-level matrix
+// instructions with W as the 16-row operand and 8 NT rows of x as the other, K dealt to 8 warps as above; the warps' sums
+// are joined in shared memory, then each lane takes some rows' outputs of one column and adds their rank products with B
+// from the rows' adapters (neighbouring lanes' rows of B are neighbours in memory; the loads of all of a lane's outputs
+// are in flight together, the first of them before the wait for h).
+// kOwn: the CTA forms h of its (one or two) rows itself, while W is on its way: a second read of A from L2 by every CTA
+// in place of a launch and its end.
+constexpr int kFewRows = 16, kOwnRows = 2;
+
+template <int T, int OT, int MT, int NT, bool kOwn>
 __global__ void __launch_bounds__(256) k_lowrank_few(const bnnk_lowrank_args p) {
-  extern __shared__ float red[];  // [8][16 MT][8 NT + 1]
-  constexpr int P = 8 * NT + 1;
+  constexpr int P = 8 * NT + 1, CN = 16 * MT;
+  __shared__ float red[8][CN][P];
+  __shared__ __align__(16) float s_h[kOwn ? kOwnRows : 1][64];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, q = lane % 4;
-  const int n0 = blockIdx.x * 16 * MT, K = p.K, rank = p.rank;
+  const int n0 = blockIdx.x * CN, K = p.K, rank = p.rank;
   const elem_t<T> *W = (const elem_t<T> *)p.w, *x = (const elem_t<T> *)p.x, *B = (const elem_t<T> *)p.b;
-  // the rows of B that the outputs here need, on their way to L2 while W is read
-  if (p.slot)
-    for (int i = threadIdx.x; i < p.rows * 16 * MT; i += 256) {
-      const int n = n0 + i % (16 * MT), s = p.slot[i / (16 * MT)];
-      if (n < p.N && s >= 0 && s < p.slots) {
-        const elem_t<T> *b = B + ((long long)s * p.N + n) * rank;
-        asm volatile("prefetch.global.L2 [%0];" ::"l"(b));
-        if (rank > 32) asm volatile("prefetch.global.L2 [%0];" ::"l"(b + rank - 1));
-      }
-    }
   float acc[MT][NT][4] = {};
-#pragma unroll 2
+#pragma unroll 4
   for (int k0 = 32 * warp; k0 < K; k0 += 256) {
     const int k = k0 + 8 * q;
     uint4 wa[MT], wb[MT];
@@ -159,14 +154,10 @@ __global__ void __launch_bounds__(256) k_lowrank_few(const bnnk_lowrank_args p) 
 #pragma unroll
   for (int m = 0; m < MT; m++)
 #pragma unroll
-    for (int j = 0; j < NT; j++) {
-      float *r = red + (warp * 16 * MT + 16 * m + g) * P + 8 * j + 2 * q;
-      r[0] = acc[m][j][0];
-      r[1] = acc[m][j][1];
-      r[8 * P] = acc[m][j][2];
-      r[8 * P + 1] = acc[m][j][3];
-    }
-  constexpr int CN = 16 * MT, OUTS = (8 * NT * CN + 255) / 256, RSTEP = 256 / CN;  // a lane's rows: r0, r0 + RSTEP, ..
+    for (int j = 0; j < NT; j++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) red[warp][16 * m + g + 8 * (e / 2)][8 * j + 2 * q + e % 2] = acc[m][j][e];
+  constexpr int OUTS = (8 * NT * CN + 255) / 256, RSTEP = 256 / CN;  // a lane's rows: r0, r0 + RSTEP, ..
   const int c = threadIdx.x % CN, r0 = threadIdx.x / CN, n = n0 + c;
   float u[OUTS];
   int s[OUTS];
@@ -177,16 +168,45 @@ __global__ void __launch_bounds__(256) k_lowrank_few(const bnnk_lowrank_args p) 
     s[o] = p.slot && r < p.rows && n < p.N ? p.slot[r] : -1;
     if (s[o] >= p.slots) s[o] = -1;
   }
+  if (kOwn) {
+    for (int r = 0; r < p.rows; r++) {
+      const int sr = p.slot[r];
+      if (sr < 0 || sr >= p.slots) continue;
+      const elem_t<T> *a = (const elem_t<T> *)p.a + (long long)sr * rank * K;
+      float h[8] = {};  // rank indexes warp, warp + 8, ..
+      for (int k = 8 * lane; k < K; k += 256) {
+        float xv[8];
+        load_elems<T, 8>(x + r * p.ldx + k, xv);
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          if (warp + 8 * j >= rank) break;
+          float av[8];
+          load_elems<T, 8>(a + (long long)(warp + 8 * j) * K + k, av);
+#pragma unroll
+          for (int e = 0; e < 8; e++) h[j] = fmaf(xv[e], av[e], h[j]);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        if (warp + 8 * j >= rank) break;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) h[j] += __shfl_xor_sync(0xffffffffu, h[j], o);
+        if (lane == 0) s_h[r][warp + 8 * j] = h[j] * (p.scale ? p.scale[sr] : 1.f);
+      }
+    }
+  }
+  __syncthreads();
   if (p.slot) {
     for (int e = 0; e < rank; e += 8) {
       uint4 b[OUTS];
 #pragma unroll
       for (int o = 0; o < OUTS; o++) b[o] = ldg16(B + ((long long)s[o] * p.N + n) * rank + e, s[o] >= 0);
-      if (e == 0) wait_launch_before();
+      if (!kOwn && e == 0) wait_launch_before();
 #pragma unroll
       for (int o = 0; o < OUTS; o++) {
         if (s[o] < 0) continue;
-        const float *h = p.hid + (long long)(r0 + o * RSTEP) * rank + e;
+        const int r = r0 + o * RSTEP;
+        const float *h = kOwn ? s_h[r] + e : p.hid + (long long)r * rank + e;
         const float4 h0 = *reinterpret_cast<const float4 *>(h), h1 = *reinterpret_cast<const float4 *>(h + 4);
         const float2 b0 = unpack2<T>(b[o].x), b1 = unpack2<T>(b[o].y), b2 = unpack2<T>(b[o].z), b3 = unpack2<T>(b[o].w);
         u[o] = fmaf(h0.x, b0.x, u[o]); u[o] = fmaf(h0.y, b0.y, u[o]);
@@ -196,7 +216,6 @@ __global__ void __launch_bounds__(256) k_lowrank_few(const bnnk_lowrank_args p) 
       }
     }
   }
-  __syncthreads();
   const float bias = p.bias && n < p.N ? p.bias[n] : 0.f;
 #pragma unroll
   for (int o = 0; o < OUTS; o++) {
@@ -204,9 +223,170 @@ __global__ void __launch_bounds__(256) k_lowrank_few(const bnnk_lowrank_args p) 
     if (r >= p.rows || n >= p.N) continue;
     float v = bias;
 #pragma unroll
-    for (int w = 0; w < 8; w++) v += red[(w * CN + c) * P + r];
+    for (int w = 0; w < 8; w++) v += red[w][c][r];
     ((elem_t<OT> *)p.y)[r * p.ldy + n] = Elem<OT>::put(v + u[o]);
   }
+}
+
+// ------------------------------------------------------------------ 17 to 64 rows
+//
+// Still bound by reading W and, with an adapter a row, B: a tcgen05 tile of the (up to 64 of 128) rows and 16 GR columns a
+// CTA, x and W streamed by TMA through a ring deep enough for the memory's latency, one thread issuing. Meanwhile 8 warps
+// load the rows of B that the tile's outputs need (a thread 4 rows' outputs in each group of 16 columns), wait for h, and
+// form the rank products in fp32 on the CUDA cores (with an adapter a row there is nothing for a matrix instruction to
+// share); the accumulator then comes from TMEM through shared memory to the threads that hold them.
+constexpr int kMidRows = 64, kMidThreads = 320, kMidStages = 8;
+
+struct MidArgs {
+  bnnk_lowrank_args p;
+  int nkb, stages;
+  int *err;
+};
+
+template <int T, int OT, int GR>
+__global__ void __launch_bounds__(kMidThreads, 1) k_lowrank_mid(const __grid_constant__ CUtensorMap mx,
+                                                               const __grid_constant__ CUtensorMap mw, const MidArgs a) {
+  constexpr int BN = 16 * GR, RI = kMidRows / 16;
+  extern __shared__ uint8_t dsmem[];
+  __shared__ __align__(8) unsigned long long b_full[kMidStages], b_empty[kMidStages], b_acc, b_out;
+  __shared__ uint32_t tmem_s;
+  __shared__ volatile int abort_s;
+  __shared__ float s_y[kMidRows][BN + 1];
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
+  const bnnk_lowrank_args &p = a.p;
+  constexpr uint32_t a_bytes = 128 * 128, stage = (128 + BN) * 128, tmem_cols = BN <= 32 ? 32 : 64;
+  const int S = a.stages, n0 = blockIdx.x * BN;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; s++) { mbar_init(smem_u32(&b_full[s]), 1); mbar_init(smem_u32(&b_empty[s]), 1); }
+    mbar_init(smem_u32(&b_acc), 1);
+    mbar_init(smem_u32(&b_out), 8);
+    abort_s = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_s)),
+                 "r"(tmem_cols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_s, 0), base = (smem_u32(dsmem) + 1023u) & ~1023u;
+  auto wait = [&](unsigned long long &bar, int parity, int code) {
+    if (__all_sync(0xffffffffu, mbar_try(smem_u32(&bar), parity))) return true;
+    bool ok = mbar_wait_asleep(smem_u32(&bar), parity);
+    ok = __all_sync(0xffffffffu, ok && !abort_s);
+    if (!ok && lane == 0) {
+      if (!abort_s) atomicExch(a.err, code);
+      abort_s = 1;
+    }
+    return ok;
+  };
+  if (warp == 0) {
+    for (int kb = 0; kb < a.nkb; kb++) {
+      const int s = kb % S;
+      if (kb >= S && !wait(b_empty[s], (kb / S - 1) & 1, BNNK_ERR_TMA_WAIT)) break;
+      const uint32_t st = base + s * stage, bar = smem_u32(&b_full[s]);
+      if (elect_one()) {
+        mbar_expect_tx(bar, kMidRows * 128 + BN * 128);  // the rows past 64 of the A tile are never written nor used
+        tma_load_2d(st, &mx, bar, kb * 64, 0);
+        tma_load_2d(st + a_bytes, &mw, bar, kb * 64, n0);
+      }
+    }
+  } else if (warp == 1) {
+    constexpr uint32_t idesc = idesc_16(T - 1, BN, 0, 0);
+    bool ok = true;
+    for (int kb = 0; kb < a.nkb && ok; kb++) {
+      const int s = kb % S;
+      if (!(ok = wait(b_full[s], (kb / S) & 1, BNNK_ERR_MMA_WAIT))) break;
+      tc_fence_after();
+      const uint64_t da = smem_desc<128>(base + s * stage), db = smem_desc<128>(base + s * stage + a_bytes);
+      if (elect_one()) {
+#pragma unroll
+        for (int kk = 0; kk < 4; kk++) mma16_ss(tmem, da + kk * 2, db + kk * 2, idesc, (kb | kk) != 0);
+        mma_commit(smem_u32(&b_empty[s]));
+      }
+    }
+    if (ok && elect_one()) mma_commit(smem_u32(&b_acc));
+  } else {
+    const int tid = threadIdx.x - 64, c = tid % 16, r0 = tid / 16, rank = p.rank;
+    const elem_t<T> *B = (const elem_t<T> *)p.b;
+    float u[GR][RI] = {};
+    int s[RI];
+    if (p.slot) {
+#pragma unroll
+      for (int i = 0; i < RI; i++) {
+        s[i] = r0 + 16 * i < p.rows ? p.slot[r0 + 16 * i] : -1;
+        if (s[i] >= p.slots) s[i] = -1;
+      }
+      for (int e = 0; e < rank; e += 16) {  // 16 of the rank at a time; a rank of 8 more ends in a half
+        uint4 b[GR][RI][2];
+#pragma unroll
+        for (int i = 0; i < RI; i++)
+#pragma unroll
+          for (int gr = 0; gr < GR; gr++) {
+            const int n = n0 + 16 * gr + c;
+            const elem_t<T> *bp = B + ((long long)s[i] * p.N + n) * rank + e;
+            b[gr][i][0] = ldg16(bp, s[i] >= 0 && n < p.N);
+            b[gr][i][1] = ldg16(bp + 8, s[i] >= 0 && n < p.N && e + 8 < rank);
+          }
+        if (e == 0) wait_launch_before();
+#pragma unroll
+        for (int i = 0; i < RI; i++) {
+          if (s[i] < 0) continue;
+          const float *h = p.hid + (long long)(r0 + 16 * i) * rank + e;
+#pragma unroll
+          for (int k = 0; k < 2; k++) {
+            if (e + 8 * k >= rank) break;
+            const float4 h0 = *reinterpret_cast<const float4 *>(h + 8 * k), h1 = *reinterpret_cast<const float4 *>(h + 8 * k + 4);
+#pragma unroll
+            for (int gr = 0; gr < GR; gr++) {
+              const uint4 w = b[gr][i][k];
+              const float2 b0 = unpack2<T>(w.x), b1 = unpack2<T>(w.y), b2 = unpack2<T>(w.z), b3 = unpack2<T>(w.w);
+              float v = u[gr][i];
+              v = fmaf(h0.x, b0.x, v); v = fmaf(h0.y, b0.y, v); v = fmaf(h0.z, b1.x, v); v = fmaf(h0.w, b1.y, v);
+              v = fmaf(h1.x, b2.x, v); v = fmaf(h1.y, b2.y, v); v = fmaf(h1.z, b3.x, v); v = fmaf(h1.w, b3.y, v);
+              u[gr][i] = v;
+            }
+          }
+        }
+      }
+    }
+    bool ok = wait(b_acc, 0, BNNK_ERR_EPI_WAIT);
+    if (ok) {
+      tc_fence_after();
+      const int qd = warp % 4;
+      if (qd < kMidRows / 32)  // the quarters that hold rows; the two warps of one share the groups
+        for (int gr = (warp - 2) / 4; gr < GR; gr += 2) {
+          uint32_t x[16];
+          tmem_ld16(tmem + 16 * gr + ((uint32_t)(32 * qd) << 16), x);
+          tmem_wait_ld(x);
+#pragma unroll
+          for (int j = 0; j < 16; j++) s_y[32 * qd + lane][16 * gr + j] = __uint_as_float(x[j]);
+        }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&b_out));
+      ok = wait(b_out, 0, BNNK_ERR_EPI_WAIT);
+    }
+    if (ok) {
+#pragma unroll
+      for (int gr = 0; gr < GR; gr++) {
+        const int n = n0 + 16 * gr + c;
+        if (n >= p.N) continue;
+        const float bias = p.bias ? p.bias[n] : 0.f;
+#pragma unroll
+        for (int i = 0; i < RI; i++) {
+          const int r = r0 + 16 * i;
+          if (r < p.rows) ((elem_t<OT> *)p.y)[r * p.ldy + n] = Elem<OT>::put(s_y[r][16 * gr + c] + bias + u[gr][i]);
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(tmem_cols));
 }
 
 // ------------------------------------------------------------------ many rows
@@ -545,26 +725,44 @@ cudaError_t launch_early(void (*kernel)(Args...), dim3 grid, int threads, size_t
 
 template <int T, int OT, int MT, int NT>
 cudaError_t few_nt(const bnnk_lowrank_args &p, cudaStream_t st) {
-  static SmemAttr attr;
-  const size_t smem = sizeof(float) * 8 * 16 * MT * (8 * NT + 1);
-  const cudaError_t e = attr.ensure(k_lowrank_few<T, OT, MT, NT>, smem);
-  if (e) return e;
   const dim3 grid((p.N + 16 * MT - 1) / (16 * MT));
-  if (p.slot) return launch_early(k_lowrank_few<T, OT, MT, NT>, grid, 256, smem, st, p);
-  k_lowrank_few<T, OT, MT, NT><<<grid, 256, smem, st>>>(p);
+  if (p.slot && p.rows > kOwnRows) return launch_early(k_lowrank_few<T, OT, MT, NT, false>, grid, 256, 0, st, p);
+  if (p.slot) k_lowrank_few<T, OT, MT, NT, true><<<grid, 256, 0, st>>>(p);
+  else k_lowrank_few<T, OT, MT, NT, false><<<grid, 256, 0, st>>>(p);
   return cudaGetLastError();
 }
 
 template <int T, int OT>
 cudaError_t run_few(const bnnk_lowrank_args &p, cudaStream_t st) {
   // 32 rows of W a CTA halve the reads of x; 16 where they would leave SMs idle
-  const bool two = (p.N + 31) / 32 >= num_sms();
-  const int nt = (p.rows + 7) / 8;
-  if (two)
-    return nt <= 1 ? few_nt<T, OT, 2, 1>(p, st) : nt <= 2 ? few_nt<T, OT, 2, 2>(p, st)
-         : nt <= 4 ? few_nt<T, OT, 2, 4>(p, st) : few_nt<T, OT, 2, 8>(p, st);
-  return nt <= 1 ? few_nt<T, OT, 1, 1>(p, st) : nt <= 2 ? few_nt<T, OT, 1, 2>(p, st)
-       : nt <= 4 ? few_nt<T, OT, 1, 4>(p, st) : few_nt<T, OT, 1, 8>(p, st);
+  if ((p.N + 31) / 32 >= num_sms()) return p.rows <= 8 ? few_nt<T, OT, 2, 1>(p, st) : few_nt<T, OT, 2, 2>(p, st);
+  return p.rows <= 8 ? few_nt<T, OT, 1, 1>(p, st) : few_nt<T, OT, 1, 2>(p, st);
+}
+
+template <int T, int OT, int GR>
+int mid_groups(const bnnk_lowrank_args &p, int *err, cudaStream_t st) {
+  constexpr int BN = 16 * GR;
+  constexpr size_t stage = (128 + BN) * 128;
+  MidArgs a = {p, (p.K + 63) / 64, kMidStages, err};
+  constexpr size_t smem = kMidStages * stage + 1024;
+  CUtensorMap mx, mw;
+  int e = encode_rows16(&mx, p.x, T == 2, p.K, p.rows, p.ldx, 64, kMidRows, 128);
+  if (!e) e = encode_rows16(&mw, p.w, T == 2, p.K, p.N, p.ldw, 64, BN, 128);
+  static SmemAttr attr;
+  if (!e) e = attr.ensure(k_lowrank_mid<T, OT, GR>, smem);
+  if (e) return e;
+  const dim3 grid((p.N + BN - 1) / BN);
+  if (p.slot) return launch_early(k_lowrank_mid<T, OT, GR>, grid, kMidThreads, smem, st, mx, mw, a);
+  k_lowrank_mid<T, OT, GR><<<grid, kMidThreads, smem, st>>>(mx, mw, a);
+  return cudaGetLastError();
+}
+
+template <int T, int OT>
+int run_mid(const bnnk_lowrank_args &p, int *err, cudaStream_t st) {
+  // as few columns a CTA as fill the SMs once, up to 48
+  const int n = (p.N + 15) / 16, sms = num_sms();
+  return n <= sms ? mid_groups<T, OT, 1>(p, err, st) : n <= 2 * sms ? mid_groups<T, OT, 2>(p, err, st)
+                                                                    : mid_groups<T, OT, 3>(p, err, st);
 }
 
 template <int T, int OT, int RB>
@@ -610,14 +808,15 @@ void run_down(const bnnk_lowrank_args &p, cudaStream_t st) {
 
 template <int T>
 int run_lowrank(const bnnk_lowrank_args &p, int *err, cudaStream_t st) {
-  if (p.slot) {
+  if (p.slot && p.rows > kOwnRows) {
     if (p.rank <= 16) run_down<T, 2>(p, st);
     else if (p.rank <= 32) run_down<T, 4>(p, st);
     else run_down<T, 8>(p, st);
     const cudaError_t e = cudaGetLastError();
     if (e) return e;
   }
-  if (p.rows <= 64) return p.otype == 0 ? run_few<T, 0>(p, st) : run_few<T, T>(p, st);
+  if (p.rows <= kFewRows) return p.otype == 0 ? run_few<T, 0>(p, st) : run_few<T, T>(p, st);
+  if (p.rows <= kMidRows) return p.otype == 0 ? run_mid<T, 0>(p, err, st) : run_mid<T, T>(p, err, st);
   if (p.otype == 0)
     return p.rank <= 16 ? run_many<T, 0, 16>(p, err, st) : p.rank <= 32 ? run_many<T, 0, 32>(p, err, st)
                                                                          : run_many<T, 0, 64>(p, err, st);
