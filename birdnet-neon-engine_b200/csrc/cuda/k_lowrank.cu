@@ -43,32 +43,31 @@ __device__ __forceinline__ uint4 ldg16(const void *p, bool in) {
 
 // ------------------------------------------------------------------ h = s_a A_a x
 //
-// One CTA per (16 rows, one of the adapters among them): the rows against the adapter's rank rows with warp-level matrix
+// One CTA per (16 MR rows, one of the adapters among them): the rows against the adapter's rank rows with warp-level matrix
 // instructions (a product of 16 rows is too small for a 128-row tile, and bound by reading A and x), K in steps of 32
 // dealt to 8 warps, their sums joined in shared memory in warp order. A lane's 16 bytes are 8 consecutive k of a row: the
 // two instructions of a step take them in the same order from both operands, so their k are a permutation of the
-// layout's, the same for both. Rows of other adapters are computed and dropped.
+// layout's, the same for both. Rows of other adapters are computed and dropped. MR 2 halves the reads of A where there
+// are rows enough (9001 rows of 1536, rank 32: 213 us for the whole operator, 217 with MR 1).
 constexpr int kDownRows = 16;
 
-template <int T, int RT>  // RT: 8-wide tiles of the rank
+template <int T, int RT, int MR>  // RT: 8-wide tiles of the rank
 __global__ void __launch_bounds__(256) k_lowrank_down(int rows, int K, const elem_t<T> *x, long long ldx,
                                                       const int32_t *slot, int slots, int rank, const elem_t<T> *A,
                                                       const float *scale, float *hid) {
-  __shared__ float red[8][kDownRows][RT * 8 + 1];
-  __shared__ int s_slot[kDownRows];
+  constexpr int R = kDownRows * MR;
+  __shared__ float red[8][R][RT * 8 + 1];
+  __shared__ int s_slot[R];
+  wait_launch_before();  // the rows may be another launch's, and h is still read by this operator's last
   launch_dependents();
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, q = lane % 4;
-  const long long r0 = (long long)blockIdx.x * kDownRows;
-  if (warp == 0) {
-    int s = -1;
-    if (lane < kDownRows && r0 + lane < rows) {
-      s = slot[r0 + lane];
-      if (s >= slots) s = -1;
-    }
-    if (lane < kDownRows) s_slot[lane] = s;
+  const long long r0 = (long long)blockIdx.x * R;
+  if (threadIdx.x < R) {
+    int s = r0 + threadIdx.x < rows ? slot[r0 + threadIdx.x] : -1;
+    s_slot[threadIdx.x] = s < slots ? s : -1;
   }
   __syncthreads();
-  const int mine = lane < kDownRows ? s_slot[lane] : -1;
+  const int mine = lane < R ? s_slot[lane] : -1;
   // the first row of each adapter here
   const unsigned same = __match_any_sync(0xffffffffu, mine);
   unsigned first = __ballot_sync(0xffffffffu, mine >= 0 && __ffs(same) - 1 == lane);
@@ -76,31 +75,37 @@ __global__ void __launch_bounds__(256) k_lowrank_down(int rows, int K, const ele
     if (e % (int)gridDim.y != (int)blockIdx.y) continue;
     const int s = s_slot[__ffs(first) - 1];
     const elem_t<T> *a = A + (long long)s * rank * K;
-    const elem_t<T> *x0 = x + (r0 + g) * ldx, *x1 = x0 + 8 * ldx;
-    const bool in0 = r0 + g < rows, in1 = r0 + g + 8 < rows;
-    float acc[RT][4] = {};
-#pragma unroll 4
+    float acc[MR][RT][4] = {};
+#pragma unroll(4 / MR)
     for (int k0 = 32 * warp; k0 < K; k0 += 256) {
       const int k = k0 + 8 * q;
-      const uint4 xa = ldg16(x0 + k, in0 && k < K), xb = ldg16(x1 + k, in1 && k < K);
+      uint4 xa[MR], xb[MR];
+#pragma unroll
+      for (int m = 0; m < MR; m++) {
+        const long long r = r0 + 16 * m + g;
+        xa[m] = ldg16(x + r * ldx + k, r < rows && k < K);
+        xb[m] = ldg16(x + (r + 8) * ldx + k, r + 8 < rows && k < K);
+      }
 #pragma unroll
       for (int j = 0; j < RT; j++) {
         const uint4 b = ldg16(a + (long long)(8 * j + g) * K + k, 8 * j + g < rank && k < K);
-        mma_sync<T>(acc[j], xa.x, xb.x, xa.y, xb.y, b.x, b.y);
-        mma_sync<T>(acc[j], xa.z, xb.z, xa.w, xb.w, b.z, b.w);
+#pragma unroll
+        for (int m = 0; m < MR; m++) {
+          mma_sync<T>(acc[m][j], xa[m].x, xb[m].x, xa[m].y, xb[m].y, b.x, b.y);
+          mma_sync<T>(acc[m][j], xa[m].z, xb[m].z, xa[m].w, xb[m].w, b.z, b.w);
+        }
       }
     }
     __syncthreads();  // the sums of the adapter before have been read
 #pragma unroll
-    for (int j = 0; j < RT; j++) {
-      red[warp][g][8 * j + 2 * q] = acc[j][0];
-      red[warp][g][8 * j + 2 * q + 1] = acc[j][1];
-      red[warp][g + 8][8 * j + 2 * q] = acc[j][2];
-      red[warp][g + 8][8 * j + 2 * q + 1] = acc[j][3];
-    }
+    for (int m = 0; m < MR; m++)
+#pragma unroll
+      for (int j = 0; j < RT; j++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) red[warp][16 * m + g + 8 * (i / 2)][8 * j + 2 * q + i % 2] = acc[m][j][i];
     __syncthreads();
     const float f = scale ? scale[s] : 1.f;
-    for (int i = threadIdx.x; i < kDownRows * rank; i += 256) {
+    for (int i = threadIdx.x; i < R * rank; i += 256) {
       const int r = i / rank, c = i % rank;
       if (s_slot[r] != s) continue;
       float v = 0.f;
@@ -129,6 +134,7 @@ __global__ void __launch_bounds__(256) k_lowrank_few(const bnnk_lowrank_args p) 
   __shared__ __align__(16) float s_h[kOwn ? kOwnRows : 1][64];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, q = lane % 4;
   const int n0 = blockIdx.x * CN, K = p.K, rank = p.rank;
+  launch_dependents();
   const elem_t<T> *W = (const elem_t<T> *)p.w, *x = (const elem_t<T> *)p.x, *B = (const elem_t<T> *)p.b;
   float acc[MT][NT][4] = {};
 #pragma unroll 4
@@ -234,7 +240,9 @@ __global__ void __launch_bounds__(256) k_lowrank_few(const bnnk_lowrank_args p) 
 // CTA, x and W streamed by TMA through a ring deep enough for the memory's latency, one thread issuing. Meanwhile 8 warps
 // load the rows of B that the tile's outputs need (a thread 4 rows' outputs in each group of 16 columns), wait for h, and
 // form the rank products in fp32 on the CUDA cores (with an adapter a row there is nothing for a matrix instruction to
-// share); the accumulator then comes from TMEM through shared memory to the threads that hold them.
+// share); the accumulators then come from TMEM through shared memory to the threads that hold them. Four accumulators take
+// a stage's four steps of 16: the tensor cores' fp32 sums lose a little at every step (K 1024 in one chain was 6.9e-7 off
+// in fp32 outputs, against 2.6e-7 for a plain fp32 sum), so the chains are kept short.
 constexpr int kMidRows = 64, kMidThreads = 320, kMidStages = 8;
 
 struct MidArgs {
@@ -254,8 +262,9 @@ __global__ void __launch_bounds__(kMidThreads, 1) k_lowrank_mid(const __grid_con
   __shared__ float s_y[kMidRows][BN + 1];
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   const bnnk_lowrank_args &p = a.p;
-  constexpr uint32_t a_bytes = 128 * 128, stage = (128 + BN) * 128, tmem_cols = BN <= 32 ? 32 : 64;
+  constexpr uint32_t a_bytes = 128 * 128, stage = (128 + BN) * 128, tmem_cols = BN == 48 ? 256 : 4 * BN;
   const int S = a.stages, n0 = blockIdx.x * BN;
+  launch_dependents();
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; s++) { mbar_init(smem_u32(&b_full[s]), 1); mbar_init(smem_u32(&b_empty[s]), 1); }
     mbar_init(smem_u32(&b_acc), 1);
@@ -303,7 +312,7 @@ __global__ void __launch_bounds__(kMidThreads, 1) k_lowrank_mid(const __grid_con
       const uint64_t da = smem_desc<128>(base + s * stage), db = smem_desc<128>(base + s * stage + a_bytes);
       if (elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < 4; kk++) mma16_ss(tmem, da + kk * 2, db + kk * 2, idesc, (kb | kk) != 0);
+        for (int kk = 0; kk < 4; kk++) mma16_ss(tmem + kk * BN, da + kk * 2, db + kk * 2, idesc, kb != 0);
         mma_commit(smem_u32(&b_empty[s]));
       }
     }
@@ -358,11 +367,19 @@ __global__ void __launch_bounds__(kMidThreads, 1) k_lowrank_mid(const __grid_con
       const int qd = warp % 4;
       if (qd < kMidRows / 32)  // the quarters that hold rows; the two warps of one share the groups
         for (int gr = (warp - 2) / 4; gr < GR; gr += 2) {
-          uint32_t x[16];
-          tmem_ld16(tmem + 16 * gr + ((uint32_t)(32 * qd) << 16), x);
-          tmem_wait_ld(x);
+          const uint32_t tq = tmem + 16 * gr + ((uint32_t)(32 * qd) << 16);
+          uint32_t x[16], y[16];
+          float v[16];
+          tmem_ld16(tq, x);
+          tmem_ld16(tq + BN, y);
+          tmem_wait_ld(x, y);
 #pragma unroll
-          for (int j = 0; j < 16; j++) s_y[32 * qd + lane][16 * gr + j] = __uint_as_float(x[j]);
+          for (int j = 0; j < 16; j++) v[j] = __uint_as_float(x[j]) + __uint_as_float(y[j]);
+          tmem_ld16(tq + 2 * BN, x);
+          tmem_ld16(tq + 3 * BN, y);
+          tmem_wait_ld(x, y);
+#pragma unroll
+          for (int j = 0; j < 16; j++) s_y[32 * qd + lane][16 * gr + j] = v[j] + (__uint_as_float(x[j]) + __uint_as_float(y[j]));
         }
       tc_fence_before();
       __syncwarp();
@@ -408,7 +425,8 @@ constexpr int kLrPad = 17;  // words a row of the stores' shared memory: blocks 
 
 struct LrArgs {
   bnnk_lowrank_args p;
-  int nkb, bn, n_tiles, tiles, stages, acc_cols, tmem_cols;
+  int nkb, bn, n_tiles, tiles, stages, tmem_cols;
+  int na, acc_cols;  // accumulators of a tile (a power of two, the sum's steps in turn) and their columns
   int *err;
 };
 
@@ -427,6 +445,7 @@ __global__ void __launch_bounds__(kLrThreads, 1) k_lowrank_many(const __grid_con
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   const bnnk_lowrank_args &p = a.p;
   const int S = a.stages, bn = a.bn;
+  launch_dependents();
   const uint32_t a_bytes = 128 * 128, stage = (128 + bn) * 128;
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; s++) { mbar_init(smem_u32(&b_full[s]), 5); mbar_init(smem_u32(&b_empty[s]), 1); }
@@ -511,14 +530,15 @@ __global__ void __launch_bounds__(kLrThreads, 1) k_lowrank_many(const __grid_con
     for (int t = blockIdx.x; t < a.tiles && ok; t += gridDim.x, lt++) {
       const int g = lt & 1;
       if (lt >= 2 && !(ok = wait(b_accempty[g], (lt / 2 - 1) & 1, BNNK_ERR_MMA_WAIT))) break;
-      const uint32_t acc = tmem + g * a.acc_cols;
+      const uint32_t acc = tmem + g * a.na * a.acc_cols;
       for (int kb = 0; kb < a.nkb; kb++, at.next(S)) {
         if (!(ok = wait(b_full[at.s], at.parity, BNNK_ERR_MMA_WAIT))) break;
         tc_fence_after();
         const uint64_t da = smem_desc<128>(base + at.s * stage), db = smem_desc<128>(base + at.s * stage + a_bytes);
         if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < 4; kk++) mma16_ss(acc, da + kk * 2, db + kk * 2, idesc, (kb | kk) != 0);
+          for (int kk = 0; kk < 4; kk++)
+            mma16_ss(acc + (kk & (a.na - 1)) * a.acc_cols, da + kk * 2, db + kk * 2, idesc, kb != 0 || kk >= a.na);
           mma_commit(smem_u32(&b_empty[at.s]));
         }
       }
@@ -642,7 +662,7 @@ __global__ void __launch_bounds__(kLrThreads, 1) k_lowrank_many(const __grid_con
       if (!wait(b_acc[g], (lt >> 1) & 1, BNNK_ERR_EPI_WAIT)) break;
       tc_fence_after();
       const bool big = T == 1 && adapters && s_big[g][32 * qd + lane];
-      const uint32_t tq = tmem + g * a.acc_cols + ((uint32_t)(32 * qd) << 16);
+      const uint32_t tq = tmem + g * a.na * a.acc_cols + ((uint32_t)(32 * qd) << 16);
       const int width = min(bn, p.N - n0), rows = min(32, p.rows - r0);
 #pragma unroll 1
       for (int c0 = h * CW; c0 < width; c0 += 2 * CW) {
@@ -657,6 +677,13 @@ __global__ void __launch_bounds__(kLrThreads, 1) k_lowrank_many(const __grid_con
 #pragma unroll
           for (int j = 0; j < 16; j++)
             v[j] = __uint_as_float(x[j]) + (p.bias && c + j < width ? __ldg(p.bias + n0 + c + j) : 0.f);
+          if (OT == 0)
+            for (int k = 1; k < a.na; k++) {
+              tmem_ld16(tq + k * a.acc_cols + c, x);
+              tmem_wait_ld(x);
+#pragma unroll
+              for (int j = 0; j < 16; j++) v[j] += __uint_as_float(x[j]);
+            }
           if (big) {  // h past fp16's range: its products here
             const int s = p.slot[r0 + lane];
             const float *hh = p.hid + (long long)(r0 + lane) * p.rank;
@@ -669,6 +696,7 @@ __global__ void __launch_bounds__(kLrThreads, 1) k_lowrank_many(const __grid_con
               for (int i = 0; i < 16; i++) v[i] += i == j ? u : 0.f;
             }
           }
+          __syncwarp();
 #pragma unroll
           for (int j = 0; j < 16; j += PW) {
             const uint32_t z = PW == 1 ? __float_as_uint(v[j]) : pack2f<T>(v[j], v[j + PW - 1]);
@@ -771,16 +799,19 @@ int run_many(const bnnk_lowrank_args &p, int *err, cudaStream_t st) {
   a.p = p;
   a.err = err;
   a.nkb = (p.K + 63) / 64;
-  // column tiles of at most 256, of equal widths, narrower while there are fewer tiles than SMs
-  const int n16 = (p.N + 15) & ~15, mt = (p.rows + 127) / 128;
-  int nt = (n16 + 255) / 256;
+  // fp32 outputs: the tensor cores' chains of fp32 sums kept to about 1024 values of K (one of 1024 was 6.9e-7 off, against
+  // 2.6e-7 for a plain fp32 sum); a 16-bit output's rounding hides them
+  a.na = OT != 0 || p.K <= 512 ? 1 : p.K <= 2048 ? 2 : 4;
+  // column tiles of at most 256 / na, of equal widths, narrower while there are fewer tiles than SMs
+  const int n16 = (p.N + 15) & ~15, mt = (p.rows + 127) / 128, most = 256 / a.na;
+  int nt = (n16 + most - 1) / most;
   while ((long long)mt * nt < num_sms() && ((n16 + nt) / (nt + 1) + 15) / 16 * 16 >= 32) nt++;
   a.bn = ((n16 + nt - 1) / nt + 15) & ~15;
   a.n_tiles = (p.N + a.bn - 1) / a.bn;
   if ((long long)mt * a.n_tiles > 0x7fffffffLL) return cudaErrorInvalidValue;
   a.tiles = mt * a.n_tiles;
   a.acc_cols = a.bn <= 32 ? 32 : a.bn <= 64 ? 64 : a.bn <= 128 ? 128 : 256;
-  a.tmem_cols = 2 * a.acc_cols;
+  a.tmem_cols = 2 * a.na * a.acc_cols;
   const size_t stage = (size_t)(128 + a.bn) * 128, out = 8 * 32 * kLrPad * 4;
   const int s = (int)((227 * 1024 - 4096 - out) / stage);
   a.stages = s > kLrStages ? kLrStages : s;
@@ -798,21 +829,24 @@ int run_many(const bnnk_lowrank_args &p, int *err, cudaStream_t st) {
   return cudaGetLastError();
 }
 
+template <int T, int RT, int MR>
+cudaError_t down_rows(const bnnk_lowrank_args &p, int adapters, cudaStream_t st) {
+  return launch_early(k_lowrank_down<T, RT, MR>, dim3((p.rows + kDownRows * MR - 1) / (kDownRows * MR), adapters), 256, 0, st,
+                      p.rows, p.K, (const elem_t<T> *)p.x, p.ldx, p.slot, p.slots, p.rank, (const elem_t<T> *)p.a, p.scale,
+                      p.hid);
+}
+
 template <int T, int RT>
-void run_down(const bnnk_lowrank_args &p, cudaStream_t st) {
+cudaError_t run_down(const bnnk_lowrank_args &p, cudaStream_t st) {
   // an adapter a CTA where there are few rows; of many rows' tiles most hold one adapter
-  const dim3 grid((p.rows + kDownRows - 1) / kDownRows, p.rows <= 512 ? kDownRows : 4);
-  k_lowrank_down<T, RT><<<grid, 256, 0, st>>>(p.rows, p.K, (const elem_t<T> *)p.x, p.ldx, p.slot, p.slots, p.rank,
-                                              (const elem_t<T> *)p.a, p.scale, p.hid);
+  if (p.rows <= 512 || RT == 8) return down_rows<T, RT, 1>(p, p.rows <= 512 ? kDownRows : 2, st);
+  return down_rows<T, RT, RT == 8 ? 1 : 2>(p, 2, st);
 }
 
 template <int T>
 int run_lowrank(const bnnk_lowrank_args &p, int *err, cudaStream_t st) {
   if (p.slot && p.rows > kOwnRows) {
-    if (p.rank <= 16) run_down<T, 2>(p, st);
-    else if (p.rank <= 32) run_down<T, 4>(p, st);
-    else run_down<T, 8>(p, st);
-    const cudaError_t e = cudaGetLastError();
+    const cudaError_t e = p.rank <= 16 ? run_down<T, 2>(p, st) : p.rank <= 32 ? run_down<T, 4>(p, st) : run_down<T, 8>(p, st);
     if (e) return e;
   }
   if (p.rows <= kFewRows) return p.otype == 0 ? run_few<T, 0>(p, st) : run_few<T, T>(p, st);
