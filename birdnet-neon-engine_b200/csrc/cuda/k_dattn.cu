@@ -283,6 +283,27 @@ __device__ __forceinline__ float warp_max(float v) {
   for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
+// Pieces of 4 values among groups of L lanes: before, piece j of lane l is piece l % L of row j of its group; after, piece
+// j of its own row (or back). A warp's memory accesses then cover L x 16 consecutive bytes of few rows.
+template <int L>
+__device__ __forceinline__ void turn_rows(float (&v)[4 * L]) {
+  const int lane = threadIdx.x % 32;
+#pragma unroll
+  for (int b = 1; b < L; b <<= 1) {
+    const bool up = lane & b;
+#pragma unroll
+    for (int j = 0; j < L; j++) {
+      if (j & b) continue;
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const float got = __shfl_xor_sync(0xffffffffu, up ? v[4 * j + e] : v[4 * (j + b) + e], b);
+        if (up) v[4 * j + e] = got;
+        else v[4 * (j + b) + e] = got;
+      }
+    }
+  }
+}
+
 __device__ __forceinline__ void sts128(uint32_t at, const uint32_t (&x)[4]) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
 }
@@ -303,9 +324,11 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
   __shared__ int s_seg[3];
   __shared__ float s_max[2][16], s_inv[2], s_dsc[2];  // fp16: the state warps' maxima, scales of S and of its sums by chunk
   __shared__ float s_pinv[L::scales][T == 1 ? kChunk : 1];  // fp16: the inverse row scales of P
+  __shared__ float s_rowmax[T == 1 ? 2 : 1][2][T == 1 ? kChunk : 1];
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   const DattnArgs &d = a.d;
   const int hk = blockIdx.y, G = kState ? 1 : d.G;
+  launch_dependents();
 
   if (warp == 0) {
     int seq = 0, part = 0;
@@ -555,6 +578,9 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
   } else if (warp >= kDaP && warp < kDaS) {
     // P: row i against the columns j <= i, blocks of 16 columns alternating between two warps
     const int qd = warp % 4, h = (warp - kDaP) / 4, i = 32 * qd + lane;
+    float fixed[16];  // lambda^(15 - j)
+#pragma unroll
+    for (int j = 0; j < 16; j++) fixed[j] = pw[15 - j];
     for (int u = 0; u < (kState ? 0 : nu); u++) {
       const int c = u / G, b = u % NB;
       const long long t = t0 + (long long)c * kChunk;
@@ -565,43 +591,54 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
       tc_fence_after();
       const uint32_t tq = tmem + L::t_qk + b * 128 + ((uint32_t)(qd * 32) << 16);
       float sc = d.scale;
-      if constexpr (T == 1) {  // the row's largest product (the dead columns' and those above the diagonal left out)
+      const int blocks = 2 * qd + 2;  // those that reach the diagonal
+      if constexpr (T == 1) {
+        // a bound of the row's products: all of these blocks' live columns, those above the diagonal too (their size
+        // matters only where it is 2^28 times the others'); the row's two warps a half each
         float m = 0.f;
 #pragma unroll 1
-        for (int blk = 0; blk < 2 * qd + 2; blk++) {
+        for (int blk = h; blk < blocks; blk += 2) {
           uint32_t x[16];
           tmem_ld16(tq + blk * 16, x);
           const uint32_t w = word_of(lw, blk / 2) >> (blk % 2 * 16);
-          const int left = i - 16 * blk;
           tmem_wait_ld(x);
+          if ((w & 0xffffu) != 0xffffu) {
 #pragma unroll
-          for (int j = 0; j < 16; j++) m = fmaxf(m, (w >> j) & 1 && j <= left ? fabsf(__uint_as_float(x[j])) : 0.f);
+            for (int j = 0; j < 16; j++) x[j] = (w >> j) & 1 ? x[j] : 0u;
+          }
+#pragma unroll
+          for (int j = 0; j < 16; j++) m = fmaxf(m, fabsf(__uint_as_float(x[j])));
         }
-        float inv;
-        sc = scale_to_f16(m, inv);
-        if (h == 0) s_pinv[u % L::scales][i] = inv;
-        // every column is read before another warp of this row writes P over it
+        s_rowmax[u & 1][h][i] = m;
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&b_row[qd]));
         if (!wait(b_row[qd], u & 1, BNNK_ERR_EPI_WAIT)) break;
+        float inv;
+        sc = scale_to_f16(fmaxf(m, s_rowmax[u & 1][h ^ 1][i]), inv);
+        if (h == 0) s_pinv[u % L::scales][i] = inv;
       }
-      const int blocks = 2 * qd + 2;  // those that reach the diagonal
       uint32_t x[16];
       if (h < blocks) tmem_ld16(tq + h * 16, x);
 #pragma unroll 1
       for (int blk = h; blk < blocks; blk += 2) {
         uint32_t p[16];
         const uint32_t w = word_of(lw, blk / 2) >> (blk % 2 * 16);
-        const float *f = pw + i - 16 * blk;  // f[-j] = lambda^(i - j), 0 above the diagonal
+        // lambda^(i - j): off the diagonal lambda^(i - 16 blk - 15) lambda^(15 - j), which no power overflows and whose
+        // second factor is the same for every row; on it from the table, 0 above
+        const float *f = pw + i - 16 * blk;
+        const bool diagonal = blk >= 2 * qd;
+        const float f0 = diagonal ? sc : f[-15] * sc;
         tmem_wait_ld(x);
         if ((w & 0xffffu) != 0xffffu) {
 #pragma unroll
           for (int j = 0; j < 16; j++) x[j] = (w >> j) & 1 ? x[j] : 0u;
         }
 #pragma unroll
-        for (int j = 0; j < 16; j += 2)
-          split2<T>(__uint_as_float(x[j]) * (f[-j] * sc), __uint_as_float(x[j + 1]) * (f[-j - 1] * sc), p[j / 2],
-                    p[8 + j / 2]);
+        for (int j = 0; j < 16; j += 2) {
+          const float a0 = __uint_as_float(x[j]) * f0, a1 = __uint_as_float(x[j + 1]) * f0;
+          if (diagonal) split2<T>(a0 * f[-j], a1 * f[-j - 1], p[j / 2], p[8 + j / 2]);
+          else split2<T>(a0 * fixed[j], a1 * fixed[j + 1], p[j / 2], p[8 + j / 2]);
+        }
         if (blk + 2 < blocks) tmem_ld16(tq + (blk + 2) * 16, x);  // the next block, while this one is stored
         tmem_st16(tq + blk * 16, p);
       }
@@ -626,12 +663,18 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
       if (a.seg_tokens) from = a.seg_state + ((long long)blockIdx.x * d.Hk + hk) * d.dk * d.dv;
       else if (d.s0 && slot >= 0) from = d.s0 + (slot * d.Hk + hk) * (long long)d.dk * d.dv;
     }
+    if (!kState && a.seg_tokens) wait_launch_before();  // the states before the segments
+    // in memory order, a row's HC columns by LP neighbouring lanes: with 16 bytes of 32 rows an access, a state of 128 x 128
+    // took 4100 cycles to load and as many to store
+    constexpr int LP = HC / 4;
+    const int mr = r - lane % LP, mc = c0 + lane % LP * 4;  // this lane's rows mr + j and columns there
 #pragma unroll
-    for (int j = 0; j < HC; j += 4) {
+    for (int j = 0; j < LP; j++) {
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (from && r < d.dk && c0 + j < d.dv) v = *reinterpret_cast<const float4 *>(from + (long long)r * d.dv + c0 + j);
-      S[j] = v.x; S[j + 1] = v.y; S[j + 2] = v.z; S[j + 3] = v.w;
+      if (from && mr + j < d.dk && mc < d.dv) v = *reinterpret_cast<const float4 *>(from + (long long)(mr + j) * d.dv + mc);
+      S[4 * j] = v.x; S[4 * j + 1] = v.y; S[4 * j + 2] = v.z; S[4 * j + 3] = v.w;
     }
+    turn_rows<LP>(S);
     // the maximum over the role's threads; a buffer is written again two calls later, when every warp has arrived at
     // the call between and so has read it
     int calls = 0;
@@ -739,9 +782,10 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
           const uint32_t off = p * L::panel + (tid + 512 * m) * 16;
           uint32_t x[4], h[4], l[4], l2[4];
           load(m, p, x);
+          if (off_row) x[0] = x[1] = x[2] = x[3] = 0;
 #pragma unroll
           for (int e = 0; e < 4; e++) {
-            const float2 f = unpack2<T>(off_row ? 0u : x[e]);
+            const float2 f = unpack2<T>(x[e]);
             if constexpr (L::parts == 3) split3<T>(f.x * wt, f.y * wt, h[e], l[e], l2[e]);
             else split2<T>(f.x * wt, f.y * wt, h[e], l[e]);
           }
@@ -801,11 +845,13 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
       } else if (s_seg[2] && d.s1 && slot >= 0) {
         to = d.s1 + (slot * d.Hk + hk) * (long long)d.dk * d.dv;
       }
-      if (to && r < d.dk) {
+      turn_rows<LP>(S);
+      if (to) {
 #pragma unroll
-        for (int j = 0; j < HC; j += 4)
-          if (c0 + j < d.dv)
-            *reinterpret_cast<float4 *>(to + (long long)r * d.dv + c0 + j) = make_float4(S[j], S[j + 1], S[j + 2], S[j + 3]);
+        for (int j = 0; j < LP; j++)
+          if (mr + j < d.dk && mc < d.dv)
+            *reinterpret_cast<float4 *>(to + (long long)(mr + j) * d.dv + mc) =
+                make_float4(S[4 * j], S[4 * j + 1], S[4 * j + 2], S[4 * j + 3]);
       }
     }
   }
@@ -822,6 +868,7 @@ __global__ void __launch_bounds__(256) k_dattn_scan(const DaArgs a) {
   __shared__ int s_first, s_parts;
   __shared__ float s_dec;
   const int i = blockIdx.z, hk = blockIdx.y;
+  launch_dependents();
   if (threadIdx.x < 32) {
     int before = 0, mine = 0;
     for (int j = threadIdx.x; j <= i; j += 32) {
@@ -855,6 +902,7 @@ __global__ void __launch_bounds__(256) k_dattn_scan(const DaArgs a) {
   const long long step = (long long)d.Hk * size;
   const int parts = s_parts;
   const float dec = s_dec;
+  wait_launch_before();  // the segments' own sums
   for (int k0 = 0; k0 < parts; k0 += 8) {  // 8 loads in flight
     float own[8];
 #pragma unroll
@@ -883,11 +931,13 @@ int run_chunk(const DaArgs &a, cudaStream_t st) {
     e = attr_s.ensure(k_dattn_chunk<T, DP, true>, smem);
     if (e) return e;
     k_dattn_chunk<T, DP, true><<<grid, kDaThreads, smem, st>>>(mq, mk, mv, a);
-    k_dattn_scan<<<dim3((d.dk * d.dv + 255) / 256, d.Hk, d.n), 256, 0, st>>>(a);
+    e = launch_early(k_dattn_scan, dim3((d.dk * d.dv + 255) / 256, d.Hk, d.n), 256, 0, st, a);
+    if (e) return e;
   }
   constexpr size_t smem = DaLayout<T, DP, false>::smem;
   e = attr.ensure(k_dattn_chunk<T, DP, false>, smem);
   if (e) return e;
+  if (a.seg_tokens) return launch_early(k_dattn_chunk<T, DP, false>, grid, kDaThreads, smem, st, mq, mk, mv, a);
   k_dattn_chunk<T, DP, false><<<grid, kDaThreads, smem, st>>>(mq, mk, mv, a);
   return cudaGetLastError();
 }

@@ -17,10 +17,6 @@
 namespace bnn {
 namespace {
 
-__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-// the launch before it has ended, its writes are visible
-__device__ __forceinline__ void wait_launch_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
 // D (16 x 8) += A (16 x 16) B (16 x 8), fp32 sums
 template <int T>
 __device__ __forceinline__ void mma_sync(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -733,22 +729,6 @@ __global__ void __launch_bounds__(kLrThreads, 1) k_lowrank_many(const __grid_con
   __syncthreads();
   if (warp == 1)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(a.tmem_cols));
-}
-
-// a launch that may start before the one before it has ended
-template <typename... Args>
-cudaError_t launch_early(void (*kernel)(Args...), dim3 grid, int threads, size_t smem, cudaStream_t st, Args... args) {
-  cudaLaunchConfig_t c = {};
-  c.gridDim = grid;
-  c.blockDim = dim3(threads);
-  c.dynamicSmemBytes = smem;
-  c.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  c.attrs = at;
-  c.numAttrs = 1;
-  return cudaLaunchKernelEx(&c, kernel, args...);
 }
 
 template <int T, int OT, int MT, int NT>

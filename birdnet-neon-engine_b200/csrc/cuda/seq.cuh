@@ -1,8 +1,9 @@
 // Element types of the operators over sequences of windows (BNN_T_F32 / F16 / BF16, include/bnneon_cuda.h): loads to
-// fp32 and the one rounding back.
+// fp32 and the one rounding back; launches that overlap the one before.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <cuda_runtime.h>
 #include <stdint.h>
 
 namespace bnn {
@@ -62,6 +63,28 @@ __device__ __forceinline__ void store_elems(elem_t<T> *p, const float (&v)[V]) {
     *reinterpret_cast<uint4 *>(p) = make_uint4(pack2f<T>(v[0], v[1]), pack2f<T>(v[2], v[3]), pack2f<T>(v[4], v[5]),
                                                pack2f<T>(v[6], v[7]));
   }
+}
+
+// Programmatic dependent launch: the next launch on the stream may start (once every CTA has come here, and as SMs have
+// room), and where the other side waits for this whole launch and its writes
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// the launch before it has ended, its writes are visible
+__device__ __forceinline__ void wait_launch_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// a launch that may start before the one before it has ended
+template <typename... Args>
+cudaError_t launch_early(void (*kernel)(Args...), dim3 grid, int threads, size_t smem, cudaStream_t st, Args... args) {
+  cudaLaunchConfig_t c = {};
+  c.gridDim = grid;
+  c.blockDim = dim3(threads);
+  c.dynamicSmemBytes = smem;
+  c.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  c.attrs = at;
+  c.numAttrs = 1;
+  return cudaLaunchKernelEx(&c, kernel, args...);
 }
 
 }  // namespace bnn
