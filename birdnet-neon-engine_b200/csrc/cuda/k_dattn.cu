@@ -6,6 +6,8 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <type_traits>
+
 #include "bnn_kernels.h"
 #include "seq.cuh"
 #include "smem_attr.cuh"
@@ -158,7 +160,7 @@ __global__ void __launch_bounds__(256) k_dattn_rec(const DattnArgs a) {
 //    scales go into the fp32 steps after the products. Values 2^28 below the maximum are the first to lose bits.
 //
 // One CTA per (segment of a sequence, k/v head) walks the segment's chunks, and for each the G q heads of the group
-// ("unit" u = (chunk, q head)). Roles: warp 0 MMA issue, warp 1 TMA, 8 warps turn QK into P (in place in TMEM, as the A
+// ("unit" u = (chunk, q head)). Roles: warps 0 and 2 MMA issue, warp 1 TMA, 8 warps turn QK into P (in place in TMEM, as the A
 // operand of the last product), 16 warps hold S in registers, form K' and the S operand; one of the two joins O1 and O2
 // into o. S in registers stays fp32: lambda^n S + DS, once a chunk. The roles' loops are rolled: unrolled, their code
 // did not stay in the instruction cache together and a unit took twice as long. The issuing warp stays converged
@@ -343,12 +345,12 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
       s_seg[2] = last;
       for (int s = 0; s < NS; s++) {
         mbar_init(smem_u32(&b_qfull[s]), 1); mbar_init(smem_u32(&b_vfull[s]), 1);
-        mbar_init(smem_u32(&b_qempty[s]), 1); mbar_init(smem_u32(&b_vempty[s]), 1);
+        mbar_init(smem_u32(&b_qempty[s]), 2); mbar_init(smem_u32(&b_vempty[s]), kState ? 1 : 2);
         mbar_init(smem_u32(&b_vfix[s]), 16); mbar_init(smem_u32(&b_kp[s]), 16);
       }
-      for (int s = 0; s < NK; s++) { mbar_init(smem_u32(&b_kfull[s]), 1); mbar_init(smem_u32(&b_kempty[s]), 1); }
+      for (int s = 0; s < NK; s++) { mbar_init(smem_u32(&b_kfull[s]), 1); mbar_init(smem_u32(&b_kempty[s]), kState ? 1 : 2); }
       for (int b = 0; b < NB; b++) { mbar_init(smem_u32(&b_qk[b]), 1); mbar_init(smem_u32(&b_p[b]), 8); }
-      mbar_init(smem_u32(&b_s), 16); mbar_init(smem_u32(&b_ds), 1); mbar_init(smem_u32(&b_o), 1);
+      mbar_init(smem_u32(&b_s), 16); mbar_init(smem_u32(&b_ds), 1); mbar_init(smem_u32(&b_o), 2);
       mbar_init(smem_u32(&b_oempty), L::o_warps); mbar_init(smem_u32(&b_kq), 1);
       mbar_init(smem_u32(&b_max), 16);
       for (int w = 0; w < 4; w++) mbar_init(smem_u32(&b_row[w]), 2);
@@ -439,6 +441,19 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
     }
     return true;
   };
+  constexpr uint32_t bt = T - 1;
+  constexpr uint32_t i_qk = idesc_16(bt, 128, 0, 0), i_qs = idesc_16(bt, DP, 0, 1), i_ds = idesc_16(bt, DP, 1, 1),
+                     i_pv = idesc_16(bt, DP, 0, 1);
+  // a descriptor's address is its low bits, in 16 bytes: K-major steps of 16 lie 32 bytes apart in a panel of 64,
+  // MN-major steps 16 rows of 128 bytes
+  auto kstep = [](int kk) { return (uint64_t)(((kk / 4) * L::panel + (kk % 4) * 32) >> 4); };
+  constexpr uint64_t mnstep = 2048 >> 4;
+  // V of chunk c for a product: its arrival, or the state warps' word that its dead rows are zero
+  auto wait_v = [&](int c, const Ring<NS> &rc) {
+    const bool whole = t1 - (t0 + (long long)c * kChunk) >= kChunk && !d.live;
+    return wait(whole ? b_vfull[rc.at] : b_vfix[rc.at], rc.parity, BNNK_ERR_MMA_WAIT);
+  };
+
   if (warp == 1) {  // TMA
     Ring<NS> rq, rc;  // tiles of Q (one a unit), of V (one a chunk)
     Ring<NK> rk;      // of K
@@ -474,18 +489,12 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
       for (int g = 1; g < G && ok; g++) load_q(g);
       rc.next();
     }
-  } else if (warp == 0) {  // MMA (the warp of the first TMEM quarter, whose scheduler has the fewest P blocks)
-    constexpr uint32_t bt = T - 1;
-    constexpr uint32_t i_qk = idesc_16(bt, 128, 0, 0), i_qs = idesc_16(bt, DP, 0, 1), i_ds = idesc_16(bt, DP, 1, 1),
-                       i_pv = idesc_16(bt, DP, 0, 1);
-    // a descriptor's address is its low bits, in 16 bytes: K-major steps of 16 lie 32 bytes apart in a panel of 64,
-    // MN-major steps 16 rows of 128 bytes
-    auto kstep = [](int kk) { return (uint64_t)(((kk / 4) * L::panel + (kk % 4) * 32) >> 4); };
-    constexpr uint64_t mnstep = 2048 >> 4;
-    Ring<NS> kq, rq, rc;  // the next QK's Q tile, this unit's, this chunk's V tile and set of K'
-    Ring<NK> kc, rn;      // the next QK's K tile, this chunk's
-    Ring<NB> kb, rb;          // and their QK / P regions
-    int kg = 0;
+  } else if (warp == 0 || warp == 2) {  // MMA
+    Ring<NS> kq, rq, rc;  // the next QK's Q tile; this unit's Q tile; this chunk's V tile and set of K'
+    Ring<NK> kc, rn;      // the next QK's K tile; this chunk's
+    Ring<NB> kb, rb;      // the next QK's region; this unit's
+    Ring<1> ro, ru, rk;   // single barriers: a phase a unit (O1, O2), a phase a chunk
+    int kg = 0, g = 0, c = 0;
     auto issue_qk = [&]() {
       if (!wait(b_qfull[kq.at], kq.parity, BNNK_ERR_MMA_WAIT)) return false;
       if (kg == 0 && !wait(b_kfull[kc.at], kc.parity, BNNK_ERR_MMA_WAIT)) return false;
@@ -496,84 +505,110 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
         for (int kk = 0; kk < DP / 16; kk++)
           mma16_ss(tmem + L::t_qk + kb.at * 128, dq + kstep(kk), dk + kstep(kk), i_qk, kk != 0);
         mma_commit(smem_u32(&b_qk[kb.at]));
-        if (L::in_place && kg == G - 1) mma_commit(smem_u32(&b_kq));
+        mma_commit(smem_u32(&b_qempty[kq.at]));
+        if (kg == G - 1) {
+          mma_commit(smem_u32(&b_kempty[kc.at]));
+          if (L::in_place) mma_commit(smem_u32(&b_kq));
+        }
       }
       kq.next();
       kb.next();
       if (++kg == G) { kg = 0; kc.next(); }
       return true;
     };
-    bool ok = kState || nu == 0 || issue_qk();
-    int g = 0;
-    Ring<1> ru, rk;  // single barriers: a phase a unit, a phase a chunk
-    for (int u = 0; u < nu && ok; u++) {
+    auto issue_o1 = [&](int u) {
+      if (!wait(b_qfull[rq.at], rq.parity, BNNK_ERR_MMA_WAIT)) return false;
+      if (g == 0 && !wait(b_s, rk.parity, BNNK_ERR_MMA_WAIT)) return false;
+      if (u && !wait(b_oempty, ro.parity ^ 1, BNNK_ERR_MMA_WAIT)) return false;
+      tc_fence_after();
+      const uint64_t dq = smem_desc<128>(base + L::q + rq.at * L::tile), ds = smem_desc_mn(base + L::st, L::s_panel);
+      if (elect_one()) {
+#pragma unroll
+        for (int part = 0; part < 2; part++)
+#pragma unroll
+          for (int kk = 0; kk < DP / 16; kk++)
+            mma16_ss(tmem + L::t_o1, dq + kstep(kk), ds + (part * L::s_tile >> 4) + kk * mnstep, i_qs, (part | kk) != 0);
+        mma_commit(smem_u32(&b_o));
+        mma_commit(smem_u32(&b_qempty[rq.at]));
+      }
+      rq.next();
+      ro.next();
+      return true;
+    };
+    auto issue_ds = [&]() {
       const int s = rc.at;
+      if (!wait_v(c, rc) || !wait(b_kp[s], rc.parity, BNNK_ERR_MMA_WAIT)) return false;
+      tc_fence_after();
+      const uint64_t dk0 = smem_desc_mn(L::kpart(base, s, 0), L::panel), dk1 = smem_desc_mn(L::kpart(base, s, 1), L::panel);
       const uint64_t dv = smem_desc_mn(base + L::v + s * L::tile, L::panel);
-      auto issue_qs = [&]() {
-        if (g == 0 && !wait(b_s, rk.parity, BNNK_ERR_MMA_WAIT)) return false;
-        if (u && !wait(b_oempty, ru.parity ^ 1, BNNK_ERR_MMA_WAIT)) return false;
-        tc_fence_after();
-        const uint64_t dq = smem_desc<128>(base + L::q + rq.at * L::tile), ds = smem_desc_mn(base + L::st, L::s_panel);
-        if (elect_one()) {
+      if (elect_one()) {
 #pragma unroll
-          for (int part = 0; part < 2; part++)
-#pragma unroll
-            for (int kk = 0; kk < DP / 16; kk++)
-              mma16_ss(tmem + L::t_o1, dq + kstep(kk), ds + (part * L::s_tile >> 4) + kk * mnstep, i_qs, (part | kk) != 0);
-          mma_commit(smem_u32(&b_qempty[rq.at]));
-        }
-        rq.next();
-        return true;
-      };
-      auto issue_ds = [&]() {
-        if (!wait(b_kp[s], rc.parity, BNNK_ERR_MMA_WAIT)) return false;
-        tc_fence_after();
-        const uint64_t dk0 = smem_desc_mn(L::kpart(base, s, 0), L::panel), dk1 = smem_desc_mn(L::kpart(base, s, 1), L::panel);
-        if (elect_one()) {
-#pragma unroll
-          for (int part = 0; part < L::parts; part++)
-#pragma unroll
-            for (int kk = 0; kk < 8; kk++)
-              mma16_ss(tmem + L::t_ds, (part ? dk1 + ((part - 1) * L::tile >> 4) : dk0) + kk * mnstep, dv + kk * mnstep, i_ds,
-                       (part | kk) != 0);
-          mma_commit(smem_u32(&b_ds));
-          mma_commit(smem_u32(&b_kempty[rn.at]));
-        }
-        rn.next();
-        return true;
-      };
-      const bool last = g == G - 1;
-      if (!kState && NB > 1 && u + 1 < nu && !(ok = issue_qk())) break;
-      if (!kState && !(ok = issue_qs())) break;
-      if (g == 0) {
-        if (!(ok = wait(b_vfull[s], rc.parity, BNNK_ERR_MMA_WAIT))) break;
-        if (!(ok = wait(b_vfix[s], rc.parity, BNNK_ERR_MMA_WAIT))) break;
-      }
-      if (last && !(ok = issue_ds())) break;
-      if (last) {
-        g = 0;
-        rk.next();
-        rc.next();
-      } else {
-        g++;
-      }
-      if (!kState) {
-        if (!(ok = wait(b_p[rb.at], rb.parity, BNNK_ERR_MMA_WAIT))) break;
-        tc_fence_after();
-        if (elect_one()) {  // P: 16 columns j a block, its first parts in 8 TMEM columns, the second parts in the next 8
+        for (int part = 0; part < L::parts; part++)
 #pragma unroll
           for (int kk = 0; kk < 8; kk++)
-#pragma unroll
-            for (int part = 0; part < 2; part++)
-              mma16_ts(tmem + L::t_o2, tmem + L::t_qk + rb.at * 128 + kk * 16 + part * 8, dv + kk * mnstep, i_pv,
-                       (part | kk) != 0);
-          mma_commit(smem_u32(&b_o));
-        }
-        rb.next();
-        ru.next();
+            mma16_ss(tmem + L::t_ds, (part ? dk1 + ((part - 1) * L::tile >> 4) : dk0) + kk * mnstep, dv + kk * mnstep, i_ds,
+                     (part | kk) != 0);
+        mma_commit(smem_u32(&b_ds));
+        mma_commit(smem_u32(&b_kempty[rn.at]));
+        mma_commit(smem_u32(&b_vempty[s]));
       }
-      if (last && elect_one()) mma_commit(smem_u32(&b_vempty[s]));
-      if (!kState && NB == 1 && u + 1 < nu) ok = issue_qk();
+      return true;
+    };
+    auto issue_o2 = [&](int u) {
+      const uint64_t dv = smem_desc_mn(base + L::v + rc.at * L::tile, L::panel);
+      if (g == 0 && !wait_v(c, rc)) return false;
+      if (u && !wait(b_oempty, ru.parity ^ 1, BNNK_ERR_MMA_WAIT)) return false;
+      if (!wait(b_p[rb.at], rb.parity, BNNK_ERR_MMA_WAIT)) return false;
+      tc_fence_after();
+      if (elect_one()) {  // P: 16 columns j a block, its first parts in 8 TMEM columns, the second parts in the next 8
+#pragma unroll
+        for (int kk = 0; kk < 8; kk++)
+#pragma unroll
+          for (int part = 0; part < 2; part++)
+            mma16_ts(tmem + L::t_o2, tmem + L::t_qk + rb.at * 128 + kk * 16 + part * 8, dv + kk * mnstep, i_pv,
+                     (part | kk) != 0);
+        mma_commit(smem_u32(&b_o));
+        if (g == G - 1) mma_commit(smem_u32(&b_vempty[rc.at]));
+      }
+      rb.next();
+      ru.next();
+      return true;
+    };
+    // Two K tiles or more: one warp issues QK (a unit ahead) and O2, the other O1 and DS, so that the waits of one do not
+    // hold up the other's products (24 x 9600 tokens, d 64: 710 us by one warp, 672 by two). One K tile: one warp, O2 after
+    // DS, so that the next K is on its way meanwhile (28800 tokens, d 128: 181 us by one warp, 194 by two).
+    constexpr bool one = L::in_place;
+    auto issue = [&](auto which) {  // each warp's own code: first QK and O2 (or all), or O1 and DS
+      constexpr bool first = decltype(which)::value;
+      bool ok = true;
+      if constexpr (first) ok = nu == 0 || issue_qk();
+      for (int u = 0; u < nu && ok; u++) {
+        const bool last = g == G - 1;
+        if constexpr (first && !one)
+          if (u + 1 < nu && !(ok = issue_qk())) break;
+        if constexpr (!kState && (!first || one))
+          if (!(ok = issue_o1(u))) break;
+        if constexpr (!first || one)
+          if (last && !(ok = issue_ds())) break;
+        if constexpr (first)
+          if (!(ok = issue_o2(u))) break;
+        if (last) {
+          g = 0;
+          c++;
+          rn.next();
+          rk.next();
+          rc.next();
+        } else {
+          g++;
+        }
+        if constexpr (one)
+          if (u + 1 < nu) ok = issue_qk();
+      }
+    };
+    if (warp == 0) {
+      if constexpr (!kState) issue(std::true_type{});
+    } else {
+      if constexpr (!one) issue(std::false_type{});
     }
   } else if (warp >= kDaP && warp < kDaS) {
     // P: row i against the columns j <= i, blocks of 16 columns alternating between two warps
@@ -633,12 +668,16 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
 #pragma unroll
           for (int j = 0; j < 16; j++) x[j] = (w >> j) & 1 ? x[j] : 0u;
         }
+        if (diagonal) {
 #pragma unroll
-        for (int j = 0; j < 16; j += 2) {
-          const float a0 = __uint_as_float(x[j]) * f0, a1 = __uint_as_float(x[j + 1]) * f0;
-          if (diagonal) split2<T>(a0 * f[-j], a1 * f[-j - 1], p[j / 2], p[8 + j / 2]);
-          else split2<T>(a0 * fixed[j], a1 * fixed[j + 1], p[j / 2], p[8 + j / 2]);
+          for (int j = 0; j < 16; j++) x[j] = __float_as_uint(__uint_as_float(x[j]) * f[-j]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; j++) x[j] = __float_as_uint(__uint_as_float(x[j]) * fixed[j]);
         }
+#pragma unroll
+        for (int j = 0; j < 16; j += 2)
+          split2<T>(__uint_as_float(x[j]) * f0, __uint_as_float(x[j + 1]) * f0, p[j / 2], p[8 + j / 2]);
         if (blk + 2 < blocks) tmem_ld16(tq + (blk + 2) * 16, x);  // the next block, while this one is stored
         tmem_st16(tq + blk * 16, p);
       }
