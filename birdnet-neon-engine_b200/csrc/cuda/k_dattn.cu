@@ -161,8 +161,8 @@ __global__ void __launch_bounds__(256) k_dattn_rec(const DattnArgs a) {
 //
 // One CTA per (segment of a sequence, k/v head) walks the segment's chunks, and for each the G q heads of the group
 // ("unit" u = (chunk, q head)). Roles: warps 0 and 2 MMA issue, warp 1 TMA, 8 warps turn QK into P (in place in TMEM, as the A
-// operand of the last product), 16 warps hold S in registers, form K' and the S operand; one of the two joins O1 and O2
-// into o. S in registers stays fp32: lambda^n S + DS, once a chunk. The roles' loops are rolled: unrolled, their code
+// operand of the last product) and join O1 and O2 into o, 16 warps hold S in registers and form K' and the S operand. S in
+// registers stays fp32: lambda^n S + DS, once a chunk. The roles' loops are rolled: unrolled, their code
 // did not stay in the instruction cache together and a unit took twice as long. The issuing warp stays converged
 // (elect.sync): from one lane's branch each tcgen05.mma took 70 cycles to issue, more than a 128 x 64 x 16 product.
 // A masked token, and a row past the segment's end, has its k and v rows taken as zero (K' zero, V zeroed in shared
@@ -226,7 +226,6 @@ template <int T, int DP, bool kState>
 struct DaLayout {
   static constexpr int parts = T == 2 ? 3 : 2;      // of K'
   static constexpr bool in_place = DP == 128 && !kState;
-  static constexpr int o_warps = in_place ? 8 : 16;  // that store o: P's, which wait for the next K there, or the state's
   static constexpr int stages = in_place ? 1 : 2;    // Q and V tiles in flight
   static constexpr int kp_sets = DP == 64 ? 2 : 1;   // sets of K': with two it is formed a chunk ahead
   static constexpr int k_stages = DP == 64 ? 3 : stages;  // K tiles: the last to be free again (after DS) and the first needed
@@ -351,7 +350,7 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
       for (int s = 0; s < NK; s++) { mbar_init(smem_u32(&b_kfull[s]), 1); mbar_init(smem_u32(&b_kempty[s]), kState ? 1 : 2); }
       for (int b = 0; b < NB; b++) { mbar_init(smem_u32(&b_qk[b]), 1); mbar_init(smem_u32(&b_p[b]), 8); }
       mbar_init(smem_u32(&b_s), 16); mbar_init(smem_u32(&b_ds), 1); mbar_init(smem_u32(&b_o), 2);
-      mbar_init(smem_u32(&b_oempty), L::o_warps); mbar_init(smem_u32(&b_kq), 1);
+      mbar_init(smem_u32(&b_oempty), 8); mbar_init(smem_u32(&b_kq), 1);
       mbar_init(smem_u32(&b_max), 16);
       for (int w = 0; w < 4; w++) mbar_init(smem_u32(&b_row[w]), 2);
       abort_s = 0;
@@ -390,7 +389,7 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
   // their rows, so that a store covers whole sectors of 32 bytes: with 16 bytes of 32 rows a store it took 3300 cycles
   // a chunk of 128 x 128
   auto put_o = [&](int c, int g, int u, int c0) {
-    constexpr int CN = DP * 4 / L::o_warps;
+    constexpr int CN = DP / 2;
     const int r = 32 * (warp % 4) + lane;
     const long long t = t0 + (long long)c * kChunk;
     const int n = (int)min((long long)kChunk, t1 - t) - 32 * (warp % 4);  // this warp's rows inside the segment
@@ -616,8 +615,9 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
     float fixed[16];  // lambda^(15 - j)
 #pragma unroll
     for (int j = 0; j < 16; j++) fixed[j] = pw[15 - j];
+    int c = 0, g = 0, c_was = 0, g_was = 0;  // this unit's chunk and q head, and those of the unit before
     for (int u = 0; u < (kState ? 0 : nu); u++) {
-      const int c = u / G, b = u % NB;
+      const int b = u % NB;
       const long long t = t0 + (long long)c * kChunk;
       const int n = (int)min((long long)kChunk, t1 - t);
       uint32_t lw[4] = {~0u, ~0u, ~0u, ~0u};
@@ -689,7 +689,15 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&b_p[b]));
-      if (L::in_place && !put_o(c, u % G, u, h * (DP / 2))) break;
+      // o: of this unit where the next QK waits for its K; else of the unit before, whose products ran meanwhile
+      if (L::in_place ? !put_o(c, g, u, h * (DP / 2)) : u && !put_o(c_was, g_was, u - 1, h * (DP / 2))) break;
+      if (!L::in_place && u + 1 == nu) put_o(c, g, u, h * (DP / 2));
+      c_was = c;
+      g_was = g;
+      if (++g == G) {
+        g = 0;
+        c++;
+      }
     }
   } else if (warp >= kDaS && seq >= 0) {
     // the state: row r = dk index, DP / 4 columns from c0 in registers
@@ -850,12 +858,9 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
       return true;
     };
     if (L::kp_sets == 2 && nc > 0 && ok) next_kp(0);
-    for (int c = 0, u = 0; c < nc && ok; c++) {
+    for (int c = 0; c < nc && ok; c++) {
       const int n = (int)min((long long)kChunk, t1 - (t0 + (long long)c * kChunk));
       if (L::kp_sets == 1 ? !next_kp(c) : c + 1 < nc && !next_kp(c + 1)) break;
-      if (!L::in_place && !kState)
-        for (int g = 0; g < G - 1 && ok; g++) ok = put_o(c, g, u++, c0);
-      if (!ok) break;
       if (!(ok = wait(b_ds, c & 1, BNNK_ERR_EPI_WAIT))) break;
       tc_fence_after();
       const float dec = pw[n];
@@ -875,7 +880,6 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
       tc_fence_before();
       if (kState) continue;
       if (c + 1 < nc) put_state(c + 1);  // the S operand's last reader, the chunk's last O1, comes before DS
-      if (!L::in_place && ok) ok = put_o(c, G - 1, u++, c0);
     }
     if (ok) {
       float *to = nullptr;
