@@ -537,6 +537,9 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
     auto issue_ds = [&]() {
       const int s = rc.at;
       if (!wait_v(c, rc) || !wait(b_kp[s], rc.parity, BNNK_ERR_MMA_WAIT)) return false;
+      // the chunk before's sum has been read: by the state warps' word that the S operand is there (which O1 waited for), or
+      // where there is none by their word after the read (K' formed ahead says nothing about it)
+      if (kState && c && !wait(b_s, rk.parity ^ 1, BNNK_ERR_MMA_WAIT)) return false;
       tc_fence_after();
       const uint64_t dk0 = smem_desc_mn(L::kpart(base, s, 0), L::panel), dk1 = smem_desc_mn(L::kpart(base, s, 1), L::panel);
       const uint64_t dv = smem_desc_mn(base + L::v + s * L::tile, L::panel);
@@ -878,7 +881,11 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
         }
       }
       tc_fence_before();
-      if (kState) continue;
+      if (kState) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&b_s));
+        continue;
+      }
       if (c + 1 < nc) put_state(c + 1);  // the S operand's last reader, the chunk's last O1, comes before DS
     }
     if (ok) {

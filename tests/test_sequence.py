@@ -267,6 +267,27 @@ def test_dattn_many_tokens_few_heads(cuda):
 
 
 @gpu
+@pytest.mark.parametrize("dtype, heads, lens, masked", [("f16", (8, 8, 32, 32), [591] * 8, 0.1),
+                                                        ("f16", (4, 2, 32, 32), [3000, 700], 0.0),
+                                                        ("bf16", (8, 8, 64, 64), [1311] * 5, 0.1),
+                                                        ("bf16", (2, 2, 128, 128), [2900, 17], 0.1),
+                                                        ("f16", (3, 1, 96, 128), [1500, 2500], 0.1)])
+def test_dattn_split_sequences_repeat(cuda, dtype, heads, lens, masked):
+    """sequences in parts of several chunks, the same bits however the warps are timed against each other"""
+    a = Attention(dtype, *heads, lens, masked, seed=12)
+    s1 = torch.zeros_like(a.s0)
+    op = a.op()
+    a.run(op, s1=s1)
+    o, s = a.o.clone(), s1.clone()
+    a.check(s1)
+    differ = torch.zeros((), device="cuda", dtype=torch.int64)
+    for _ in range(200):
+        a.run(op, s1=s1)
+        differ += (a.o != o).sum() + (s1 != s).sum()
+    assert int(differ) == 0 and op.error == 0
+
+
+@gpu
 def test_dattn_offsets_past_32_bits(cuda):
     """states and rows more than 2^32 bytes and 2^31 elements into their buffers"""
     torch.cuda.empty_cache()
