@@ -520,6 +520,19 @@ def test_norm_gate_zero_rows_and_zero_values(cuda):
     assert bool((xo == 0).all()) and bool((h == 0).all())
 
 
+@gpu
+def test_station_context_example(cuda):
+    """the operators together: whole recordings against window by window. The two ways round h, q, k, v, o and f to bf16
+    (2^-8 each) at different sums: some roundings' difference, in logits of about the weights' size"""
+    import importlib.util  # pylint: disable=import-outside-toplevel
+    import os  # pylint: disable=import-outside-toplevel
+    from conftest import REPO  # pylint: disable=import-outside-toplevel
+    spec = importlib.util.spec_from_file_location("station_context", os.path.join(REPO, "examples", "station_context.py"))
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    assert example.main() < 8 * 2.0 ** -8
+
+
 # ------------------------------------------------------------------ refusals (no GPU needed)
 
 
