@@ -55,6 +55,8 @@ __global__ void __launch_bounds__(256) k_dattn_rec(const DattnArgs a) {
   const int hk = blockIdx.y, i = blockIdx.x, cs = blockIdx.z * 32, c0 = cs + (lane % 8) * 4;
   const int dk = a.dk, dv = a.dv;
   const bool col = c0 < dv;
+  wait_launch_before();
+  launch_dependents();
   const long long slot = a.slot ? a.slot[i] : i;
   float4 S[4];
   int row[4];
@@ -1021,9 +1023,8 @@ extern "C" int bnnk_dattn(const bnnk_dattn_args *p, bnn_stream_t st) {
   if (!p->cu || p->tokens <= 8ll * p->n) {
     const int warps = (p->dk + 15) / 16;
     const dim3 grid(p->n, p->Hk, (p->dv + 31) / 32);
-    if (p->type == 1) k_dattn_rec<1><<<grid, 32 * warps, 0, s>>>(d);
-    else k_dattn_rec<2><<<grid, 32 * warps, 0, s>>>(d);
-    return cudaGetLastError();
+    return p->type == 1 ? launch_early(k_dattn_rec<1>, grid, 32 * warps, 0, s, d)
+                        : launch_early(k_dattn_rec<2>, grid, 32 * warps, 0, s, d);
   }
   DaArgs a = {d, segment_tokens(p->n, p->Hk, p->tokens), p->n, p->scratch, p->err};
   if (a.seg_tokens) a.segs += (int)(p->tokens / a.seg_tokens);

@@ -130,6 +130,7 @@ __global__ void __launch_bounds__(256) k_lowrank_few(const bnnk_lowrank_args p) 
   __shared__ __align__(16) float s_h[kOwn ? kOwnRows : 1][64];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, q = lane % 4;
   const int n0 = blockIdx.x * CN, K = p.K, rank = p.rank;
+  if (kOwn) wait_launch_before();  // the only launch; else it follows the one that forms h, which has waited
   launch_dependents();
   const elem_t<T> *W = (const elem_t<T> *)p.w, *x = (const elem_t<T> *)p.x, *B = (const elem_t<T> *)p.b;
   float acc[MT][NT][4] = {};
@@ -735,8 +736,8 @@ template <int T, int OT, int MT, int NT>
 cudaError_t few_nt(const bnnk_lowrank_args &p, cudaStream_t st) {
   const dim3 grid((p.N + 16 * MT - 1) / (16 * MT));
   if (p.slot && p.rows > kOwnRows) return launch_early(k_lowrank_few<T, OT, MT, NT, false>, grid, 256, 0, st, p);
-  if (p.slot) k_lowrank_few<T, OT, MT, NT, true><<<grid, 256, 0, st>>>(p);
-  else k_lowrank_few<T, OT, MT, NT, false><<<grid, 256, 0, st>>>(p);
+  if (p.slot) return launch_early(k_lowrank_few<T, OT, MT, NT, true>, grid, 256, 0, st, p);
+  k_lowrank_few<T, OT, MT, NT, false><<<grid, 256, 0, st>>>(p);
   return cudaGetLastError();
 }
 
