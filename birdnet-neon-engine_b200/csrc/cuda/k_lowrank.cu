@@ -500,9 +500,15 @@ __global__ void __launch_bounds__(kLrThreads, 1) k_lowrank_many(const __grid_con
   };
 
   if (warp == 0) {
+    int ahead = 0;      // places that may be used before the last tile's adapters have had theirs
+    bool owed = false;  // whether they are still to say so
     for (int t = blockIdx.x; t < a.tiles && ok; t += gridDim.x, lt++) {
       const int r0 = t / a.n_tiles * 128, n0 = t % a.n_tiles * bn;
       for (int kb = 0; kb < a.nkb; kb++, at.next(S)) {
+        if (owed && ahead-- == 0) {
+          if (!(ok = wait(b_back[(lt - 1) & 1], ((lt - 1) >> 1) & 1, BNNK_ERR_TMA_WAIT))) break;
+          owed = false;
+        }
         if (at.used && !(ok = wait(b_empty[at.s], at.parity ^ 1, BNNK_ERR_TMA_WAIT))) break;
         const uint32_t st = base + at.s * stage, bar = smem_u32(&b_full[at.s]);
         if (elect_one()) {
@@ -513,14 +519,17 @@ __global__ void __launch_bounds__(kLrThreads, 1) k_lowrank_many(const __grid_con
         }
       }
       // the ring's next places are the adapters': handed over and back, so that each side waits for a place whose use
-      // before has begun (a parity tells one use from the next, not from the one after)
+      // before has begun (a parity tells one use from the next, not from the one after). Until it comes to a place that
+      // they had, this warp goes on with the next tile.
       if (!ok || !adapters) continue;
+      if (owed && !(ok = wait(b_back[(lt - 1) & 1], ((lt - 1) >> 1) & 1, BNNK_ERR_TMA_WAIT))) break;
       if (elect_one()) mbar_arrive(smem_u32(&b_turn[lt & 1]));
       int n = 0;
       if (!(ok = extra(n))) break;
       list_read();
       for (int k = 0; k < n; k++) at.next(S);
-      if (!(ok = wait(b_back[lt & 1], (lt >> 1) & 1, BNNK_ERR_TMA_WAIT))) break;
+      ahead = max(0, S - n);
+      owed = true;
     }
   } else if (warp == 1) {
     const uint32_t idesc = idesc_16(T - 1, bn, 0, 0);
@@ -582,8 +591,13 @@ __global__ void __launch_bounds__(kLrThreads, 1) k_lowrank_many(const __grid_con
           const unsigned same = __match_any_sync(0xffffffffu, all[w]);  // every lane takes part, those without an adapter too
           bool first = all[w] >= 0 && __ffs(same) - 1 == lane;
 #pragma unroll
-          for (int v = 0; v < w; v++)
-            for (int l = 0; l < 32; l++) first &= __shfl_sync(0xffffffffu, all[v], l) != all[w];
+          for (int v = 0; v < w; v++) {
+            // neighbouring rows are mostly one request's: 32 rows all the same need one comparison
+            const int s0 = __shfl_sync(0xffffffffu, all[v], 0);
+            if (__all_sync(0xffffffffu, all[v] == s0)) first &= s0 != all[w];
+            else
+              for (int l = 0; l < 32; l++) first &= __shfl_sync(0xffffffffu, all[v], l) != all[w];
+          }
           firsts[w] = __ballot_sync(0xffffffffu, first);
           if (w < warp - 2) before += __popc(firsts[w]);
           count += __popc(firsts[w]);
@@ -591,11 +605,18 @@ __global__ void __launch_bounds__(kLrThreads, 1) k_lowrank_many(const __grid_con
         const unsigned own = firsts[0] * (warp == 2) | firsts[1] * (warp == 3) | firsts[2] * (warp == 4) | firsts[3] * (warp == 5);
         if ((own >> lane) & 1) s_list[g][before + __popc(own & ((1u << lane) - 1))] = mine;
         if (warp == 2 && lane == 0) s_n[g] = count;
-        // this row's h: rows past fp16's range are added when y is stored
-        const float *h = p.hid + (long long)(r0 + row) * p.rank;
+        // this row's h, read while W's steps run: rows past fp16's range are added when y is stored
+        float h[RB];
+#pragma unroll
+        for (int c = 0; c < RB; c += 4) {
+          float4 u = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (mine >= 0 && c < p.rank) u = *reinterpret_cast<const float4 *>(p.hid + (long long)(r0 + row) * p.rank + c);
+          h[c] = u.x, h[c + 1] = u.y, h[c + 2] = u.z, h[c + 3] = u.w;
+        }
         bool big = false;
-        if (T == 1 && mine >= 0)
-          for (int e = 0; e < p.rank; e++) big |= fabsf(h[e]) > 65504.f && fabsf(h[e]) < __int_as_float(0x7f800000);
+        if constexpr (T == 1)
+#pragma unroll
+          for (int e = 0; e < RB; e++) big |= fabsf(h[e]) > 65504.f && fabsf(h[e]) < __int_as_float(0x7f800000);
         s_big[g][row] = big;
         __threadfence_block();
         __syncwarp();
@@ -612,19 +633,15 @@ __global__ void __launch_bounds__(kLrThreads, 1) k_lowrank_many(const __grid_con
 #pragma unroll 1
             for (int e = 0; e < here; e++) {
               const bool on = mine >= 0 && s_list[g][e0 + e] == mine && !big;
-#pragma unroll 1
-              for (int c = 0; c < RB; c += 8) {
-                uint32_t z[4] = {0, 0, 0, 0};
-                if (on && c < p.rank) {
-                  const float4 u = *reinterpret_cast<const float4 *>(h + c), v = *reinterpret_cast<const float4 *>(h + c + 4);
-                  const float f[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
 #pragma unroll
-                  for (int i = 0; i < 4; i++) {
-                    uint32_t x0, x1, x2 = 0;
-                    if constexpr (PARTS == 3) split3<T>(f[2 * i], f[2 * i + 1], x0, x1, x2);
-                    else split2<T>(f[2 * i], f[2 * i + 1], x0, x1);
-                    z[i] = part == 0 ? x0 : part == 1 ? x1 : x2;
-                  }
+              for (int c = 0; c < RB; c += 8) {
+                uint32_t z[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                  uint32_t x0, x1, x2 = 0;
+                  if constexpr (PARTS == 3) split3<T>(h[c + 2 * i], h[c + 2 * i + 1], x0, x1, x2);
+                  else split2<T>(h[c + 2 * i], h[c + 2 * i + 1], x0, x1);
+                  z[i] = !on ? 0 : part == 0 ? x0 : part == 1 ? x1 : x2;
                 }
                 uint32_t off = e * 128 * RB * 2 + row * RB * 2 + c * 2;
                 off ^= (off >> 3) & (RB == 64 ? 0x70 : RB == 32 ? 0x30 : 0x10);  // the swizzle of 2 RB bytes a row
