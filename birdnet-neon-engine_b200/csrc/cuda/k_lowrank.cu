@@ -418,7 +418,7 @@ __global__ void __launch_bounds__(kMidThreads, 1) k_lowrank_mid(const __grid_con
 // any row alignment.
 constexpr int kLrThreads = 448;
 constexpr int kLrStages = 8;
-constexpr int kLrPad = 17;  // words a row of the stores' shared memory: blocks of 16 words
+constexpr int kLrPad = 20;  // words a row of the stores' shared memory: blocks of 16 words; 16-byte accesses meet no bank twice
 
 struct LrArgs {
   bnnk_lowrank_args p;
@@ -626,38 +626,44 @@ __global__ void __launch_bounds__(kLrThreads, 1) k_lowrank_many(const __grid_con
         // the ring's places of W's steps
         for (int kb = 0; kb < a.nkb; kb++) at.next(S);
         for (int e0 = 0; e0 < count && ok; e0 += GS) {
+          const int here = min(GS, count - e0);
+          int my = -1;  // this row's adapter among the stage's
+          for (int e = 0; e < here; e++)
+            if (mine >= 0 && !big && s_list[g][e0 + e] == mine) my = e;
+#pragma unroll 1
           for (int part = 0; part < PARTS; part++, at.next(S)) {
             if (at.used && !(ok = wait(b_empty[at.s], at.parity ^ 1, BNNK_ERR_TMA_WAIT))) break;
             const uint32_t st = base + at.s * stage, bar = smem_u32(&b_full[at.s]);
-            const int here = min(GS, count - e0);
-#pragma unroll 1
-            for (int e = 0; e < here; e++) {
-              const bool on = mine >= 0 && s_list[g][e0 + e] == mine && !big;
+            if (warp == 2 && elect_one()) {
+              mbar_expect_tx(bar, here * bn * RB * 2);
+              for (int e = 0; e < here; e++)
+                tma_load_3d(st + a_bytes + e * bn * RB * 2, &mb, bar, 0, n0, s_list[g][e0 + e]);
+            }
 #pragma unroll
-              for (int c = 0; c < RB; c += 8) {
-                uint32_t z[4];
+            for (int c = 0; c < RB; c += 8) {
+              uint32_t z[4] = {0, 0, 0, 0};
+              if (my >= 0) {  // a part: what the parts before have left, rounded
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                  uint32_t x0, x1, x2 = 0;
-                  if constexpr (PARTS == 3) split3<T>(h[c + 2 * i], h[c + 2 * i + 1], x0, x1, x2);
-                  else split2<T>(h[c + 2 * i], h[c + 2 * i + 1], x0, x1);
-                  z[i] = !on ? 0 : part == 0 ? x0 : part == 1 ? x1 : x2;
+                  float &u = h[c + 2 * i], &v = h[c + 2 * i + 1];
+                  z[i] = pack2f<T>(u, v);
+                  const float2 f = unpack2<T>(z[i]);
+                  u -= f.x, v -= f.y;
                 }
+              }
+#pragma unroll 1
+              for (int e = 0; e < here; e++) {
+                const bool on = e == my;
                 uint32_t off = e * 128 * RB * 2 + row * RB * 2 + c * 2;
                 off ^= (off >> 3) & (RB == 64 ? 0x70 : RB == 32 ? 0x30 : 0x10);  // the swizzle of 2 RB bytes a row
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(st + off), "r"(z[0]), "r"(z[1]), "r"(z[2]),
-                             "r"(z[3])
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(st + off), "r"(on ? z[0] : 0),
+                             "r"(on ? z[1] : 0), "r"(on ? z[2] : 0), "r"(on ? z[3] : 0)
                              : "memory");
               }
             }
             fence_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar);
-            if (warp == 2 && elect_one()) {
-              mbar_expect_tx(bar, here * bn * RB * 2);
-              for (int e = 0; e < here; e++)
-                tma_load_3d(st + a_bytes + e * bn * RB * 2, &mb, bar, 0, n0, s_list[g][e0 + e]);
-            }
           }
         }
         if (!ok) break;
@@ -671,6 +677,8 @@ __global__ void __launch_bounds__(kLrThreads, 1) k_lowrank_many(const __grid_con
     const int qd = warp % 4, h = (warp - 6) / 4;
     const uint32_t buf = base + S * stage + (warp - 6) * 32 * kLrPad * 4;
     const bool even = PW == 1 || (((uintptr_t)p.y | (uintptr_t)(p.ldy * 2)) & 3) == 0;  // word-aligned rows
+    const bool bias16 = p.bias && ((uintptr_t)p.bias & 15) == 0;
+    const bool wide = (((uintptr_t)p.y | (uintptr_t)(p.ldy * (4 / PW))) & 15) == 0;  // rows of whole 16 bytes
     for (int t = blockIdx.x; t < a.tiles; t += gridDim.x, lt++) {
       const int r0 = t / a.n_tiles * 128 + 32 * qd, n0 = t % a.n_tiles * bn, g = lt & 1;
       if (!wait(b_acc[g], (lt >> 1) & 1, BNNK_ERR_EPI_WAIT)) break;
@@ -689,8 +697,17 @@ __global__ void __launch_bounds__(kLrThreads, 1) k_lowrank_many(const __grid_con
           tmem_wait_ld(x);
           float v[16];
 #pragma unroll
-          for (int j = 0; j < 16; j++)
-            v[j] = __uint_as_float(x[j]) + (p.bias && c + j < width ? __ldg(p.bias + n0 + c + j) : 0.f);
+          for (int j = 0; j < 16; j++) v[j] = __uint_as_float(x[j]);
+          if (bias16 && c + 16 <= width) {
+#pragma unroll
+            for (int j = 0; j < 16; j += 4) {
+              const float4 u = __ldg(reinterpret_cast<const float4 *>(p.bias + n0 + c + j));
+              v[j] += u.x, v[j + 1] += u.y, v[j + 2] += u.z, v[j + 3] += u.w;
+            }
+          } else if (p.bias) {
+#pragma unroll
+            for (int j = 0; j < 16; j++) v[j] += c + j < width ? __ldg(p.bias + n0 + c + j) : 0.f;
+          }
           if (OT == 0)
             for (int k = 1; k < a.na; k++) {
               tmem_ld16(tq + k * a.acc_cols + c, x);
@@ -712,12 +729,31 @@ __global__ void __launch_bounds__(kLrThreads, 1) k_lowrank_many(const __grid_con
           }
           __syncwarp();
 #pragma unroll
-          for (int j = 0; j < 16; j += PW) {
-            const uint32_t z = PW == 1 ? __float_as_uint(v[j]) : pack2f<T>(v[j], v[j + PW - 1]);
-            asm volatile("st.shared.b32 [%0], %1;" ::"r"(buf + (lane * kLrPad + (16 * w0 + j) / PW) * 4), "r"(z) : "memory");
+          for (int j = 0; j < 16; j += 4 * PW) {
+            uint32_t z[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+              z[i] = PW == 1 ? __float_as_uint(v[j + i]) : pack2f<T>(v[j + PW * i], v[j + PW * i + PW - 1]);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(buf + (lane * kLrPad + (16 * w0 + j) / PW) * 4),
+                         "r"(z[0]), "r"(z[1]), "r"(z[2]), "r"(z[3])
+                         : "memory");
           }
         }
         __syncwarp();
+        if (wide && c0 + CW <= width) {
+          char *y = (char *)p.y + ((long long)(r0 + lane / 4) * p.ldy + n0 + c0) * (4 / PW) + lane % 4 * 16;
+#pragma unroll
+          for (int r = lane / 4; r < 32; r += 8, y += 8 * p.ldy * (4 / PW)) {
+            uint4 z;
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(z.x), "=r"(z.y), "=r"(z.z), "=r"(z.w)
+                         : "r"(buf + (r * kLrPad + lane % 4 * 4) * 4)
+                         : "memory");
+            if (r < rows) *reinterpret_cast<uint4 *>(y) = z;
+          }
+          __syncwarp();
+          continue;
+        }
         const int c = c0 + lane % 16 * PW;
         elem_t<OT> *y = (elem_t<OT> *)p.y + (long long)(r0 + lane / 16) * p.ldy + n0 + c;
 #pragma unroll 4
