@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(256) k_lowrank_down(int rows, int K, const ele
     const int s = s_slot[__ffs(first) - 1];
     const elem_t<T> *a = A + (long long)s * rank * K;
     float acc[MR][RT][4] = {};
-#pragma unroll(4 / MR)
+#pragma unroll(RT <= 2 ? 6 / MR + 1 : RT <= 4 ? 3 : 2)
     for (int k0 = 32 * warp; k0 < K; k0 += 256) {
       const int k = k0 + 8 * q;
       uint4 xa[MR], xb[MR];
