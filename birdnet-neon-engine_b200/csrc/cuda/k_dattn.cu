@@ -30,6 +30,7 @@ struct DattnArgs {
   long long ots;
   const float *pow;  // [Hk][kDattnPow]: lambda^0 .. lambda^128
   float scale;
+  int over;  // not 0: the recurrent form has the sequences of up to so many tokens, the chunk form the others
 };
 
 // a sequence's tokens [t0, t1): cu offsets kept inside the buffers, or token i for sequence i where cu is NULL
@@ -70,6 +71,7 @@ __global__ void __launch_bounds__(256) k_dattn_rec(const DattnArgs a) {
   }
   long long t0, t1;
   seq_range(a, i, t0, t1);
+  if (a.over && t1 - t0 > a.over) return;
   const float lam = a.pow[hk * kDattnPow + 1];
   int buf = 0;
   for (long long t = t0; t < t1; t++) {
@@ -182,11 +184,11 @@ struct DaArgs {
 };
 
 // the sequence, part, tokens and last-part flag of segment s: sequence i has max(1, ceil(length / seg_tokens)) segments,
-// in order. One warp; false past the last segment.
+// or none where the recurrent form has it, in order. One warp; false past the last segment.
 __device__ bool find_segment(const DaArgs &a, int s, int &seq, int &part, long long &t0, long long &t1, bool &last) {
   const int lane = threadIdx.x % 32;
   long long b0, b1;
-  if (!a.seg_tokens) {
+  if (!a.seg_tokens && !a.d.over) {
     if (s >= a.d.n) return false;
     seq = s; part = 0; last = true;
     seq_range(a.d, s, t0, t1);
@@ -198,7 +200,7 @@ __device__ bool find_segment(const DaArgs &a, int s, int &seq, int &part, long l
     int parts = 0;
     if (i < a.d.n) {
       seq_range(a.d, i, b0, b1);
-      parts = max(1, (int)((b1 - b0 + a.seg_tokens - 1) / a.seg_tokens));
+      parts = a.d.over ? b1 - b0 > a.d.over : max(1, (int)((b1 - b0 + a.seg_tokens - 1) / a.seg_tokens));
     }
     int sum = parts;
     for (int o = 1; o < 32; o <<= 1) {
@@ -1017,18 +1019,31 @@ extern "C" long long bnnk_dattn_scratch_states(int n, int Hk, long long tokens) 
 extern "C" int bnnk_dattn(const bnnk_dattn_args *p, bnn_stream_t st) {
   if (p->n <= 0) return 0;
   const DattnArgs d = {p->n, p->H, p->Hk, p->H / p->Hk, p->dk, p->dv, p->tokens, p->cu, p->slot, p->live, p->q, p->k, p->v,
-                       p->qts, p->kts, p->vts, p->s0, p->s1, p->o, p->ots, p->pow, p->scale};
+                       p->qts, p->kts, p->vts, p->s0, p->s1, p->o, p->ots, p->pow, p->scale, 0};
   const cudaStream_t s = (cudaStream_t)st;
-  // short sequences: the recurrent form
-  if (!p->cu || p->tokens <= 8ll * p->n) {
-    const int warps = (p->dk + 15) / 16;
-    const dim3 grid(p->n, p->Hk, (p->dv + 31) / 32);
-    return p->type == 1 ? launch_early(k_dattn_rec<1>, grid, 32 * warps, 0, s, d)
-                        : launch_early(k_dattn_rec<2>, grid, 32 * warps, 0, s, d);
-  }
-  DaArgs a = {d, segment_tokens(p->n, p->Hk, p->tokens), p->n, p->scratch, p->err};
-  if (a.seg_tokens) a.segs += (int)(p->tokens / a.seg_tokens);
   const bool wide = p->dk > 64 || p->dv > 64;
+  DaArgs a = {d, segment_tokens(p->n, p->Hk, p->tokens), p->n, p->scratch, p->err};
+  // The recurrent form for single tokens (cu NULL) and where the sequences are short on average: a token costs a CTA about
+  // 2 us of latency, or a state's share of the SMs' arithmetic where CTAs are many; a chunk costs its 128 rows, filled or
+  // not. Measured (8 heads, us, recurrent / chunk): 16 sequences, d 64, of 1 token 8 / 14, of 4 16.4 / 14.3, d 128, of 8
+  // 26.6 / 18.4; 300 sequences, d 64, of 12 tokens 111 / 136, of 16 144 / 135, d 128, of 4 183 / 200, of 8 326 / 202.
+  // Lengths are known on the device alone, and one of 1000 tokens would take the recurrent form 2 ms: those far above the
+  // average go to the chunk form in a second launch, of as many CTAs a head as there can be such sequences (2 us for every
+  // num_sms() of them that find none). Where the CTAs are few it costs what it saves: the chunk form has them all.
+  const bool few = (long long)p->n * p->Hk <= num_sms();
+  if (!p->cu || p->tokens <= (few ? 4ll : (wide ? 4ll : 12ll) * p->n)) {
+    const int over = wide ? 32 : 64, warps = (p->dk + 15) / 16;
+    if (p->cu && p->tokens > over) a.d.over = over;
+    const dim3 grid(p->n, p->Hk, (p->dv + 31) / 32);
+    const int e = p->type == 1 ? launch_early(k_dattn_rec<1>, grid, 32 * warps, 0, s, a.d)
+                               : launch_early(k_dattn_rec<2>, grid, 32 * warps, 0, s, a.d);
+    if (e || !a.d.over) return e;
+    const long long longer = p->tokens / (over + 1);
+    a.segs = longer < p->n ? (int)longer : p->n;
+    a.seg_tokens = 0;
+  } else if (a.seg_tokens) {
+    a.segs += (int)(p->tokens / a.seg_tokens);
+  }
   if (p->type == 1) return wide ? run_chunk<1, 128>(a, s) : run_chunk<1, 64>(a, s);
   return wide ? run_chunk<2, 128>(a, s) : run_chunk<2, 64>(a, s);
 }

@@ -172,6 +172,34 @@ def test_dattn_against_64_bits(cuda, case):
     a.s0 = keep
 
 
+MIXED = [
+    # short sequences on average, some of them long: neighbours of the lengths where the forms change, empty ones
+    ("bf16", 4, 2, 64, 64, [1] * 40 + [300] + [2] * 20 + [0] * 10 + [64, 65, 1, 66, 0] + [3] * 15, 0.1),
+    ("f16", 2, 2, 40, 64, [0, 200] + [5] * 100, 0),
+    ("bf16", 2, 2, 128, 128, [1] * 60 + [32, 33, 0, 140] + [1] * 60, 0),
+    ("f16", 2, 2, 96, 72, [2] * 80 + [34], 0.2),
+    ("bf16", 1, 1, 128, 64, [1, 0, 3], 0),
+    ("f16", 3, 3, 64, 64, [1] * 5, 0),
+]
+
+
+@gpu
+@pytest.mark.parametrize("case", range(len(MIXED)))
+def test_dattn_long_among_short(cuda, case):
+    dtype, H, Hk, dk, dv, lens, masked = MIXED[case]
+    a = Attention(dtype, H, Hk, dk, dv, lens, masked, seed=100 + case)
+    s1 = torch.full_like(a.s0, 9.0)
+    op = a.op()
+    a.run(op, s1=s1)
+    a.check(s1)
+    untouched = [i for i in range(len(a.s0)) if i not in set(a.slot.tolist())]
+    assert bool((s1[untouched] == 9.0).all())
+    assert op.error == 0
+    o = a.o.clone()
+    a.run(op, s1=a.s0)
+    assert torch.equal(a.o, o) and torch.equal(a.s0[a.slot.long()], s1[a.slot.long()])
+
+
 @gpu
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 @pytest.mark.parametrize("heads", [(2, 2, 128, 128), (8, 2, 64, 64), (3, 1, 96, 72), (12, 1, 8, 104), (1, 1, 24, 128)])
@@ -401,6 +429,62 @@ LOWRANK = [
 def test_lowrank_against_64_bits(cuda, case):
     lowrank_case(*LOWRANK[case], seed=case, bias=case % 3 != 1, scale=case % 4 != 2, xpad=8 * (case % 2),
                  ypad=case % 5, wpad=8 * (case % 3))
+
+
+LOWRANK_EDGES = [
+    ("bf16", "bf16", 2, 77, 264, 64, 3, "any"),
+    ("f16", "f16", 3, 128, 1000, 8, 3, "any"),
+    ("bf16", "f32", 8, 40, 2048, 32, 9, "any"),
+    ("f16", "f32", 9, 2500, 64, 24, 4, "any"),
+    ("bf16", "bf16", 65, 300, 136, 64, 70, "any"),
+    ("f16", "f32", 127, 6522, 128, 16, 200, "any"),
+    ("bf16", "f32", 128, 50, 80, 48, 128, "any"),
+    ("bf16", "bf16", 129, 300, 136, 64, 140, "any"),
+    ("f16", "f16", 513, 260, 72, 24, 9, "any"),
+    ("bf16", "f32", 300, 130, 2304, 64, 5, "runs"),
+    ("f16", "f32", 200, 3000, 1024, 64, 3, "runs"),
+    ("bf16", "bf16", 6000, 1000, 64, 64, 40, "runs"),
+]
+
+
+@gpu
+@pytest.mark.parametrize("case", range(len(LOWRANK_EDGES)))
+def test_lowrank_row_counts_where_forms_change(cuda, case):
+    lowrank_case(*LOWRANK_EDGES[case], seed=50 + case, bias=case % 2 == 0, scale=case % 3 != 1, xpad=8 * (case % 3),
+                 ypad=(0, 1, 8)[case % 3], wpad=8 * (case % 2))
+
+
+@gpu
+@pytest.mark.parametrize("rows", [1, 9, 50, 300])
+@pytest.mark.parametrize("out", ["f16", "f32"])
+def test_lowrank_fp16_h_past_the_type(cuda, rows, out):
+    """h is fp32: rows whose h passes fp16's largest value keep it, beside rows of the same adapter whose h does not"""
+    gen, K, N, rank, slots = generator(rows), 256, 200, 16, 3
+    x = rand(gen, rows, K)
+    x[::3] *= 300.0
+    x, w = x.half(), (rand(gen, N, K) * 2.0 ** -4).half()
+    A, B = rand(gen, slots, rank, K).half(), (rand(gen, slots, N, rank) * 2.0 ** -11).half()
+    s = torch.full((slots,), 60.0, device="cuda")
+    slot = torch.randint(-1, slots, (rows,), device="cuda", generator=gen).int()
+    slot[0] = 0
+    y = torch.empty(rows, N, device="cuda", dtype=DT[out])
+    op = sequence.LowRank("f16", out, N, K, w.data_ptr(), None, slots, rank, A.data_ptr(), B.data_ptr(), s.data_ptr(),
+                          rows=rows)
+    op.run(rows, x.data_ptr(), slot.data_ptr(), y.data_ptr())
+    assert op.error == 0
+    xd, wd = x.double(), w.double()
+    want, M = xd @ wd.t(), xd.abs() @ wd.abs().t()
+    most = 0.0
+    for a in range(slots):
+        at = torch.nonzero(slot == a).flatten()
+        if not len(at):
+            continue
+        h = 60.0 * (xd[at] @ A[a].double().t())
+        most = max(most, float(h.abs().max()))
+        want[at] += h @ B[a].double().t()
+        M[at] += 60.0 * ((xd[at].abs() @ A[a].double().abs().t()) @ B[a].double().abs().t())
+    assert most > 65504.0
+    check(y, want, (2.0 ** -15 + (K + rank + 4) * 2.0 ** -24) * M, out, "y")
 
 
 @gpu
