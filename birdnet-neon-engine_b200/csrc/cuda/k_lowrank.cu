@@ -3,8 +3,8 @@
 //   y_r = W x_r + bias + h_r B_a^T,   h_r = s_a A_a x_r,   a = slot[r] (none where it is outside [0, slots))
 //
 // W [N][K], A [slots][rank][K], B [slots][N][rank]; sums in fp32. Two launches: h (k_lowrank_down), then y in one of three
-// forms by the number of rows (one launch for one or two rows); the second launch starts while the first runs (programmatic dependent launch) and waits
-// for h only where it is used, after its sums over K.
+// forms by the number of rows (one launch for one row); the second launch starts while the first runs (programmatic
+// dependent launch) and waits for h only where it is used, after its sums over K.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -43,8 +43,8 @@ __device__ __forceinline__ uint4 ldg16(const void *p, bool in) {
 // instructions (a product of 16 rows is too small for a 128-row tile, and bound by reading A and x), K in steps of 32
 // dealt to 8 warps, their sums joined in shared memory in warp order. A lane's 16 bytes are 8 consecutive k of a row: the
 // two instructions of a step take them in the same order from both operands, so their k are a permutation of the
-// layout's, the same for both. Rows of other adapters are computed and dropped. MR 2 halves the reads of A where there
-// are rows enough (9001 rows of 1536, rank 32: 213 us for the whole operator, 217 with MR 1).
+// layout's, the same for both. Rows of other adapters are computed and dropped. Bound by latency: K over 8 warps is a
+// few rounds of loads (9001 rows of 1536, rank 32, 1200 rows an adapter: 27 us, 1.1 TB/s).
 constexpr int kDownRows = 16;
 
 template <int T, int RT, int MR>  // RT: 8-wide tiles of the rank
@@ -114,18 +114,20 @@ __global__ void __launch_bounds__(256) k_lowrank_down(int rows, int K, const ele
 
 // ------------------------------------------------------------------ up to 16 rows
 //
-// Bound by reading W (and the adapters' B) once, and by latency. One CTA per 16 MT rows of W: warp-level matrix
+// Bound by reading W (and the adapters' B) once, and by latency. One CTA per 16 rows of W: warp-level matrix
 // instructions with W as the 16-row operand and 8 NT rows of x as the other, K dealt to 8 warps as above; the warps' sums
 // are joined in shared memory, then each lane takes some rows' outputs of one column and adds their rank products with B
 // from the rows' adapters (neighbouring lanes' rows of B are neighbours in memory; the loads of all of a lane's outputs
 // are in flight together, the first of them before the wait for h).
-// kOwn: the CTA forms h of its (one or two) rows itself, while W is on its way: a second read of A from L2 by every CTA
-// in place of a launch and its end.
-constexpr int kFewRows = 16, kOwnRows = 2;
+// kOwn: the CTA forms h of its one row itself, while W is on its way: a second read of A from L2 by every CTA in place of
+// a launch and its end (1 row, 1024 x 1024, calls one after another: 7.5 us, with the launch 9.7; 2 rows: 17.3 us, with the
+// launch 11.3). 16 rows of W a CTA: with 32, which halve the reads of x, 8 rows of 6522 x 1024 took 15.4 us in place of
+// 13.3. Against the next form at 16 rows: 14.2 us, 19.5 (6522 x 1024), 11.9 and 13.3 (1024 x 1024).
+constexpr int kFewRows = 16, kOwnRows = 1;
 
-template <int T, int OT, int MT, int NT, bool kOwn>
+template <int T, int OT, int NT, bool kOwn>
 __global__ void __launch_bounds__(256) k_lowrank_few(const bnnk_lowrank_args p) {
-  constexpr int P = 8 * NT + 1, CN = 16 * MT;
+  constexpr int P = 8 * NT + 1, CN = 16;
   __shared__ float red[8][CN][P];
   __shared__ __align__(16) float s_h[kOwn ? kOwnRows : 1][64];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, q = lane % 4;
@@ -133,33 +135,23 @@ __global__ void __launch_bounds__(256) k_lowrank_few(const bnnk_lowrank_args p) 
   if (kOwn) wait_launch_before();  // the only launch; else it follows the one that forms h, which has waited
   launch_dependents();
   const elem_t<T> *W = (const elem_t<T> *)p.w, *x = (const elem_t<T> *)p.x, *B = (const elem_t<T> *)p.b;
-  float acc[MT][NT][4] = {};
+  float acc[NT][4] = {};
 #pragma unroll 4
   for (int k0 = 32 * warp; k0 < K; k0 += 256) {
-    const int k = k0 + 8 * q;
-    uint4 wa[MT], wb[MT];
-#pragma unroll
-    for (int m = 0; m < MT; m++) {
-      const int n = n0 + 16 * m + g;
-      wa[m] = ldg16(W + (long long)n * p.ldw + k, n < p.N && k < K);
-      wb[m] = ldg16(W + (long long)(n + 8) * p.ldw + k, n + 8 < p.N && k < K);
-    }
+    const int k = k0 + 8 * q, n = n0 + g;
+    const uint4 wa = ldg16(W + (long long)n * p.ldw + k, n < p.N && k < K);
+    const uint4 wb = ldg16(W + (long long)(n + 8) * p.ldw + k, n + 8 < p.N && k < K);
 #pragma unroll
     for (int j = 0; j < NT; j++) {
       const uint4 b = ldg16(x + (8 * j + g) * p.ldx + k, 8 * j + g < p.rows && k < K);
-#pragma unroll
-      for (int m = 0; m < MT; m++) {
-        mma_sync<T>(acc[m][j], wa[m].x, wb[m].x, wa[m].y, wb[m].y, b.x, b.y);
-        mma_sync<T>(acc[m][j], wa[m].z, wb[m].z, wa[m].w, wb[m].w, b.z, b.w);
-      }
+      mma_sync<T>(acc[j], wa.x, wb.x, wa.y, wb.y, b.x, b.y);
+      mma_sync<T>(acc[j], wa.z, wb.z, wa.w, wb.w, b.z, b.w);
     }
   }
 #pragma unroll
-  for (int m = 0; m < MT; m++)
+  for (int j = 0; j < NT; j++)
 #pragma unroll
-    for (int j = 0; j < NT; j++)
-#pragma unroll
-      for (int e = 0; e < 4; e++) red[warp][16 * m + g + 8 * (e / 2)][8 * j + 2 * q + e % 2] = acc[m][j][e];
+    for (int e = 0; e < 4; e++) red[warp][g + 8 * (e / 2)][8 * j + 2 * q + e % 2] = acc[j][e];
   constexpr int OUTS = (8 * NT * CN + 255) / 256, RSTEP = 256 / CN;  // a lane's rows: r0, r0 + RSTEP, ..
   const int c = threadIdx.x % CN, r0 = threadIdx.x / CN, n = n0 + c;
   float u[OUTS];
@@ -231,7 +223,7 @@ __global__ void __launch_bounds__(256) k_lowrank_few(const bnnk_lowrank_args p) 
   }
 }
 
-// ------------------------------------------------------------------ 17 to 64 rows
+// ------------------------------------------------------------------ 17 to 128 rows
 //
 // Still bound by reading W and, with an adapter a row, B: a tcgen05 tile of the (up to 64 of 128) rows and 16 GR columns a
 // CTA, x and W streamed by TMA through a ring deep enough for the memory's latency, one thread issuing. Meanwhile 8 warps
@@ -240,7 +232,11 @@ __global__ void __launch_bounds__(256) k_lowrank_few(const bnnk_lowrank_args p) 
 // share); the accumulators then come from TMEM through shared memory to the threads that hold them. Four accumulators take
 // a stage's four steps of 16: the tensor cores' fp32 sums lose a little at every step (K 1024 in one chain was 6.9e-7 off
 // in fp32 outputs, against 2.6e-7 for a plain fp32 sum), so the chains are kept short.
-constexpr int kMidRows = 64, kMidThreads = 320, kMidStages = 8;
+// Class head of 64 stations with an adapter each (64 x 1024 x 6522, rank 16, fp32 logits): 14 us.
+// More rows than 64 take one CTA per 64 of them. The many-row form gives each adapter of a tile its own steps; an adapter a
+// row is its worst case, one adapter its best (128 rows of 1024 x 6522, rank 32, fp32, us, this form / that one: an adapter
+// a row 43 / 103, 8 rows each 37 / 43, 64 each 36 / 25; 512 rows: 113 / 202, 100 / 70, 100 / 33). 128 rows are the middle.
+constexpr int kMidRows = 64, kMidMost = 128, kMidThreads = 320, kMidStages = 8;
 
 struct MidArgs {
   bnnk_lowrank_args p;
@@ -260,7 +256,7 @@ __global__ void __launch_bounds__(kMidThreads, 1) k_lowrank_mid(const __grid_con
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   const bnnk_lowrank_args &p = a.p;
   constexpr uint32_t a_bytes = 128 * 128, stage = (128 + BN) * 128, tmem_cols = BN == 48 ? 256 : 4 * BN;
-  const int S = a.stages, n0 = blockIdx.x * BN;
+  const int S = a.stages, n0 = blockIdx.x * BN, m0 = blockIdx.y * kMidRows;
   launch_dependents();
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; s++) { mbar_init(smem_u32(&b_full[s]), 1); mbar_init(smem_u32(&b_empty[s]), 1); }
@@ -295,7 +291,7 @@ __global__ void __launch_bounds__(kMidThreads, 1) k_lowrank_mid(const __grid_con
       const uint32_t st = base + s * stage, bar = smem_u32(&b_full[s]);
       if (elect_one()) {
         mbar_expect_tx(bar, kMidRows * 128 + BN * 128);  // the rows past 64 of the A tile are never written nor used
-        tma_load_2d(st, &mx, bar, kb * 64, 0);
+        tma_load_2d(st, &mx, bar, kb * 64, m0);
         tma_load_2d(st + a_bytes, &mw, bar, kb * 64, n0);
       }
     }
@@ -315,7 +311,7 @@ __global__ void __launch_bounds__(kMidThreads, 1) k_lowrank_mid(const __grid_con
     }
     if (ok && elect_one()) mma_commit(smem_u32(&b_acc));
   } else {
-    const int tid = threadIdx.x - 64, c = tid % 16, r0 = tid / 16, rank = p.rank;
+    const int tid = threadIdx.x - 64, c = tid % 16, r0 = m0 + tid / 16, rank = p.rank;
     const elem_t<T> *B = (const elem_t<T> *)p.b;
     float u[GR][RI] = {};
     int s[RI];
@@ -392,7 +388,7 @@ __global__ void __launch_bounds__(kMidThreads, 1) k_lowrank_mid(const __grid_con
 #pragma unroll
         for (int i = 0; i < RI; i++) {
           const int r = r0 + 16 * i;
-          if (r < p.rows) ((elem_t<OT> *)p.y)[r * p.ldy + n] = Elem<OT>::put(s_y[r][16 * gr + c] + bias + u[gr][i]);
+          if (r < p.rows) ((elem_t<OT> *)p.y)[(long long)r * p.ldy + n] = Elem<OT>::put(s_y[r - m0][16 * gr + c] + bias + u[gr][i]);
         }
       }
     }
@@ -415,7 +411,10 @@ __global__ void __launch_bounds__(kMidThreads, 1) k_lowrank_mid(const __grid_con
 // One persistent CTA per SM, column tiles fastest. Warp 0 streams 64-wide steps of x and W into a ring by TMA; warp 1
 // issues the MMAs into one of two accumulators; warps 2 .. 5 make the list and h's operand tiles and load the B_a tiles;
 // warps 6 .. 13 store y: accumulator rows through shared memory, so that a store covers 32 neighbouring words of a row at
-// any row alignment.
+// any row alignment; 16 bytes a lane where y's rows are whole 16 bytes.
+// Bound by reading x and W from L2 (48 KB for 1040 cycles of products at 256 columns). 9001 x 1536 x 6144 without adapters
+// 130 us, 1.31 PFLOP/s (the library's product: 123 us); adapters of 700 rows and rank 32 on top 37 us, 27 of them to form h. Tiles of 256
+// rows, which read half of W, left no TMEM for a second accumulator: 241 us in place of 212 at the time.
 constexpr int kLrThreads = 448;
 constexpr int kLrStages = 8;
 constexpr int kLrPad = 20;  // words a row of the stores' shared memory: blocks of 16 words; 16-byte accesses meet no bank twice
@@ -785,20 +784,18 @@ __global__ void __launch_bounds__(kLrThreads, 1) k_lowrank_many(const __grid_con
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(a.tmem_cols));
 }
 
-template <int T, int OT, int MT, int NT>
+template <int T, int OT, int NT>
 cudaError_t few_nt(const bnnk_lowrank_args &p, cudaStream_t st) {
-  const dim3 grid((p.N + 16 * MT - 1) / (16 * MT));
-  if (p.slot && p.rows > kOwnRows) return launch_early(k_lowrank_few<T, OT, MT, NT, false>, grid, 256, 0, st, p);
-  if (p.slot) return launch_early(k_lowrank_few<T, OT, MT, NT, true>, grid, 256, 0, st, p);
-  k_lowrank_few<T, OT, MT, NT, false><<<grid, 256, 0, st>>>(p);
+  const dim3 grid((p.N + 15) / 16);
+  if (p.slot && p.rows > kOwnRows) return launch_early(k_lowrank_few<T, OT, NT, false>, grid, 256, 0, st, p);
+  if (p.slot) return launch_early(k_lowrank_few<T, OT, NT, true>, grid, 256, 0, st, p);
+  k_lowrank_few<T, OT, NT, false><<<grid, 256, 0, st>>>(p);
   return cudaGetLastError();
 }
 
 template <int T, int OT>
 cudaError_t run_few(const bnnk_lowrank_args &p, cudaStream_t st) {
-  // 32 rows of W a CTA halve the reads of x; 16 where they would leave SMs idle
-  if ((p.N + 31) / 32 >= num_sms()) return p.rows <= 8 ? few_nt<T, OT, 2, 1>(p, st) : few_nt<T, OT, 2, 2>(p, st);
-  return p.rows <= 8 ? few_nt<T, OT, 1, 1>(p, st) : few_nt<T, OT, 1, 2>(p, st);
+  return p.rows <= 8 ? few_nt<T, OT, 1>(p, st) : few_nt<T, OT, 2>(p, st);
 }
 
 template <int T, int OT, int GR>
@@ -813,7 +810,7 @@ int mid_groups(const bnnk_lowrank_args &p, int *err, cudaStream_t st) {
   static SmemAttr attr;
   if (!e) e = attr.ensure(k_lowrank_mid<T, OT, GR>, smem);
   if (e) return e;
-  const dim3 grid((p.N + BN - 1) / BN);
+  const dim3 grid((p.N + BN - 1) / BN, (p.rows + kMidRows - 1) / kMidRows);
   if (p.slot) return launch_early(k_lowrank_mid<T, OT, GR>, grid, kMidThreads, smem, st, mx, mw, a);
   k_lowrank_mid<T, OT, GR><<<grid, kMidThreads, smem, st>>>(mx, mw, a);
   return cudaGetLastError();
@@ -821,8 +818,8 @@ int mid_groups(const bnnk_lowrank_args &p, int *err, cudaStream_t st) {
 
 template <int T, int OT>
 int run_mid(const bnnk_lowrank_args &p, int *err, cudaStream_t st) {
-  // as few columns a CTA as fill the SMs once, up to 48
-  const int n = (p.N + 15) / 16, sms = num_sms();
+  // as few columns a CTA as fill the SMs once, up to 48 (64 rows of 6522 x 1024 with 16, 32, 48: 31.7, 24.0, 21.5 us)
+  const int n = (p.N + 15) / 16 * ((p.rows + kMidRows - 1) / kMidRows), sms = num_sms();
   return n <= sms ? mid_groups<T, OT, 1>(p, err, st) : n <= 2 * sms ? mid_groups<T, OT, 2>(p, err, st)
                                                                     : mid_groups<T, OT, 3>(p, err, st);
 }
@@ -834,7 +831,8 @@ int run_many(const bnnk_lowrank_args &p, int *err, cudaStream_t st) {
   a.err = err;
   a.nkb = (p.K + 63) / 64;
   // fp32 outputs: the tensor cores' chains of fp32 sums kept to about 1024 values of K (one of 1024 was 6.9e-7 off, against
-  // 2.6e-7 for a plain fp32 sum); a 16-bit output's rounding hides them
+  // 2.6e-7 for a plain fp32 sum), for narrower tiles (2000 rows of 2720, us with 1, 2, 4 accumulators: K 512 25.6, 28.2,
+  // 33.8, K 1536 35.8, 37.9, 50.2, K 4096 64.5, 68.9, 105); a 16-bit output's rounding hides them
   a.na = OT != 0 || p.K <= 512 ? 1 : p.K <= 2048 ? 2 : 4;
   // column tiles of at most 256 / na, of equal widths, narrower while there are fewer tiles than SMs
   const int n16 = (p.N + 15) & ~15, mt = (p.rows + 127) / 128, most = 256 / a.na;
@@ -872,9 +870,14 @@ cudaError_t down_rows(const bnnk_lowrank_args &p, int adapters, cudaStream_t st)
 
 template <int T, int RT>
 cudaError_t run_down(const bnnk_lowrank_args &p, cudaStream_t st) {
-  // an adapter a CTA where there are few rows; of many rows' tiles most hold one adapter
-  if (p.rows <= 512 || RT == 8) return down_rows<T, RT, 1>(p, p.rows <= 512 ? kDownRows : 2, st);
-  return down_rows<T, RT, RT == 8 ? 1 : 2>(p, 2, st);
+  // 32-row tiles halve the reads of A; 16 where rows are few, or the sums would not fit (700 rows an adapter, K 1536, rank
+  // 32, us for the operator with 16 / 32: 300 rows 30.7 / 24.6, 9001 rows 171 / 164; 64 adapters, K 1024, rank 16, 64 rows
+  // 13.6 / 16.6). As many CTAs a tile as its rows can have adapters while the tiles are few, two where they fill the SMs,
+  // since most then hold one or two (an adapter a row, 300 rows, 2 / 16: 57 / 35; 700 rows an adapter, 9001 rows 164 / 180)
+  const bool small = RT == 8 || p.rows <= kMidMost;
+  const int tiles = (p.rows + (small ? 15 : 31)) / (small ? 16 : 32), share = 512 / tiles;
+  const int y = share < 2 ? 2 : share > 16 ? 16 : share;
+  return small ? down_rows<T, RT, 1>(p, y, st) : down_rows<T, RT, RT == 8 ? 1 : 2>(p, y, st);
 }
 
 template <int T>
@@ -884,7 +887,7 @@ int run_lowrank(const bnnk_lowrank_args &p, int *err, cudaStream_t st) {
     if (e) return e;
   }
   if (p.rows <= kFewRows) return p.otype == 0 ? run_few<T, 0>(p, st) : run_few<T, T>(p, st);
-  if (p.rows <= kMidRows) return p.otype == 0 ? run_mid<T, 0>(p, err, st) : run_mid<T, T>(p, err, st);
+  if (p.rows <= kMidMost) return p.otype == 0 ? run_mid<T, 0>(p, err, st) : run_mid<T, T>(p, err, st);
   if (p.otype == 0)
     return p.rank <= 16 ? run_many<T, 0, 16>(p, err, st) : p.rank <= 32 ? run_many<T, 0, 32>(p, err, st)
                                                                          : run_many<T, 0, 64>(p, err, st);
