@@ -46,7 +46,8 @@ __device__ __forceinline__ void seq_range(const DattnArgs &a, int i, long long &
 // + 4 warps p), a warp's access is 4 rows of 128 consecutive bytes. Per token the update and, for each q head of the
 // group, the partial sums over the thread's rows, joined over the warp's 4 row groups by shuffles and over the warps
 // through shared memory, in a fixed order.
-// Bound by memory for single tokens: S is read once and written once (at most 8 + 8 KB a CTA).
+// Bound by memory for single tokens: S is read once and written once (at most 8 + 8 KB a CTA). 300 sequences of 16 heads of
+// 64 x 64 (160 MB): 32 us, 4.9 TB/s; one sequence: 8 us, a launch and two waits for memory.
 constexpr int kRecG = 8;  // q heads whose partial sums are in shared memory at once
 
 template <int T>
@@ -164,13 +165,19 @@ __global__ void __launch_bounds__(256) k_dattn_rec(const DattnArgs a) {
 //    scales go into the fp32 steps after the products. Values 2^28 below the maximum are the first to lose bits.
 //
 // One CTA per (segment of a sequence, k/v head) walks the segment's chunks, and for each the G q heads of the group
-// ("unit" u = (chunk, q head)). Roles: warps 0 and 2 MMA issue, warp 1 TMA, 8 warps turn QK into P (in place in TMEM, as the A
-// operand of the last product) and join O1 and O2 into o, 16 warps hold S in registers and form K' and the S operand. S in
-// registers stays fp32: lambda^n S + DS, once a chunk. The roles' loops are rolled: unrolled, their code
-// did not stay in the instruction cache together and a unit took twice as long. The issuing warp stays converged
+// ("unit" u = (chunk, q head)). Roles: warps 0 and 2 MMA issue, warp 1 TMA, 8 warps turn QK into P (in place in TMEM, as the
+// A operand of the last product) and join O1 and O2 into o, 16 warps hold S in registers and form K' and the S operand. S
+// in registers stays fp32: lambda^n S + DS, once a chunk. The roles' loops are rolled: unrolled, their code did not stay in
+// the instruction cache together and a unit took twice as long. The issuing warp stays converged
 // (elect.sync): from one lane's branch each tcgen05.mma took 70 cycles to issue, more than a 128 x 64 x 16 product.
 // A masked token, and a row past the segment's end, has its k and v rows taken as zero (K' zero, V zeroed in shared
 // memory, its P column zero by selection, so that NaN and infinities there stay out); its o row is zero or not stored.
+//
+// Bound by its roles' chain through a chunk and by shared memory's bandwidth, not by the products: DP 64 takes 4900 cycles a
+// chunk and head, of which the products are 2400 (each operand's parts are products of their own). 24 sequences of 9600
+// tokens, 16 heads of 64 (bf16, 1.9 GB): 657 us, 2.9 TB/s; 384 CTAs on 148 SMs are 2.6 rounds that take 3. DP 128 has
+// shared memory for one stage only: one sequence of 28800 tokens, 12 heads of 128 (0.35 GB): 183 us, 62 of them the first
+// pass for the parts' states. 37 sequences of 1 to 611 tokens, 4 heads of 96 x 72 shared by 3 (fp16): 76 us.
 constexpr int kChunk = 128;
 constexpr int kDaThreads = 896;
 constexpr int kDaP = 4, kDaS = 12;  // first warps of the P and state roles
@@ -224,8 +231,8 @@ __device__ bool find_segment(const DaArgs &a, int s, int &seq, int &part, long l
   return false;
 }
 
-// Shared memory and TMEM. A pass for the state alone has no Q and no S operand. Else, DP 128: one stage of Q, K, V, and the first part of K' in K's place (it waits for QK to have
-// read K); DP 64: two stages (three of K), two QK / P regions, two sets of K', formed a chunk ahead.
+// Shared memory and TMEM. A pass for the state alone has no Q and no S operand. Else, DP 128: one stage of Q, K, V, and the
+// first part of K' in K's place (it waits for QK to have read K); DP 64: two stages (three of K), two QK / P regions, two sets of K', formed a chunk ahead.
 template <int T, int DP, bool kState>
 struct DaLayout {
   static constexpr int parts = T == 2 ? 3 : 2;      // of K'
@@ -240,7 +247,8 @@ struct DaLayout {
   static constexpr uint32_t q = 0, k = q + (kState ? 0 : stages * tile), v = k + k_stages * tile, kp = v + stages * tile,
                             st = kp + (in_place ? parts - 1 : kp_sets * parts) * tile, end = st + (kState ? 0 : 2 * s_tile);
   static constexpr uint32_t t_qk = 0, t_o1 = qk_bufs * 128, t_o2 = t_o1 + DP, t_ds = t_o2 + DP;  // TMEM columns
-  static constexpr size_t smem = end + 1024 + (kState && DP == 64 ? panel : 0);  // the last part's second panel is read, not used
+  // kState: the last part's second panel is read, not used
+  static constexpr size_t smem = end + 1024 + (kState && DP == 64 ? panel : 0);
   static constexpr int scales = T == 1 ? (qk_bufs == 2 ? 4 : 2) : 1;  // P row scales: units until o has read them
   // part x of K' of set s
   static __device__ __forceinline__ uint32_t kpart(uint32_t base, int s, int x) {
@@ -1001,8 +1009,11 @@ int run_chunk(const DaArgs &a, cudaStream_t st) {
 
 using namespace bnn;
 
-// Tokens of a segment, 0 for whole sequences. Whole sequences where they are enough CTAs for the SMs: one pass. Fewer:
-// parts of about equal length, one per SM, whose states come from a first pass over K and V.
+// Tokens of a segment, 0 for whole sequences. Whole sequences where they are enough CTAs for half of the SMs: one pass.
+// Fewer: parts of about equal length, one per SM, whose states come from a first pass over K and V. 8 heads, d 64, us whole
+// / in parts: 1 sequence of 2400 tokens 56 / 25, of 9600 185 / 39; 4 of 2400 57 / 41; 8 of 2400 59 / 69, of 9600 195 / 180;
+// 12 of 9600 199 / 280; d 128: 1 of 2400 94 / 36. The lengths are known on the device alone: 8 even sequences lose 10 us
+// by parts, a long one among 7 short ones gains 146.
 static int segment_tokens(int n, int Hk, long long tokens) {
   const long long sms = num_sms(), ctas = (long long)n * Hk;
   if (ctas * 2 > sms) return 0;
