@@ -247,7 +247,9 @@ bnn_dattn *bnn_dattn_new(int type, int heads, int kv_heads, int dk, int dv, cons
  * slot, slot = d_slot[i] (d_slot NULL: i; a negative slot starts from zero and its state is dropped; no two sequences
  * of a call share a slot). d_s0 NULL: all start from zero; d_s1 NULL: no state is kept; d_s1 may be d_s0. A token whose
  * byte of d_live (NULL: all live) is 0 is a window that failed or is missing: its q, k and v are not used, its o is 0,
- * and the state decays by its step. */
+ * and the state decays by its step. A live token with an infinity or a NaN makes its own head's state and all later
+ * outputs of its sequence non-finite, and may do so to outputs up to 127 tokens before it (they are formed in chunks);
+ * other sequences keep theirs. */
 int bnn_dattn_run(bnn_dattn *op, int n, long long tokens, const int32_t *d_cu, const int32_t *d_slot,
                   const uint8_t *d_live, const void *d_q, long long qts, const void *d_k, long long kts, const void *d_v,
                   long long vts, const float *d_s0, float *d_s1, void *d_o, long long ots, void *stream);
@@ -269,7 +271,9 @@ typedef struct bnn_lowrank bnn_lowrank;
 bnn_lowrank *bnn_lowrank_new(int type, int out_type, int N, int K, const void *d_w, long long ldw, const float *d_bias,
                              int slots, int rank, const void *d_a, const void *d_b, const float *d_scale, int rows);
 /* d_x [rows][K] at row stride ldx (a multiple of 8, 16-byte aligned) -> d_y [rows][N] at row stride ldy; d_slot [rows]:
- * the rows' adapters in any order (outside 0 .. slots - 1: none), NULL: none for all */
+ * the rows' adapters in any order (outside 0 .. slots - 1: none), NULL: none for all. An infinity or a NaN in d_x stays
+ * in its row; one in d_b of an adapter may reach, in a call of more than 128 rows, the rows of others beside its own
+ * rows (they share tiles of 128). */
 int bnn_lowrank_run(bnn_lowrank *op, int rows, const void *d_x, long long ldx, const int32_t *d_slot, void *d_y,
                     long long ldy, void *stream);
 /* the op's device error word (0 = no bounded wait ran out); synchronous */
