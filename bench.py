@@ -637,7 +637,8 @@ def perch_int8(torch, stream, batch=512, steps=5, cpu=True):
     finally:
         m.close()
     base = checked = None
-    if cpu:
+    from oracle import ref  # pylint: disable=import-outside-toplevel
+    if cpu and ref.available():  # the port has no fp32 body ops: only the reference build runs this package on the CPU
         cores = os.cpu_count() or 1
         n = min(batch, cores)
         kind, crun, what = cpu_runner(pkg, mode=4)
@@ -646,7 +647,6 @@ def perch_int8(torch, stream, batch=512, steps=5, cpu=True):
         dt = time.perf_counter() - t0
         base = {"value": round(n / dt, 3), "unit": "windows/s", "cores": cores, "kind": kind,
                 "sample": f"{n} windows, one per thread, {dt:.1f} s: {what}"}
-        from oracle import ref  # pylint: disable=import-outside-toplevel
         idx = chunk_boundary_sample(batch, batch, 4)
         want, wemb, rc = ref.run_many(pkg, 4, np.ascontiguousarray(pcm[idx]), threads=min(len(idx), cores))
         bad = int(sum(not (np.array_equal(got[w].view(np.int32), want[j].view(np.int32)) and
