@@ -114,14 +114,18 @@ SIGNATURES = {
     "bnn_dattn_new": (_P, [_I, _I, _I, _I, _I, _P, ctypes.c_float, _I, _LL]),
     "bnn_dattn_run": (_I, [_P, _I, _LL, _P, _P, _P, _P, _LL, _P, _LL, _P, _LL, _P, _P, _P, _LL, _P]),
     "bnn_dattn_step": (_I, [_P, _I, _P, _P, _P, _LL, _P, _LL, _P, _LL, _P, _P, _P, _LL, _P]),
+    "bnn_dattn_run_words": (_I, [_P, _P]),
+    "bnn_dattn_step_words": (_I, [_P, _P]),
     "bnn_dattn_error": (_I, [_P]),
     "bnn_dattn_free": (None, [_P]),
     "bnn_lowrank_new": (_P, [_I, _I, _I, _I, _P, _LL, _P, _I, _I, _P, _P, _P, _I]),
     "bnn_lowrank_run": (_I, [_P, _I, _P, _LL, _P, _P, _LL, _P]),
+    "bnn_lowrank_run_words": (_I, [_P, _P]),
     "bnn_lowrank_error": (_I, [_P]),
     "bnn_lowrank_free": (None, [_P]),
     "bnn_norm_gate_new": (_P, [_I, _I, _I, _I, _I, ctypes.c_float, ctypes.c_float, _P, _P, _P, _P, _P]),
     "bnn_norm_gate_run": (_I, [_P, _I, _P, _LL, _P, _LL, _P, _LL, _P, _P, _LL, _P, _LL, _P]),
+    "bnn_norm_gate_run_words": (_I, [_P, _P]),
     "bnn_norm_gate_free": (None, [_P]),
 }
 

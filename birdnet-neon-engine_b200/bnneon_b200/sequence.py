@@ -9,6 +9,8 @@ Buffers are device pointers (ints, e.g. a torch tensor's data_ptr()) and `stream
 legacy default stream), as Model.infer_device takes them; calls are asynchronous. Strides default to packed rows.
 An object's calls share its scratch: order them on one stream, or give each stream an object of its own.
 """
+import struct
+
 import numpy as np
 
 from . import BnnError, last_error, load_library
@@ -16,6 +18,9 @@ from . import BnnError, last_error, load_library
 TYPES = {"f32": 0, "f16": 1, "bf16": 2}
 NORMS = {"rms": 0, "layer": 1}
 GATES = {"none": 0, "sigmoid": 1, "silu": 2}
+
+# a call's arguments as 64-bit words: ctypes takes about 0.1 us for each argument, more than a small call's launch
+_WORDS = {n: struct.Struct(f"{n}q").pack for n in (7, 13, 14, 16)}
 
 
 def _code(table, what, name):
@@ -36,10 +41,6 @@ class _Op:
         if not op:
             raise last_error(self.h)
         self.op = op
-
-    def _check(self, rc):
-        if rc:
-            raise last_error(self.h)
 
     def close(self):
         if self.op:
@@ -77,14 +78,18 @@ class DecayAttention(_Op):
     def run(self, n, tokens, cu, q, k, v, o, s0=None, s1=None, slot=None, live=None, qts=None, kts=None, vts=None,
             ots=None, stream=None):
         """n sequences, sequence i the tokens cu[i] .. cu[i + 1] - 1"""
-        self._check(self.h.bnn_dattn_run(self.op, n, tokens, cu, slot, live, q, qts or self.q_row, k, kts or self.k_row,
-                                         v, vts or self.v_row, s0, s1, o, ots or self.o_row, stream))
+        if self.h.bnn_dattn_run_words(self.op, _WORDS[16](
+                n, tokens, cu or 0, slot or 0, live or 0, q or 0, qts or self.q_row, k or 0, kts or self.k_row, v or 0,
+                vts or self.v_row, s0 or 0, s1 or 0, o or 0, ots or self.o_row, stream or 0)):
+            raise last_error(self.h)
 
     def step(self, n, q, k, v, o, s0=None, s1=None, slot=None, live=None, qts=None, kts=None, vts=None, ots=None,
              stream=None):
         """n sequences of one token each"""
-        self._check(self.h.bnn_dattn_step(self.op, n, slot, live, q, qts or self.q_row, k, kts or self.k_row, v,
-                                          vts or self.v_row, s0, s1, o, ots or self.o_row, stream))
+        if self.h.bnn_dattn_step_words(self.op, _WORDS[14](
+                n, slot or 0, live or 0, q or 0, qts or self.q_row, k or 0, kts or self.k_row, v or 0, vts or self.v_row,
+                s0 or 0, s1 or 0, o or 0, ots or self.o_row, stream or 0)):
+            raise last_error(self.h)
 
     @property
     def error(self):
@@ -103,7 +108,9 @@ class LowRank(_Op):
         self.N, self.K = N, K
 
     def run(self, rows, x, slot, y, ldx=None, ldy=None, stream=None):
-        self._check(self.h.bnn_lowrank_run(self.op, rows, x, ldx or self.K, slot, y, ldy or self.N, stream))
+        if self.h.bnn_lowrank_run_words(self.op, _WORDS[7](rows, x or 0, ldx or self.K, slot or 0, y or 0, ldy or self.N,
+                                                          stream or 0)):
+            raise last_error(self.h)
 
     @property
     def error(self):
@@ -125,5 +132,7 @@ class NormGate(_Op):
 
     def run(self, rows, x, f, g, xo, h, live=None, xs=None, fs=None, gs=None, xos=None, hs=None, stream=None):
         D = self.D
-        self._check(self.h.bnn_norm_gate_run(self.op, rows, x, xs or D, f, fs or D, g, gs or D, live, xo, xos or D, h,
-                                             hs or D, stream))
+        if self.h.bnn_norm_gate_run_words(self.op, _WORDS[13](
+                rows, x or 0, xs or D, f or 0, fs or D, g or 0, gs or D, live or 0, xo or 0, xos or D, h or 0, hs or D,
+                stream or 0)):
+            raise last_error(self.h)

@@ -134,6 +134,20 @@ int bnn_dattn_step(bnn_dattn *o, int n, const int32_t *d_slot, const uint8_t *d_
                       stream);
 }
 
+#define P(i) ((void *)(uintptr_t)w[i])
+/* a count that an int does not hold is refused as a negative one */
+static int count_of(long long v) { return v < 0 || v > 0x7fffffff ? -1 : (int)v; }
+
+int bnn_dattn_run_words(bnn_dattn *o, const long long *w) {
+  return bnn_dattn_run(o, count_of(w[0]), w[1], P(2), P(3), P(4), P(5), w[6], P(7), w[8], P(9), w[10], P(11), P(12), P(13),
+                       w[14], P(15));
+}
+
+int bnn_dattn_step_words(bnn_dattn *o, const long long *w) {
+  return bnn_dattn_step(o, count_of(w[0]), P(1), P(2), P(3), w[4], P(5), w[6], P(7), w[8], P(9), P(10), P(11), w[12],
+                        P(13));
+}
+
 int bnn_dattn_error(bnn_dattn *o) { return o ? read_word(o->err) : -1; }
 
 void bnn_dattn_free(bnn_dattn *o) {
@@ -193,6 +207,10 @@ int bnn_lowrank_run(bnn_lowrank *o, int rows, const void *d_x, long long ldx, co
   return launch_rc("bnn_lowrank_run", bnnk_lowrank(&a, (bnn_stream_t)stream));
 }
 
+int bnn_lowrank_run_words(bnn_lowrank *o, const long long *w) {
+  return bnn_lowrank_run(o, count_of(w[0]), P(1), w[2], P(3), P(4), w[5], P(6));
+}
+
 int bnn_lowrank_error(bnn_lowrank *o) { return o ? read_word(o->a.err) : -1; }
 
 void bnn_lowrank_free(bnn_lowrank *o) {
@@ -250,6 +268,10 @@ int bnn_norm_gate_run(bnn_norm_gate *o, int rows, const void *d_x, long long xs,
   a.x = d_x; a.xs = xs; a.f = d_f; a.fs = fs; a.g = d_g; a.gs = gs; a.live = d_live;
   a.xo = d_xo; a.xos = xos; a.h = d_h; a.hs = hs;
   return launch_rc("bnn_norm_gate_run", bnnk_norm_gate(&a, (bnn_stream_t)stream));
+}
+
+int bnn_norm_gate_run_words(bnn_norm_gate *o, const long long *w) {
+  return bnn_norm_gate_run(o, count_of(w[0]), P(1), w[2], P(3), w[4], P(5), w[6], P(7), P(8), w[9], P(10), w[11], P(12));
 }
 
 void bnn_norm_gate_free(bnn_norm_gate *o) { free(o); }

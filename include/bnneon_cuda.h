@@ -257,6 +257,10 @@ int bnn_dattn_run(bnn_dattn *op, int n, long long tokens, const int32_t *d_cu, c
 int bnn_dattn_step(bnn_dattn *op, int n, const int32_t *d_slot, const uint8_t *d_live, const void *d_q, long long qts,
                    const void *d_k, long long kts, const void *d_v, long long vts, const float *d_s0, float *d_s1,
                    void *d_o, long long ots, void *stream);
+/* the same calls with the arguments after op as 64-bit words in their order (16 and 14 of them): one pointer for
+ * bindings that pay for every argument */
+int bnn_dattn_run_words(bnn_dattn *op, const long long *words);
+int bnn_dattn_step_words(bnn_dattn *op, const long long *words);
 /* the op's device error word (0 = no bounded wait ran out); synchronous */
 int bnn_dattn_error(bnn_dattn *op);
 void bnn_dattn_free(bnn_dattn *op);
@@ -276,6 +280,7 @@ bnn_lowrank *bnn_lowrank_new(int type, int out_type, int N, int K, const void *d
  * rows (they share tiles of 128). */
 int bnn_lowrank_run(bnn_lowrank *op, int rows, const void *d_x, long long ldx, const int32_t *d_slot, void *d_y,
                     long long ldy, void *stream);
+int bnn_lowrank_run_words(bnn_lowrank *op, const long long *words); /* the 7 arguments after op as words */
 /* the op's device error word (0 = no bounded wait ran out); synchronous */
 int bnn_lowrank_error(bnn_lowrank *op);
 void bnn_lowrank_free(bnn_lowrank *op);
@@ -295,6 +300,7 @@ bnn_norm_gate *bnn_norm_gate_new(int D, int x_type, int type, int norm, int gate
 int bnn_norm_gate_run(bnn_norm_gate *op, int rows, const void *d_x, long long xs, const void *d_f, long long fs,
                       const void *d_g, long long gs, const uint8_t *d_live, void *d_xo, long long xos, void *d_h,
                       long long hs, void *stream);
+int bnn_norm_gate_run_words(bnn_norm_gate *op, const long long *words); /* the 13 arguments after op as words */
 void bnn_norm_gate_free(bnn_norm_gate *op);
 
 /* the current device's error word of the per-op entry points (0 = no bounded device wait ran out; then reset to 0;

@@ -715,3 +715,75 @@ def test_new_reports_out_of_memory(cuda):
         assert e.value.kind == "OOM"
     finally:
         h.bnn_debug_fail_alloc(0, 0)
+
+
+# ------------------------------------------------------------------ the entry points' two forms, captured calls
+
+
+def block(seed=0, n=5, lens=(3, 140, 0, 1, 260)):
+    """one of each operator with its buffers: (objects, calls by the plain entry points, calls by the Python methods)"""
+    a = Attention("bf16", 2, 2, 64, 64, list(lens), 0.2, seed=seed)
+    att, s1 = a.op(), torch.zeros_like(a.s0)
+    gen = generator(seed)
+    x, w = rand(gen, 40, 64).bfloat16(), rand(gen, 96, 64).bfloat16()
+    A, B = rand(gen, 2, 8, 64).bfloat16(), rand(gen, 2, 96, 8).bfloat16()
+    slot, y = torch.randint(-1, 2, (40,), device="cuda", generator=gen).int(), torch.zeros(40, 96, device="cuda")
+    low = sequence.LowRank("bf16", "f32", 96, 64, w.data_ptr(), None, 2, 8, A.data_ptr(), B.data_ptr(), rows=40)
+    r, f, g = rand(gen, 30, 72), rand(gen, 30, 72).bfloat16(), rand(gen, 30, 72).bfloat16()
+    ro, h = torch.zeros_like(r), torch.zeros_like(f)
+    norm = sequence.NormGate(72, "f32", "bf16", "layer", "silu")
+    b = Attention("bf16", 2, 2, 64, 64, [1] * n, seed=seed + 1)
+    bs1 = torch.zeros_like(b.s0)
+    p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+
+    def plain(st):
+        c = att.h
+        assert not c.bnn_dattn_run(att.op, len(lens), sum(lens), p(a.cu), p(a.slot), p(a.live), p(a.q), a.ts, p(a.k), a.ts,
+                                   p(a.v), a.ts, p(a.s0), p(s1), p(a.o), 128, st)
+        assert not c.bnn_dattn_step(att.op, n, p(b.slot), None, p(b.q), b.ts, p(b.k), b.ts, p(b.v), b.ts, p(b.s0), p(bs1),
+                                    p(b.o), 128, st)
+        assert not c.bnn_lowrank_run(low.op, 40, p(x), 64, p(slot), p(y), 96, st)
+        assert not c.bnn_norm_gate_run(norm.op, 30, p(r), 72, p(f), 72, p(g), 72, None, p(ro), 72, p(h), 72, st)
+
+    def methods(st):
+        a.run(att, s1=s1, stream=st)
+        b.run(att, s1=bs1, stream=st, step=True)
+        low.run(40, p(x), p(slot), p(y), stream=st)
+        norm.run(30, p(r), p(f), p(g), p(ro), p(h), stream=st)
+
+    return (x, w, A, B, att, low, norm, slot), (a.o, s1, b.o, bs1, y, ro, h), plain, methods
+
+
+@gpu
+def test_plain_entry_points_give_what_the_methods_give(cuda):
+    keep, outs, plain, methods = block()
+    st = torch.cuda.current_stream().cuda_stream
+    methods(st)
+    want = [t.clone() for t in outs]
+    for t in outs:
+        t.zero_()
+    plain(st)
+    assert all(torch.equal(t, w) for t, w in zip(outs, want))
+    del keep
+
+
+@gpu
+def test_calls_in_a_captured_graph(cuda):
+    keep, outs, _, methods = block(seed=3)
+    methods(torch.cuda.current_stream().cuda_stream)
+    want = [t.clone() for t in outs]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        methods(torch.cuda.current_stream().cuda_stream)
+    for _ in range(3):
+        for t in outs:
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(t, w) for t, w in zip(outs, want))
+    del keep
+
+
+def test_counts_past_an_int_are_refused():
+    norm = sequence.NormGate(64, "f32", "bf16")
+    usage(lambda: norm.run((1 << 32) + 1, 4096, None, None, 4096, None), "-1 rows")
