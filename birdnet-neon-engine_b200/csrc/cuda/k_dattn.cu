@@ -590,7 +590,8 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
     };
     // Two K tiles or more: one warp issues QK (a unit ahead) and O2, the other O1 and DS, so that the waits of one do not
     // hold up the other's products (24 x 9600 tokens, d 64: 710 us by one warp, 672 by two). One K tile: one warp, O2 after
-    // DS, so that the next K is on its way meanwhile (28800 tokens, d 128: 181 us by one warp, 194 by two).
+    // DS, so that the next K is on its way meanwhile (28800 tokens, d 128: 181 us by one warp, 194 by two); the last O2, with
+    // no next K, before DS.
     constexpr bool one = L::in_place;
     auto issue = [&](auto which) {  // each warp's own code: first QK and O2 (or all), or O1 and DS
       constexpr bool first = decltype(which)::value;
@@ -602,10 +603,17 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
           if (u + 1 < nu && !(ok = issue_qk())) break;
         if constexpr (!kState && (!first || one))
           if (!(ok = issue_o1(u))) break;
-        if constexpr (!first || one)
-          if (last && !(ok = issue_ds())) break;
-        if constexpr (first)
+        if constexpr (one) {
+#pragma unroll 1
+          for (int step = 0; step < 2 && ok; step++)
+            if ((step == 0) == (u + 1 < nu)) ok = !last || issue_ds();
+            else ok = issue_o2(u);
+          if (!ok) break;
+        } else if constexpr (first) {
           if (!(ok = issue_o2(u))) break;
+        } else {
+          if (last && !(ok = issue_ds())) break;
+        }
         if (last) {
           g = 0;
           c++;
