@@ -32,6 +32,7 @@ struct NormArgs {
   long long xos, hs;
   float eps, alpha;
   int layer, gate;
+  int shift;  // k_norm_gate<.., kShift>: the first row's start past a 16-byte boundary of f, in elements
 };
 
 __device__ __forceinline__ float gate_of(int gate, float g) {
@@ -72,6 +73,15 @@ struct Raw {
       }
     }
   }
+  // the elements j of the group's in the mask
+  __device__ __forceinline__ void load_some(const elem_t<T> *p, unsigned mask) {
+#pragma unroll
+    for (int j = 0; j < V; j++)
+      if ((mask >> j) & 1) {
+        if constexpr (T == 0) w[j] = __float_as_uint(p[j]);
+        else w[j / 2] |= (uint32_t)reinterpret_cast<const uint16_t *>(p)[j] << 16 * (j & 1);
+      }
+  }
   __device__ __forceinline__ void zero() {
 #pragma unroll
     for (int i = 0; i < words; i++) w[i] = 0;
@@ -85,14 +95,37 @@ struct Raw {
   }
 };
 
+// the elements in the mask of a group of 8
+template <int T, int V>
+__device__ __forceinline__ void store_some(elem_t<T> *p, const float (&v)[V], unsigned mask) {
+#pragma unroll
+  for (int j = 0; j < V; j++)
+    if ((mask >> j) & 1) p[j] = Elem<T>::put(v[j]);
+}
+
 // A block a row, each thread NV groups of V consecutive columns (D <= blockDim NV V), the same for all its rows: the
 // vectors' values for them are read once and stay in registers (alpha gamma wpost as one). B: with bpost and bpre.
-template <int XT, int FT, int V, int NV, bool B>
+// kShift (V 8): rows that start anywhere, all tensors' at the same distance past 16 bytes; the groups lie on the 16-byte
+// boundaries, the first and the last one partly outside the row: their loads take the neighbours' elements too, which are
+// left out of the sums, their stores go element by element. A block's rows are 8 apart or a multiple, so the distance is
+// one for all of them.
+template <int XT, int FT, int V, int NV, bool B, bool kShift>
 __global__ void __launch_bounds__(256) k_norm_gate(const NormArgs a) {
   __shared__ float red[2][8];
   int calls = 0;
   const int D = a.D;
   const float inv = 1.f / (float)D;
+  const int shift = kShift ? (int)((a.shift + blockIdx.x * (a.xs & 7)) & 7) : 0;
+  auto column = [&](int k) { return (k * (int)blockDim.x + (int)threadIdx.x) * V - shift; };
+  unsigned some[NV];  // the group's elements inside the row
+#pragma unroll
+  for (int k = 0; k < NV; k++) {
+    some[k] = 0;
+#pragma unroll
+    for (int j = 0; j < V; j++) some[k] |= (column(k) + j >= 0 && column(k) + j < D ? 1u : 0u) << j;
+  }
+  constexpr unsigned kAll = (1u << V) - 1;
+  auto inside = [&](int k, int j) { return !kShift || ((some[k] >> j) & 1); };
   wait_launch_before();
   launch_dependents();
   float cu[NV][V], bu[NV][B ? V : 1], ch[NV][V], bh[NV][B ? V : 1];
@@ -100,10 +133,10 @@ __global__ void __launch_bounds__(256) k_norm_gate(const NormArgs a) {
   for (int k = 0; k < NV; k++)
 #pragma unroll
     for (int j = 0; j < V; j++) {
-      const int c = (k * blockDim.x + threadIdx.x) * V + j;
-      const bool in = c < D;
+      const int c = column(k) + j;
+      const bool in = c >= 0 && c < D;
       const float gm = a.alpha * (a.gamma && in ? a.gamma[c] : 1.f);
-      cu[k][j] = gm * (a.wpost && in ? a.wpost[c] : 1.f);
+      cu[k][j] = in ? gm * (a.wpost ? a.wpost[c] : 1.f) : 0.f;
       ch[k][j] = a.wpre && in ? a.wpre[c] : 1.f;
       if constexpr (B) {
         bu[k][j] = a.bpost && in ? gm * a.bpost[c] : 0.f;
@@ -118,11 +151,18 @@ __global__ void __launch_bounds__(256) k_norm_gate(const NormArgs a) {
     const elem_t<FT> *f = (const elem_t<FT> *)a.f + r * a.fs, *g = (const elem_t<FT> *)a.g + r * a.gs;
 #pragma unroll
     for (int k = 0; k < NV; k++) {
-      const int c = (k * blockDim.x + threadIdx.x) * V;
+      const int c = column(k);
       vx[k].zero();
       vf[k].zero();
       vg[k].zero();
-      if (c < D) {
+      // past the row's ends another row's elements, read and left out; past the first and the last row's nothing
+      if (kShift && ((c < 0 && r == 0) || (c + V > D && r == a.rows - 1))) {
+        vx[k].load_some(x + c, some[k]);
+        if (a.f && live) {
+          vf[k].load_some(f + c, some[k]);
+          if (a.gate) vg[k].load_some(g + c, some[k]);
+        }
+      } else if (c < D) {
         vx[k].load(x + c);
         if (a.f && live) {
           vf[k].load(f + c);
@@ -147,21 +187,21 @@ __global__ void __launch_bounds__(256) k_norm_gate(const NormArgs a) {
 #pragma unroll
       for (int j = 0; j < V; j++) y[k][j] = rx[k].at(j);
     // v is zero past the row's end, and stays out of the squares there
-    auto in_row = [&](int k) { return (k * (int)blockDim.x + (int)threadIdx.x) * V < D; };
+    auto in_row = [&](int k) { return column(k) < D; };
     if (upd) {
       float mean = 0.f, ss = 0.f;
       if (a.layer) {
 #pragma unroll
         for (int k = 0; k < NV; k++)
 #pragma unroll
-          for (int j = 0; j < V; j++) mean += rf[k].at(j);
+          for (int j = 0; j < V; j++) mean += inside(k, j) ? rf[k].at(j) : 0.f;
         mean = block_sum(mean, red, calls) * inv;
       }
 #pragma unroll
       for (int k = 0; k < NV; k++)
         if (in_row(k))
 #pragma unroll
-          for (int j = 0; j < V; j++) ss += (rf[k].at(j) - mean) * (rf[k].at(j) - mean);
+          for (int j = 0; j < V; j++) ss += inside(k, j) ? (rf[k].at(j) - mean) * (rf[k].at(j) - mean) : 0.f;
       const float rs = rsqrtf(block_sum(ss, red, calls) * inv + a.eps);
 #pragma unroll
       for (int k = 0; k < NV; k++)
@@ -176,7 +216,10 @@ __global__ void __launch_bounds__(256) k_norm_gate(const NormArgs a) {
       elem_t<XT> *xo = (elem_t<XT> *)a.xo + r * a.xos;
 #pragma unroll
       for (int k = 0; k < NV; k++)
-        if (in_row(k)) store_elems<XT, V>(xo + (k * blockDim.x + threadIdx.x) * V, y[k]);
+        if (in_row(k)) {
+          if (!kShift || some[k] == kAll) store_elems<XT, V>(xo + column(k), y[k]);
+          else if constexpr (kShift) store_some<XT, V>(xo + column(k), y[k], some[k]);
+        }
     }
     if (a.h) {
       float mean = 0.f, ss = 0.f;
@@ -185,14 +228,14 @@ __global__ void __launch_bounds__(256) k_norm_gate(const NormArgs a) {
         for (int k = 0; k < NV; k++)
           if (in_row(k))
 #pragma unroll
-            for (int j = 0; j < V; j++) mean += y[k][j];
+            for (int j = 0; j < V; j++) mean += inside(k, j) ? y[k][j] : 0.f;
         mean = block_sum(mean, red, calls) * inv;
       }
 #pragma unroll
       for (int k = 0; k < NV; k++)
         if (in_row(k))
 #pragma unroll
-          for (int j = 0; j < V; j++) ss += (y[k][j] - mean) * (y[k][j] - mean);
+          for (int j = 0; j < V; j++) ss += inside(k, j) ? (y[k][j] - mean) * (y[k][j] - mean) : 0.f;
       const float rs = rsqrtf(block_sum(ss, red, calls) * inv + a.eps);
       elem_t<FT> *h = (elem_t<FT> *)a.h + r * a.hs;
 #pragma unroll
@@ -205,7 +248,8 @@ __global__ void __launch_bounds__(256) k_norm_gate(const NormArgs a) {
           if constexpr (B) o[j] += bh[k][j];
           if (!live) o[j] = 0.f;
         }
-        store_elems<FT, V>(h + (k * blockDim.x + threadIdx.x) * V, o);
+        if (!kShift || some[k] == kAll) store_elems<FT, V>(h + column(k), o);
+        else if constexpr (kShift) store_some<FT, V>(h + column(k), o, some[k]);
       }
     }
 #pragma unroll
@@ -277,21 +321,25 @@ __global__ void __launch_bounds__(kNormThreads) k_norm_gate_wide(const NormArgs 
   }
 }
 
-template <int XT, int FT, int V, int NV>
+template <int XT, int FT, int V, int NV, bool kShift = false>
 cudaError_t launch_rows(const NormArgs &a, cudaStream_t st) {
-  const int warps = (a.D + 32 * V * NV - 1) / (32 * V * NV);
-  const long long most = (long long)num_sms() * (24 / warps);
+  const int warps = (a.D + (kShift ? 7 : 0) + 32 * V * NV - 1) / (32 * V * NV);
+  const long long most = (long long)num_sms() * (24 / warps) & (kShift ? ~7ll : ~0ll);
   const int blocks = (int)(a.rows < most ? a.rows : most);
-  auto kernel = a.bpost || a.bpre ? k_norm_gate<XT, FT, V, NV, true> : k_norm_gate<XT, FT, V, NV, false>;
+  auto kernel = a.bpost || a.bpre ? k_norm_gate<XT, FT, V, NV, true, kShift> : k_norm_gate<XT, FT, V, NV, false, kShift>;
   // An early start hides a small call's latency (one row 8.5 -> 8.1 us). A full grid of blocks that stay would settle
-  // unevenly in what the launch before leaves free (3000 x 1021: 24.6 -> 29.4 us)
+  // unevenly in what the launch before leaves free (3000 x 1021, one element an access: 24.6 -> 29.4 us)
   if (blocks < num_sms()) return launch_early(kernel, dim3(blocks), 32 * warps, 0, st, a);
   kernel<<<blocks, 32 * warps, 0, st>>>(a);
   return cudaGetLastError();
 }
 
 template <int XT, int FT>
-cudaError_t launch_norm(const NormArgs &a, bool vec, cudaStream_t st) {
+cudaError_t launch_norm(const NormArgs &a, bool vec, bool shifted, cudaStream_t st) {
+  // 20000 rows, fp16, layer norm, us with groups of 8 between ends one by one / one element an access: 100 wide 20.6 / 18.7,
+  // 193 22.5 / 34.9, 1533 150 / 281, 2001 152 / 379; 1021 wide, 1 row 5.5 / 3.9, 592 rows 8.8 / 8.2, 1184 12.3 / 13.9, 3000
+  // 22.5 / 28.3 (1024 wide on 16 bytes: 16.5)
+  if (shifted && a.D >= 192 && a.D <= 2041 && a.rows > 4 * num_sms()) return launch_rows<XT, FT, 8, 1, true>(a, st);
   if (vec) {
     if (a.D <= 2048) return launch_rows<XT, FT, 8, 1>(a, st);
     if (a.D <= 8192) return launch_rows<XT, FT, 8, 4>(a, st);
@@ -319,11 +367,25 @@ extern "C" int bnnk_norm_gate(const bnnk_norm_gate_args *p, bnn_stream_t st) {
                        (uintptr_t)a.bpre;
   const bool vec = a.D % 8 == 0 && !(at & 15) &&
                    !((a.xs | (a.f ? a.fs : 0) | (a.f && a.gate ? a.gs : 0) | (a.xo ? a.xos : 0) | (a.h ? a.hs : 0)) & 7);
+  // rows of any start and width, all tensors' at the same elements of 8: the same with the ends one by one
+  bool shifted = !vec;
+  a.shift = -1;
+  auto same = [&](const void *p, long long stride, int type) {
+    if (!p) return;
+    const int size = type == 0 ? 4 : 2, off = (int)((uintptr_t)p / size & 7);
+    if ((uintptr_t)p % size || (stride & 7) != (a.xs & 7) || (a.shift >= 0 && off != a.shift)) shifted = false;
+    a.shift = off;
+  };
+  same(a.x, a.xs, p->xtype);
+  same(a.f, a.fs, p->type);
+  if (a.f && a.gate) same(a.g, a.gs, p->type);
+  same(a.xo, a.xos, p->xtype);
+  same(a.h, a.hs, p->type);
   const cudaStream_t s = (cudaStream_t)st;
-  if (p->xtype == 0 && p->type == 0) return launch_norm<0, 0>(a, vec, s);
-  if (p->xtype == 0 && p->type == 1) return launch_norm<0, 1>(a, vec, s);
-  if (p->xtype == 0 && p->type == 2) return launch_norm<0, 2>(a, vec, s);
-  if (p->xtype == 1 && p->type == 1) return launch_norm<1, 1>(a, vec, s);
-  if (p->xtype == 2 && p->type == 2) return launch_norm<2, 2>(a, vec, s);
+  if (p->xtype == 0 && p->type == 0) return launch_norm<0, 0>(a, vec, shifted, s);
+  if (p->xtype == 0 && p->type == 1) return launch_norm<0, 1>(a, vec, shifted, s);
+  if (p->xtype == 0 && p->type == 2) return launch_norm<0, 2>(a, vec, shifted, s);
+  if (p->xtype == 1 && p->type == 1) return launch_norm<1, 1>(a, vec, shifted, s);
+  if (p->xtype == 2 && p->type == 2) return launch_norm<2, 2>(a, vec, shifted, s);
   return cudaErrorInvalidValue;
 }

@@ -594,6 +594,18 @@ def test_norm_gate_forms(cuda, case, norm, gate, types):
 
 
 @gpu
+@pytest.mark.parametrize("case", [
+    dict(D=192, offset=1), dict(D=193), dict(D=1021, offset=5, masked=True), dict(D=1023, pad=6), dict(D=200, offset=4, pad=4),
+    dict(D=2041, offset=7), dict(D=2042), dict(D=777, inplace=True, masked=True), dict(D=1024, offset=3, inplace=True),
+    dict(D=300, offset=2, vectors="none", outputs="h"), dict(D=509, f=False, pad=1), dict(D=255, outputs="xo", masked=True)])
+@pytest.mark.parametrize("norm, gate, types", [("rms", "silu", ("bf16", "bf16")), ("layer", "sigmoid", ("f32", "f16")),
+                                               ("layer", "none", ("f32", "f32"))])
+def test_norm_gate_rows_that_start_anywhere(cuda, case, norm, gate, types):
+    kw = dict(case)
+    norm_case(kw.pop("D"), *types, norm, gate, rows=1301, seed=4, **kw)
+
+
+@gpu
 def test_norm_gate_zero_rows_and_zero_values(cuda):
     op = sequence.NormGate(64, "f32", "bf16", "rms", "none")
     x = torch.zeros(4, 64, device="cuda")
