@@ -15,13 +15,23 @@ static int launch_rc(const char *what, int e) {
   return -1;
 }
 
-/* device memory of an op, the first word zero (an error word); -1 with the error set */
+/* device memory of an op; -1 with the error set */
 static int dev_alloc(const char *what, void **p, size_t bytes) {
-  cudaError_t e = bnn_fail_dev_alloc() ? cudaErrorMemoryAllocation : cudaMalloc(p, bytes);
-  if (!e) e = cudaMemset(*p, 0, sizeof(int));
+  const cudaError_t e = bnn_fail_dev_alloc() ? cudaErrorMemoryAllocation : cudaMalloc(p, bytes);
   if (!e) return 0;
   ERR(e == cudaErrorMemoryAllocation ? BNN_ERR_OOM : BNN_ERR_CPU, "%s: %zu bytes of device memory: CUDA error %d (%s)",
       what, bytes, (int)e, cudaGetErrorString(e));
+  return -1;
+}
+
+/* an op's error word cleared, and table (NULL: none) copied to d_table; both have happened when it returns: the copies go
+ * to the legacy stream, which streams made non-blocking do not wait for, and the first run may be on one of those */
+static int dev_set(const char *what, int *err, float *d_table, const float *table, size_t bytes) {
+  cudaError_t e = cudaMemset(err, 0, sizeof(int));
+  if (!e && table) e = cudaMemcpy(d_table, table, bytes, cudaMemcpyHostToDevice);
+  if (!e) e = cudaStreamSynchronize(cudaStreamLegacy);
+  if (!e) return 0;
+  ERR(BNN_ERR_CPU, "%s: CUDA error %d (%s)", what, (int)e, cudaGetErrorString(e));
   return -1;
 }
 
@@ -86,8 +96,7 @@ bnn_dattn *bnn_dattn_new(int type, int heads, int kv_heads, int dk, int dv, cons
           th[kDattnPow2 + 2 * k + 1] = (float)(p - (double)(float)p);
         }
     }
-    const cudaError_t e = cudaMemcpy(o->pow, t, bytes, cudaMemcpyHostToDevice);
-    if (e) { ERR(BNN_ERR_CPU, "bnn_dattn_new: CUDA error %d (%s)", (int)e, cudaGetErrorString(e)); bad = 1; }
+    bad = dev_set("bnn_dattn_new", o->err, o->pow, t, bytes);
   }
   free(t);
   if (bad) { bnn_dattn_free(o); return NULL; }
@@ -181,7 +190,8 @@ bnn_lowrank *bnn_lowrank_new(int type, int out_type, int N, int K, const void *d
   o->a.type = type; o->a.otype = out_type; o->a.N = N; o->a.K = K; o->a.slots = slots; o->a.rank = rank;
   o->a.w = d_w; o->a.ldw = ldw; o->a.bias = d_bias; o->a.a = d_a; o->a.b = d_b; o->a.scale = d_scale;
   if (dev_alloc("bnn_lowrank_new", (void **)&o->a.hid, sizeof(float) * (size_t)rows * rank) ||
-      dev_alloc("bnn_lowrank_new", (void **)&o->a.err, sizeof(int))) {
+      dev_alloc("bnn_lowrank_new", (void **)&o->a.err, sizeof(int)) ||
+      dev_set("bnn_lowrank_new", o->a.err, NULL, NULL, 0)) {
     bnn_lowrank_free(o);
     return NULL;
   }

@@ -629,6 +629,48 @@ def test_station_context_example(cuda):
     assert example.main() < 8 * 2.0 ** -8
 
 
+# ------------------------------------------------------------------ streams
+
+
+def busy(ms=50):
+    """work of about so many ms on the current stream"""
+    torch.cuda._sleep(int(ms * 1.9e6))  # pylint: disable=protected-access
+
+
+@gpu
+def test_op_made_while_the_default_stream_is_busy(cuda):
+    """an op's set-up is over when it exists: its first run may be on a side stream, and what the default stream still has
+    to do must not write into the op's memory after that"""
+    gen, K, N, rank = generator(2), 64, 96, 8
+    w, A, B = rand(gen, N, K).bfloat16(), rand(gen, 2, rank, K).bfloat16(), rand(gen, 2, N, rank).bfloat16()
+    side = torch.cuda.Stream()
+    for rows in (1, 9, 50, 300):
+        x, slot = rand(gen, rows, K).bfloat16(), torch.zeros(rows, device="cuda").int()
+        outs = []
+        for late in (False, True):
+            y = torch.empty(rows, N, device="cuda")
+            torch.cuda.synchronize()
+            if late:
+                busy()
+            op = sequence.LowRank("bf16", "f32", N, K, w.data_ptr(), None, 2, rank, A.data_ptr(), B.data_ptr(), rows=rows)
+            op.run(rows, x.data_ptr(), slot.data_ptr(), y.data_ptr(), stream=side.cuda_stream)
+            side.synchronize()
+            outs.append(y)
+            torch.cuda.synchronize()
+        assert torch.equal(*outs), rows
+    a = Attention("bf16", 2, 2, 64, 64, [150, 4], seed=13)
+    s1 = torch.zeros_like(a.s0)
+    a.run(a.op(), s1=s1)
+    want, state = a.o.clone(), s1.clone()
+    a.o.zero_()
+    torch.cuda.synchronize()
+    busy()
+    op = a.op()
+    a.run(op, s1=s1, stream=side.cuda_stream)
+    side.synchronize()
+    assert torch.equal(a.o, want) and torch.equal(s1, state)
+
+
 # ------------------------------------------------------------------ refusals (no GPU needed)
 
 
