@@ -43,9 +43,10 @@ static void *host_alloc(const char *what, size_t bytes) {
 
 static int misaligned(const void *p) { return ((uintptr_t)p & 15) != 0; }
 
+/* a device word after all work issued so far, on streams that the copy alone would not wait for too */
 static int read_word(const int *d) {
   int v = 0;
-  if (d && cudaMemcpy(&v, d, sizeof v, cudaMemcpyDeviceToHost)) return -1;
+  if (d && (cudaDeviceSynchronize() || cudaMemcpy(&v, d, sizeof v, cudaMemcpyDeviceToHost))) return -1;
   return v;
 }
 

@@ -261,7 +261,8 @@ int bnn_dattn_step(bnn_dattn *op, int n, const int32_t *d_slot, const uint8_t *d
  * bindings that pay for every argument */
 int bnn_dattn_run_words(bnn_dattn *op, const long long *words);
 int bnn_dattn_step_words(bnn_dattn *op, const long long *words);
-/* the op's device error word (0 = no bounded wait ran out); synchronous */
+/* the op's device error word after all work issued so far on the device (0 = no bounded wait ran out in any of the op's
+ * runs: once set it stays); synchronous */
 int bnn_dattn_error(bnn_dattn *op);
 void bnn_dattn_free(bnn_dattn *op);
 
@@ -281,7 +282,7 @@ bnn_lowrank *bnn_lowrank_new(int type, int out_type, int N, int K, const void *d
 int bnn_lowrank_run(bnn_lowrank *op, int rows, const void *d_x, long long ldx, const int32_t *d_slot, void *d_y,
                     long long ldy, void *stream);
 int bnn_lowrank_run_words(bnn_lowrank *op, const long long *words); /* the 7 arguments after op as words */
-/* the op's device error word (0 = no bounded wait ran out); synchronous */
+/* as bnn_dattn_error */
 int bnn_lowrank_error(bnn_lowrank *op);
 void bnn_lowrank_free(bnn_lowrank *op);
 

@@ -671,6 +671,26 @@ def test_op_made_while_the_default_stream_is_busy(cuda):
     assert torch.equal(a.o, want) and torch.equal(s1, state)
 
 
+@gpu
+def test_error_word_waits_for_the_runs(cuda):
+    """the error word is that of every run issued before, on a non-blocking stream too"""
+    a = Attention("bf16", 2, 2, 64, 64, [150, 4], seed=14)
+    att = a.op()
+    w, y = torch.zeros(16, 64, device="cuda").bfloat16(), torch.empty(4, 16, device="cuda")
+    low = sequence.LowRank("bf16", "f32", 16, 64, w.data_ptr(), None, 1, 8, w.data_ptr(), w.data_ptr(), rows=4)
+    side, done = torch.cuda.Stream(), torch.cuda.Event()
+    for op, run in ((att, lambda: a.run(att, stream=side.cuda_stream)),
+                    (low, lambda: low.run(4, w.data_ptr(), None, y.data_ptr(), stream=side.cuda_stream))):
+        run()  # a kernel's first launch may wait for the device
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            busy()
+            run()
+            done.record()
+        assert not done.query()
+        assert op.error == 0 and done.query()
+
+
 # ------------------------------------------------------------------ refusals (no GPU needed)
 
 
