@@ -42,6 +42,8 @@ static void *host_alloc(const char *what, size_t bytes) {
 }
 
 static int misaligned(const void *p) { return ((uintptr_t)p & 15) != 0; }
+/* not where 4-byte values can be */
+static int misaligned4(const void *p) { return ((uintptr_t)p & 3) != 0; }
 
 /* a device word after all work issued so far, on streams that the copy alone would not wait for too */
 static int read_word(const int *d) {
@@ -114,6 +116,11 @@ static int dattn_launch(const char *what, bnn_dattn *o, int n, long long tokens,
     return -1;
   }
   if (n == 0) return 0;
+  if (misaligned4(d_cu) || misaligned4(d_slot)) {
+    ERR(BNN_ERR_USAGE, "%s: offsets %p, slots %p: not aligned to their elements", what, (const void *)d_cu,
+        (const void *)d_slot);
+    return -1;
+  }
   if ((tokens > 0 && (!d_q || !d_k || !d_v || !d_o)) || misaligned(d_q) || misaligned(d_k) || misaligned(d_v) ||
       misaligned(d_o) || misaligned(d_s0) || misaligned(d_s1) || qts < (long long)o->H * o->dk || qts % 8 ||
       kts < (long long)o->Hk * o->dk || kts % 8 || vts < (long long)o->Hk * o->dv || vts % 8 ||
@@ -145,15 +152,21 @@ int bnn_dattn_step(bnn_dattn *o, int n, const int32_t *d_slot, const uint8_t *d_
 }
 
 #define P(i) ((void *)(uintptr_t)w[i])
+static int no_words(const char *what, const long long *w) {
+  if (!w) ERR(BNN_ERR_USAGE, "%s: no arguments", what);
+  return !w;
+}
 /* a count that an int does not hold is refused as a negative one */
 static int count_of(long long v) { return v < 0 || v > 0x7fffffff ? -1 : (int)v; }
 
 int bnn_dattn_run_words(bnn_dattn *o, const long long *w) {
+  if (no_words("bnn_dattn_run_words", w)) return -1;
   return bnn_dattn_run(o, count_of(w[0]), w[1], P(2), P(3), P(4), P(5), w[6], P(7), w[8], P(9), w[10], P(11), P(12), P(13),
                        w[14], P(15));
 }
 
 int bnn_dattn_step_words(bnn_dattn *o, const long long *w) {
+  if (no_words("bnn_dattn_step_words", w)) return -1;
   return bnn_dattn_step(o, count_of(w[0]), P(1), P(2), P(3), w[4], P(5), w[6], P(7), w[8], P(9), P(10), P(11), w[12],
                         P(13));
 }
@@ -179,10 +192,12 @@ bnn_lowrank *bnn_lowrank_new(int type, int out_type, int N, int K, const void *d
                              int slots, int rank, const void *d_a, const void *d_b, const float *d_scale, int rows) {
   if ((type != BNN_T_F16 && type != BNN_T_BF16) || (out_type != BNN_T_F32 && out_type != type) || N < 1 || K < 8 ||
       K % 8 || N > (1 << 24) || K > (1 << 24) || !d_w || ldw < K || ldw % 8 || slots < 1 || rank < 8 || rank > 64 ||
-      rank % 8 || !d_a || !d_b || rows < 1 || misaligned(d_w) || misaligned(d_a) || misaligned(d_b)) {
-    ERR(BNN_ERR_USAGE, "bnn_lowrank_new: type %d out %d N %d K %d ldw %lld slots %d rank %d rows %d w %p a %p b %p (type "
-        "fp16 or bf16, out fp32 or the same, K and ldw >= K multiples of 8, N and K up to 2^24, rank a multiple of 8 in 8 "
-        ".. 64, 16-byte aligned weights)", type, out_type, N, K, ldw, slots, rank, rows, d_w, d_a, d_b);
+      rank % 8 || !d_a || !d_b || rows < 1 || misaligned(d_w) || misaligned(d_a) || misaligned(d_b) ||
+      misaligned4(d_bias) || misaligned4(d_scale)) {
+    ERR(BNN_ERR_USAGE, "bnn_lowrank_new: type %d out %d N %d K %d ldw %lld slots %d rank %d rows %d w %p a %p b %p bias %p scale %p "
+        "(type fp16 or bf16, out fp32 or the same, K and ldw >= K multiples of 8, N and K up to 2^24, rank a multiple of 8 in 8 "
+        ".. 64, 16-byte aligned weights, bias and scale aligned to their elements)", type, out_type, N, K, ldw, slots, rank,
+        rows, d_w, d_a, d_b, (const void *)d_bias, (const void *)d_scale);
     return NULL;
   }
   bnn_lowrank *o = host_alloc("bnn_lowrank_new", sizeof *o);
@@ -202,9 +217,11 @@ bnn_lowrank *bnn_lowrank_new(int type, int out_type, int N, int K, const void *d
 int bnn_lowrank_run(bnn_lowrank *o, int rows, const void *d_x, long long ldx, const int32_t *d_slot, void *d_y,
                     long long ldy, void *stream) {
   if (!o || rows < 0 || rows > o->rows || (rows > 0 && (!d_x || !d_y || ldx < o->a.K || ldx % 8 || ldy < o->a.N ||
-                                                        misaligned(d_x) || ((uintptr_t)d_y & (o->a.otype ? 1 : 3))))) {
+                                                        misaligned(d_x) || misaligned4(d_slot) ||
+                                                        ((uintptr_t)d_y & (o->a.otype ? 1 : 3))))) {
     ERR(BNN_ERR_USAGE, "bnn_lowrank_run: %d rows (capacity %d) x %p stride %lld (>= K %d, a multiple of 8, 16-byte "
-        "aligned) y %p stride %lld (>= N %d)", rows, o ? o->rows : 0, d_x, ldx, o ? o->a.K : 0, d_y, ldy, o ? o->a.N : 0);
+        "aligned) y %p stride %lld (>= N %d) slots %p (y and slots aligned to their elements)", rows, o ? o->rows : 0, d_x,
+        ldx, o ? o->a.K : 0, d_y, ldy, o ? o->a.N : 0, (const void *)d_slot);
     return -1;
   }
   if (rows == 0) return 0;
@@ -219,6 +236,7 @@ int bnn_lowrank_run(bnn_lowrank *o, int rows, const void *d_x, long long ldx, co
 }
 
 int bnn_lowrank_run_words(bnn_lowrank *o, const long long *w) {
+  if (no_words("bnn_lowrank_run_words", w)) return -1;
   return bnn_lowrank_run(o, count_of(w[0]), P(1), w[2], P(3), P(4), w[5], P(6));
 }
 
@@ -242,9 +260,11 @@ bnn_norm_gate *bnn_norm_gate_new(int D, int x_type, int type, int norm, int gate
                                  const float *d_bpre) {
   if (D < 1 || D > (1 << 24) || type < BNN_T_F32 || type > BNN_T_BF16 || (x_type != BNN_T_F32 && x_type != type) ||
       (norm != BNN_NORM_RMS && norm != BNN_NORM_LAYER) || gate < BNN_GATE_NONE || gate > BNN_GATE_SILU || !(eps >= 0.f) ||
-      !isfinite(eps) || !isfinite(alpha)) {
+      !isfinite(eps) || !isfinite(alpha) || misaligned4(d_wpost) || misaligned4(d_bpost) || misaligned4(d_gamma) ||
+      misaligned4(d_wpre) || misaligned4(d_bpre)) {
     ERR(BNN_ERR_USAGE, "bnn_norm_gate_new: D %d x_type %d type %d norm %d gate %d eps %g alpha %g (D in 1 .. 2^24, x_type "
-        "fp32 or type, BNN_NORM_*, BNN_GATE_*, finite eps >= 0 and alpha)", D, x_type, type, norm, gate, eps, alpha);
+        "fp32 or type, BNN_NORM_*, BNN_GATE_*, finite eps >= 0 and alpha, vectors aligned to their elements)", D, x_type,
+        type, norm, gate, eps, alpha);
     return NULL;
   }
   bnn_norm_gate *o = host_alloc("bnn_norm_gate_new", sizeof *o);
@@ -282,6 +302,7 @@ int bnn_norm_gate_run(bnn_norm_gate *o, int rows, const void *d_x, long long xs,
 }
 
 int bnn_norm_gate_run_words(bnn_norm_gate *o, const long long *w) {
+  if (no_words("bnn_norm_gate_run_words", w)) return -1;
   return bnn_norm_gate_run(o, count_of(w[0]), P(1), w[2], P(3), w[4], P(5), w[6], P(7), P(8), w[9], P(10), w[11], P(12));
 }
 

@@ -11,7 +11,7 @@ import math
 import numpy as np
 import pytest
 
-from bnneon_b200 import BnnError, load_library, sequence
+from bnneon_b200 import BnnError, last_error, load_library, sequence
 
 torch = pytest.importorskip("torch")
 gpu = pytest.mark.gpu
@@ -861,3 +861,37 @@ def test_calls_in_a_captured_graph(cuda):
 def test_counts_past_an_int_are_refused():
     norm = sequence.NormGate(64, "f32", "bf16")
     usage(lambda: norm.run((1 << 32) + 1, 4096, None, None, 4096, None), "-1 rows")
+
+
+@pytest.mark.parametrize("vector", ["wpost", "bpost", "gamma", "wpre", "bpre"])
+def test_norm_gate_new_refuses_misaligned_vectors(vector):
+    usage(lambda: sequence.NormGate(64, "f32", "bf16", **{vector: P + 2}), "vectors aligned")
+
+
+@pytest.mark.parametrize("kw", [dict(bias=P + 2), dict(scale=P + 1)])
+def test_lowrank_new_refuses_misaligned_vectors(kw):
+    a = dict(dtype="bf16", out="bf16", N=10, K=64, w=P, bias=P, slots=2, rank=8, a=P, b=P, scale=P, rows=4)
+    usage(lambda: sequence.LowRank(**dict(a, **kw)), "aligned to their elements")
+
+
+def test_words_entry_points_refuse_no_words():
+    h = load_library()
+    norm = sequence.NormGate(64, "f32", "bf16")
+    for call, op in ((h.bnn_dattn_run_words, None), (h.bnn_dattn_step_words, None), (h.bnn_lowrank_run_words, None),
+                     (h.bnn_norm_gate_run_words, norm.op)):
+        assert call(op, None) == -1
+        e = last_error(h)
+        assert e.kind == "USAGE" and "no arguments" in str(e)
+
+
+@gpu
+def test_run_refuses_misaligned_offsets_and_slots(cuda):
+    """on the host: in a kernel such an address would be a fault"""
+    op = sequence.DecayAttention("bf16", 4, 64, 32, [0.9, 0.5], kv_heads=2, seqs=2, tokens=10)
+    ok = dict(n=2, tokens=10, cu=P, q=P, k=P, v=P, o=P)
+    for kw in (dict(cu=P + 2), dict(slot=P + 2), dict(slot=P + 1)):
+        usage(lambda kw=kw: op.run(**dict(ok, **kw)), "not aligned to their elements")
+    usage(lambda: op.step(1, P, P, P, P, slot=P + 3), "not aligned to their elements")
+    w = torch.zeros(10, 64, device="cuda").bfloat16()
+    low = sequence.LowRank("bf16", "f32", 10, 64, w.data_ptr(), None, 1, 8, w.data_ptr(), w.data_ptr(), rows=4)
+    usage(lambda: low.run(4, P, P + 2, P), "aligned to their elements")
