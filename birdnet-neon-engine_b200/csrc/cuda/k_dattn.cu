@@ -459,10 +459,14 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
   // MN-major steps 16 rows of 128 bytes
   auto kstep = [](int kk) { return (uint64_t)(((kk / 4) * L::panel + (kk % 4) * 32) >> 4); };
   constexpr uint64_t mnstep = 2048 >> 4;
-  // V of chunk c for a product: its arrival, or the state warps' word that its dead rows are zero
+  // V of chunk c for a product: its arrival, then the state warps' word that its dead rows are zero. The word alone would
+  // not do: its parity says as much while the word on the tile's chunk before is still on its way, which nothing else that
+  // this warp has waited for excludes. The tile's arrival does: the tile was free after that chunk's DS, which waited for
+  // K', and the state warps give their word on K' after the one on V.
   auto wait_v = [&](int c, const Ring<NS> &rc) {
     const bool whole = t1 - (t0 + (long long)c * kChunk) >= kChunk && !d.live;
-    return wait(whole ? b_vfull[rc.at] : b_vfix[rc.at], rc.parity, BNNK_ERR_MMA_WAIT);
+    if (!wait(b_vfull[rc.at], rc.parity, BNNK_ERR_MMA_WAIT)) return false;
+    return whole || wait(b_vfix[rc.at], rc.parity, BNNK_ERR_MMA_WAIT);
   };
 
   if (warp == 1) {  // TMA

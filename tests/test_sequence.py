@@ -316,6 +316,30 @@ def test_dattn_split_sequences_repeat(cuda, dtype, heads, lens, masked):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_dattn_ends_inside_a_chunk_repeat(cuda, dtype):
+    """heads up to 64, no mask, an end inside the third or a later chunk: the rows past it are the next sequence's (here
+    NaN), and are zeroed in a tile that was used before; the same bits however the warps are timed against each other"""
+    lens = [257, 300, 383, 511, 700] * 6
+    a = Attention(dtype, 6, 6, 64, 64, [x for n in lens for x in (n, 130)], seed=15)
+    odd = torch.cat([a.cu[i:i + 2] for i in range(0, 2 * len(lens), 2)])
+    mine = torch.zeros(len(a.buf), dtype=torch.bool, device="cuda")
+    for lo, hi in odd.view(-1, 2).tolist():
+        mine[lo:hi] = True
+    s1 = torch.zeros_like(a.s0)
+    op = a.op()
+    a.run(op, s1=s1)
+    a.check(s1)
+    o, s = a.o[mine].clone(), s1[a.slot[::2].long()].clone()
+    a.buf[~mine] = math.nan
+    differ = torch.zeros((), device="cuda", dtype=torch.int64)
+    for _ in range(100):
+        a.run(op, s1=s1)
+        differ += (a.o[mine] != o).sum() + (s1[a.slot[::2].long()] != s).sum()
+    assert int(differ) == 0 and op.error == 0
+
+
+@gpu
 def test_dattn_offsets_past_32_bits(cuda):
     """states and rows more than 2^32 bytes and 2^31 elements into their buffers"""
     torch.cuda.empty_cache()
