@@ -162,7 +162,10 @@ __global__ void __launch_bounds__(256) k_dattn_rec(const DattnArgs a) {
 //    it was 2.4e-6 off, against 4.5e-7 for fp32 products).
 //  - fp16: two parts are 22 bits, but only within the type's range, so each is scaled by a power of two that a maximum
 //    gives: P by its row's, S and K' by their tile's, and K' has the decays counted from the chunk's last live token. The
-//    scales go into the fp32 steps after the products. Values 2^28 below the maximum are the first to lose bits.
+//    scales go into the fp32 steps after the products. The maxima are those of the decayed values, so that a loud token
+//    long ago takes no bits from the present. The maximum comes to 2^14 .. 2^15 and the second part ends at 2^-24: 22 bits
+//    for values down to 2^17 below the maximum, 11 at 2^28. That far below, P and S are under the rounding of an fp16 output
+//    beside the others; in K' it is a feature of k that small beside the chunk's largest.
 //
 // One CTA per (segment of a sequence, k/v head) walks the segment's chunks, and for each the G q heads of the group
 // ("unit" u = (chunk, q head)). Roles: warps 0 and 2 MMA issue, warp 1 TMA, 8 warps turn QK into P (in place in TMEM, as the
@@ -655,8 +658,7 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
       float sc = d.scale;
       const int blocks = 2 * qd + 2;  // those that reach the diagonal
       if constexpr (T == 1) {
-        // a bound of the row's products: all of these blocks' live columns, those above the diagonal too (their size
-        // matters only where it is 2^28 times the others'); the row's two warps a half each
+        // the largest of the row's decayed products; the row's two warps a half each
         float m = 0.f;
 #pragma unroll 1
         for (int blk = h; blk < blocks; blk += 2) {
@@ -668,8 +670,16 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
 #pragma unroll
             for (int j = 0; j < 16; j++) x[j] = (w >> j) & 1 ? x[j] : 0u;
           }
+          const float *f = pw + i - 16 * blk;  // the decays, as below
+          float mb = 0.f;
+          if (blk >= 2 * qd) {
 #pragma unroll
-          for (int j = 0; j < 16; j++) m = fmaxf(m, fabsf(__uint_as_float(x[j])));
+            for (int j = 0; j < 16; j++) m = fmaxf(m, fabsf(__uint_as_float(x[j]) * f[-j]));
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16; j++) mb = fmaxf(mb, fabsf(__uint_as_float(x[j]) * fixed[j]));
+            m = fmaxf(m, mb * f[-15]);
+          }
         }
         s_rowmax[u & 1][h][i] = m;
         __syncwarp();
@@ -826,20 +836,23 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
       };
       if constexpr (T == 1) {
         float mx = 0.f;
+        if (n < kChunk || d.live)
+          from_j = lw[3] ? 127 - __clz(lw[3]) : lw[2] ? 95 - __clz(lw[2]) : lw[1] ? 63 - __clz(lw[1]) : lw[0] ? 31 - __clz(lw[0]) : 0;
 #pragma unroll 1
         for (int m = 0; m < 2; m++)
-          if (!dead(m))
+          if (!dead(m)) {
+            float rm = 0.f;
             for (int p = 0; p < PN; p++) {
               uint32_t x[4];
               load(m, p, x);
 #pragma unroll
               for (int e = 0; e < 4; e++) {
                 const float2 f = unpack2<T>(x[e]);
-                mx = fmaxf(mx, fmaxf(fabsf(f.x), fabsf(f.y)));
+                rm = fmaxf(rm, fmaxf(fabsf(f.x), fabsf(f.y)));
               }
             }
-        if (n < kChunk || d.live)
-          from_j = lw[3] ? 127 - __clz(lw[3]) : lw[2] ? 95 - __clz(lw[2]) : lw[1] ? 63 - __clz(lw[1]) : lw[0] ? 31 - __clz(lw[0]) : 0;
+            mx = fmaxf(mx, rm * pw[from_j - tid / 8 - 64 * m]);
+          }
         float inv;
         ksc = scale_to_f16(role_max(mx), inv);
         if (!ok) return false;

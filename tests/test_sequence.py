@@ -340,6 +340,31 @@ def test_dattn_ends_inside_a_chunk_repeat(cuda, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("heads", [(2, 1, 64, 64), (1, 1, 128, 128), (3, 3, 40, 72)])
+@pytest.mark.parametrize("masked", [0.0, 0.2])
+def test_dattn_loud_tokens_long_ago(cuda, heads, masked):
+    """fp16: a token 2^28 times as loud as the others, decayed to nothing 60 tokens later, takes nothing from the state and
+    the outputs there. The scale brings the quiet outputs to about 1, the loud ones past the type"""
+    lens = [128, 300, 77]
+    a = Attention("f16", *heads, lens, masked, seed=16, decay=[0.5] * heads[1], k_scale=2.0 ** -13)
+    a.scale = 1000.0
+    loud = [0, 128, 128 + 140, 128 + 300 + 3]
+    quiet = torch.ones(sum(lens), dtype=torch.bool, device="cuda")
+    for t in loud:
+        a.k[t] = (a.k[t].float() * 2.0 ** 28).clamp(-6e4, 6e4).half()
+        quiet[t:t + 60] = False
+    s1 = torch.zeros_like(a.s0)
+    op = a.op()
+    a.run(op, s0=False, s1=s1)
+    (o, mo), states = a.want(s0=False)
+    rel = 2.0 ** -15 + (max(lens) + a.dk + 4) * 2.0 ** -24
+    check(a.o[quiet], o[quiet], rel * mo[quiet], "f16", "quiet o")
+    for i, (S, M) in enumerate(states):
+        check(s1[int(a.slot[i])], S, rel * M, "f32", f"state {i}")
+    assert op.error == 0
+
+
+@gpu
 def test_dattn_offsets_past_32_bits(cuda):
     """states and rows more than 2^32 bytes and 2^31 elements into their buffers"""
     torch.cuda.empty_cache()
