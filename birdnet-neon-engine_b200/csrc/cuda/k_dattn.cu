@@ -175,6 +175,10 @@ __global__ void __launch_bounds__(256) k_dattn_rec(const DattnArgs a) {
 // (elect.sync): from one lane's branch each tcgen05.mma took 70 cycles to issue, more than a 128 x 64 x 16 product.
 // A masked token, and a row past the segment's end, has its k and v rows taken as zero (K' zero, V zeroed in shared
 // memory, its P column zero by selection, so that NaN and infinities there stay out); its o row is zero or not stored.
+// A live token's NaN or infinity meets the rows before it in the same products (0 NaN) and makes them NaN. It also makes
+// the state so, for good, which the state warps look for once the segment is done: chunks that hold such a token are then
+// formed again token by token (redo_chunks; 1 to 2 % of a call without one). To keep it out of the products instead took 8
+// to 12 % of every call (a selection above P's diagonal and a pass over each tile of V by a warp of its own).
 //
 // Bound by its roles' chain through a chunk and by shared memory's bandwidth, not by the products: DP 64 takes 4900 cycles a
 // chunk and head, of which the products are 2400 (each operand's parts are products of their own). 24 sequences of 9600
@@ -324,6 +328,75 @@ __device__ __forceinline__ void sts128(uint32_t at, const uint32_t (&x)[4]) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
 }
 
+template <int T>
+__device__ __forceinline__ bool no_number(elem_t<T> v) {
+  return !(fabsf(Elem<T>::get(v)) < __int_as_float(0x7f800000));
+}
+
+// The outputs of the chunks from the first to the last that holds a live token whose k or v is not finite, by the
+// definition: S_t = lambda S_(t-1) + k_t^T v_t from the segment's start (`from`, NULL: zero), o_t = scale q_t S_t. A warp
+// has 4 columns of S at a time, a lane the rows lane + 32 p. All of the CTA's threads; span: two shared words.
+template <int T>
+__device__ __forceinline__ void redo_chunks(const DattnArgs &d, int hk, long long t0, long long t1, const float *from, float lam,
+                                         int *span) {
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  if (threadIdx.x == 0) { span[0] = 0x7fffffff; span[1] = -1; }
+  __syncthreads();
+  for (long long t = t0 + warp; t < t1; t += kDaThreads / 32) {
+    if (d.live && !d.live[t]) continue;
+    const elem_t<T> *k = (const elem_t<T> *)d.k + t * d.kts + (long long)hk * d.dk;
+    const elem_t<T> *v = (const elem_t<T> *)d.v + t * d.vts + (long long)hk * d.dv;
+    bool bad = false;
+    for (int c = lane; c < d.dk; c += 32) bad |= no_number<T>(k[c]);
+    for (int c = lane; c < d.dv; c += 32) bad |= no_number<T>(v[c]);
+    if (bad) {
+      atomicMin(&span[0], (int)((t - t0) / kChunk));
+      atomicMax(&span[1], (int)((t - t0) / kChunk));
+    }
+  }
+  __syncthreads();
+  const long long first = t0 + (long long)span[0] * kChunk, end = min(t1, t0 + (long long)(span[1] + 1) * kChunk);
+  for (int c0 = 4 * warp; c0 < d.dv && span[1] >= 0; c0 += kDaThreads / 8) {
+    float S[4][4];
+#pragma unroll
+    for (int p = 0; p < 4; p++)
+#pragma unroll
+      for (int c = 0; c < 4; c++)
+        S[p][c] = from && lane + 32 * p < d.dk ? from[(long long)(lane + 32 * p) * d.dv + c0 + c] : 0.f;
+    for (long long t = t0; t < end; t++) {
+      const bool live = !d.live || d.live[t];
+      const elem_t<T> *k = (const elem_t<T> *)d.k + t * d.kts + (long long)hk * d.dk;
+      const elem_t<T> *v = (const elem_t<T> *)d.v + t * d.vts + (long long)hk * d.dv + c0;
+#pragma unroll
+      for (int p = 0; p < 4; p++) {
+        const float kk = live && lane + 32 * p < d.dk ? Elem<T>::get(k[lane + 32 * p]) : 0.f;
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+          S[p][c] = live && lane + 32 * p < d.dk ? fmaf(kk, Elem<T>::get(v[c]), lam * S[p][c]) : lam * S[p][c];
+      }
+      if (t < first || !live) continue;  // a dead token's o is zero already
+      for (int g = 0; g < d.G; g++) {
+        const elem_t<T> *q = (const elem_t<T> *)d.q + t * d.qts + (long long)(hk * d.G + g) * d.dk;
+        elem_t<T> *o = (elem_t<T> *)d.o + t * d.ots + (long long)(hk * d.G + g) * d.dv + c0;
+        float u[4] = {};
+#pragma unroll
+        for (int p = 0; p < 4; p++) {
+          if (lane + 32 * p >= d.dk) continue;
+          const float qq = Elem<T>::get(q[lane + 32 * p]);
+#pragma unroll
+          for (int c = 0; c < 4; c++) u[c] = fmaf(qq, S[p][c], u[c]);
+        }
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+#pragma unroll
+          for (int m = 16; m; m >>= 1) u[c] += __shfl_xor_sync(0xffffffffu, u[c], m);
+          if (lane == c) o[c] = Elem<T>::put(d.scale * u[c]);
+        }
+      }
+    }
+  }
+}
+
 template <int T, int DP, bool kState>
 __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_constant__ CUtensorMap mq,
                                                               const __grid_constant__ CUtensorMap mk,
@@ -337,7 +410,8 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
   __shared__ volatile int abort_s;
   __shared__ float s_pow[32 + 129];  // s_pow[32 + x] = lambda^x, 0 for x < 0
   __shared__ long long s_range[2];
-  __shared__ int s_seg[3];
+  __shared__ int s_seg[3], s_span[2];
+  __shared__ volatile int s_bad;  // the segment's state is not finite
   __shared__ float s_max[2][16], s_inv[2], s_dsc[2];  // fp16: the state warps' maxima, scales of S and of its sums by chunk
   __shared__ float s_pinv[L::scales][T == 1 ? kChunk : 1];  // fp16: the inverse row scales of P
   __shared__ float s_rowmax[T == 1 ? 2 : 1][2][T == 1 ? kChunk : 1];
@@ -369,6 +443,7 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
       mbar_init(smem_u32(&b_max), 16);
       for (int w = 0; w < 4; w++) mbar_init(smem_u32(&b_row[w]), 2);
       abort_s = 0;
+      s_bad = 0;
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncwarp();
@@ -388,6 +463,18 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
   const bool work = seq >= 0 && !(kState && s_seg[2]);
   const int nc = work ? (int)((t1 - t0 + kChunk - 1) / kChunk) : 0, nu = nc * G;
   const float *pw = s_pow + 32;
+  // the state before the segment
+  auto state_before = [&]() -> const float * {
+    if (a.seg_tokens) return a.seg_state + ((long long)blockIdx.x * d.Hk + hk) * d.dk * d.dv;
+    const long long slot = d.slot ? d.slot[seq] : seq;
+    return d.s0 && slot >= 0 ? d.s0 + (slot * d.Hk + hk) * (long long)d.dk * d.dv : nullptr;
+  };
+  // where the segment's state goes
+  auto state_after = [&]() -> float * {
+    if (kState) return work ? a.seg_state + ((long long)blockIdx.x * d.Hk + hk) * d.dk * d.dv : nullptr;
+    const long long slot = d.slot ? d.slot[seq] : seq;
+    return s_seg[2] && d.s1 && slot >= 0 ? d.s1 + (slot * d.Hk + hk) * (long long)d.dk * d.dv : nullptr;
+  };
   // a whole warp waits; false (and the error word set) when the time limit or another role's ran out
   auto wait = [&](unsigned long long &bar, int parity, int code) {
     if (__all_sync(0xffffffffu, mbar_try(smem_u32(&bar), parity))) return true;
@@ -741,12 +828,7 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
     constexpr int HC = DP / 4;
     const int r = 32 * (warp % 4) + lane, c0 = (warp - kDaS) / 4 * HC, tid = threadIdx.x - 32 * kDaS;
     float S[HC];
-    const long long slot = d.slot ? d.slot[seq] : seq;
-    const float *from = nullptr;
-    if (!kState) {
-      if (a.seg_tokens) from = a.seg_state + ((long long)blockIdx.x * d.Hk + hk) * d.dk * d.dv;
-      else if (d.s0 && slot >= 0) from = d.s0 + (slot * d.Hk + hk) * (long long)d.dk * d.dv;
-    }
+    const float *from = kState ? nullptr : state_before();
     if (!kState && a.seg_tokens) wait_launch_before();  // the states before the segments
     // in memory order, a row's HC columns by LP neighbouring lanes: with 16 bytes of 32 rows an access, a state of 128 x 128
     // took 4100 cycles to load and as many to store
@@ -925,14 +1007,19 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
       }
       if (c + 1 < nc) put_state(c + 1);  // the S operand's last reader, the chunk's last O1, comes before DS
     }
-    if (ok) {
-      float *to = nullptr;
-      if (kState) {
-        if (work) to = a.seg_state + ((long long)blockIdx.x * d.Hk + hk) * d.dk * d.dv;
-      } else if (s_seg[2] && d.s1 && slot >= 0) {
-        to = d.s1 + (slot * d.Hk + hk) * (long long)d.dk * d.dv;
-      }
+    {
+      float *to = ok ? state_after() : nullptr;
       turn_rows<LP>(S);
+      if constexpr (!kState) {
+        float z = 0.f;
+#pragma unroll
+        for (int e = 0; e < HC; e++) z = fmaf(S[e], 0.f, z);
+        if (z != 0.f && r < DP) s_bad = 1;
+        asm volatile("bar.sync 1, 512;" ::: "memory");  // the state warps
+      }
+      // chunks formed again start from the state before the segment, which this one's place may be: until then it waits in
+      // the S operand's place, which DS of the last chunk has come after
+      if (!kState && s_bad && ok) to = reinterpret_cast<float *>(dsmem + (base - smem_u32(dsmem)) + L::st);
       if (to) {
 #pragma unroll
         for (int j = 0; j < LP; j++)
@@ -946,6 +1033,14 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
   __syncthreads();
   if (warp == 1)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+  if constexpr (!kState)
+    if (s_bad && !abort_s) {
+      if (nc) redo_chunks<T>(d, hk, t0, t1, state_before(), pw[1], s_span);
+      __syncthreads();  // the state before the segment has been read
+      if (float *to = state_after())
+        for (int e = threadIdx.x; e < d.dk * d.dv; e += kDaThreads)
+          to[e] = reinterpret_cast<const float *>(dsmem + (base - smem_u32(dsmem)) + L::st)[e];
+    }
 }
 
 // the states before each segment: S = s0, then S = lambda^seg_tokens S + (the segment's own sum), in place in seg_state.

@@ -247,9 +247,8 @@ bnn_dattn *bnn_dattn_new(int type, int heads, int kv_heads, int dk, int dv, cons
  * slot, slot = d_slot[i] (d_slot NULL: i; a negative slot starts from zero and its state is dropped; no two sequences
  * of a call share a slot). d_s0 NULL: all start from zero; d_s1 NULL: no state is kept; d_s1 may be d_s0. A token whose
  * byte of d_live (NULL: all live) is 0 is a window that failed or is missing: its q, k and v are not used, its o is 0,
- * and the state decays by its step. A live token with an infinity or a NaN makes its own head's state and all later
- * outputs of its sequence non-finite, and may do so to outputs up to 127 tokens before it (they are formed in chunks);
- * other sequences keep theirs. */
+ * and the state decays by its step. A live token's infinities and NaN make NaN or infinities where the formulas
+ * have either, in its own head's state and outputs from it on; all that comes before it keeps its values. */
 int bnn_dattn_run(bnn_dattn *op, int n, long long tokens, const int32_t *d_cu, const int32_t *d_slot,
                   const uint8_t *d_live, const void *d_q, long long qts, const void *d_k, long long kts, const void *d_v,
                   long long vts, const float *d_s0, float *d_s1, void *d_o, long long ots, void *stream);

@@ -365,6 +365,51 @@ def test_dattn_loud_tokens_long_ago(cuda, heads, masked):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("heads, lens, bad", [((2, 2, 64, 64), [300, 140], [100, 257, 311]), ((3, 1, 96, 72), [300, 140], [0, 130, 299]),
+                                              ((2, 1, 128, 128), [700], [127, 128, 640]), ((1, 1, 64, 64), [3000], [1500]),
+                                              ((1, 1, 128, 64), [2500], [1000, 1001, 2499]), ((2, 2, 40, 24), [5, 9, 2], [6])])
+@pytest.mark.parametrize("part", "qkv")
+@pytest.mark.parametrize("value", [math.nan, -math.inf])
+def test_dattn_live_tokens_without_numbers(cuda, dtype, heads, lens, bad, part, value):
+    """a live token's NaN or infinity: other heads and other sequences keep their bits, the outputs and states that the
+    definition has finite (those before the token, and columns that it does not reach) their values, the others are not
+    finite"""
+    a = Attention(dtype, *heads, lens, seed=17)
+    op = a.op()
+    s1 = torch.zeros_like(a.s0)
+    a.run(op, s1=s1)
+    o, s = a.o.clone(), s1.clone()
+    x = {"q": a.q, "k": a.k, "v": a.v}[part]
+    G, ends = a.H // a.Hk, a.cu.tolist()
+    same = torch.full((sum(lens), a.H), True, device="cuda")
+    for i, t in enumerate(bad):
+        h = i % x.shape[1]
+        x[t, h, (7 * i + 3) % x.shape[2]] = value
+        first, end = max(e for e in ends if e <= t), min(e for e in ends if e > t)
+        same[first:end, slice(h, h + 1) if part == "q" else slice(h * G, (h + 1) * G)] = False
+    s1.zero_()
+    a.s0, keep = a.s0.clone(), a.s0
+    a.run(op, s1=a.s0)  # in place
+    s1, a.s0 = a.s0, keep
+    (want, mo), states = a.want()
+    rel = 2.0 ** -15 + (max(lens) + a.dk + 4) * 2.0 ** -24
+
+    def finite_ones(got, w, m, dt, what):
+        fin = torch.isfinite(w)
+        assert torch.equal(torch.isfinite(got), fin), what
+        check(got[fin], w[fin], rel * m[fin], dt, what)
+
+    finite_ones(a.o, want, mo, dtype, "o")
+    for i, (S, M) in enumerate(states):
+        finite_ones(s1[int(a.slot[i])], S, M, "f32", f"state {i}")
+    assert torch.equal(a.o[same], o[same])
+    if part == "q":
+        assert torch.equal(s1[a.slot.long()], s[a.slot.long()])
+    assert op.error == 0
+
+
+@gpu
 def test_dattn_offsets_past_32_bits(cuda):
     """states and rows more than 2^32 bytes and 2^31 elements into their buffers"""
     torch.cuda.empty_cache()
