@@ -404,12 +404,16 @@ __global__ void __launch_bounds__(kMidThreads, 1) k_lowrank_mid(const __grid_con
 // A tcgen05 GEMM of 128-row tiles, y's accumulators in TMEM, with the adapters as more steps of the sum: for each
 // adapter among the tile's rows (the list that 4 warps make from the rows' slots while W's steps run) the A operand is h
 // in the rows of that adapter and zero in the others, the B operand B_a. h is fp32 and goes as 16-bit parts: three for
-// bf16 (all 24 bits), two for fp16 (22 bits); a row with an |h| past fp16's range is left out of the operand and its
-// products are added in fp32 when y is stored. Slots of 64 / RB adapters share a stage (RB: the rank rounded up to 16, 32
-// or 64, a row of that many bytes swizzled as such).
+// bf16 (all 24 bits), two for fp16, which leave 2^-25 at most: 2^-23 of a row's largest |h| from 0.25 up. Slots of 64 / RB
+// adapters share a stage (RB: the rank rounded up to 16, 32 or 64, a row of that many bytes swizzled as such).
+// A tile of fp16 rows with an |h| past the type, or a row whose largest is below 0.25 (two parts would leave 1.7e-5 of an h of
+// 1e-3), has kind::tf32 steps instead: h as two parts of 11 bits, which leave 2^-22 of it whatever its size, and B's values
+// exact. 16 columns of the adapters back to back are a step: a row of A is 16 first parts and 16 second ones, a row of B 16
+// values for both, made of the 16-bit ones that TMA puts behind them. 9001 x 1536 x 6144, rank 32, runs of 700, cold caches:
+// 173 us, with 16-bit parts 158; 300 rows with an adapter each, 1024 x 6522, rank 16: 127 and 79.
 //
-// One persistent CTA per SM, column tiles fastest. Warp 0 streams 64-wide steps of x and W into a ring by TMA; warp 1
-// issues the MMAs into one of two accumulators; warps 2 .. 5 make the list and h's operand tiles and load the B_a tiles;
+// One persistent CTA per SM, column tiles fastest. Warp 0 streams 64-wide steps of x and W, then the adapters' B, into a
+// ring by TMA; warp 1 issues the MMAs into one of two accumulators; warps 2 .. 5 make the list and h's operand tiles;
 // warps 6 .. 13 store y: accumulator rows through shared memory, so that a store covers 32 neighbouring words of a row at
 // any row alignment; 16 bytes a lane where y's rows are whole 16 bytes.
 // Bound by reading x and W from L2 (48 KB for 1040 cycles of products at 256 columns). 9001 x 1536 x 6144 without adapters
@@ -426,33 +430,36 @@ struct LrArgs {
   int *err;
 };
 
+// the nearest tf32 (11 bits), ties away from zero; not for a NaN whose payload would carry over
+__device__ __forceinline__ float to_tf32(float v) { return __uint_as_float((__float_as_uint(v) + 0x1000u) & 0xffffe000u); }
+
 template <int T, int OT, int RB>
 __global__ void __launch_bounds__(kLrThreads, 1) k_lowrank_many(const __grid_constant__ CUtensorMap mx,
                                                                const __grid_constant__ CUtensorMap mw,
-                                                               const __grid_constant__ CUtensorMap mb, const LrArgs a) {
+                                                               const __grid_constant__ CUtensorMap mb,
+                                                               const __grid_constant__ CUtensorMap mb8, const LrArgs a) {
   constexpr int PARTS = T == 2 ? 3 : 2, GS = 64 / RB;  // adapters a stage
   extern __shared__ uint8_t dsmem[];
   __shared__ __align__(8) unsigned long long b_full[kLrStages], b_empty[kLrStages], b_acc[2], b_accempty[2], b_list[2],
-      b_listempty[2], b_turn[2], b_back[2];
+      b_listempty[2], b_place[kLrStages], b_base;
   __shared__ uint32_t tmem_s;
   __shared__ volatile int abort_s;
   __shared__ int s_n[2], s_list[2][128];
-  __shared__ volatile uint8_t s_big[2][128];
+  __shared__ volatile uint8_t s_wide[2][4];  // tf32 steps, as warps 2 .. 5 found for their rows
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   const bnnk_lowrank_args &p = a.p;
   const int S = a.stages, bn = a.bn;
   launch_dependents();
   const uint32_t a_bytes = 128 * 128, stage = (128 + bn) * 128;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < S; s++) { mbar_init(smem_u32(&b_full[s]), 5); mbar_init(smem_u32(&b_empty[s]), 1); }
+    for (int s = 0; s < S; s++) { mbar_init(smem_u32(&b_full[s]), 5); mbar_init(smem_u32(&b_empty[s]), 1); mbar_init(smem_u32(&b_place[s]), 1); }
     for (int g = 0; g < 2; g++) {
       mbar_init(smem_u32(&b_acc[g]), 1);
       mbar_init(smem_u32(&b_accempty[g]), 8);
       mbar_init(smem_u32(&b_list[g]), 4);
-      mbar_init(smem_u32(&b_listempty[g]), 14);
-      mbar_init(smem_u32(&b_turn[g]), 1);
-      mbar_init(smem_u32(&b_back[g]), 4);
+      mbar_init(smem_u32(&b_listempty[g]), 6);
     }
+    mbar_init(smem_u32(&b_base), 1);
     abort_s = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -483,14 +490,24 @@ __global__ void __launch_bounds__(kLrThreads, 1) k_lowrank_many(const __grid_con
       if (++s == S) { s = 0; parity ^= 1; used = 1; }
     }
   } at;
+  // 8 columns of the list's adapters back to back: the adapter's place in the list, the columns' in the adapter
+  struct Columns {
+    int e = 0, off = 0;
+    __device__ __forceinline__ void next(int rank) {
+      if ((off += 8) == rank) off = 0, e++;
+    }
+  };
   int lt = 0;       // tiles done
   bool ok = true;
-  // the stages that the tile's adapters take (after list lt % 2 is made)
-  auto extra = [&](int &n) {
+  // the stages that the tile's adapters take, and their kind (after list lt % 2 is made)
+  auto extra = [&](int &n, bool &wide) {
     n = 0;
+    wide = false;
     if (!adapters) return true;
-    if (!wait(b_list[lt & 1], (lt >> 1) & 1, BNNK_ERR_TMA_WAIT)) return false;
-    n = (s_n[lt & 1] + GS - 1) / GS * PARTS;
+    const int g = lt & 1;
+    if (!wait(b_list[g], (lt >> 1) & 1, BNNK_ERR_TMA_WAIT)) return false;
+    wide = T == 1 && (s_wide[g][0] | s_wide[g][1] | s_wide[g][2] | s_wide[g][3]);
+    n = wide ? (s_n[g] * p.rank + 15) / 16 : (s_n[g] + GS - 1) / GS * PARTS;
     return true;
   };
   auto list_read = [&]() {
@@ -499,15 +516,9 @@ __global__ void __launch_bounds__(kLrThreads, 1) k_lowrank_many(const __grid_con
   };
 
   if (warp == 0) {
-    int ahead = 0;      // places that may be used before the last tile's adapters have had theirs
-    bool owed = false;  // whether they are still to say so
     for (int t = blockIdx.x; t < a.tiles && ok; t += gridDim.x, lt++) {
-      const int r0 = t / a.n_tiles * 128, n0 = t % a.n_tiles * bn;
+      const int r0 = t / a.n_tiles * 128, n0 = t % a.n_tiles * bn, g = lt & 1;
       for (int kb = 0; kb < a.nkb; kb++, at.next(S)) {
-        if (owed && ahead-- == 0) {
-          if (!(ok = wait(b_back[(lt - 1) & 1], ((lt - 1) >> 1) & 1, BNNK_ERR_TMA_WAIT))) break;
-          owed = false;
-        }
         if (at.used && !(ok = wait(b_empty[at.s], at.parity ^ 1, BNNK_ERR_TMA_WAIT))) break;
         const uint32_t st = base + at.s * stage, bar = smem_u32(&b_full[at.s]);
         if (elect_one()) {
@@ -517,21 +528,41 @@ __global__ void __launch_bounds__(kLrThreads, 1) k_lowrank_many(const __grid_con
           tma_load_2d(st + a_bytes, &mw, bar, kb * 64, n0);
         }
       }
-      // the ring's next places are the adapters': handed over and back, so that each side waits for a place whose use
-      // before has begun (a parity tells one use from the next, not from the one after). Until it comes to a place that
-      // they had, this warp goes on with the next tile.
-      if (!ok || !adapters) continue;
-      if (owed && !(ok = wait(b_back[(lt - 1) & 1], ((lt - 1) >> 1) & 1, BNNK_ERR_TMA_WAIT))) break;
-      if (elect_one()) mbar_arrive(smem_u32(&b_turn[lt & 1]));
-      int n = 0;
-      if (!(ok = extra(n))) break;
+      int n;
+      bool wide;
+      if (!ok || !(ok = extra(n, wide))) break;
+      // the adapters' places: B here, b_place tells the warps that make A that a place is free for them (b_empty could not:
+      // a parity tells one use from the next, not from the one after) and, for tf32 steps, that its 16-bit B is there
+      Columns col;
+      for (int k = 0; k < n; k++, at.next(S)) {
+        if (at.used && !(ok = wait(b_empty[at.s], at.parity ^ 1, BNNK_ERR_TMA_WAIT))) break;
+        const uint32_t st = base + at.s * stage + a_bytes, full = smem_u32(&b_full[at.s]), place = smem_u32(&b_place[at.s]);
+        if (!wide) {
+          const int e0 = k / PARTS * GS, here = min(GS, s_n[g] - e0);
+          if (elect_one()) {
+            mbar_arrive(place);
+            mbar_expect_tx(full, here * bn * RB * 2);
+            for (int e = 0; e < here; e++) tma_load_3d(st + e * bn * RB * 2, &mb, full, 0, n0, s_list[g][e0 + e]);
+          }
+        } else {
+          const Columns c0 = col;
+          col.next(p.rank);
+          const Columns c1 = col;
+          col.next(p.rank);
+          const bool both = c1.e < s_n[g];
+          if (elect_one()) {
+            mbar_arrive(full);
+            mbar_expect_tx(place, bn * (both ? 32 : 16));
+            tma_load_3d(st + bn * 64, &mb8, place, c0.off, n0, s_list[g][c0.e]);
+            if (both) tma_load_3d(st + bn * 80, &mb8, place, c1.off, n0, s_list[g][c1.e]);
+          }
+        }
+      }
       list_read();
-      for (int k = 0; k < n; k++) at.next(S);
-      ahead = max(0, S - n);
-      owed = true;
     }
   } else if (warp == 1) {
     const uint32_t idesc = idesc_16(T - 1, bn, 0, 0);
+    int base_parity = 0;
     for (int t = blockIdx.x; t < a.tiles && ok; t += gridDim.x, lt++) {
       const int g = lt & 1;
       if (lt >= 2 && !(ok = wait(b_accempty[g], (lt / 2 - 1) & 1, BNNK_ERR_MMA_WAIT))) break;
@@ -547,15 +578,32 @@ __global__ void __launch_bounds__(kLrThreads, 1) k_lowrank_many(const __grid_con
           mma_commit(smem_u32(&b_empty[at.s]));
         }
       }
-      int n = 0;
-      if (!ok || !(ok = extra(n))) break;
+      int n;
+      bool wide;
+      if (!ok || !(ok = extra(n, wide))) break;
       const int used = n ? s_n[g] : 0;
       list_read();
+      if (T == 1 && wide) {  // instructions of another kind: nothing says that they follow W's into the sum, so W's end first
+        if (elect_one()) mma_commit(smem_u32(&b_base));
+        if (!(ok = wait(b_base, base_parity, BNNK_ERR_MMA_WAIT))) break;
+        base_parity ^= 1;
+        tc_fence_after();
+      }
       for (int k = 0; k < n; k++, at.next(S)) {
         if (!(ok = wait(b_full[at.s], at.parity, BNNK_ERR_MMA_WAIT))) break;
         tc_fence_after();
+        const uint32_t st = base + at.s * stage;
+        if (T == 1 && wide) {
+          const uint64_t da = smem_desc<128>(st), db = smem_desc<64>(st + a_bytes);
+          if (elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < 4; kk++) mma32_ss(acc, da + kk * 2, db + (kk & 1) * 2, idesc_tf32(bn), 1);
+            mma_commit(smem_u32(&b_empty[at.s]));
+          }
+          continue;
+        }
         const int here = min(GS, used - k / PARTS * GS);
-        const uint64_t da = smem_desc<2 * RB>(base + at.s * stage), db = smem_desc<2 * RB>(base + at.s * stage + a_bytes);
+        const uint64_t da = smem_desc<2 * RB>(st), db = smem_desc<2 * RB>(st + a_bytes);
         if (elect_one()) {
           for (int e = 0; e < here; e++)
 #pragma unroll
@@ -569,9 +617,15 @@ __global__ void __launch_bounds__(kLrThreads, 1) k_lowrank_many(const __grid_con
   } else if (warp < 6) {
     if (adapters) {
       const int row = threadIdx.x - 64;
+      uint32_t place_parity = 0;  // by place
+      auto wait_place = [&]() {
+        if (!(ok = wait(b_place[at.s], (place_parity >> at.s) & 1, BNNK_ERR_TMA_WAIT))) return false;
+        place_parity ^= 1u << at.s;
+        return true;
+      };
       wait_launch_before();
       for (int t = blockIdx.x; t < a.tiles && ok; t += gridDim.x, lt++) {
-        const int r0 = t / a.n_tiles * 128, n0 = t % a.n_tiles * bn, g = lt & 1;
+        const int r0 = t / a.n_tiles * 128, g = lt & 1;
         if (lt >= 2 && !(ok = wait(b_listempty[g], (lt / 2 - 1) & 1, BNNK_ERR_TMA_WAIT))) break;
         // the tile's adapters, in the order of their first rows: every warp makes the whole list from all 128 slots and
         // writes its own part of it
@@ -604,40 +658,112 @@ __global__ void __launch_bounds__(kLrThreads, 1) k_lowrank_many(const __grid_con
         const unsigned own = firsts[0] * (warp == 2) | firsts[1] * (warp == 3) | firsts[2] * (warp == 4) | firsts[3] * (warp == 5);
         if ((own >> lane) & 1) s_list[g][before + __popc(own & ((1u << lane) - 1))] = mine;
         if (warp == 2 && lane == 0) s_n[g] = count;
-        // this row's h, read while W's steps run: rows past fp16's range are added when y is stored
-        float h[RB];
+        // this row's h, read while W's steps run
+        float h[RB], most = 0.f;
 #pragma unroll
         for (int c = 0; c < RB; c += 4) {
           float4 u = make_float4(0.f, 0.f, 0.f, 0.f);
           if (mine >= 0 && c < p.rank) u = *reinterpret_cast<const float4 *>(p.hid + (long long)(r0 + row) * p.rank + c);
           h[c] = u.x, h[c + 1] = u.y, h[c + 2] = u.z, h[c + 3] = u.w;
         }
-        bool big = false;
-        if constexpr (T == 1)
+        if constexpr (T == 1) {
 #pragma unroll
-          for (int e = 0; e < RB; e++) big |= fabsf(h[e]) > 65504.f && fabsf(h[e]) < __int_as_float(0x7f800000);
-        s_big[g][row] = big;
+          for (int c = 0; c < RB; c++) most = fmaxf(most, fabsf(h[c]));
+          const bool wide = (most > 0.f && most < 0.25f) || (most > 65504.f && most < __int_as_float(0x7f800000));
+          const bool any = __any_sync(0xffffffffu, wide);
+          if (lane == 0) s_wide[g][warp - 2] = any;
+        }
         __threadfence_block();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&b_list[g]));
-        if (!(ok = wait(b_list[g], (lt >> 1) & 1, BNNK_ERR_TMA_WAIT))) break;
-        if (!(ok = wait(b_turn[g], (lt >> 1) & 1, BNNK_ERR_TMA_WAIT))) break;
+        int steps;
+        bool wide;
+        if (!(ok = extra(steps, wide))) break;
         // the ring's places of W's steps
         for (int kb = 0; kb < a.nkb; kb++) at.next(S);
+        if constexpr (T == 1)
+          if (wide) {
+#pragma unroll
+            for (int c = 0; c < RB; c++) h[c] = h[c] == h[c] ? h[c] : __uint_as_float(0x7fc00000u);  // for to_tf32
+            uint8_t *ring = dsmem + (base - smem_u32(dsmem));
+            Columns col;
+#pragma unroll 1
+            for (int k = 0; k < steps; k++, at.next(S)) {
+              if (!wait_place()) break;
+              uint8_t *st = ring + at.s * stage;
+              int s[2], off[2];
+              uint4 w[2][2];
+#pragma unroll
+              for (int j = 0; j < 2; j++, col.next(p.rank)) {
+                s[j] = col.e < count ? s_list[g][col.e] : -1;
+                off[j] = col.off;
+#pragma unroll
+                for (int q = 0; q < 2; q++) {
+                  const int n = row + 128 * q;
+                  w[j][q] = make_uint4(0, 0, 0, 0);
+                  if (s[j] >= 0 && n < bn) w[j][q] = *reinterpret_cast<const uint4 *>(st + a_bytes + bn * 64 + (j * bn + n) * 16);
+                }
+              }
+              // A: 128 bytes a row, first parts of 16 columns and second ones, 16-byte places with the 128-byte swizzle
+#pragma unroll
+              for (int j = 0; j < 2; j++) {
+                uint8_t *ra = st + row * 128;
+                const int sw = (row & 7) * 16;
+                const bool on = s[j] >= 0 && s[j] == mine;
+                float u[8] = {}, v[8] = {};
+                if (__any_sync(0xffffffffu, on)) {
+#pragma unroll
+                  for (int i = 0; i < RB / 8; i++)
+                    if (off[j] == 8 * i) {
+#pragma unroll
+                      for (int c = 0; c < 8; c++) v[c] = on ? h[8 * i + c] : 0.f;
+                    }
+#pragma unroll
+                  for (int c = 0; c < 8; c++) {
+                    u[c] = to_tf32(v[c]);
+                    v[c] = to_tf32(v[c] - u[c]);
+                  }
+                }
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                  float4 *first = reinterpret_cast<float4 *>(ra + ((2 * j + i) * 16 ^ sw));
+                  float4 *second = reinterpret_cast<float4 *>(ra + ((4 + 2 * j + i) * 16 ^ sw));
+                  *first = make_float4(u[4 * i], u[4 * i + 1], u[4 * i + 2], u[4 * i + 3]);
+                  *second = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                }
+              }
+              // B: 64 bytes a row, the 64-byte swizzle
+#pragma unroll
+              for (int q = 0; q < 2; q++) {
+                const int n = row + 128 * q;
+                if (n >= bn) break;
+                uint8_t *rb = st + a_bytes + n * 64;
+                const int sw = (n >> 1 & 3) * 16;
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                  const float2 b0 = unpack2<T>(w[j][q].x), b1 = unpack2<T>(w[j][q].y), b2 = unpack2<T>(w[j][q].z),
+                               b3 = unpack2<T>(w[j][q].w);
+                  *reinterpret_cast<float4 *>(rb + (2 * j * 16 ^ sw)) = make_float4(b0.x, b0.y, b1.x, b1.y);
+                  *reinterpret_cast<float4 *>(rb + ((2 * j + 1) * 16 ^ sw)) = make_float4(b2.x, b2.y, b3.x, b3.y);
+                }
+              }
+              fence_async_smem();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(smem_u32(&b_full[at.s]));
+            }
+            if (!ok) break;
+            list_read();
+            continue;
+          }
         for (int e0 = 0; e0 < count && ok; e0 += GS) {
           const int here = min(GS, count - e0);
           int my = -1;  // this row's adapter among the stage's
           for (int e = 0; e < here; e++)
-            if (mine >= 0 && !big && s_list[g][e0 + e] == mine) my = e;
+            if (mine >= 0 && s_list[g][e0 + e] == mine) my = e;
 #pragma unroll 1
           for (int part = 0; part < PARTS; part++, at.next(S)) {
-            if (at.used && !(ok = wait(b_empty[at.s], at.parity ^ 1, BNNK_ERR_TMA_WAIT))) break;
-            const uint32_t st = base + at.s * stage, bar = smem_u32(&b_full[at.s]);
-            if (warp == 2 && elect_one()) {
-              mbar_expect_tx(bar, here * bn * RB * 2);
-              for (int e = 0; e < here; e++)
-                tma_load_3d(st + a_bytes + e * bn * RB * 2, &mb, bar, 0, n0, s_list[g][e0 + e]);
-            }
+            if (!wait_place()) break;
+            const uint32_t st = base + at.s * stage;
 #pragma unroll
             for (int c = 0; c < RB; c += 8) {
               uint32_t z[4] = {0, 0, 0, 0};
@@ -662,12 +788,11 @@ __global__ void __launch_bounds__(kLrThreads, 1) k_lowrank_many(const __grid_con
             }
             fence_async_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(bar);
+            if (lane == 0) mbar_arrive(smem_u32(&b_full[at.s]));
           }
         }
         if (!ok) break;
         list_read();
-        if (lane == 0) mbar_arrive(smem_u32(&b_back[g]));
       }
     }
   } else {
@@ -682,7 +807,6 @@ __global__ void __launch_bounds__(kLrThreads, 1) k_lowrank_many(const __grid_con
       const int r0 = t / a.n_tiles * 128 + 32 * qd, n0 = t % a.n_tiles * bn, g = lt & 1;
       if (!wait(b_acc[g], (lt >> 1) & 1, BNNK_ERR_EPI_WAIT)) break;
       tc_fence_after();
-      const bool big = T == 1 && adapters && s_big[g][32 * qd + lane];
       const uint32_t tq = tmem + g * a.na * a.acc_cols + ((uint32_t)(32 * qd) << 16);
       const int width = min(bn, p.N - n0), rows = min(32, p.rows - r0);
 #pragma unroll 1
@@ -714,18 +838,6 @@ __global__ void __launch_bounds__(kLrThreads, 1) k_lowrank_many(const __grid_con
 #pragma unroll
               for (int j = 0; j < 16; j++) v[j] += __uint_as_float(x[j]);
             }
-          if (big) {  // h past fp16's range: its products here
-            const int s = p.slot[r0 + lane];
-            const float *hh = p.hid + (long long)(r0 + lane) * p.rank;
-#pragma unroll 1
-            for (int j = 0; j < 16 && c + j < width; j++) {
-              const elem_t<T> *b = (const elem_t<T> *)p.b + ((long long)s * p.N + n0 + c + j) * p.rank;
-              float u = 0.f;
-              for (int e = 0; e < p.rank; e++) u = fmaf(hh[e], Elem<T>::get(b[e]), u);
-#pragma unroll
-              for (int i = 0; i < 16; i++) v[i] += i == j ? u : 0.f;
-            }
-          }
           __syncwarp();
 #pragma unroll
           for (int j = 0; j < 16; j += 4 * PW) {
@@ -772,10 +884,7 @@ __global__ void __launch_bounds__(kLrThreads, 1) k_lowrank_many(const __grid_con
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(smem_u32(&b_accempty[g]));
-        if (adapters) mbar_arrive(smem_u32(&b_listempty[g]));
-      }
+      if (lane == 0) mbar_arrive(smem_u32(&b_accempty[g]));
     }
   }
   tc_fence_before();
@@ -848,16 +957,17 @@ int run_many(const bnnk_lowrank_args &p, int *err, cudaStream_t st) {
   const int s = (int)((227 * 1024 - 4096 - out) / stage);
   a.stages = s > kLrStages ? kLrStages : s;
   const size_t smem = a.stages * stage + out + 1024;
-  CUtensorMap mx, mw, mb;
+  CUtensorMap mx, mw, mb, mb8;
   int e = encode_rows16(&mx, p.x, T == 2, p.K, p.rows, p.ldx, 64, 128, 128);
   if (!e) e = encode_rows16(&mw, p.w, T == 2, p.K, p.N, p.ldw, 64, a.bn, 128);
   if (!e) e = encode_slots16(&mb, p.b, T == 2, p.rank, p.N, p.slots, RB, a.bn);
+  if (!e) e = encode_slots16(&mb8, p.b, T == 2, p.rank, p.N, p.slots, 8, a.bn);
   static SmemAttr attr;
   if (!e) e = attr.ensure(k_lowrank_many<T, OT, RB>, smem);
   if (e) return e;
   const int grid = a.tiles < num_sms() ? a.tiles : num_sms();
-  if (p.slot) return launch_early(k_lowrank_many<T, OT, RB>, dim3(grid), kLrThreads, smem, st, mx, mw, mb, a);
-  k_lowrank_many<T, OT, RB><<<grid, kLrThreads, smem, st>>>(mx, mw, mb, a);
+  if (p.slot) return launch_early(k_lowrank_many<T, OT, RB>, dim3(grid), kLrThreads, smem, st, mx, mw, mb, mb8, a);
+  k_lowrank_many<T, OT, RB><<<grid, kLrThreads, smem, st>>>(mx, mw, mb, mb8, a);
   return cudaGetLastError();
 }
 

@@ -58,7 +58,10 @@ int bnn::encode_slots16(CUtensorMap *m, const void *base, int bf16, int width, i
   const cuuint32_t box[3] = {(cuuint32_t)box_w, (cuuint32_t)box_rows, 1}, es[3] = {1, 1, 1};
   return enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void *>(base),
              dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-             box_w == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : box_w == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B,
+             box_w == 64   ? CU_TENSOR_MAP_SWIZZLE_128B
+             : box_w == 32 ? CU_TENSOR_MAP_SWIZZLE_64B
+             : box_w == 16 ? CU_TENSOR_MAP_SWIZZLE_32B
+                           : CU_TENSOR_MAP_SWIZZLE_NONE,
              CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE)
              ? cudaErrorInvalidValue
              : 0;

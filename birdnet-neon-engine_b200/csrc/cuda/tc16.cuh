@@ -1,4 +1,5 @@
-// tcgen05 kind::f16 building blocks of the operators over sequences (inline PTX): fp16 or bf16 operands (both of a type),
+// tcgen05 kind::f16 building blocks of the operators over sequences (inline PTX): fp16 or bf16 operands (both of a type; a
+// kind::tf32 product too),
 // fp32 accumulators in TMEM, A from shared memory or TMEM, K-major and MN-major shared-memory tiles, TMEM loads and
 // stores. Host side: the descriptor encoder and 3-D maps of [rows][heads][width] tensors.
 #pragma once
@@ -16,6 +17,10 @@ __host__ __device__ constexpr uint32_t idesc_16(int t, int n, int a_mn, int b_mn
   return (1u << 4) | ((uint32_t)t << 7) | ((uint32_t)t << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
          ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
+// the same for kind::tf32, both operands K-major: 32 bytes of a row are its 8 K elements
+__host__ __device__ constexpr uint32_t idesc_tf32(int n) {
+  return (1u << 4) | (2u << 7) | (2u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
 // descriptor of an MN-major tile: k rows of 64 elements (128 bytes, 128-byte swizzle), 8-row groups back to back, the
 // next 64 elements of the M or N index `panel` bytes on
 __device__ __forceinline__ uint64_t smem_desc_mn(uint32_t addr, uint32_t panel) {
@@ -27,6 +32,14 @@ __device__ __forceinline__ void mma16_ss(uint32_t d, uint64_t da, uint64_t db, u
       "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(da), "l"(db), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma32_ss(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::tf32 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
       "l"(da), "l"(db), "r"(idesc), "r"(accumulate)
       : "memory");
 }
@@ -130,6 +143,7 @@ int encode_heads(CUtensorMap *m, const void *base, int bf16, int width, int head
 int encode_rows16(CUtensorMap *m, const void *base, int bf16, int width, long long rows, long long rs, int box_w,
                   int box_rows, int sw);
 // host: a 3-D map of [slots][rows][width] back to back, boxes of box_w x box_rows x 1 slot, swizzle 2 box_w bytes
+// (8 wide: none)
 int encode_slots16(CUtensorMap *m, const void *base, int bf16, int width, int rows, int slots, int box_w, int box_rows);
 
 }  // namespace bnn

@@ -582,6 +582,59 @@ def test_lowrank_fp16_h_past_the_type(cuda, rows, out):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("rows", [1, 16, 128, 129, 500])
+@pytest.mark.parametrize("scale", [1.0, 1e-2, 1e-4, 1e-6])
+def test_lowrank_keeps_h_of_any_size(cuda, dtype, rows, scale):
+    """h is fp32 however small and however many rows share the call. Without W: the error is that of the two sums, K and
+    rank terms of 2^-24 each at worst, in rms no more than 2^-24 times the root of their number (2^-20), twice that where
+    the tensor cores cut sums off"""
+    gen, K, N, rank, slots = generator(rows), 256, 130, 24, 3
+    x, w = rand(gen, rows, K).to(DT[dtype]), torch.zeros(N, K, device="cuda", dtype=DT[dtype])
+    A, B = (rand(gen, slots, rank, K) * 2.0 ** -4).to(DT[dtype]), rand(gen, slots, N, rank).to(DT[dtype])
+    s = torch.full((slots,), scale, device="cuda")
+    slot = torch.randint(0, slots, (rows,), device="cuda", generator=gen).int()
+    y = torch.empty(rows, N, device="cuda")
+    op = sequence.LowRank(dtype, "f32", N, K, w.data_ptr(), None, slots, rank, A.data_ptr(), B.data_ptr(), s.data_ptr(),
+                          rows=rows)
+    op.run(rows, x.data_ptr(), slot.data_ptr(), y.data_ptr())
+    h = torch.einsum("rk,rjk->rj", x.double(), A.double()[slot.long()]) * s.double()[0]
+    want = torch.einsum("rj,rnj->rn", h, B.double()[slot.long()])
+    assert float((y.double() - want).norm() / want.norm()) < 2.0 ** -19
+    assert op.error == 0
+
+
+@gpu
+@pytest.mark.parametrize("rank, out", [(8, "f32"), (24, "f16"), (64, "f32")])
+def test_lowrank_fp16_tiles_of_both_kinds(cuda, rank, out):
+    """blocks of rows whose h is ordinary, small, past fp16 or absent, several tiles for each SM: every block to the
+    accuracy of its own size"""
+    gen, rows, K, N, slots = generator(rank), 5001, 64, 3000, 5
+    size = torch.tensor([1.0, 1e-3, 1.0, 3e4, 1e-5, 0.0], device="cuda")[torch.arange(rows, device="cuda") // 100 % 6]
+    x, w = rand(gen, rows, K).half(), (rand(gen, N, K) * 2.0 ** -3).half()
+    A, B = (rand(gen, slots, rank, K) * 2.0 ** -3).half(), (rand(gen, slots, N, rank) * 2.0 ** -6).half()
+    # the size by the adapter's scale: adapter 5 a + b has scale sizes[b]
+    sizes = torch.tensor([1.0, 1e-3, 3e4, 1e-5], device="cuda")
+    A4, B4 = A.repeat_interleave(4, 0).contiguous(), B.repeat_interleave(4, 0).contiguous()
+    s = sizes.repeat(slots)
+    which = torch.stack([(size == v).int() * i for i, v in enumerate(sizes)]).sum(0)
+    slot = torch.randint(0, slots, (rows,), device="cuda", generator=gen) * 4 + which
+    slot = torch.where(size == 0, -1, slot).int()
+    y = torch.empty(rows, N, device="cuda", dtype=DT[out])
+    op = sequence.LowRank("f16", out, N, K, w.data_ptr(), None, 4 * slots, rank, A4.data_ptr(), B4.data_ptr(), s.data_ptr(),
+                          rows=rows)
+    op.run(rows, x.data_ptr(), slot.data_ptr(), y.data_ptr())
+    assert op.error == 0
+    xd, wd = x.double(), w.double()
+    want, M = xd @ wd.t(), xd.abs() @ wd.abs().t()
+    for a in range(4 * slots):
+        at = torch.nonzero(slot == a).flatten()
+        want[at] += s[a].double() * ((xd[at] @ A4[a].double().t()) @ B4[a].double().t())
+        M[at] += s[a].double() * ((xd[at].abs() @ A4[a].double().abs().t()) @ B4[a].double().abs().t())
+    check(y, want, (K + rank + 8) * 2.0 ** -23 * M, out, "y")  # the tensor cores cut off: 2^-23 a term
+
+
+@gpu
 def test_lowrank_adapter_replaced_between_runs(cuda):
     """the adapters are read by every run: one that is written in stream order counts from the next run on"""
     gen = generator(1)
