@@ -412,6 +412,9 @@ __global__ void __launch_bounds__(kMidThreads, 1) k_lowrank_mid(const __grid_con
 // values for both, made of the 16-bit ones that TMA puts behind them. 9001 x 1536 x 6144, rank 32, runs of 700, cold caches:
 // 173 us, with 16-bit parts 158; 300 rows with an adapter each, 1024 x 6522, rank 16: 127 and 79.
 //
+// A NaN or an infinity in an adapter's B meets the zeros of the rows of others in the same products: y that is not finite
+// where the row's own x and h are is formed again in fp32 when it is stored (row_product).
+//
 // One persistent CTA per SM, column tiles fastest. Warp 0 streams 64-wide steps of x and W, then the adapters' B, into a
 // ring by TMA; warp 1 issues the MMAs into one of two accumulators; warps 2 .. 5 make the list and h's operand tiles;
 // warps 6 .. 13 store y: accumulator rows through shared memory, so that a store covers 32 neighbouring words of a row at
@@ -432,6 +435,54 @@ struct LrArgs {
 
 // the nearest tf32 (11 bits), ties away from zero; not for a NaN whose payload would carry over
 __device__ __forceinline__ float to_tf32(float v) { return __uint_as_float((__float_as_uint(v) + 0x1000u) & 0xffffe000u); }
+
+__device__ __forceinline__ bool any_not_finite(const float (&v)[8]) {
+  float z = 0.f;
+#pragma unroll
+  for (int c = 0; c < 8; c++) z = fmaf(v[c], 0.f, z);
+  return z != 0.f;
+}
+// whether row r's own inputs, its h or without an adapter its x, hold a NaN or an infinity
+template <int T>
+__device__ __forceinline__ bool row_not_finite(const bnnk_lowrank_args &p, long long r, int s) {
+  float v[8];
+  bool bad = false;
+  if (s >= 0)
+    for (int e = 0; e < p.rank; e += 8) {
+      load_elems<0, 8>(p.hid + r * p.rank + e, v);
+      bad |= any_not_finite(v);
+    }
+  else
+    for (int k = 0; k < p.K; k += 8) {
+      load_elems<T, 8>((const elem_t<T> *)p.x + r * p.ldx + k, v);
+      bad |= any_not_finite(v);
+    }
+  return bad;
+}
+// y of row r, whose adapter is s, and column n
+template <int T>
+__device__ __forceinline__ float row_product(const bnnk_lowrank_args &p, long long r, int s, int n) {
+  float sum = p.bias ? p.bias[n] : 0.f;
+#pragma unroll 1
+  for (int k = 0; k < p.K; k += 8) {
+    float xv[8], wv[8];
+    load_elems<T, 8>((const elem_t<T> *)p.x + r * p.ldx + k, xv);
+    load_elems<T, 8>((const elem_t<T> *)p.w + n * p.ldw + k, wv);
+#pragma unroll
+    for (int c = 0; c < 8; c++) sum = fmaf(xv[c], wv[c], sum);
+  }
+  float u = 0.f;
+  if (s >= 0)
+#pragma unroll 1
+    for (int e = 0; e < p.rank; e += 8) {
+      float h[8], b[8];
+      load_elems<0, 8>(p.hid + r * p.rank + e, h);
+      load_elems<T, 8>((const elem_t<T> *)p.b + ((long long)s * p.N + n) * p.rank + e, b);
+#pragma unroll
+      for (int c = 0; c < 8; c++) u = fmaf(h[c], b[c], u);
+    }
+  return sum + u;
+}
 
 template <int T, int OT, int RB>
 __global__ void __launch_bounds__(kLrThreads, 1) k_lowrank_many(const __grid_constant__ CUtensorMap mx,
@@ -809,6 +860,7 @@ __global__ void __launch_bounds__(kLrThreads, 1) k_lowrank_many(const __grid_con
       tc_fence_after();
       const uint32_t tq = tmem + g * a.na * a.acc_cols + ((uint32_t)(32 * qd) << 16);
       const int width = min(bn, p.N - n0), rows = min(32, p.rows - r0);
+      int own_bad = -1, own = -1;  // this lane's row: row_not_finite (-1: not looked at yet), its adapter
 #pragma unroll 1
       for (int c0 = h * CW; c0 < width; c0 += 2 * CW) {
 #pragma unroll
@@ -838,6 +890,28 @@ __global__ void __launch_bounds__(kLrThreads, 1) k_lowrank_many(const __grid_con
 #pragma unroll
               for (int j = 0; j < 16; j++) v[j] += __uint_as_float(x[j]);
             }
+          if (adapters) {
+            float z = 0.f;
+#pragma unroll
+            for (int j = 0; j < 16; j++) z = fmaf(v[j], 0.f, z);
+            if (__any_sync(0xffffffffu, z != 0.f)) {
+              if (z != 0.f && lane < rows && own_bad < 0) {
+                own = p.slot[r0 + lane];
+                if (own >= p.slots) own = -1;
+                own_bad = row_not_finite<T>(p, r0 + lane, own);
+              }
+#pragma unroll 1
+              for (int j = 0; j < 16 && c + j < width; j++) {
+                float u = 0.f;
+#pragma unroll
+                for (int i = 0; i < 16; i++) u = i == j ? v[i] : u;
+                if (lane >= rows || own_bad || u * 0.f == 0.f) continue;
+                u = row_product<T>(p, r0 + lane, own, n0 + c + j);
+#pragma unroll
+                for (int i = 0; i < 16; i++) v[i] = i == j ? u : v[i];
+              }
+            }
+          }
           __syncwarp();
 #pragma unroll
           for (int j = 0; j < 16; j += 4 * PW) {

@@ -276,8 +276,7 @@ bnn_lowrank *bnn_lowrank_new(int type, int out_type, int N, int K, const void *d
                              int slots, int rank, const void *d_a, const void *d_b, const float *d_scale, int rows);
 /* d_x [rows][K] at row stride ldx (a multiple of 8, 16-byte aligned) -> d_y [rows][N] at row stride ldy; d_slot [rows]:
  * the rows' adapters in any order (outside 0 .. slots - 1: none), NULL: none for all. An infinity or a NaN in d_x stays
- * in its row; one in d_b of an adapter may reach, in a call of more than 128 rows, the rows of others beside its own
- * rows (they share tiles of 128). */
+ * in its row, one in an adapter in that adapter's rows. */
 int bnn_lowrank_run(bnn_lowrank *op, int rows, const void *d_x, long long ldx, const int32_t *d_slot, void *d_y,
                     long long ldy, void *stream);
 int bnn_lowrank_run_words(bnn_lowrank *op, const long long *words); /* the 7 arguments after op as words */

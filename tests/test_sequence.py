@@ -635,6 +635,36 @@ def test_lowrank_fp16_tiles_of_both_kinds(cuda, rank, out):
 
 
 @gpu
+@pytest.mark.parametrize("dtype, out", [("f16", "f16"), ("f16", "f32"), ("bf16", "bf16"), ("bf16", "f32")])
+@pytest.mark.parametrize("rows", [1, 12, 100, 128, 129, 300, 1000])
+@pytest.mark.parametrize("where, value", [("a", math.nan), ("b", math.nan), ("b", math.inf), ("x", math.nan), ("scale", math.inf)])
+@pytest.mark.parametrize("size", [1.0, 1e-3])
+def test_lowrank_values_that_are_no_numbers(cuda, dtype, out, rows, where, value, size):
+    """what is not finite in one adapter or one row stays in its rows, whatever shares the call"""
+    gen, K, N, rank, slots = generator(rows), 72, 300, 24, 6
+    x, w = rand(gen, rows, K).to(DT[dtype]), rand(gen, N, K).to(DT[dtype])
+    A, B = (rand(gen, slots, rank, K) * 2.0 ** -3).to(DT[dtype]), rand(gen, slots, N, rank).to(DT[dtype])
+    bias, s = rand(gen, N), torch.full((slots,), size, device="cuda")
+    slot = torch.randint(-1, slots, (rows,), device="cuda", generator=gen).int()
+    slot[:2] = torch.tensor([1, 2][:rows]).int()
+    {"a": A[1, 3], "b": B[1, 7:20], "x": x[rows // 2], "scale": s[1:2]}[where][..., 0] = value
+    y = torch.full((rows, N), 7.0, device="cuda", dtype=DT[out])
+    op = sequence.LowRank(dtype, out, N, K, w.data_ptr(), bias.data_ptr(), slots, rank, A.data_ptr(), B.data_ptr(),
+                          s.data_ptr(), rows=rows)
+    op.run(rows, x.data_ptr(), slot.data_ptr(), y.data_ptr())
+    assert op.error == 0
+    xd, wd = x.double(), w.double()
+    want, M = xd @ wd.t() + bias.double(), xd.abs() @ wd.abs().t() + bias.double().abs()
+    for a in range(slots):
+        at = torch.nonzero(slot == a).flatten()
+        want[at] += (s[a].double() * (xd[at] @ A[a].double().t())) @ B[a].double().t()
+        M[at] += (s[a].double() * (xd[at].abs() @ A[a].double().abs().t())) @ B[a].double().abs().t()
+    fin = torch.isfinite(want)
+    assert torch.equal(torch.isfinite(y), fin)
+    check(y[fin], want[fin], (2.0 ** -15 + (K + rank + 4) * 2.0 ** -24) * M[fin], out, "y")
+
+
+@gpu
 def test_lowrank_adapter_replaced_between_runs(cuda):
     """the adapters are read by every run: one that is written in stream order counts from the next run on"""
     gen = generator(1)
