@@ -783,6 +783,22 @@ def test_norm_gate_rows_that_start_anywhere(cuda, case, norm, gate, types):
 
 
 @gpu
+@pytest.mark.parametrize("gate", ["sigmoid", "silu"])
+@pytest.mark.parametrize("D", [64, 1021, 9001])
+def test_norm_gate_fp32_gates_of_any_size(cuda, D, gate):
+    """u is 1 everywhere, so that x' is the gate: of fp32 g to a few roundings (the exponential's 2 ulp, the quotient's 2, the
+    products'), however large g is"""
+    x, f = torch.zeros(800, D, device="cuda"), torch.ones(800, D, device="cuda")
+    g = torch.linspace(-80.0, 80.0, 800 * D, device="cuda").view(800, D)
+    xo = torch.empty_like(x)
+    op = sequence.NormGate(D, "f32", "f32", "rms", gate, eps=0.0)
+    op.run(800, x.data_ptr(), f.data_ptr(), g.data_ptr(), xo.data_ptr(), None)
+    want = torch.sigmoid(g.double()) * (g.double() if gate == "silu" else 1.0)
+    # the norm of ones: its sum is exact, its root's reciprocal 2 ulp
+    check(xo, want, 8 * 2.0 ** -23 * want.abs(), "f32", "gate")
+
+
+@gpu
 def test_norm_gate_zero_rows_and_zero_values(cuda):
     op = sequence.NormGate(64, "f32", "bf16", "rms", "none")
     x = torch.zeros(4, 64, device="cuda")
