@@ -1143,8 +1143,12 @@ static int segment_tokens(int n, int Hk, long long tokens) {
 }
 
 extern "C" long long bnnk_dattn_scratch_states(int n, int Hk, long long tokens) {
-  if ((long long)n * Hk * 2 > num_sms()) n = num_sms() / (2 * Hk);  // the most sequences that are split
-  return n < 1 ? 0 : (long long)(n + num_sms() / Hk + 1) * Hk;
+  // the most sequences that are split: no more than half of the SMs have, and of more than a chunk each on average
+  long long most = num_sms() / (2 * Hk), parts = num_sms() / Hk;
+  if (most > n) most = n;
+  if (most > (tokens - 1) / kChunk) most = (tokens - 1) / kChunk;
+  if (parts > tokens / kChunk) parts = tokens / kChunk;
+  return most < 1 ? 0 : (most + parts + 1) * Hk;
 }
 
 extern "C" int bnnk_dattn(const bnnk_dattn_args *p, bnn_stream_t st) {
@@ -1160,7 +1164,9 @@ extern "C" int bnnk_dattn(const bnnk_dattn_args *p, bnn_stream_t st) {
   // 26.6 / 18.4; 300 sequences, d 64, of 12 tokens 111 / 136, of 16 144 / 135, d 128, of 4 183 / 200, of 8 326 / 202.
   // Lengths are known on the device alone, and one of 1000 tokens would take the recurrent form 2 ms: those far above the
   // average go to the chunk form in a second launch, of as many CTAs a head as there can be such sequences (2 us for every
-  // num_sms() of them that find none). Where the CTAs are few it costs what it saves: the chunk form has them all.
+  // num_sms() of them that find none). Where the CTAs are few that costs what it saves, and the call's tokens may all be one
+  // sequence's (16 tokens of one: 30 us recurrent, 15 by chunks; of 16: 8 and 14): the recurrent form has up to 4 tokens of
+  // the whole call there, the chunk form the others. Callers that know of single tokens have the step.
   const bool few = (long long)p->n * p->Hk <= num_sms();
   if (!p->cu || p->tokens <= (few ? 4ll : (wide ? 4ll : 12ll) * p->n)) {
     const int over = wide ? 32 : 64, warps = (p->dk + 15) / 16;

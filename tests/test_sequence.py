@@ -410,6 +410,30 @@ def test_dattn_live_tokens_without_numbers(cuda, dtype, heads, lens, bad, part, 
 
 
 @gpu
+def test_dattn_scratch_is_what_calls_can_use(cuda):
+    """none for an op of single tokens; for any capacity, at least a state for each head and part of every call it allows.
+    The parts of a call: those of `segment_tokens` in k_dattn.cu"""
+    import ctypes  # pylint: disable=import-outside-toplevel
+    states = load_library().bnnk_dattn_scratch_states
+    states.restype, states.argtypes = ctypes.c_longlong, [ctypes.c_int, ctypes.c_int, ctypes.c_longlong]
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    assert states(1, 8, 1) == 0 and states(300, 16, 300) == 0 and states(1, 1, 128) == 0
+
+    def parts(n, hk, tokens):
+        if n * hk * 2 > sms:
+            return 0
+        length = -(-(-(-tokens // max(1, sms // hk))) // 128) * 128
+        return 0 if tokens <= n * length else n + tokens // length
+
+    rng = np.random.default_rng(1)
+    for _ in range(20000):
+        hk, seqs, tokens = int(rng.integers(1, 100)), int(rng.integers(1, 160)), int(2 ** rng.uniform(0, 18))
+        n, used = int(rng.integers(1, seqs + 1)), int(rng.integers(1, tokens + 1))
+        for t in (used, tokens):
+            assert parts(n, hk, t) * hk <= states(seqs, hk, tokens), (n, t, hk, seqs, tokens)
+
+
+@gpu
 def test_dattn_offsets_past_32_bits(cuda):
     """states and rows more than 2^32 bytes and 2^31 elements into their buffers"""
     torch.cuda.empty_cache()
