@@ -1165,8 +1165,9 @@ extern "C" int bnnk_dattn(const bnnk_dattn_args *p, bnn_stream_t st) {
   // Lengths are known on the device alone, and one of 1000 tokens would take the recurrent form 2 ms: those far above the
   // average go to the chunk form in a second launch, of as many CTAs a head as there can be such sequences (2 us for every
   // num_sms() of them that find none). Where the CTAs are few that costs what it saves, and the call's tokens may all be one
-  // sequence's (16 tokens of one: 30 us recurrent, 15 by chunks; of 16: 8 and 14): the recurrent form has up to 4 tokens of
-  // the whole call there, the chunk form the others. Callers that know of single tokens have the step.
+  // sequence's (d 64: 16 tokens of one sequence 35 us recurrent, 14.3 by chunks; of 16 8.3 and 14.4; 4 of one 14.3 and 14.3):
+  // the recurrent form has up to 4 tokens of the whole call there, the chunk form the others. Callers that know of single
+  // tokens have the step.
   const bool few = (long long)p->n * p->Hk <= num_sms();
   if (!p->cu || p->tokens <= (few ? 4ll : (wide ? 4ll : 12ll) * p->n)) {
     const int over = wide ? 32 : 64, warps = (p->dk + 15) / 16;

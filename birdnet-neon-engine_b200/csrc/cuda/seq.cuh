@@ -38,12 +38,11 @@ __device__ __forceinline__ uint32_t pack2f(float a, float b) {
   else { const __nv_bfloat162 v = __floats2bfloat162_rn(a, b); return *reinterpret_cast<const uint32_t *>(&v); }
 }
 
-// V consecutive elements (V = 8: 16-byte accesses on 16-byte aligned addresses; V = 1: one element)
+// 8 consecutive elements by 16-byte accesses on 16-byte aligned addresses; stores of one element too (V = 1)
 template <int T, int V>
 __device__ __forceinline__ void load_elems(const elem_t<T> *p, float (&v)[V]) {
-  if constexpr (V == 1) {
-    v[0] = Elem<T>::get(*p);
-  } else if constexpr (T == 0) {
+  static_assert(V == 8, "8 elements");
+  if constexpr (T == 0) {
     const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
     v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
   } else {

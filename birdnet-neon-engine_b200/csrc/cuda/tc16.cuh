@@ -57,20 +57,12 @@ __device__ __forceinline__ void mma16_ts(uint32_t d, uint32_t ta, uint64_t db, u
 #define BNN_I4(r, i) "r"((r)[i]), "r"((r)[(i) + 1]), "r"((r)[(i) + 2]), "r"((r)[(i) + 3])
 #define BNN_P4(r, i) "+r"((r)[i]), "+r"((r)[(i) + 1]), "+r"((r)[(i) + 2]), "+r"((r)[(i) + 3])
 
-// this thread's lane, 16 or 32 consecutive 32-bit columns
+// this thread's lane, 16 consecutive 32-bit columns
 __device__ __forceinline__ void tmem_ld16(uint32_t t, uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
       "[%16];"
       : BNN_O4(r, 0), BNN_O4(r, 4), BNN_O4(r, 8), BNN_O4(r, 12)
-      : "r"(t));
-}
-__device__ __forceinline__ void tmem_ld32(uint32_t t, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : BNN_O4(r, 0), BNN_O4(r, 4), BNN_O4(r, 8), BNN_O4(r, 12), BNN_O4(r, 16), BNN_O4(r, 20), BNN_O4(r, 24),
-        BNN_O4(r, 28)
       : "r"(t));
 }
 __device__ __forceinline__ void tmem_st16(uint32_t t, const uint32_t (&r)[16]) {
@@ -81,11 +73,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t t, const uint32_t (&r)[16]) {
       : "memory");
 }
 // waits for this thread's TMEM loads; the registers they fill are operands, so that no use of them moves above
-__device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[32]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : BNN_P4(r, 0), BNN_P4(r, 4), BNN_P4(r, 8), BNN_P4(r, 12), BNN_P4(r, 16), BNN_P4(r, 20), BNN_P4(r, 24),
-                 BNN_P4(r, 28)::"memory");
-}
 __device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : BNN_P4(r, 0), BNN_P4(r, 4), BNN_P4(r, 8), BNN_P4(r, 12)::"memory");
