@@ -410,14 +410,48 @@ def test_dattn_live_tokens_without_numbers(cuda, dtype, heads, lens, bad, part, 
 
 
 @gpu
+@pytest.mark.parametrize("dtype, adds", [("bf16", 24), ("f16", 16)])
+@pytest.mark.parametrize("heads, lens", [((2, 2, 64, 64), [1000, 640]), ((2, 1, 128, 128), [1000, 640]), ((1, 1, 128, 128), [6000])])
+def test_dattn_states_are_fp32(cuda, dtype, adds, heads, lens):
+    """the states' error in rms: the products are exact but for the fp32 sums, a chunk's one chain of 8 steps for each of
+    K's parts (three for bf16, two for fp16), of which the tensor cores cut off at most 2^-24 of the sum at a step. With a
+    part less (16 or 11 bits of K') it would be above"""
+    a = Attention(dtype, *heads, lens, seed=18, decay=[0.99] * heads[1])
+    s1 = torch.zeros_like(a.s0)
+    a.run(a.op(), s1=s1)
+    _, states = a.want()
+    for i, (S, _) in enumerate(states):
+        assert float((s1[int(a.slot[i])].double() - S).norm() / S.norm()) < adds * 2.0 ** -24
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_dattn_steps_after_a_prompt_against_64_bits(cuda, dtype, d):
+    """outputs and state of single steps on the state that a prompt left, as of one sequence"""
+    a = Attention(dtype, 4, 2, d, d, [140], 0.1, seed=19)
+    state, op = a.s0.clone(), a.op()
+    cu = torch.tensor([0, 130]).int().cuda()
+    kw = dict(slot=a.slot.data_ptr(), qts=a.ts, kts=a.ts, vts=a.ts)
+
+    def at(t):
+        return [x[t].data_ptr() for x in (a.q, a.k, a.v, a.o)] + [state.data_ptr()] * 2
+
+    op.run(1, 130, cu.data_ptr(), *at(0), live=a.live.data_ptr(), **kw)
+    for t in range(130, 140):
+        op.step(1, *at(t), live=a.live[t:].data_ptr(), **kw)
+    a.check(state)
+
+
+@gpu
 def test_dattn_scratch_is_what_calls_can_use(cuda):
-    """none for an op of single tokens; for any capacity, at least a state for each head and part of every call it allows.
-    The parts of a call: those of `segment_tokens` in k_dattn.cu"""
+    """none where no call has more tokens than a chunk; for any capacity, at least a state for each head and part of every
+    call it allows. The parts of a call: those of `segment_tokens` in k_dattn.cu"""
     import ctypes  # pylint: disable=import-outside-toplevel
     states = load_library().bnnk_dattn_scratch_states
     states.restype, states.argtypes = ctypes.c_longlong, [ctypes.c_int, ctypes.c_int, ctypes.c_longlong]
     sms = torch.cuda.get_device_properties(0).multi_processor_count
-    assert states(1, 8, 1) == 0 and states(300, 16, 300) == 0 and states(1, 1, 128) == 0
+    assert states(1, 8, 1) == 0 and states(1, 1, 128) == 0 and states(100, 16, 100) == 0
 
     def parts(n, hk, tokens):
         if n * hk * 2 > sms:
@@ -626,6 +660,26 @@ def test_lowrank_keeps_h_of_any_size(cuda, dtype, rows, scale):
     want = torch.einsum("rj,rnj->rn", h, B.double()[slot.long()])
     assert float((y.double() - want).norm() / want.norm()) < 2.0 ** -19
     assert op.error == 0
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("rows, K, adds", [(12, 1024, 16), (64, 1024, 16), (128, 1024, 16), (300, 4096, 64)])
+def test_lowrank_fp32_outputs_are_fp32(cuda, dtype, rows, K, adds):
+    """the error in rms of fp32 outputs: of chains of so many steps of the tensor cores (K / 16 over the form's accumulators),
+    which cut off up to 2^-24 of the sum at each, half of it on average"""
+    gen, N, rank, slots = generator(rows), 260, 16, 4
+    x, w = rand(gen, rows, K).to(DT[dtype]), (rand(gen, N, K) * K ** -0.5).to(DT[dtype])
+    A, B = (rand(gen, slots, rank, K) * K ** -0.5).to(DT[dtype]), rand(gen, slots, N, rank).to(DT[dtype])
+    slot = torch.randint(-1, slots, (rows,), device="cuda", generator=gen).int()
+    y = torch.empty(rows, N, device="cuda")
+    op = sequence.LowRank(dtype, "f32", N, K, w.data_ptr(), None, slots, rank, A.data_ptr(), B.data_ptr(), rows=rows)
+    op.run(rows, x.data_ptr(), slot.data_ptr(), y.data_ptr())
+    want = x.double() @ w.double().t()
+    for a in range(slots):
+        at = torch.nonzero(slot == a).flatten()
+        want[at] += (x[at].double() @ A[a].double().t()) @ B[a].double().t()
+    assert float((y.double() - want).norm() / want.norm()) < adds * 2.0 ** -25
 
 
 @gpu
