@@ -725,7 +725,7 @@ static int *op_err_word(void) {
   if (cudaGetDevice(&dev) || dev < 0 || dev >= 64) return NULL;
   pthread_mutex_lock(&g_op_err_mu);
   if (!g_op_err[dev] && !cudaMalloc((void **)&g_op_err[dev], sizeof(int)) &&
-      cudaMemset(g_op_err[dev], 0, sizeof(int))) {
+      (cudaMemset(g_op_err[dev], 0, sizeof(int)) || cudaStreamSynchronize(cudaStreamLegacy))) {
     cudaFree(g_op_err[dev]);
     g_op_err[dev] = NULL;
   }
@@ -743,8 +743,9 @@ int bnn_cuda_device_init(void) {
 
 int bnn_cuda_op_error(void) {
   int *w = op_err_word(), v = 0;
-  if (!w || cudaMemcpy(&v, w, sizeof v, cudaMemcpyDeviceToHost)) return -1;
-  if (v) cudaMemset(w, 0, sizeof(int));
+  /* the copy alone does not wait for operators on streams made non-blocking */
+  if (!w || cudaDeviceSynchronize() || cudaMemcpy(&v, w, sizeof v, cudaMemcpyDeviceToHost)) return -1;
+  if (v && (cudaMemset(w, 0, sizeof(int)) || cudaStreamSynchronize(cudaStreamLegacy))) return -1;
   return v;
 }
 

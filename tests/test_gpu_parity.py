@@ -416,3 +416,24 @@ def test_two_gpus_in_one_context(lib, mini_pkg):
         out2, emb2 = m2.infer_batch(pcm)
     assert bits_equal(out1, out2), mismatch_report(out1, out2)
     assert bits_equal(emb1, emb2), mismatch_report(emb1, emb2)
+
+
+def test_op_error_waits_for_the_operators(lib):
+    """bnn_cuda_op_error is that of every operator issued before, on a non-blocking stream too"""
+    x, q = torch.rand(64, 32, device="cuda"), torch.zeros(64 * 32, dtype=torch.int8, device="cuda")
+    sa, za = torch.zeros(64, device="cuda"), torch.zeros(64, dtype=torch.int32, device="cuda")
+    side, done = torch.cuda.Stream(), torch.cuda.Event()
+
+    def run():
+        assert lib.bnn_cuda_quant_rows(64, 64, x.data_ptr(), 64 * 32, 32, 32, 32, None, 0, q.data_ptr(), sa.data_ptr(),
+                                       za.data_ptr(), side.cuda_stream) == 0, lib.bnn_last_error()
+
+    run()  # a kernel's first launch may wait for the device
+    assert lib.bnn_cuda_op_error() == 0
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(100_000_000)  # pylint: disable=protected-access
+        run()
+        done.record()
+    assert not done.query()
+    assert lib.bnn_cuda_op_error() == 0 and done.query()
