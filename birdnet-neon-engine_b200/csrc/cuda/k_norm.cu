@@ -8,9 +8,10 @@
 // gets h = 0 whatever its f and g hold (they are not read).
 //
 // Bound by memory: f, g, x in, x', h out. 28800 rows of 1536 (x fp32, the rest bf16, 619 MB): 119 us, 5.2 TB/s. A row
-// over the warps of a block keeps a thread's share small (56 registers); a warp a row took 242 us (250 registers, few
-// rows in flight), the same without the next row's loads ahead of this row's sums 141 us, without the vectors in registers
-// 149 us. Four blocks of 6 warps an SM: with five 143 us, with eight 120 us.
+// over the warps of a block keeps a thread's share small (75 registers, 94 with biases); a warp a row took 242 us (250
+// registers, few rows in flight), the same without the next row's loads ahead of this row's sums 141 us, without the vectors
+// in registers 149 us. 24 warps an SM stay: with 16 and 32, 256 wide 43.3 -> 47.3 and 52.5 us (60000 rows), 1024 77.8 -> 89.3
+// and 94.9 (28800), 1536 118 -> 168 and 148, 2048 90 -> 103 and 111 (16384), 4096 117 -> 111 and 122 (10000), cold caches.
 #include <cuda_runtime.h>
 
 #include "bnn_kernels.h"
@@ -340,6 +341,13 @@ cudaError_t launch_rows(const NormArgs &a, cudaStream_t st) {
 
 template <int XT, int FT>
 cudaError_t launch_norm(const NormArgs &a, bool vec, bool shifted, cudaStream_t st) {
+  // Up to 2048 wide a thread has one group of 8 elements, up to 8192 four: 255 registers there and up to 350 bytes of them
+  // spilled, and still ahead of the form without (fp32 residual, bf16, RMS, us with four groups / wide form: 16320 rows of
+  // 2056 152 / 299, 8192 of 4096 100 / 283, 4096 of 8192 115 / 317, 300 of 4096 18.5 / 27.0; all fp32, layer norm, biases: 8192
+  // of 4096 228 / 394). Past that, and for rows off 16 bytes past 2048, the wide form: 4092 of 8200 320 us, 1677 of 20000 408,
+  // 8184 of 4100 293. Off 16 bytes with few rows, one element an access (500 rows, this form / wide: fp16, layer norm, 1021
+  // wide 14.2 / 16.4, 1500 24.6 / 19.6, 2001 24.6 / 22.5; bf16, RMS, 1500 14.3 / 16.4, 2001 15.1 / 18.4; 20000 rows of 100, fp16
+  // 22.5 / 129). Rows of any start, wide and many enough, by groups of 8 on the 16-byte boundaries:
   // 20000 rows, fp16, layer norm, us with groups of 8 between ends one by one / one element an access: 100 wide 20.6 / 18.7,
   // 193 22.5 / 34.9, 1533 150 / 281, 2001 152 / 379; 1021 wide, 1 row 5.5 / 3.9, 592 rows 8.8 / 8.2, 1184 12.3 / 13.9, 3000
   // 22.5 / 28.3 (1024 wide on 16 bytes: 16.5)
