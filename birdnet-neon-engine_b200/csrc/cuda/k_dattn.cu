@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(256) k_dattn_rec(const DattnArgs a) {
 //  - fp16: two parts are 22 bits, but only within the type's range, so each is scaled by a power of two that a maximum
 //    gives: P by its row's, S and K' by their tile's, and K' has the decays counted from the chunk's last live token. The
 //    scales go into the fp32 steps after the products. The maxima are those of the decayed values, so that a loud token
-//    long ago takes no bits from the present. The maximum comes to 2^14 .. 2^15 and the second part ends at 2^-24: 22 bits
+//    long ago takes no bits from the present (24 x 9600 tokens, cold caches: 761 us without the decays, 808 with). The maximum comes to 2^14 .. 2^15 and the second part ends at 2^-24: 22 bits
 //    for values down to 2^17 below the maximum, 11 at 2^28. That far below, P and S are under the rounding of an fp16 output
 //    beside the others; in K' it is a feature of k that small beside the chunk's largest.
 //
@@ -182,9 +182,9 @@ __global__ void __launch_bounds__(256) k_dattn_rec(const DattnArgs a) {
 //
 // Bound by its roles' chain through a chunk and by shared memory's bandwidth, not by the products: DP 64 takes 4900 cycles a
 // chunk and head, of which the products are 2400 (each operand's parts are products of their own). 24 sequences of 9600
-// tokens, 16 heads of 64 (bf16, 1.9 GB): 657 us, 2.9 TB/s; 384 CTAs on 148 SMs are 2.6 rounds that take 3. DP 128 has
-// shared memory for one stage only: one sequence of 28800 tokens, 12 heads of 128 (0.35 GB): 183 us, 62 of them the first
-// pass for the parts' states. 37 sequences of 1 to 611 tokens, 4 heads of 96 x 72 shared by 3 (fp16): 76 us.
+// tokens, 16 heads of 64 (bf16, 1.9 GB): 667 us, 2.8 TB/s; 384 CTAs on 148 SMs are 2.6 rounds that take 3. DP 128 has
+// shared memory for one stage only: one sequence of 28800 tokens, 12 heads of 128 (0.35 GB): 185 us, 62 of them the first
+// pass for the parts' states. 37 sequences of 1 to 611 tokens, 4 heads of 96 x 72 shared by 3 (fp16): 81 us.
 constexpr int kChunk = 128;
 constexpr int kDaThreads = 896;
 constexpr int kDaP = 4, kDaS = 12;  // first warps of the P and state roles

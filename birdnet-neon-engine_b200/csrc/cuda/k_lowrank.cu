@@ -234,8 +234,9 @@ __global__ void __launch_bounds__(256) k_lowrank_few(const bnnk_lowrank_args p) 
 // in fp32 outputs, against 2.6e-7 for a plain fp32 sum), so the chains are kept short.
 // Class head of 64 stations with an adapter each (64 x 1024 x 6522, rank 16, fp32 logits): 14 us.
 // More rows than 64 take one CTA per 64 of them. The many-row form gives each adapter of a tile its own steps; an adapter a
-// row is its worst case, one adapter its best (128 rows of 1024 x 6522, rank 32, fp32, us, this form / that one: an adapter
-// a row 43 / 103, 8 rows each 37 / 43, 64 each 36 / 25; 512 rows: 113 / 202, 100 / 70, 100 / 33). 128 rows are the middle.
+// row is its worst case, one adapter its best (1024 x 6522, rank 32, bf16 to fp32, cold caches, us, this form / that one: 128
+// rows with an adapter each 48 / 143, 8 rows each 38 / 39, 64 each 38 / 26; 300 rows 91 / 206, 65 / 46, 63 / 28; 512 rows 136 /
+// 296, 97 / 58, 97 / 30; fp16's that one 128 rows 108, 36, 26). 128 rows are the middle.
 constexpr int kMidRows = 64, kMidMost = 128, kMidThreads = 320, kMidStages = 8;
 
 struct MidArgs {
@@ -419,9 +420,11 @@ __global__ void __launch_bounds__(kMidThreads, 1) k_lowrank_mid(const __grid_con
 // ring by TMA; warp 1 issues the MMAs into one of two accumulators; warps 2 .. 5 make the list and h's operand tiles;
 // warps 6 .. 13 store y: accumulator rows through shared memory, so that a store covers 32 neighbouring words of a row at
 // any row alignment; 16 bytes a lane where y's rows are whole 16 bytes.
-// Bound by reading x and W from L2 (48 KB for 1040 cycles of products at 256 columns). 9001 x 1536 x 6144 without adapters
-// 130 us, 1.31 PFLOP/s (the library's product: 123 us); adapters of 700 rows and rank 32 on top 37 us, 27 of them to form h. Tiles of 256
-// rows, which read half of W, left no TMEM for a second accumulator: 241 us in place of 212 at the time.
+// Bound by reading x and W from L2 (48 KB for 1040 cycles of products at 256 columns). 9001 x 1536 x 6144, fp16, calls apart
+// with cold caches: 126 us without adapters, 1.35 PFLOP/s (the library's product: 123 us); with adapters of 700 rows and rank
+// 32 158, 27 of them to form h; one call after another, at the clocks that lasting load leaves, 186. Tiles of 256 rows, which
+// read half of W, left no TMEM for a second accumulator: 241 us in place of 212 at the time. Adapters that change from row to
+// row: 331 us (bf16 373).
 constexpr int kLrThreads = 448;
 constexpr int kLrStages = 8;
 constexpr int kLrPad = 20;  // words a row of the stores' shared memory: blocks of 16 words; 16-byte accesses meet no bank twice
