@@ -860,6 +860,11 @@ __global__ void __launch_bounds__(kDaThreads, 1) k_dattn_chunk(const __grid_cons
         float m = 0.f, inv;
 #pragma unroll
         for (int j = 0; j < HC; j++) m = fmaxf(m, fabsf(S[j]));
+        if (m == __int_as_float(0x7f800000)) {  // infinities are their columns' alone: the others' scale leaves them out
+          m = 0.f;
+#pragma unroll
+          for (int j = 0; j < HC; j++) m = fmaxf(m, isinf(S[j]) ? 0.f : fabsf(S[j]));
+        }
         sc = scale_to_f16(role_max(r < DP ? m : 0.f), inv);
         if (tid == 0) s_inv[c & 1] = inv;
       }

@@ -444,6 +444,34 @@ def test_dattn_steps_after_a_prompt_against_64_bits(cuda, dtype, d):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("heads", [(2, 1, 64, 64), (1, 1, 128, 72)])
+@pytest.mark.parametrize("where", ["v", "s0"])
+def test_dattn_infinite_columns_of_large_states(cuda, dtype, heads, where):
+    """a column of the state that is infinite, from a v or from the state that a sequence starts with, leaves the other
+    columns what they are, past fp16's largest value too"""
+    a = Attention(dtype, *heads, [300, 200], seed=20)
+    a.s0 *= 1e6
+    a.q *= 2.0 ** -10
+    if where == "v":
+        a.v[10, 0, 3] = math.inf
+    else:
+        a.s0[int(a.slot[0]), 0, 5, 3] = math.inf
+    s1, op = torch.zeros_like(a.s0), a.op()
+    a.run(op, s1=s1)
+    (want, mo), states = a.want()
+    fin = torch.isfinite(want)
+    rel = 2.0 ** -15 + (300 + a.dk + 4) * 2.0 ** -24
+    assert torch.equal(torch.isfinite(a.o), fin)
+    check(a.o[fin], want[fin], rel * mo[fin], dtype, "o")
+    for i, (S, M) in enumerate(states):
+        fin = torch.isfinite(S)
+        assert torch.equal(torch.isfinite(s1[int(a.slot[i])]), fin)
+        check(s1[int(a.slot[i])][fin], S[fin], rel * M[fin], "f32", f"state {i}")
+    assert op.error == 0
+
+
+@gpu
 def test_dattn_scratch_is_what_calls_can_use(cuda):
     """none where no call has more tokens than a chunk; for any capacity, at least a state for each head and part of every
     call it allows. The parts of a call: those of `segment_tokens` in k_dattn.cu"""
